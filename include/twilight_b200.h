@@ -333,6 +333,43 @@ TWL_API int twl_append_kv(const void* new_k, const void* new_v, int dtype, void*
                   int32_t num_kv_heads, int32_t num_pages_total, int32_t* status,
                   void* stream);
 
+/* ---- a prompt's way into the cache --------------------------------------------------------
+ * twl_rope_append_kv: rotary positions and the append of any number of new tokens per sequence in
+ * one pass (twl_append_kv for one token whose K is rotated already).  Replaces the RoPE and cache
+ * update of attention_forward (twilight/pyimpl/attention.py:82-126) on the paged layout.
+ * Sequence b's new tokens are rows qo_indptr[b]..qo_indptr[b+1] of q [T][H_q], k and v [T][H_kv]
+ * (heads of 128 contiguous elements; token and head strides in elements, multiples of 4, bases
+ * 8-byte aligned, so parts of one fused projection can be passed as they lie).  They are the LAST
+ * tokens of the sequence its page table describes: new token i has cache position
+ * len_b - n_b + i.  A sequence without new tokens is left alone (n_b = 0), one that has fewer tokens
+ * than new ones is skipped and flagged (TWL_FLAG_BAD_INDEX).  Written: the rotated q to q_out (which
+ * may be q itself), rotated K and V rows to the pages, and, unless null, the INT4 slabs (the
+ * arithmetic of twl_quantize_k_pages) and the page metadata (a page whose first row is new starts
+ * afresh, others fold).  A page that gets new tokens must not belong to a second sequence.
+ * Rotation of channels 0..rotary_dim (a multiple of 8 up to 128; 0 = none): pair i turns by
+ * position * freqs[i] (freqs: double [rotary_dim/2], radians per position), its channels are i and
+ * i + rotary_dim/2, or 2i and 2i+1 with `interleaved`; cos and sin are multiplied by
+ * attention_scale.  positions: int32 or int64 [T], or null for the cache positions.
+ * twl_dequantize_k_pages: the values of INT4 slabs, code*scale + min in fp32 rounded to `dtype`:
+ * out[n_pages][H_kv][16][128] of the pages page_ids[n_pages], or of the first n_pages when null.  A page
+ * id out of range gives zeros and a flag. */
+TWL_API int twl_rope_append_kv(const void* q, const void* k, const void* v, int dtype,
+                               int64_t q_token_stride, int64_t q_head_stride,
+                               int64_t k_token_stride, int64_t k_head_stride,
+                               int64_t v_token_stride, int64_t v_head_stride, void* q_out,
+                               int64_t out_token_stride, int64_t out_head_stride,
+                               const void* positions, int32_t positions_are_64bit,
+                               const double* freqs, int32_t rotary_dim, int32_t interleaved,
+                               float attention_scale, void* k_pages, void* v_pages,
+                               uint8_t* k4_pages, void* kmeta, const int32_t* qo_indptr,
+                               const int32_t* kv_indptr, const int32_t* kv_indices,
+                               const int32_t* kv_last_page_len, int32_t num_tokens, int32_t batch,
+                               int32_t num_q_heads, int32_t num_kv_heads, int32_t num_pages_total,
+                               int32_t* status, void* stream);
+TWL_API int twl_dequantize_k_pages(const uint8_t* k4_pages, const int32_t* page_ids, int64_t n_pages,
+                                   void* out, int dtype, int32_t num_kv_heads,
+                                   int32_t num_pages_total, int32_t* status, void* stream);
+
 /* Index list -> dense byte mask [rows][d] (the mask interface of twilight/pyimpl: selectors
  * and pruners return bool[B,H,1,L], attention.py:199-281).  mask must be zeroed by the caller. */
 TWL_API int twl_indices_to_mask(const int32_t* indices, int32_t index_stride, const int32_t* budget,

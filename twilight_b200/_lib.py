@@ -50,6 +50,10 @@ SIGNATURES = {
     "twl_select_prune_attend_step": (C.c_int, [ptr, C.c_int, ptr, ptr, ptr, ptr, ptr, ptr, ptr, i32, i32, i32,
                                                i32, i32, i32, i32, f32, ptr, f32, i32, i32, i32, ptr, ptr, sz,
                                                ptr, ptr]),
+    "twl_rope_append_kv": (C.c_int, [ptr, ptr, ptr, C.c_int, i64, i64, i64, i64, i64, i64, ptr, i64, i64, ptr, i32, ptr,
+                                     i32, i32, f32, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, i32, i32, i32, i32, i32,
+                                     ptr, ptr]),
+    "twl_dequantize_k_pages": (C.c_int, [ptr, ptr, i64, ptr, C.c_int, i32, i32, ptr, ptr]),
     "twl_round_scores": (C.c_int, [ptr, i64, C.c_int, f32, ptr]),
 }
 

@@ -15,6 +15,9 @@ from .ops import (  # noqa: F401
     quantize_k_pages,
     build_page_meta,
     append_kv,
+    rope_frequencies,
+    rope_append_kv,
+    dequantize_k_pages,
     indices_to_mask,
     batched_sparse_gemv_int4_k,
 )

@@ -491,6 +491,156 @@ def append_kv(new_k, new_v, k_pages, v_pages, k4_pages, kmeta, kv_indptr, kv_ind
             k_pages=k_pages, v_pages=v_pages, k4_pages=k4_pages, kmeta=kmeta, status=status)
 
 
+# ---------------------------------------------------------------------------------------------
+# a prompt's way into the cache
+# ---------------------------------------------------------------------------------------------
+def rope_frequencies(rotary_dim: int = HEAD_DIM, base: float = 10000.0, *, scaling: Optional[dict] = None,
+                     seq_len: Optional[int] = None, device="cuda") -> Tuple[torch.Tensor, float]:
+    """Angles per position of the ``rotary_dim/2`` rotary pairs (float64, for :func:`rope_append_kv`) and the
+    factor on cos and sin.  ``scaling`` takes the dictionaries that model configurations state
+    (``rope_scaling``), by ``rope_type``: ``"default"``; ``"linear"`` (positions divided by ``factor``);
+    ``"dynamic"`` (the base grows with ``seq_len`` beyond ``original_max_position_embeddings``); ``"llama3"``
+    (long wavelengths divided by ``factor``, short ones kept, a ramp between) and ``"yarn"`` (the same in terms
+    of the pair's index, with an attention factor)."""
+    if rotary_dim % 8 or not 8 <= rotary_dim <= HEAD_DIM:
+        raise _lib.TwilightError(f"rotary_dim must be a multiple of 8 from 8 to {HEAD_DIM}")
+    kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
+    pair = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    factor = 1.0 if scaling is None else float(scaling.get("factor", 1.0))
+    attention_scale = 1.0
+    if kind == "dynamic":
+        limit = scaling["original_max_position_embeddings"]
+        n = max(limit, seq_len or limit)
+        base = base * (factor * n / limit - (factor - 1)) ** (rotary_dim / (rotary_dim - 2))
+    freqs = base ** (-pair / rotary_dim)
+    if kind == "linear":
+        freqs = freqs / factor
+    elif kind == "llama3":
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        turns = scaling["original_max_position_embeddings"] * freqs / (2 * math.pi)  # within the original context
+        keep = ((turns - low) / (high - low)).clamp(0, 1)
+        freqs = freqs * (keep + (1 - keep) / factor)
+    elif kind == "yarn":
+        limit = scaling["original_max_position_embeddings"]
+
+        def index_of(turns):  # of the pair that makes this many turns within the original context
+            return rotary_dim * math.log(limit / (turns * 2 * math.pi)) / (2 * math.log(base))
+        first = max(math.floor(index_of(float(scaling.get("beta_fast", 32)))), 0)
+        last = min(math.ceil(index_of(float(scaling.get("beta_slow", 1)))), rotary_dim - 1)
+        ramp = ((pair / 2 - first) / max(last - first, 0.001)).clamp(0, 1)
+        freqs = freqs * (1 - ramp + ramp / factor)
+        attention_scale = scaling.get("attention_factor")
+        if attention_scale is None:
+            attention_scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif kind not in ("default", "dynamic"):
+        raise _lib.TwilightError(f"unknown rope_type {kind!r}")
+    return freqs.to(device), float(attention_scale)
+
+
+def _cuda(t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise _lib.TwilightError("the operators take CUDA tensors only (there is no CPU path)")
+
+
+def _rows(t: torch.Tensor, name: str, heads: Optional[int] = None) -> torch.Tensor:
+    if t.dim() != 3 or t.shape[-1] != HEAD_DIM or t.stride(-1) != 1:
+        raise _lib.TwilightError(f"{name} must be [tokens, heads, {HEAD_DIM}] with contiguous heads")
+    if heads is not None and t.shape[1] != heads:
+        raise _lib.TwilightError(f"{name} has {t.shape[1]} heads, the cache {heads}")
+    return t
+
+
+def _pages(dtype: torch.dtype, **pools: torch.Tensor) -> None:
+    """K/V pools (and metadata) of the queries' type, contiguous, with the layout's trailing dimensions."""
+    for name, t in pools.items():
+        want = (2, HEAD_DIM) if name == "kmeta" else (PAGE, HEAD_DIM)
+        if t.dim() != 4 or tuple(t.shape[2:]) != want or not t.is_contiguous():
+            raise _lib.TwilightError(f"{name} must be contiguous [pages, kv heads, {want[0]}, {want[1]}]")
+        if t.dtype != dtype:
+            raise _lib.TwilightError(f"{name} is {t.dtype}, q is {dtype}")
+
+
+def _table(batch: int, **tables: torch.Tensor) -> None:
+    """Page-table tensors: int32, contiguous, ``*indptr`` of batch+1 and ``*last_page_len`` of batch entries."""
+    for name, t in tables.items():
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise _lib.TwilightError(f"{name} must be contiguous int32")
+        want = batch + 1 if name.endswith("indptr") else batch if name.endswith("last_page_len") else None
+        if want is not None and t.numel() != want:
+            raise _lib.TwilightError(f"{name} must have {want} entries")
+
+
+def rope_append_kv(q, k, v, freqs, k_pages, v_pages, k4_pages, kmeta, qo_indptr, kv_indptr, kv_indices,
+                   kv_last_page_len, *, positions=None, interleaved: bool = False, attention_scale: float = 1.0,
+                   out=None, status=None) -> torch.Tensor:
+    """Rotary positions and the cache append of a ragged batch's new tokens in one pass; returns the rotated q.
+
+    ``q [T,Hq,128]``, ``k, v [T,Hkv,128]`` (views of one fused projection will do): sequence b's new tokens are
+    rows ``qo_indptr[b]:qo_indptr[b+1]`` and the last tokens of the sequence that the page table describes.
+    ``freqs`` (from :func:`rope_frequencies`) rotates the first ``2*len(freqs)`` channels, as halves or
+    ``interleaved`` pairs; None rotates nothing.  ``positions`` (int32 or int64 ``[T]``) replaces the cache
+    positions.  K and V rows, INT4 slabs (``k4_pages``) and page metadata (``kmeta``) are written in place; the
+    last two may be None.  ``out`` may be q itself."""
+    q, k, v = _rows(q, "q"), _rows(k, "k", k_pages.shape[1]), _rows(v, "v", k_pages.shape[1])
+    t, hq, _ = q.shape
+    batch = qo_indptr.numel() - 1
+    if k.shape[0] != t or v.shape[0] != t or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise _lib.TwilightError("q, k and v must have the same tokens and type")
+    if hq % k_pages.shape[1]:
+        raise _lib.TwilightError("query heads must be a multiple of KV heads")
+    _pages(q.dtype, k_pages=k_pages, v_pages=v_pages, **({} if kmeta is None else {"kmeta": kmeta}))
+    if v_pages.shape != k_pages.shape or (kmeta is not None and kmeta.shape[:2] != k_pages.shape[:2]):
+        raise _lib.TwilightError("k_pages, v_pages and kmeta must have the same pages and heads")
+    if k4_pages is not None and (k4_pages.dtype != torch.uint8 or not k4_pages.is_contiguous()
+                                 or k4_pages.shape != (*k_pages.shape[:2], K4_SLAB_BYTES)):
+        raise _lib.TwilightError(f"k4_pages must be contiguous uint8 [pages, kv heads, {K4_SLAB_BYTES}]")
+    _table(batch, qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices,
+           kv_last_page_len=kv_last_page_len)
+    if freqs is not None and (freqs.dtype != torch.float64 or not freqs.is_contiguous()):
+        raise _lib.TwilightError("freqs must be contiguous float64 (see rope_frequencies)")
+    if positions is not None and (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (t,)
+                                  or not positions.is_contiguous()):
+        raise _lib.TwilightError("positions must be contiguous int32 or int64, one for each token")
+    if out is None:
+        out = torch.empty(t, hq, HEAD_DIM, dtype=q.dtype, device=q.device)
+    elif _rows(out, "out").shape != q.shape or out.dtype != q.dtype:
+        raise _lib.TwilightError("out must have q's shape and type")
+    _cuda(q)
+    if t == 0:
+        return out
+    _launch("rope_append_kv", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(q), q.stride(0), q.stride(1),
+            k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+            _p(positions), int(positions is not None and positions.dtype == torch.int64), _p(freqs),
+            0 if freqs is None else 2 * freqs.numel(), int(interleaved), float(attention_scale), k_pages.data_ptr(),
+            v_pages.data_ptr(), _p(k4_pages), _p(kmeta), qo_indptr.data_ptr(), kv_indptr.data_ptr(),
+            kv_indices.data_ptr(), kv_last_page_len.data_ptr(), t, batch, hq, k_pages.shape[1], k_pages.shape[0],
+            _p(status), _stream(q.device), k=k, v=v, out=out, positions=positions, freqs=freqs, k_pages=k_pages,
+            v_pages=v_pages, k4_pages=k4_pages, kmeta=kmeta, qo_indptr=qo_indptr, kv_indptr=kv_indptr,
+            kv_indices=kv_indices, kv_last_page_len=kv_last_page_len, status=status)
+    return out
+
+
+def dequantize_k_pages(k4_pages, page_ids=None, *, dtype: torch.dtype, out=None, status=None) -> torch.Tensor:
+    """Values of INT4 slabs, ``code*scale + minimum`` rounded to ``dtype``: ``[n,Hkv,16,128]`` of the pages
+    ``page_ids`` (int32 ``[n]``), or of every page."""
+    _cuda_contig(k4_pages, "k4_pages")
+    if k4_pages.dtype != torch.uint8 or k4_pages.dim() != 3 or k4_pages.shape[2] != K4_SLAB_BYTES:
+        raise _lib.TwilightError(f"k4_pages must be uint8 [pages, kv heads, {K4_SLAB_BYTES}]")
+    pages, hkv = k4_pages.shape[0], k4_pages.shape[1]
+    if page_ids is not None and (page_ids.dtype != torch.int32 or page_ids.dim() != 1 or not page_ids.is_contiguous()):
+        raise _lib.TwilightError("page_ids must be contiguous int32 [n]")
+    n = pages if page_ids is None else page_ids.numel()
+    if out is None:
+        out = torch.empty(n, hkv, PAGE, HEAD_DIM, dtype=dtype, device=k4_pages.device)
+    elif out.shape != (n, hkv, PAGE, HEAD_DIM) or out.dtype != dtype or not out.is_contiguous():
+        raise _lib.TwilightError(f"out must be contiguous {dtype} [{n}, {hkv}, {PAGE}, {HEAD_DIM}]")
+    if out.numel() == 0:
+        return out
+    _launch("dequantize_k_pages", k4_pages, k4_pages.data_ptr(), _p(page_ids), n, out.data_ptr(), _dtype_code(out),
+            hkv, pages, _p(status), _stream(k4_pages.device), page_ids=page_ids, out=out, status=status)
+    return out
+
+
 def indices_to_mask(indices, budget, seq_len: int) -> torch.Tensor:
     """Index lists -> the reference's mask layout ``bool[B,H,1,L]`` (attention.py:199-281)."""
     b, hq, stride = indices.shape

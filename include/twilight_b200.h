@@ -370,6 +370,70 @@ TWL_API int twl_dequantize_k_pages(const uint8_t* k4_pages, const int32_t* page_
                                    void* out, int dtype, int32_t num_kv_heads,
                                    int32_t num_pages_total, int32_t* status, void* stream);
 
+/* ---- attention of more than one token at a time -------------------------------------------
+ * twl_prompt_attn: attention of a ragged batch's new tokens over the paged cache (the dense prefill of
+ * twilight/pyimpl/attention.py:157-182 on pages; chunks of a prompt and several tokens to verify are
+ * the same call).  Sequence b's queries are rows qo_indptr[b]..qo_indptr[b+1] of q [T][H_q][128] (token
+ * stride in elements, heads contiguous) and the LAST tokens its page table describes; with `causal`
+ * query i sees positions 0..len_b - n_b + i, else all len_b.  A row that sees nothing gives zeros.
+ * block_pages/block_npages (null: all pages) restrict every block of query_block queries (a multiple
+ * of 16) of a KV head to a list of ascending logical pages, as twl_quest_select_blocks writes it:
+ * block j of sequence b is row qo_indptr[b]/query_block + b + j of [slots][H_kv][max_k], slots =
+ * T/query_block + batch.
+ * out [T][H_q][128]; lse (nullable) fp32 [T][H_q], natural logarithm of the sum of exponentials, -inf
+ * for a row without keys.  Rows of q behind qo_indptr[batch] are left as they were.
+ * Softmax statistics and accumulators are fp32; weights are rounded to `dtype` for the product with V.
+ * max_pages = the largest page count of a sequence (sizes the workspace).  workspace: at least
+ * twl_prompt_attn_workspace_bytes(...) bytes, 256-byte aligned, contents irrelevant; calls that can
+ * overlap on the GPU need one each.  V rows of tokens that a query does not see must be finite where they
+ * share a tile of keys with tokens that it sees (rows behind a sequence's end may hold anything).
+ *
+ * twl_quest_select_blocks: the pages a block of queries attends to: all pages from the one that
+ * holds its first position on, and of the pages before that the max(1,budget/16)+(budget%16!=0) with the
+ * largest sums over the block's rows (tokens x query heads of the KV head) of Quest's bound
+ * sum_d max(q_d*kmax_d, q_d*kmin_d) (twilight/pyimpl/quest.py:37-99 applied to a block), ties to the
+ * lower page, in fp32.  pooled: fp32 [slots][H_kv][256] and page_scores: fp32
+ * [slots][H_kv][max_pages], caller scratch (kept as outputs for inspection: sums of min(q,0) and
+ * max(q,0); scores of the pages before the block).
+ *
+ * twl_shared_prefix_attn: decode attention (one token per sequence) of groups of sequences that share a
+ * prefix.  Group i is the sequences group_indptr[i]..group_indptr[i+1] of the batch; its prefix is a page
+ * list of its own (prefix_indptr[num_groups+1], prefix_indices, prefix_last_page_len), read once for the
+ * whole group; kv_indptr/kv_indices/kv_last_page_len describe what each sequence has behind it (no
+ * page: nothing; last_page_len is not read then).  out = attention over both parts; zeros where both
+ * are empty.  A sequence that no group names has no prefix.  max_pages = the largest page count of a
+ * prefix or a sequence's own part. */
+TWL_API size_t twl_prompt_attn_workspace_bytes(int32_t num_tokens, int32_t batch, int32_t num_q_heads,
+                                               int32_t num_kv_heads, int32_t max_pages,
+                                               int32_t query_block);
+TWL_API int twl_prompt_attn(const void* q, int dtype, int64_t q_token_stride, const void* k_pages,
+                            const void* v_pages, const int32_t* qo_indptr, const int32_t* kv_indptr,
+                            const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                            int32_t num_tokens, int32_t batch, int32_t num_q_heads,
+                            int32_t num_kv_heads, int32_t num_pages_total, int32_t max_pages,
+                            int32_t causal, const int32_t* block_pages, const int32_t* block_npages,
+                            int32_t max_k, int32_t query_block, float sm_scale, void* out, float* lse,
+                            void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+TWL_API int twl_quest_select_blocks(const void* q, int dtype, int64_t q_token_stride, const void* kmeta,
+                                    const int32_t* qo_indptr, const int32_t* kv_indptr,
+                                    const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                                    int32_t num_tokens, int32_t batch, int32_t num_q_heads,
+                                    int32_t num_kv_heads, int32_t num_pages_total, int32_t token_budget,
+                                    int32_t query_block, int32_t max_pages, float* pooled,
+                                    float* page_scores, int32_t* block_pages, int32_t* block_npages,
+                                    int32_t max_k, int32_t* status, void* stream);
+TWL_API size_t twl_shared_prefix_workspace_bytes(int32_t batch, int32_t num_groups, int32_t num_q_heads,
+                                                 int32_t num_kv_heads, int32_t max_pages);
+TWL_API int twl_shared_prefix_attn(const void* q, int dtype, int64_t q_token_stride, const void* k_pages,
+                                   const void* v_pages, const int32_t* group_indptr,
+                                   const int32_t* prefix_indptr, const int32_t* prefix_indices,
+                                   const int32_t* prefix_last_page_len, const int32_t* kv_indptr,
+                                   const int32_t* kv_indices, const int32_t* kv_last_page_len,
+                                   int32_t batch, int32_t num_groups, int32_t num_q_heads,
+                                   int32_t num_kv_heads, int32_t num_pages_total, int32_t max_pages,
+                                   float sm_scale, void* out, float* lse, void* workspace,
+                                   size_t workspace_bytes, int32_t* status, void* stream);
+
 /* Index list -> dense byte mask [rows][d] (the mask interface of twilight/pyimpl: selectors
  * and pruners return bool[B,H,1,L], attention.py:199-281).  mask must be zeroed by the caller. */
 TWL_API int twl_indices_to_mask(const int32_t* indices, int32_t index_stride, const int32_t* budget,

@@ -1,0 +1,371 @@
+"""Attention of ragged prompts (dense, and over selected pages) and of decode batches with a shared prefix, against plain
+64-bit implementations."""
+import math
+
+import pytest
+import torch
+
+from twilight_b200.cache import PAGE, PagedKVCache
+from twilight_b200.kernel import ops
+
+pytestmark = pytest.mark.gpu
+DEV, D = "cuda", 128
+SCALE = 1.0 / math.sqrt(D)
+I32 = dict(dtype=torch.int32, device=DEV)
+
+
+def tol_of(dtype, p, v, ref):
+    """Bound on |out - ref| per element: the output's rounding (half a step), the weights' rounding (half a step of each,
+    which adds up to at most eps/2 * sum p|v|), and 32-bit arithmetic over the row (2^-18 of sum p|v| covers logits up to
+    64 in size, whose 32-bit products and scaled differences are off by 64 * 2^-24, and the sums)."""
+    eps = torch.finfo(dtype).eps
+    mass = p @ v.abs()
+    return eps / 2 * ref.abs() + (eps / 2 + 2.0 ** -18) * mass + torch.finfo(dtype).smallest_normal * eps
+
+
+def attend64(q, k, v, keep, scale=SCALE):
+    """q [R,D], k/v [L,D], keep [R,L] -> out, lse, p in 64 bits; rows without keys give zeros and -inf."""
+    x = (q @ k.T) * scale
+    x = x.masked_fill(~keep, -math.inf)
+    lse = torch.logsumexp(x, -1) if k.shape[0] else torch.full((q.shape[0],), -math.inf, dtype=torch.float64, device=q.device)
+    p = torch.exp(x - torch.where(lse == -math.inf, torch.zeros_like(lse), lse)[:, None])
+    return p @ v, lse, p
+
+
+def pool(pages, hkv, dtype, seed):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    lean = torch.randn(hkv, 1, D, generator=g, device=DEV)
+    heavy = torch.rand(pages, hkv, PAGE, 1, generator=g, device=DEV) < 0.02
+    k = (torch.randn(pages, hkv, PAGE, D, generator=g, device=DEV) + (0.1 + 0.6 * heavy) * lean).to(dtype)
+    v = torch.randn(pages, hkv, PAGE, D, generator=g, device=DEV).to(dtype)
+    return k, v, lean, g
+
+
+def table(lens, seed, at=0, total=None):
+    n = [(x + PAGE - 1) // PAGE for x in lens]
+    ptr = torch.tensor([0] + torch.tensor(n).cumsum(0).tolist(), **I32)
+    order = torch.randperm(total or sum(n), generator=torch.Generator().manual_seed(seed))[at: at + sum(n)]
+    last = torch.tensor([(x - 1) % PAGE + 1 if x else 0 for x in lens], **I32)
+    return ptr, order.to(**I32), last
+
+
+def dense(pages, ptr, idx, b, n, h):
+    ids = idx[int(ptr[b]): int(ptr[b + 1])].long()
+    return pages[ids, h].reshape(-1, D)[:n].double()
+
+
+def poison_tails(k, v, ptr, idx, lens):
+    """Whatever lies behind a sequence's end in its last page must not matter."""
+    for b, n in enumerate(lens):
+        if n % PAGE:
+            page = int(idx[int(ptr[b + 1]) - 1])
+            k[page, :, n % PAGE:] = float("nan")
+            v[page, :, n % PAGE:] = float("inf")
+
+
+def make_prompt(new, old, hq, hkv, dtype, seed=0, strided=False):
+    lens = [a + b for a, b in zip(new, old)]
+    ptr, idx, last = table(lens, seed + 1)
+    k, v, lean, g = pool(max(1, idx.numel()), hkv, dtype, seed)
+    q = torch.randn(sum(new), hkv, hq // hkv, D, generator=g, device=DEV) + 0.3 * lean
+    q = q.reshape(sum(new), hq, D).to(dtype)
+    if strided:  # a part of a wider projection
+        wide = torch.randn(sum(new), hq + 3, D, generator=g, device=DEV).to(dtype)
+        wide[:, :hq] = q
+        q = wide[:, :hq]
+    qo = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), **I32)
+    return q, k, v, qo, (ptr, idx, last), lens
+
+
+def check_prompt(q, k, v, qo, tab, lens, out, lse, causal=True, pages_of=None, block=64):
+    hq, hkv, dtype = q.shape[1], k.shape[1], q.dtype
+    g = hq // hkv
+    for b, n in enumerate(lens):
+        a, e = int(qo[b]), int(qo[b + 1])
+        m = e - a
+        if m == 0:
+            continue
+        at = torch.arange(n, device=DEV)
+        where = n - m + torch.arange(m, device=DEV)
+        for h in range(hkv):
+            kk, vv = (dense(x, tab[0], tab[1], b, n, h) for x in (k, v))
+            keep = (at <= where[:, None]) if causal else torch.ones(m, n, dtype=torch.bool, device=DEV)
+            if pages_of is not None:
+                allowed = torch.zeros(m, n, dtype=torch.bool, device=DEV)
+                for t0 in range(0, m, block):
+                    allowed[t0: t0 + block] = torch.isin(at // PAGE, pages_of(b, t0 // block, h))
+                keep = keep & allowed
+            keep = keep[:, None].expand(m, g, n).reshape(m * g, n)
+            ref, ref_lse, p = attend64(q[a:e, h * g: (h + 1) * g].double().reshape(m * g, D), kk, vv, keep)
+            got = out[a:e, h * g: (h + 1) * g].double().reshape(m * g, D)
+            bad = (got - ref).abs() > tol_of(dtype, p, vv, ref)
+            assert not bad.any(), (b, h, int(bad.sum()), float((got - ref).abs().max()))
+            got_lse = lse[a:e, h * g: (h + 1) * g].double().reshape(-1)
+            none = ref_lse == -math.inf
+            assert (got_lse[none] == -math.inf).all() and not got[none].any()
+            # 32-bit logits and sums: 2^-18 absolute for logits up to 64, 2^-22 of the logarithm itself
+            assert ((got_lse - ref_lse)[~none].abs() <= 2.0 ** -18 + 2.0 ** -22 * ref_lse[~none].abs()).all()
+
+
+PROMPTS = [
+    # new, old, hq, hkv, dtype
+    ([1], [0], 4, 1, torch.bfloat16),
+    ([1, 1, 1], [0, 15, 16], 8, 8, torch.float16),
+    ([3, 0, 17, 5], [0, 40, 0, 300], 8, 2, torch.bfloat16),
+    ([64, 1, 2], [64, 1000, 0], 7, 1, torch.float16),
+    ([129, 33, 300], [1, 0, 77], 6, 2, torch.bfloat16),
+    ([1000], [24], 4, 4, torch.float16),
+    ([257, 255], [0, 513], 16, 2, torch.bfloat16),
+    ([40, 3], [2500, 4000], 5, 1, torch.bfloat16),
+    ([2, 70], [31, 9], 48, 2, torch.float16),
+    ([600], [0], 40, 8, torch.bfloat16),
+]
+
+
+@pytest.mark.parametrize("case", PROMPTS, ids=[str(i) for i in range(len(PROMPTS))])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_attention(case, causal):
+    new, old, hq, hkv, dtype = case
+    q, k, v, qo, tab, lens = make_prompt(new, old, hq, hkv, dtype, seed=len(new), strided=sum(new) % 2 == 0)
+    poison_tails(k, v, tab[0], tab[1], lens)
+    status = torch.zeros(1, **I32)
+    out, lse = ops.prompt_attn(q, k, v, qo, *tab, max_pages=max((n + 15) // 16 for n in lens), causal=causal, lse=True,
+                               status=status)
+    assert int(status) == 0
+    k, v = torch.nan_to_num(k, 0, 0, 0), torch.nan_to_num(v, 0, 0, 0)
+    check_prompt(q, k, v, qo, tab, lens, out, lse, causal)
+
+
+SPARSE = [
+    # new, old, hq, hkv, dtype, budget, block
+    ([200], [1000], 8, 2, torch.bfloat16, 256, 64),
+    ([130, 1, 64], [37, 700, 0], 4, 4, torch.float16, 100, 32),
+    ([300, 20], [5, 2000], 16, 2, torch.bfloat16, 64, 128),
+    ([513], [511], 7, 1, torch.float16, 17, 16),
+    ([100, 90], [0, 3000], 6, 2, torch.bfloat16, 5000, 64),      # the budget covers everything
+    ([2, 3, 1], [900, 0, 1500], 8, 1, torch.bfloat16, 128, 64),  # a few tokens each
+]
+
+
+def plain_blocks(q, meta, qo, tab, lens, budget, block, b, j, h, g):
+    """Pages of block j of sequence b for KV head h, and the history's scores, in 64 bits."""
+    a, e = int(qo[b]), int(qo[b + 1])
+    t0 = j * block
+    rows = q[a + t0: min(e, a + t0 + block), h * g: (h + 1) * g].double().reshape(-1, D)
+    first = lens[b] - (e - a) + t0
+    last = first + rows.shape[0] // g - 1
+    n = first // PAGE
+    ids = tab[1][int(tab[0][b]): int(tab[0][b + 1])].long()[:n]
+    lo, hi = meta[ids, h, 0].double(), meta[ids, h, 1].double()
+    score = torch.maximum(rows[:, None] * lo, rows[:, None] * hi).sum((0, 2)) if n else torch.zeros(0, device=DEV)
+    k = max(1, budget // PAGE) + (budget % PAGE != 0)
+    return score, min(k, n), torch.arange(n, last // PAGE + 1, device=DEV), rows
+
+
+@pytest.mark.parametrize("case", SPARSE, ids=[str(i) for i in range(len(SPARSE))])
+def test_selected_pages_and_sparse_prompt_attention(case):
+    new, old, hq, hkv, dtype, budget, block = case
+    q, k, v, qo, tab, lens = make_prompt(new, old, hq, hkv, dtype, seed=7)
+    g = hq // hkv
+    most = max((n + 15) // 16 for n in lens)
+    meta = ops.build_page_meta(k, *tab, max_pages=most)
+    poison_tails(k, v, tab[0], tab[1], lens)
+    status = torch.zeros(1, **I32)
+    pages, count = ops.quest_select_blocks(q, meta, qo, *tab, budget, max_pages=most, query_block=block, status=status)
+    assert int(status) == 0
+
+    def slot(b, j):
+        return int(qo[b]) // block + b + j
+
+    for b in range(len(new)):
+        for j in range((new[b] + block - 1) // block):
+            for h in range(hkv):
+                got = pages[slot(b, j), h, : int(count[slot(b, j), h])].long()
+                score, n, mine, rows = plain_blocks(q, meta, qo, tab, lens, budget, block, b, j, h, g)
+                assert got.numel() == n + mine.numel() and (got[1:] > got[:-1]).all()
+                assert torch.equal(got[n:], mine)
+                if n < score.numel():  # a 32-bit sum of rows*256 products: near ties may go either way
+                    cut = score.sort(descending=True).values[n - 1]
+                    off = 2.0 ** -20 * (rows.abs().sum(0) * meta.double().abs().amax()).sum()
+                    chosen = torch.zeros_like(score, dtype=torch.bool)
+                    chosen[got[:n]] = True
+                    assert chosen[score > cut + off].all() and not chosen[score < cut - off].any()
+    out, lse = ops.prompt_attn(q, k, v, qo, *tab, max_pages=most, block_pages=pages, block_npages=count,
+                               query_block=block, lse=True, status=status)
+    assert int(status) == 0
+    k, v = torch.nan_to_num(k, 0, 0, 0), torch.nan_to_num(v, 0, 0, 0)
+    check_prompt(q, k, v, qo, tab, lens, out, lse, True,
+                 lambda b, j, h: pages[slot(b, j), h, : int(count[slot(b, j), h])], block)
+
+
+def test_lists_of_a_caller_empty_rows_and_bad_pages():
+    new, old = [70, 40], [100, 10]
+    q, k, v, qo, tab, lens = make_prompt(new, old, 4, 2, torch.bfloat16, seed=3)
+    block, slots = 32, sum(new) // 32 + 2
+    pages = torch.full((slots, 2, 5), -7, **I32)
+    count = torch.zeros(slots, 2, **I32)
+    # block 0 of sequence 0: page 1 only; block 1: nothing; block 2: only a page behind all its queries but the last ones
+    pages[0, :, 0], count[0] = 1, 1
+    pages[2, :, 0], count[2] = 10, 1
+    first = 110 // 32 * 0 + int(qo[1]) // block + 1
+    pages[first, :, :2], count[first] = torch.tensor([0, 2], **I32), 2
+    pages[first + 1, :, :1], count[first + 1] = torch.tensor([3], **I32), 1
+    status = torch.zeros(1, **I32)
+    out, lse = ops.prompt_attn(q, k, v, qo, *tab, max_pages=11, block_pages=pages, block_npages=count,
+                               query_block=block, lse=True, status=status)
+    assert int(status) == 0
+    base = [0, first]
+    check_prompt(q, k, v, qo, tab, lens, out, lse, True, lambda b, j, h: pages[base[b] + j, h, : int(count[base[b] + j, h])],
+                 block)
+    assert not out[32:64].any() and (lse[32:64] == -math.inf).all()
+    # a page that is not there is skipped and flagged
+    pages[0, :, 1], count[0] = 500, 2
+    got = ops.prompt_attn(q, k, v, qo, *tab, max_pages=11, block_pages=pages, block_npages=count, query_block=block,
+                          status=status)
+    assert int(status) == ops.FLAG_BAD_INDEX and torch.equal(got, out)
+    status.zero_()
+    idx = tab[1].clone()
+    idx[1] = -1
+    ops.prompt_attn(q, k, v, qo, tab[0], idx, tab[2], max_pages=11, status=status)
+    assert int(status) == ops.FLAG_BAD_INDEX
+
+
+def test_rows_behind_the_last_sequence_are_left_and_extreme_logits():
+    q, k, v, qo, tab, lens = make_prompt([20, 30], [0, 200], 4, 2, torch.bfloat16, seed=5)
+    out = torch.full_like(q, 7.0)
+    short = qo.clone()
+    short[2] = 41
+    # the second sequence then has 21 new tokens, its last ones
+    ops.prompt_attn(q, k, v, short, *tab, max_pages=15, out=out)
+    assert (out[41:] == 7.0).all() and not (out[:41] == 7.0).all(-1).any()
+    # logits of +-1000: the softmax is one key's, or an even split between equal ones
+    q2 = torch.zeros_like(q)
+    q2[:, :, 0] = 100.0
+    k2 = torch.zeros_like(k)
+    k2[..., 0] = -100.0
+    page = int(tab[1][0])
+    k2[page, :, 3, 0] = 100.0
+    got = ops.prompt_attn(q2, k2, v, qo, *tab, max_pages=15)
+    want = v[page, :, 3].repeat_interleave(2, 0)
+    assert torch.equal(got[5:20], want.expand(15, 4, D))
+    assert torch.isfinite(got.float()).all()
+
+
+PREFIXES = [
+    # group sizes, prefix lengths, own lengths (cycled), hq, hkv, dtype
+    ([1], [0], [0], 4, 1, torch.bfloat16),
+    ([2, 1], [40, 0], [0, 17, 0], 8, 2, torch.float16),
+    ([3, 5], [1, 300], [0, 1, 16, 33], 8, 8, torch.bfloat16),
+    ([40], [1000], [5, 0, 130], 8, 2, torch.bfloat16),
+    ([7, 33, 1], [129, 2047, 16], [700, 3], 7, 1, torch.float16),
+    ([150], [777], [1], 16, 2, torch.bfloat16),
+    ([20, 0, 13], [100, 50, 4100], [64, 65, 0], 40, 8, torch.bfloat16),
+    ([70], [5000], [20], 32, 1, torch.float16),
+    ([300], [513], [0, 40], 4, 4, torch.float16),
+]
+
+
+@pytest.mark.parametrize("case", PREFIXES, ids=[str(i) for i in range(len(PREFIXES))])
+def test_shared_prefix_attention(case):
+    sizes, prefix, own, hq, hkv, dtype = case
+    n = sum(sizes)
+    own = [own[i % len(own)] for i in range(n)]
+    pages = sum((x + 15) // 16 for x in prefix + own)
+    total = max(pages, 1)
+    ptr, idx, last = table(own, 4, 0, total)
+    pptr, pidx, plast = table(prefix, 4, idx.numel(), total)
+    k, v, lean, g = pool(total, hkv, dtype, 9)
+    q = (torch.randn(n, hkv, hq // hkv, D, generator=g, device=DEV) + 0.3 * lean).reshape(n, hq, D).to(dtype)
+    poison_tails(k, v, ptr, idx, own)
+    poison_tails(k, v, pptr, pidx, prefix)
+    group = torch.tensor([0] + torch.tensor(sizes).cumsum(0).tolist(), **I32)
+    status = torch.zeros(1, **I32)
+    args = (q, k, v, group, pptr, pidx, plast, ptr, idx, last)
+    out, lse = ops.shared_prefix_attn(*args, lse=True, status=status)
+    assert int(status) == 0
+    most = max(1, max((x + 15) // 16 for x in prefix + own))
+    again = ops.shared_prefix_attn(*args[:1], *args[1:], max_pages=most)
+    assert torch.equal(again, out)                              # the same with the exact bound, and twice
+    k, v = torch.nan_to_num(k, 0, 0, 0), torch.nan_to_num(v, 0, 0, 0)
+    gq = hq // hkv
+    for i in range(len(sizes)):
+        for b in range(int(group[i]), int(group[i + 1])):
+            for h in range(hkv):
+                kk = torch.cat([dense(k, pptr, pidx, i, prefix[i], h), dense(k, ptr, idx, b, own[b], h)])
+                vv = torch.cat([dense(v, pptr, pidx, i, prefix[i], h), dense(v, ptr, idx, b, own[b], h)])
+                keep = torch.ones(gq, kk.shape[0], dtype=torch.bool, device=DEV)
+                ref, ref_lse, p = attend64(q[b, h * gq: (h + 1) * gq].double(), kk, vv, keep)
+                got = out[b, h * gq: (h + 1) * gq].double()
+                assert ((got - ref).abs() <= tol_of(dtype, p, vv, ref)).all(), (i, b, h, float((got - ref).abs().max()))
+                got_lse = lse[b, h * gq: (h + 1) * gq].double()
+                if kk.shape[0] == 0:
+                    assert (got_lse == -math.inf).all() and not got.any()
+                else:
+                    assert ((got_lse - ref_lse).abs() <= 2.0 ** -18 + 2.0 ** -22 * ref_lse.abs()).all()
+
+
+def test_a_sequence_in_no_group_has_no_prefix():
+    own = [20, 30, 5]
+    ptr, idx, last = table(own + [64], 2)
+    k, v, lean, g = pool(idx.numel(), 2, torch.bfloat16, 1)
+    q = torch.randn(3, 4, D, generator=g, device=DEV).to(torch.bfloat16)
+    pptr, pidx, plast = torch.tensor([0, 4], **I32), idx[-4:].contiguous(), torch.tensor([16], **I32)
+    args = (ptr[:4].contiguous(), idx, last[:3].contiguous())
+    got = ops.shared_prefix_attn(q, k, v, torch.tensor([1, 2], **I32), pptr, pidx, plast, *args)
+    alone = ops.prompt_attn(q, k, v, torch.arange(4, **I32), *args, max_pages=2)
+    all_in = ops.shared_prefix_attn(q, k, v, torch.tensor([0, 3], **I32), pptr, pidx, plast, *args)
+    for b, want in ((0, alone), (1, all_in), (2, alone)):
+        assert (got[b].float() - want[b].float()).abs().max() <= 2.0 ** -7 * want[b].float().abs().max()
+
+
+def test_graph_side_stream_and_a_workspace_of_the_callers():
+    q, k, v, qo, tab, lens = make_prompt([300, 40], [500, 0], 8, 2, torch.bfloat16, seed=2)
+    want = ops.prompt_attn(q, k, v, qo, *tab, max_pages=50)
+    ws = torch.full((ops.prompt_attn_workspace_bytes(340, 2, 8, 2, 50),), 255, dtype=torch.uint8, device=DEV)
+    out = torch.empty_like(want)
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=s):
+        ops.prompt_attn(q, k, v, qo, *tab, max_pages=50, out=out, workspace=ws)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_a_prompts_whole_way_through_the_operators():
+    """Append with rotation, select, attend in two chunks; then a decode step over the prompt as a shared prefix.  The
+    same prompt in one chunk gives the same, within what rounding twice allows."""
+    hq, hkv, dtype, n = 8, 2, torch.bfloat16, 700
+    g = torch.Generator(device=DEV).manual_seed(11)
+    proj = torch.randn(n, hq + 2 * hkv, D, generator=g, device=DEV).to(dtype)
+    parts = proj[:, :hq], proj[:, hq: hq + hkv], proj[:, hq + hkv:]
+    freqs, scale = ops.rope_frequencies(D, 500000.0, device=DEV)
+    ptr, idx, last = table([n], 5)
+    results = []
+    for cuts in ([0, n], [0, 400, n]):
+        k, v = (torch.zeros(idx.numel(), hkv, PAGE, D, dtype=dtype, device=DEV) for _ in range(2))
+        k4 = torch.zeros(idx.numel(), hkv, 1280, dtype=torch.uint8, device=DEV)
+        meta = torch.zeros(idx.numel(), hkv, 2, D, dtype=dtype, device=DEV)
+        outs = []
+        for a, e in zip(cuts, cuts[1:]):
+            p1, i1, l1 = PagedKVCache.page_table([e], DEV)[:3]
+            tab = (p1, idx[: p1[-1]].contiguous(), l1)
+            qo = torch.tensor([0, e - a], **I32)
+            q = ops.rope_append_kv(*(x[a:e] for x in parts), freqs, k, v, k4, meta, qo, *tab, attention_scale=scale)
+            sel = ops.quest_select_blocks(q, meta, qo, *tab, 1024, max_pages=44, query_block=16)
+            outs.append(ops.prompt_attn(q, k, v, qo, *tab, max_pages=44, block_pages=sel[0], block_npages=sel[1],
+                                        query_block=16))
+        results.append((torch.cat(outs), k, v, k4, meta))
+    for a, b in zip(results[0][1:], results[1][1:]):
+        assert torch.equal(a, b)
+    x, y = results[0][0].float(), results[1][0].float()
+    assert ((x - y).abs() <= 2.0 ** -7 * y.abs() + 2.0 ** -7 * v.float().abs().max()).all()
+    k, v = results[0][1:3]
+    qd = torch.randn(3, hq, D, generator=g, device=DEV).to(dtype)
+    none = torch.zeros(4, **I32), torch.zeros(0, **I32), torch.zeros(3, **I32)
+    got = ops.shared_prefix_attn(qd, k, v, torch.tensor([0, 3], **I32), ptr, idx, last, *none)
+    kk, vv = (dense(x, ptr, idx, 0, n, 0) for x in (k, v))
+    ref, _, p = attend64(qd[1, :4].double(), kk, vv, torch.ones(4, n, dtype=torch.bool, device=DEV))
+    assert ((got[1, :4].double() - ref).abs() <= tol_of(dtype, p, vv, ref)).all()

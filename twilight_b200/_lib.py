@@ -54,6 +54,14 @@ SIGNATURES = {
                                      i32, i32, f32, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, i32, i32, i32, i32, i32,
                                      ptr, ptr]),
     "twl_dequantize_k_pages": (C.c_int, [ptr, ptr, i64, ptr, C.c_int, i32, i32, ptr, ptr]),
+    "twl_prompt_attn_workspace_bytes": (sz, [i32] * 6),
+    "twl_prompt_attn": (C.c_int, [ptr, C.c_int, i64, ptr, ptr, ptr, ptr, ptr, ptr, i32, i32, i32, i32, i32, i32, i32,
+                                  ptr, ptr, i32, i32, f32, ptr, ptr, ptr, sz, ptr, ptr]),
+    "twl_quest_select_blocks": (C.c_int, [ptr, C.c_int, i64, ptr, ptr, ptr, ptr, ptr, i32, i32, i32, i32, i32, i32,
+                                          i32, i32, ptr, ptr, ptr, ptr, i32, ptr, ptr]),
+    "twl_shared_prefix_workspace_bytes": (sz, [i32] * 5),
+    "twl_shared_prefix_attn": (C.c_int, [ptr, C.c_int, i64, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, i32, i32, i32,
+                                         i32, i32, i32, f32, ptr, ptr, ptr, sz, ptr, ptr]),
     "twl_round_scores": (C.c_int, [ptr, i64, C.c_int, f32, ptr]),
 }
 

@@ -652,6 +652,193 @@ static int launch_scores_g(const ScoreParams& p, cudaStream_t st) {
   }
 }
 
+// ---- pages of query blocks (prompts) -------------------------------------------------------------
+// A block of query tokens (all their G heads of a KV head: rows r) picks its pages by the sum of Quest's bounds over
+// its rows, which is linear in the metadata,
+//   sum_r sum_d max(q_rd kmax_d, q_rd kmin_d) = sum_d (sum_r min(q_rd, 0)) kmin_d + (sum_r max(q_rd, 0)) kmax_d,
+// so a block is pooled once into 256 numbers and a page costs it 256 multiply-adds whatever its rows.  All of it
+// in 32 bits.  Three launches: pool, scores, selection.
+// Slots: query block j of sequence b is slot qo_indptr[b]/query_block + b + j.
+struct BlockSelParams {
+  const void *q, *kmeta;
+  int64_t q_ts;
+  const int32_t *qo_indptr, *indptr, *indices, *last_len;
+  float *pooled, *scores;  // [slots][Hkv][256], [slots][Hkv][max_pages]
+  int32_t *block_pages, *block_npages, *status;
+  int32_t batch, Hq, Hkv, num_tokens, num_pages_total, query_block, max_pages, max_k, budget_k, slots;
+};
+struct QueryBlock {
+  int b, row0, rows, first, last, pages;  // sequence, first query row, tokens, positions of the first and last, its pages
+};
+
+// The query block of a slot, found by the warp; rows = 0 where there is none.
+__device__ __forceinline__ QueryBlock query_block_of(const BlockSelParams& p, int slot) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = p.batch;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) >> 5, c = lo + lane * step;
+    const int n = __popc(__ballot_sync(0xffffffffu, c < hi && p.qo_indptr[c] / p.query_block + c <= slot));
+    lo += (n > 0 ? n - 1 : 0) * step;
+    hi = min(hi, lo + step);
+  }
+  QueryBlock r;
+  r.b = lo;
+  const int t0 = p.qo_indptr[lo], n_new = p.qo_indptr[lo + 1] - t0;
+  const int at = (slot - (t0 / p.query_block + lo)) * p.query_block;
+  const int n_pages = p.indptr[lo + 1] - p.indptr[lo], ll = p.last_len[lo];
+  const bool bad = t0 < 0 || t0 + n_new > p.num_tokens || (n_pages > 0 && (ll < 1 || ll > kPage));
+  const int len = n_pages > 0 && !bad ? (n_pages - 1) * kPage + ll : 0;
+  r.row0 = t0 + at;
+  r.rows = bad || at >= n_new ? 0 : min(p.query_block, n_new - at);
+  r.first = len - n_new + at;
+  r.last = r.first + r.rows - 1;
+  r.pages = min(max(n_pages, 0), p.max_pages);
+  return r;
+}
+// pages wholly before the block's first position: the ones it chooses from
+__device__ __forceinline__ int history_pages(const QueryBlock& r) {
+  return r.rows > 0 && r.first > 0 ? min(r.first / kPage, r.pages) : 0;
+}
+
+// block = (slot, KV head): 16 lanes of 8 channels x 16 rows at a time
+template <typename T>
+__global__ void __launch_bounds__(256) pool_query_blocks_kernel(const BlockSelParams p) {
+  __shared__ float part[16][2][kD];
+  pdl_wait();
+  const int slot = blockIdx.x, kvh = blockIdx.y, G = p.Hq / p.Hkv;
+  const QueryBlock qb = query_block_of(p, slot);
+  if (history_pages(qb) == 0) return;
+  const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  float lo[8] = {}, hi[8] = {};
+  for (int r = r0; r < qb.rows * G; r += 16) {
+    const int tok = r / G;
+    const T* src = static_cast<const T*>(p.q) + (int64_t)(qb.row0 + tok) * p.q_ts + (kvh * G + r - tok * G) * kD;
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + c);
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = Elem<T>::to_f2(u[k]);
+      lo[2 * k] += fminf(f.x, 0.f);
+      hi[2 * k] += fmaxf(f.x, 0.f);
+      lo[2 * k + 1] += fminf(f.y, 0.f);
+      hi[2 * k + 1] += fmaxf(f.y, 0.f);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    part[r0][0][8 * c + k] = lo[k];
+    part[r0][1][8 * c + k] = hi[k];
+  }
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s += (&part[r][0][0])[threadIdx.x];
+  p.pooled[((size_t)slot * p.Hkv + kvh) * 256 + threadIdx.x] = s;
+}
+
+// block = 64 pages x 16 slots of one KV head; a thread owns one page and four slots.  Both operands are staged in
+// shared memory (metadata as it lies in HBM, rows padded by 8 bytes: conflict-free 8-byte reads).
+constexpr int kBlkPages = 64, kBlkSlots = 16, kBlkMetaPitch = 260;
+constexpr int kBlkSmem = kBlkSlots * 256 * 4 + kBlkPages * kBlkMetaPitch * 2;
+template <typename T>
+__global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelParams p) {
+  extern __shared__ __align__(16) uint8_t blk_smem[];
+  float (*pooled)[256] = reinterpret_cast<float (*)[256]>(blk_smem);
+  T* meta = reinterpret_cast<T*>(blk_smem + kBlkSlots * 256 * sizeof(float));
+  __shared__ int hist_s[kBlkSlots], seq_s[kBlkSlots];
+  pdl_wait();
+  const int slot0 = blockIdx.z * kBlkSlots, kvh = blockIdx.y, page0 = blockIdx.x * kBlkPages;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int i = warp; i < kBlkSlots; i += 8) {
+    QueryBlock qb;
+    qb.rows = 0;
+    qb.b = -1;
+    if (slot0 + i < p.slots) qb = query_block_of(p, slot0 + i);
+    if (lane == 0) {
+      hist_s[i] = history_pages(qb);
+      seq_s[i] = qb.b;
+    }
+  }
+  __syncthreads();
+  bool any = false;
+  for (int i = 0; i < kBlkSlots; ++i) any |= hist_s[i] > page0;
+  if (!any) return;
+  for (int i = threadIdx.x; i < kBlkSlots * 64; i += 256) {
+    const int s = i >> 6;
+    if (hist_s[s] > page0)
+      reinterpret_cast<float4*>(pooled[s])[i & 63] =
+          reinterpret_cast<const float4*>(p.pooled + ((size_t)(slot0 + s) * p.Hkv + kvh) * 256)[i & 63];
+  }
+  const int page = threadIdx.x & 63, sg = threadIdx.x >> 6;
+  for (int i0 = 0; i0 < kBlkSlots;) {  // the slots of one sequence at a time
+    const int b = seq_s[i0];
+    int i1 = i0 + 1, n = hist_s[i0];
+    while (i1 < kBlkSlots && seq_s[i1] == b) n = max(n, hist_s[i1++]);
+    n = min(n - page0, kBlkPages);
+    if (n > 0) {
+      __syncthreads();  // the metadata of the sequence before has been used
+      const int32_t* idx = p.indices + p.indptr[b] + page0;
+      for (int i = threadIdx.x; i < n * 32; i += 256) {
+        const int pg = i >> 5;
+        const int phys = idx[pg];
+        const bool ok = phys >= 0 && phys < p.num_pages_total;
+        if (!ok && (i & 31) == 0) raise_flag(p.status, TWL_FLAG_BAD_INDEX);
+        const uint4 v = ldg_stream_u4(static_cast<const T*>(p.kmeta) + ((size_t)(ok ? phys : 0) * p.Hkv + kvh) * 2 * kD +
+                                      8 * (i & 31));
+        uint2* to = reinterpret_cast<uint2*>(meta + pg * kBlkMetaPitch + 8 * (i & 31));
+        to[0] = make_uint2(v.x, v.y);
+        to[1] = make_uint2(v.z, v.w);
+      }
+      __syncthreads();
+      float acc[4] = {};
+      if (page < n) {
+        const uint2* m = reinterpret_cast<const uint2*>(meta + page * kBlkMetaPitch);
+#pragma unroll 4
+        for (int d = 0; d < 64; ++d) {
+          const uint2 u = m[d];
+          const float2 x = Elem<T>::to_f2(u.x), y = Elem<T>::to_f2(u.y);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 w = reinterpret_cast<const float4*>(pooled[4 * sg + j])[d];
+            acc[j] += (x.x * w.x + x.y * w.y) + (y.x * w.z + y.y * w.w);
+          }
+        }
+        const int phys = idx[page];
+        const bool ok = phys >= 0 && phys < p.num_pages_total;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int s = 4 * sg + j;
+          if (s >= i0 && s < i1 && page0 + page < hist_s[s])
+            p.scores[((size_t)(slot0 + s) * p.Hkv + kvh) * p.max_pages + page0 + page] = ok ? acc[j] : -INFINITY;
+        }
+      }
+    }
+    i0 = i1;
+  }
+}
+
+// block = (slot, KV head): the budget's best of the pages before the block, then the pages it lies in
+__global__ void __launch_bounds__(kTopkThreads) select_query_blocks_kernel(const BlockSelParams p) {
+  extern __shared__ __align__(16) uint32_t keys[];
+  __shared__ TopkScratch sc;
+  pdl_wait();
+  const int slot = blockIdx.x, kvh = blockIdx.y;
+  const QueryBlock qb = query_block_of(p, slot);
+  if (qb.rows == 0) return;
+  const size_t row = (size_t)slot * p.Hkv + kvh;
+  int32_t* out = p.block_pages + row * p.max_k;
+  const int n = history_pages(qb), k = min(min(n, p.budget_k), p.max_k);
+  if (k == n) {
+    for (int i = threadIdx.x; i < n; i += kTopkThreads) out[i] = i;
+  } else if (k > 0) {
+    topk_row(p.scores + row * p.max_pages, n, k, out, keys, sc);
+  }
+  // its own pages, up to the one of its last position
+  const int own = qb.last < 0 ? 0 : max(0, min(min(qb.last / kPage + 1, qb.pages) - n, p.max_k - k));
+  for (int i = threadIdx.x; i < own; i += kTopkThreads) out[k + i] = n + i;
+  if (threadIdx.x == 0) p.block_npages[row] = k + own;
+}
+
 }  // namespace twl
 
 extern "C" int twl_quest_page_scores(const void* q, int dtype, const void* kmeta,
@@ -722,5 +909,54 @@ extern "C" int twl_quest_topk_pages(const float* page_scores, int32_t max_pages,
   TWL_CUDA_TRY(launch_chain(quest_topk_pages_kernel, dim3(batch * num_q_heads), dim3(kTopkThreads), smem,
                             reinterpret_cast<cudaStream_t>(stream), tp));
   TWL_CHECK_LAUNCH();
+  return TWL_OK;
+}
+
+extern "C" int twl_quest_select_blocks(const void* q, int dtype, int64_t q_token_stride, const void* kmeta,
+                                       const int32_t* qo_indptr, const int32_t* kv_indptr, const int32_t* kv_indices,
+                                       const int32_t* kv_last_page_len, int32_t num_tokens, int32_t batch,
+                                       int32_t num_q_heads, int32_t num_kv_heads, int32_t num_pages_total,
+                                       int32_t token_budget, int32_t query_block, int32_t max_pages, float* pooled,
+                                       float* page_scores, int32_t* block_pages, int32_t* block_npages, int32_t max_k,
+                                       int32_t* status, void* stream) {
+  using namespace twl;
+  if (!q || !kmeta || !qo_indptr || !kv_indptr || !kv_indices || !kv_last_page_len || !pooled || !page_scores ||
+      !block_pages || !block_npages)
+    return TWL_ERR_BAD_ARG;
+  if (num_tokens <= 0 || batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_pages_total <= 0 ||
+      token_budget <= 0 || max_pages <= 0 || max_k <= 0 || num_q_heads % num_kv_heads != 0)
+    return TWL_ERR_BAD_ARG;
+  if (query_block < kPage || query_block % kPage != 0) return TWL_ERR_UNSUPPORTED;
+  if (dtype != TWL_F16 && dtype != TWL_BF16) return TWL_ERR_UNSUPPORTED;
+  if (!aligned(q, 16) || q_token_stride % 8 != 0 || !aligned(kmeta, 16) || !aligned(pooled, 16))
+    return TWL_ERR_MISALIGNED;
+  const int64_t slots = (int64_t)num_tokens / query_block + batch;
+  const size_t smem = (size_t)max_pages * 4;
+  const int64_t slot_tiles = (slots + kBlkSlots - 1) / kBlkSlots;
+  if (smem > 200 * 1024 || slots > 0x7fffffffLL || slot_tiles > 65535 || num_kv_heads > 65535) return TWL_ERR_TOO_LARGE;
+  BlockSelParams p;
+  p.q = q; p.kmeta = kmeta; p.q_ts = q_token_stride;
+  p.qo_indptr = qo_indptr; p.indptr = kv_indptr; p.indices = kv_indices; p.last_len = kv_last_page_len;
+  p.pooled = pooled; p.scores = page_scores; p.block_pages = block_pages; p.block_npages = block_npages;
+  p.status = status; p.batch = batch; p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.num_tokens = num_tokens;
+  p.num_pages_total = num_pages_total; p.query_block = query_block; p.max_pages = max_pages; p.max_k = max_k;
+  p.budget_k = (token_budget / kPage > 1 ? token_budget / kPage : 1) + (token_budget % kPage ? 1 : 0);
+  p.slots = (int32_t)slots;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const dim3 per_slot((unsigned)slots, (unsigned)num_kv_heads);
+  const dim3 tiles((unsigned)((max_pages + kBlkPages - 1) / kBlkPages), (unsigned)num_kv_heads, (unsigned)slot_tiles);
+  if (dtype == TWL_F16) {
+    TWL_CUDA_TRY(launch_chain(pool_query_blocks_kernel<__half>, per_slot, dim3(256), 0, st, p));
+    TWL_CUDA_TRY(cudaFuncSetAttribute(score_query_blocks_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      kBlkSmem));
+    TWL_CUDA_TRY(launch_chain(score_query_blocks_kernel<__half>, tiles, dim3(256), kBlkSmem, st, p));
+  } else {
+    TWL_CUDA_TRY(launch_chain(pool_query_blocks_kernel<__nv_bfloat16>, per_slot, dim3(256), 0, st, p));
+    TWL_CUDA_TRY(cudaFuncSetAttribute(score_query_blocks_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      kBlkSmem));
+    TWL_CUDA_TRY(launch_chain(score_query_blocks_kernel<__nv_bfloat16>, tiles, dim3(256), kBlkSmem, st, p));
+  }
+  TWL_CUDA_TRY(cudaFuncSetAttribute(select_query_blocks_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  TWL_CUDA_TRY(launch_chain(select_query_blocks_kernel, per_slot, dim3(kTopkThreads), smem, st, p));
   return TWL_OK;
 }

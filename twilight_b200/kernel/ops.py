@@ -641,6 +641,190 @@ def dequantize_k_pages(k4_pages, page_ids=None, *, dtype: torch.dtype, out=None,
     return out
 
 
+# ---------------------------------------------------------------------------------------------
+# attention of more than one token at a time
+# ---------------------------------------------------------------------------------------------
+def _queries(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor) -> torch.Tensor:
+    _rows(q, "q")
+    if q.shape[1] > 1 and q.stride(1) != HEAD_DIM:
+        raise _lib.TwilightError("the heads of a token of q must be contiguous")
+    _pages(q.dtype, k_pages=k_pages, v_pages=v_pages)
+    if k_pages.shape != v_pages.shape:
+        raise _lib.TwilightError("k_pages and v_pages must have the same shape")
+    if q.shape[1] % k_pages.shape[1]:
+        raise _lib.TwilightError("query heads must be a multiple of KV heads")
+    return q
+
+
+def _result(q: torch.Tensor, out, lse) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Checked or fresh output, and the log-sum-exp buffer where one is wanted (``lse``: True or a tensor)."""
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise _lib.TwilightError("out must be contiguous, of q's shape and type")
+    if lse is None or lse is False:
+        return out, None
+    if lse is True:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+    elif lse.shape != q.shape[:2] or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise _lib.TwilightError("lse must be contiguous float32 [tokens, query heads]")
+    return out, lse
+
+
+def _workspace(t: Optional[torch.Tensor], nbytes: int, device) -> torch.Tensor:
+    if t is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if t.dtype != torch.uint8 or not t.is_contiguous():
+        raise _lib.TwilightError("workspace must be contiguous uint8")
+    return t
+
+
+def prompt_attn_workspace_bytes(num_tokens: int, batch: int, num_q_heads: int, num_kv_heads: int, max_pages: int,
+                                query_block: int = 0) -> int:
+    """Bytes of :func:`prompt_attn`'s workspace; ``query_block`` is 0 without block lists."""
+    return int(_lib.load().twl_prompt_attn_workspace_bytes(num_tokens, batch, num_q_heads, num_kv_heads, max_pages,
+                                                           query_block))
+
+
+def prompt_attn(q, k_pages, v_pages, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, *, max_pages: int,
+                causal: bool = True, block_pages=None, block_npages=None, query_block: int = 64,
+                sm_scale: Optional[float] = None, out=None, lse=None, workspace=None, status=None):
+    """Attention of a ragged batch's new tokens over the paged cache: whole prompts, chunks of them, or a few tokens
+    to verify (the dense prefill of twilight/pyimpl/attention.py:157-182, on pages).
+
+    ``q [T,Hq,128]``: sequence b's queries are rows ``qo_indptr[b]:qo_indptr[b+1]`` and the last tokens that its page
+    table describes (append them first, :func:`rope_append_kv`).  ``block_pages``/``block_npages`` from
+    :func:`quest_select_blocks` restrict every block of ``query_block`` queries to its pages.  ``max_pages``: the
+    largest page count of a sequence.  Returns ``out [T,Hq,128]``, and with ``lse`` (True or a tensor) also the fp32
+    ``[T,Hq]`` logarithms of the sums of exponentials.  ``workspace``: ``prompt_attn_workspace_bytes`` bytes, one for
+    each call that may overlap with another."""
+    _queries(q, k_pages, v_pages)
+    t, hq, _ = q.shape
+    batch, hkv = qo_indptr.numel() - 1, k_pages.shape[1]
+    _table(batch, qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices, kv_last_page_len=kv_last_page_len)
+    out, lse = _result(q, out, lse)
+    if (block_pages is None) != (block_npages is None):
+        raise _lib.TwilightError("block_pages and block_npages go together")
+    max_k = 0
+    if block_pages is not None:
+        _table(batch, block_pages=block_pages, block_npages=block_npages)
+        slots, max_k = t // query_block + batch, block_pages.shape[-1]
+        if block_pages.shape != (slots, hkv, max_k) or block_npages.shape != (slots, hkv):
+            raise _lib.TwilightError(f"block_pages must be [{slots}, {hkv}, max_k], block_npages [{slots}, {hkv}]")
+    else:
+        query_block = 0
+    _cuda(q)
+    if t > 0:
+        workspace = _workspace(workspace, prompt_attn_workspace_bytes(t, batch, hq, hkv, max_pages, query_block), q.device)
+        _launch("prompt_attn", q, q.data_ptr(), _dtype_code(q), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
+                qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), t, batch,
+                hq, hkv, k_pages.shape[0], max_pages, int(causal), _p(block_pages), _p(block_npages), max_k, query_block,
+                1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, out.data_ptr(), _p(lse),
+                workspace.data_ptr(), workspace.numel(), _p(status), _stream(q.device), k_pages=k_pages, v_pages=v_pages,
+                qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices, kv_last_page_len=kv_last_page_len,
+                block_pages=block_pages, block_npages=block_npages, out=out, lse=lse, workspace=workspace, status=status)
+    return out if lse is None else (out, lse)
+
+
+def quest_select_blocks(q, kmeta, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, token_budget: int, *,
+                        max_pages: int, query_block: int = 64, block_pages=None, block_npages=None, pooled=None,
+                        page_scores=None, status=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Pages that every block of ``query_block`` queries (a multiple of 16) of a prompt attends to, for
+    :func:`prompt_attn`: all from the page of its first position on, and of those before it the token budget's best
+    by the sum of Quest's bounds over the block's rows (twilight/pyimpl/quest.py:37-99 applied to a block).
+
+    Returns ``(block_pages [slots,Hkv,max_k] int32 ascending, block_npages [slots,Hkv] int32)`` with
+    ``slots = T//query_block + batch``; block j of sequence b is row ``qo_indptr[b]//query_block + b + j``."""
+    _rows(q, "q")
+    t, hq, _ = q.shape
+    if hq > 1 and q.stride(1) != HEAD_DIM:
+        raise _lib.TwilightError("the heads of a token of q must be contiguous")
+    batch = qo_indptr.numel() - 1
+    _pages(q.dtype, kmeta=kmeta)
+    hkv = kmeta.shape[1]
+    if hq % hkv:
+        raise _lib.TwilightError("query heads must be a multiple of KV heads")
+    _table(batch, qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices, kv_last_page_len=kv_last_page_len)
+    if token_budget <= 0 or max_pages <= 0:
+        raise _lib.TwilightError("token_budget and max_pages must be positive")
+    if query_block < PAGE or query_block % PAGE:
+        raise _lib.TwilightError(f"query_block must be a multiple of {PAGE}")
+    _cuda(q)
+    slots = t // query_block + batch
+    # a block that starts inside a page lies in one page more than its tokens fill
+    max_k = min(max(1, token_budget // PAGE) + (1 if token_budget % PAGE else 0) + query_block // PAGE + 1, max_pages)
+    dev = q.device
+    if block_pages is None:
+        block_pages = torch.empty(slots, hkv, max_k, dtype=torch.int32, device=dev)
+    if block_npages is None:
+        block_npages = torch.empty(slots, hkv, dtype=torch.int32, device=dev)
+    if pooled is None:
+        pooled = torch.empty(slots, hkv, 2 * HEAD_DIM, dtype=torch.float32, device=dev)
+    if page_scores is None:
+        page_scores = torch.empty(slots, hkv, max_pages, dtype=torch.float32, device=dev)
+    _table(batch, block_pages=block_pages, block_npages=block_npages)
+    if block_pages.dim() != 3 or block_pages.shape[:2] != (slots, hkv) or block_pages.shape[2] < max_k \
+            or block_npages.shape != (slots, hkv):
+        raise _lib.TwilightError(f"block_pages must be [{slots}, {hkv}, at least {max_k}], block_npages [{slots}, {hkv}]")
+    for name, x, width in (("pooled", pooled, 2 * HEAD_DIM), ("page_scores", page_scores, max_pages)):
+        if x.shape != (slots, hkv, width) or x.dtype != torch.float32 or not x.is_contiguous():
+            raise _lib.TwilightError(f"{name} must be contiguous float32 [{slots}, {hkv}, {width}]")
+    if t > 0:
+        _launch("quest_select_blocks", q, q.data_ptr(), _dtype_code(q), q.stride(0), kmeta.data_ptr(),
+                qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), t, batch,
+                hq, hkv, kmeta.shape[0], token_budget, query_block, max_pages, pooled.data_ptr(), page_scores.data_ptr(),
+                block_pages.data_ptr(), block_npages.data_ptr(), block_pages.shape[2], _p(status), _stream(dev),
+                kmeta=kmeta, qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices,
+                kv_last_page_len=kv_last_page_len, pooled=pooled, page_scores=page_scores, block_pages=block_pages,
+                block_npages=block_npages, status=status)
+    return block_pages, block_npages
+
+
+def shared_prefix_workspace_bytes(batch: int, num_groups: int, num_q_heads: int, num_kv_heads: int, max_pages: int) -> int:
+    return int(_lib.load().twl_shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads, max_pages))
+
+
+def shared_prefix_attn(q, k_pages, v_pages, group_indptr, prefix_indptr, prefix_indices, prefix_last_page_len, kv_indptr,
+                       kv_indices, kv_last_page_len, *, max_pages: Optional[int] = None, sm_scale: Optional[float] = None,
+                       out=None, lse=None, workspace=None, status=None):
+    """Decode attention of groups of sequences over a prefix that a group shares (read once for the whole group) and
+    each sequence's own pages behind it.
+
+    ``q [B,Hq,128]`` (or ``[B,Hq,1,128]``), one token per sequence.  Group i is sequences
+    ``group_indptr[i]:group_indptr[i+1]``; the three ``prefix_*`` tensors are its page table, the three ``kv_*``
+    tensors that of the sequences' own parts (no pages: nothing of its own).  ``max_pages``: the largest page count of
+    any of them; None takes the lengths of the index lists, which is an upper bound.  Returns ``out [B,Hq,128]``, and
+    with ``lse`` also the fp32 ``[B,Hq]`` logarithms of the sums of exponentials."""
+    if q.dim() == 4:
+        if q.shape[2] != 1:
+            raise _lib.TwilightError("decode step only: q_len must be 1")
+        q = q[:, :, 0, :]
+    _queries(q, k_pages, v_pages)
+    b, hq, _ = q.shape
+    groups, hkv = group_indptr.numel() - 1, k_pages.shape[1]
+    _table(groups, group_indptr=group_indptr, prefix_indptr=prefix_indptr, prefix_indices=prefix_indices,
+           prefix_last_page_len=prefix_last_page_len)
+    _table(b, kv_indptr=kv_indptr, kv_indices=kv_indices, kv_last_page_len=kv_last_page_len)
+    if groups < 1:
+        raise _lib.TwilightError("group_indptr must have at least two entries")
+    out, lse = _result(q, out, lse)
+    _cuda(q)
+    if b > 0:
+        if max_pages is None:
+            max_pages = max(prefix_indices.numel(), kv_indices.numel(), 1)
+        workspace = _workspace(workspace, shared_prefix_workspace_bytes(b, groups, hq, hkv, max_pages), q.device)
+        _launch("shared_prefix_attn", q, q.data_ptr(), _dtype_code(q), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
+                group_indptr.data_ptr(), prefix_indptr.data_ptr(), prefix_indices.data_ptr(),
+                prefix_last_page_len.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(),
+                b, groups, hq, hkv, k_pages.shape[0], max_pages,
+                1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, out.data_ptr(), _p(lse),
+                workspace.data_ptr(), workspace.numel(), _p(status), _stream(q.device), k_pages=k_pages, v_pages=v_pages,
+                group_indptr=group_indptr, prefix_indptr=prefix_indptr, prefix_indices=prefix_indices,
+                prefix_last_page_len=prefix_last_page_len, kv_indptr=kv_indptr, kv_indices=kv_indices,
+                kv_last_page_len=kv_last_page_len, out=out, lse=lse, workspace=workspace, status=status)
+    return out if lse is None else (out, lse)
+
+
 def indices_to_mask(indices, budget, seq_len: int) -> torch.Tensor:
     """Index lists -> the reference's mask layout ``bool[B,H,1,L]`` (attention.py:199-281)."""
     b, hq, stride = indices.shape

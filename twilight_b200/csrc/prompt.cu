@@ -528,7 +528,7 @@ static WorkspaceLayout workspace_layout(int64_t tokens, int64_t n_seg, int64_t H
   const int64_t tt = kPage * 8 / G;  // tokens of a 128-row tile
   const int64_t blocks = query_block > 0 ? tokens / query_block + n_seg : n_seg;  // runs that are cut into tiles
   // items per KV head without key chunks, and at most two targets more where keys are split
-  const int64_t row_u = tokens * G / 8 + 2 * blocks + n_seg;
+  const int64_t row_u = n_seg * (kFewRows / 8);  // at most 16 rows a segment, in tiles of 8 or 16
   const int64_t tile_u = tokens / (2 * tt) + blocks;
   w.row_cap = (int32_t)(row_u + 2 * row_target + 1);
   w.tile_cap = (int32_t)(tile_u + 2 * tile_target + 1);
@@ -579,6 +579,10 @@ static int run_attention(const AttnParams& p, int dtype, bool need_merge, cudaSt
     TWL_CUDA_TRY(cudaFuncSetAttribute(prompt_rows_kernel<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem));
     TWL_CUDA_TRY(launch_chain(prompt_rows_kernel<T, 2>, rows_grid, dim3(kRowWarps * 32), kRowSmem, st, p));
   }
+  if ((int64_t)p.num_tokens * p.G > p.few_rows) {
+    const int bad = tile_attention_launch(p, dtype, st);
+    if (bad != TWL_OK) return bad;
+  }
   if (need_merge) {
     const int64_t blocks = ((int64_t)p.num_tokens * p.Hq + 7) / 8, most = (int64_t)num_sms() * 8;
     TWL_CUDA_TRY(launch_chain(prompt_merge_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, p));
@@ -595,6 +599,7 @@ static int check_attention(int dtype, int32_t num_tokens, int32_t batch, int32_t
     return TWL_ERR_BAD_ARG;
   if (dtype != TWL_F16 && dtype != TWL_BF16) return TWL_ERR_UNSUPPORTED;
   if (num_q_heads / num_kv_heads > 128) return TWL_ERR_UNSUPPORTED;
+  if ((int64_t)num_pages_total * num_kv_heads * TWL_PAGE_SIZE >= 0x7fffffffLL) return TWL_ERR_TOO_LARGE;
   return TWL_OK;
 }
 
@@ -620,6 +625,7 @@ extern "C" int twl_prompt_attn(const void* q, int dtype, int64_t q_token_stride,
   const int bad = check_attention(dtype, num_tokens, batch, num_q_heads, num_kv_heads, num_pages_total, max_pages);
   if (bad != TWL_OK) return bad;
   if (block_pages && query_block % kPage != 0) return TWL_ERR_UNSUPPORTED;
+  if (!(sm_scale > 0.f)) return TWL_ERR_BAD_ARG;  // the running maximum is that of the scaled products
   if (!aligned(q, 16) || q_token_stride % 8 != 0 || !aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(out, 16))
     return TWL_ERR_MISALIGNED;
   const WorkspaceLayout w = workspace_layout(num_tokens, batch, num_q_heads, num_kv_heads, max_pages,
@@ -633,7 +639,7 @@ extern "C" int twl_prompt_attn(const void* q, int dtype, int64_t q_token_stride,
   p.block_pages = block_pages; p.block_npages = block_npages; p.max_k = max_k;
   p.query_block = query_block > 0 ? query_block : 1;
   p.num_tokens = num_tokens; p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = num_q_heads / num_kv_heads;
-  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; p.row_tile = 16; p.few_rows = 0x7fffffff;
+  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; p.row_tile = 16; p.few_rows = kFewRows;
   p.scale_log2 = sm_scale * 1.44269504088896341f;
   p.status = status;
   place_workspace(p, w, workspace);
@@ -664,6 +670,7 @@ extern "C" int twl_shared_prefix_attn(const void* q, int dtype, int64_t q_token_
     return TWL_ERR_BAD_ARG;
   const int bad = check_attention(dtype, batch, batch, num_q_heads, num_kv_heads, num_pages_total, max_pages);
   if (bad != TWL_OK) return bad;
+  if (!(sm_scale > 0.f)) return TWL_ERR_BAD_ARG;
   if (!aligned(q, 16) || q_token_stride % 8 != 0 || !aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(out, 16))
     return TWL_ERR_MISALIGNED;
   const WorkspaceLayout w =
@@ -676,7 +683,7 @@ extern "C" int twl_shared_prefix_attn(const void* q, int dtype, int64_t q_token_
   p.qo2 = group_indptr; p.indptr2 = prefix_indptr; p.indices2 = prefix_indices; p.last2 = prefix_last_page_len;
   p.n_second = num_groups; p.always_partial = 1; p.query_block = 1;
   p.num_tokens = batch; p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = num_q_heads / num_kv_heads;
-  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; p.row_tile = p.G <= 8 ? 8 : 16; p.few_rows = 0x7fffffff;
+  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; p.row_tile = p.G <= 8 ? 8 : 16; p.few_rows = kFewRows;
   p.scale_log2 = sm_scale * 1.44269504088896341f;
   p.status = status;
   place_workspace(p, w, workspace);

@@ -1,0 +1,618 @@
+// Attention tiles of up to 256 query rows on the fifth-generation tensor cores: the part of prompt_attn and
+// shared_prefix_attn whose segments have more than a few rows.
+//
+// A block (one per SM, persistent) works on one item at a time: two subtiles of 128 packed rows (tokens x query heads
+// of one KV head) over one run of its pages, 128 keys (eight pages) a step.  Per subtile and step
+//   S = Q K^T          tcgen05.mma, both operands in shared memory (128-byte swizzle), S in TMEM, fp32
+//   P = 2^(S c - m)    one softmax thread per row: S from TMEM, running maximum and sum in registers, P back to TMEM
+//   O += P V           tcgen05.mma, P from TMEM, V in shared memory as it lies in the cache (keys x channels)
+// The two subtiles share K and V and alternate on the tensor cores: while one subtile's weights are computed, the
+// other's products run.  TMEM (512 columns): S of both subtiles (P takes the place of S once it is read), O of both.
+// The reference maximum m of a row is only moved when the true one has grown by more than 2^8, so O is rescaled a
+// few times per row; weights then stay below 2^8, which fp16 and the fp32 sums hold without loss.
+//
+// Warps: 0-3 and 4-7 softmax of subtile 0 and 1, 8 page loads (TMA: a page is two boxes of 16 rows x 128 bytes, issued by
+// sixteen lanes), 9 tensor-core issue (10 and 11 only complete the warpgroup).  K and V tiles share a ring of five 32 KiB stages.
+//
+// Bound: two products of 128 x 128 x 128 (512 clocks each at the tensor peak) and 128 x 128 exponentials per subtile and
+// step; with few rows per KV head, reading K and V.
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "prompt.cuh"
+
+namespace twl {
+
+constexpr int kTileThreads = 384;  // three warpgroups, the unit of the register split
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
+static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "registers of the launch: 168 a thread at 384 threads");
+constexpr int kStages = 5;
+constexpr int kStageBytes = 128 * kD * 2;      // 128 keys (or 128 query rows)
+constexpr int kHalfBytes = kStageBytes / 2;    // 64 channels of 128 rows
+constexpr int kInfoSlots = 8;                  // key tiles whose positions are kept
+constexpr uint32_t kWaitLimit = 1u << 31;      // clocks (about a second)
+
+struct alignas(64) TileParams {
+  CUtensorMap tq, tk, tv;
+  AttnParams a;
+};
+
+struct TileShared {
+  uint64_t q_full, q_free, kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], o_full[2], drain;
+  uint32_t tmem;
+  int32_t hi[kInfoSlots];      // largest position of the tile's keys, INT_MAX when a page is missing
+  int32_t tail[kInfoSlots];    // which of its pages the sequence ends in, -1 for none
+  int32_t pos[kInfoSlots][8];  // position of every page's first key
+};
+constexpr int kTileSmem = 2 * kStageBytes + kStages * kStageBytes + 1024 + (int)sizeof(TileShared);
+static_assert(kTileSmem <= 232448, "shared memory of a block");
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint64_t* b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+      : "=r"(ok) : "r"(smem_u32(b)), "r"(parity) : "memory");
+  return ok != 0;
+}
+// Bounded wait of a whole warp for the completion of the phase with this parity; false when the limit ran out.
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity) {
+  bool ok = mbar_try(b, parity);
+  if (!ok) {
+    const long long t0 = clock64();
+    do ok = mbar_try(b, parity);
+    while (!ok && clock64() - t0 <= (long long)kWaitLimit);
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(m), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(m), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Shared-memory operand descriptor, 128-byte swizzle.  Rows of 128 bytes, eight rows to a swizzle atom (1024 bytes):
+// `stride` is from one group of eight rows to the next, `lead` (operands whose rows are the K side) from one 64-element
+// column block to the next.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(stride >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// Instruction descriptor: fp32 accumulators, 128 x 128, A and B of the model type, B's rows the N side or the K side.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t mma_desc(bool b_rows_are_k) {
+  const uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_rows_are_k ? 1u : 0u) << 16) | (16u << 17) | (8u << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a),
+      "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a),
+      "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 columns of the thread's TMEM lane.  The wait names the registers, so that nothing uses them before it.
+__device__ __forceinline__ void tmem_ld32(float* r, uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait_ld32(float* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]),
+        "+f"(r[8]), "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]),
+        "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]),
+        "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31])
+               :: "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+      "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ float tile_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t tile_pack2(float a, float b) {
+  typename Elem<T>::T2 v;
+  v.x = Elem<T>::from_f(a);
+  v.y = Elem<T>::from_f(b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// One work item as every role of the block sees it.
+struct Item {
+  Segment s;
+  const int32_t* list;  // block list, or null
+  int t0, ntok, chunk, kvh;
+  int first, n_pages;   // its pages: numbers first .. first + n_pages of the segment's (or of the list)
+  int steps[2];         // key tiles of the two subtiles
+};
+__device__ __forceinline__ Item load_item(const AttnParams& p, int i) {
+  Item it;
+  const int4 w = p.tile_list[i / p.Hkv];
+  it.kvh = i % p.Hkv;
+  it.s = p.segs[w.x];
+  it.t0 = w.y;
+  it.ntok = w.z;
+  it.chunk = w.w;
+  it.list = nullptr;
+  int avail = 0;
+  if (p.block_pages) {
+    const int64_t slot = (int64_t)(it.s.tok0 / p.query_block + w.x + it.t0 / p.query_block) * p.Hkv + it.kvh;
+    it.list = p.block_pages + slot * p.max_k;
+    avail = min(max(p.block_npages[slot], 0), p.max_k);
+  }
+  it.first = it.chunk * it.s.chunk_pages;
+  it.n_pages = 0;
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    const int n = min(it.ntok - a * p.tok_tile, p.tok_tile);
+    int pages = 0;
+    if (n > 0) {
+      if (!it.list) avail = pages_seen(it.s, it.t0 + a * p.tok_tile + n - 1, p.causal);
+      pages = max(0, min(avail - it.first, it.s.chunk_pages));
+    }
+    it.steps[a] = (pages + 7) >> 3;
+    it.n_pages = max(it.n_pages, pages);
+  }
+  return it;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __grid_constant__ TileParams tp) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* q_s = smem;
+  uint8_t* kv_s = smem + 2 * kStageBytes;
+  TileShared& sh = *reinterpret_cast<TileShared*>(smem + (2 + kStages) * kStageBytes);
+  const AttnParams& p = tp.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.q_full, 1);
+    mbar_init(&sh.q_free, 1);
+    mbar_init(&sh.drain, 1);
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&sh.kv_full[i], 1);
+      mbar_init(&sh.kv_empty[i], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&sh.s_full[a], 1);
+      mbar_init(&sh.p_full[a], 128);
+      mbar_init(&sh.o_full[a], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 9) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  pdl_wait();
+  const int n_items = p.hdr->tile_items * p.Hkv;
+  bool ok = true;
+  if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+
+  if (warp == 8) {
+    // ---- loads ----
+    uint32_t stage = 0, round = 0, q_round = 0;
+    uint32_t tiles = 0;  // key tiles so far, over all items
+    uint32_t used = 0;  // stages filled so far, at most kStages: what an early end has to wait for
+    const int page_of_lane = (lane & 15) >> 1, half = lane & 1;
+    const int gone = p.num_pages_total * p.Hkv * kPage;  // a row behind the pool: reads as zeros
+    auto put = [&](const CUtensorMap* map, int row) {
+      ok = mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1);
+      if (!ok) return;
+      if (lane == 0) mbar_expect(&sh.kv_full[stage], kStageBytes);
+      __syncwarp();
+      if (lane < 16)
+        tma_2d(smem_u32(kv_s + stage * kStageBytes) + half * kHalfBytes + page_of_lane * 2048, map, half * 64, row,
+               &sh.kv_full[stage]);
+      used = max(used, stage + 1);
+      if (++stage == kStages) {
+        stage = 0;
+        ++round;
+      }
+    };
+    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+      const Item it = load_item(p, i);
+      const int32_t* indices = (it.s.second ? p.indices2 : p.indices1) + it.s.kvbase;
+      const int steps = max(it.steps[0], it.steps[1]);
+      if (steps == 0) continue;
+      const int subs = it.steps[1] > 0 ? 2 : 1;
+      ok = mbar_wait(&sh.q_free, (q_round & 1) ^ 1);
+      if (!ok) break;
+      ++q_round;
+      if (lane == 0) {
+        mbar_expect(&sh.q_full, (uint32_t)(subs * 2 * 64 * 2 * p.G * p.tok_tile));
+        for (int a = 0; a < subs; ++a)
+          for (int h = 0; h < 2; ++h)
+            tma_3d(smem_u32(q_s) + a * kStageBytes + h * kHalfBytes, &tp.tq, h * 64, it.kvh * p.G,
+                   it.s.tok0 + it.t0 + a * p.tok_tile, &sh.q_full);
+      }
+      __syncwarp();
+      auto look_up = [&](int j, int& lp, int& phys) {
+        const int at = 8 * j + page_of_lane;
+        lp = -1;
+        phys = -1;
+        if (j < steps && at < it.n_pages) {
+          lp = it.list ? it.list[it.first + at] : it.first + at;
+          if (lp >= 0 && lp < it.s.npages) phys = indices[lp];
+          if (phys < 0 || phys >= p.num_pages_total) {
+            phys = -1;
+            raise_flag(p.status, TWL_FLAG_BAD_INDEX);
+          }
+        }
+      };
+      int lp, phys, lp_next, phys_next;
+      look_up(0, lp, phys);
+      for (int j = 0; j < steps && ok; ++j) {
+        look_up(j + 1, lp_next, phys_next);
+        const int row = phys < 0 ? gone : (phys * p.Hkv + it.kvh) * kPage;
+        const int pos = phys < 0 ? 0x3fffffff : lp * kPage;
+        const int hi = __reduce_max_sync(0xffffffffu, phys < 0 ? 0x7fffffff : pos + kPage - 1);
+        const bool last = phys >= 0 && lp == it.s.npages - 1 && (it.s.len & (kPage - 1)) != 0;
+        const uint32_t tail = __ballot_sync(0xffffffffu, last);
+        // Room for K means that V of three tiles ago has been used, so every reader of the info of that tile and of
+        // those before it is done: of the eight slots three are still in use.
+        ok = mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1);
+        if (!ok) break;
+        const int slot = tiles++ & (kInfoSlots - 1);
+        if (lane < 16 && half == 0) sh.pos[slot][page_of_lane] = pos;
+        if (lane == 0) {
+          sh.hi[slot] = hi;
+          sh.tail[slot] = tail ? (__ffs(tail) - 1) >> 1 : -1;
+        }
+        __syncwarp();
+        put(&tp.tk, row);
+        if (ok) put(&tp.tv, row);
+        lp = lp_next;
+        phys = phys_next;
+      }
+    }
+    if (!ok) {  // an early end: the copies in flight still write to shared memory
+      for (uint32_t s = 0; s < used; ++s) mbar_wait(&sh.kv_full[s], (s < stage ? round : round - 1) & 1);
+      if (q_round) mbar_wait(&sh.q_full, (q_round - 1) & 1);
+    }
+  } else if (warp == 9) {
+    // ---- tensor cores ----
+    uint32_t stage = 0, round = 0, q_round = 0, p_round[2] = {0, 0}, tiles = 0;
+    const uint32_t kS = mma_desc<T>(false), kO = mma_desc<T>(true);
+    const uint32_t q_a = smem_u32(q_s), kv_a = smem_u32(kv_s);
+    auto next = [&]() {
+      if (++stage == kStages) {
+        stage = 0;
+        ++round;
+      }
+    };
+    auto scores = [&](int a, uint32_t k_stage) {  // S = Q K^T
+      if (lane == 0) {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const uint32_t off = (ks >> 2) * kHalfBytes + (ks & 3) * 32;
+          mma_ss(tmem + a * 128, smem_desc(q_a + a * kStageBytes + off, 16, 1024),
+                 smem_desc(kv_a + k_stage * kStageBytes + off, 16, 1024), kS, ks > 0);
+        }
+        mma_commit(&sh.s_full[a]);
+      }
+      __syncwarp();
+    };
+    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+      const Item it = load_item(p, i);
+      const int steps = max(it.steps[0], it.steps[1]);
+      if (steps == 0) continue;
+      ok = mbar_wait(&sh.q_full, q_round & 1);
+      if (!ok) break;
+      ++q_round;
+      ok = mbar_wait(&sh.kv_full[stage], round & 1);
+      if (!ok) break;
+      tc_fence_after();
+      if (it.steps[0] > 0) scores(0, stage);
+      if (it.steps[1] > 0) scores(1, stage);
+      if (lane == 0) {
+        mma_commit(&sh.kv_empty[stage]);
+        if (steps == 1) mma_commit(&sh.q_free);
+      }
+      __syncwarp();
+      next();
+      for (int j = 0; j < steps && ok; ++j) {
+        const uint32_t v_stage = stage;
+        ok = mbar_wait(&sh.kv_full[v_stage], round & 1);
+        if (!ok) break;
+        next();
+        const int tail = sh.tail[tiles++ & (kInfoSlots - 1)];
+        if (tail >= 0) {
+          // rows behind the sequence's end may hold anything, and 0 x NaN is not 0
+          const int r0 = it.s.len & (kPage - 1);
+          uint4* page = reinterpret_cast<uint4*>(kv_s + v_stage * kStageBytes + tail * 2048);
+          for (int c = r0 * 8 + lane; c < kPage * 8; c += 32) {
+            page[c] = make_uint4(0, 0, 0, 0);
+            page[kHalfBytes / 16 + c] = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        bool k_here = false;
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          if (j >= it.steps[a]) continue;
+          ok = mbar_wait(&sh.p_full[a], p_round[a] & 1);
+          if (!ok) break;
+          ++p_round[a];
+          tc_fence_after();
+          if (lane == 0) {
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              mma_ts(tmem + 256 + a * 128, tmem + a * 128 + ks * 8,
+                     smem_desc(kv_a + v_stage * kStageBytes + ks * 2048, kHalfBytes, 1024), kO, j > 0 || ks > 0);
+          }
+          __syncwarp();
+          if (j + 1 < it.steps[a]) {
+            if (!k_here) {
+              ok = mbar_wait(&sh.kv_full[stage], round & 1);
+              if (!ok) break;
+              k_here = true;
+              tc_fence_after();
+            }
+            scores(a, stage);
+          } else if (lane == 0) {
+            mma_commit(&sh.o_full[a]);
+          }
+        }
+        if (!ok) break;
+        if (lane == 0) {
+          mma_commit(&sh.kv_empty[v_stage]);
+          if (k_here) mma_commit(&sh.kv_empty[stage]);
+          if (j + 2 == steps) mma_commit(&sh.q_free);  // the last product with Q has been issued
+        }
+        __syncwarp();
+        if (k_here) next();
+      }
+    }
+    if (!ok) {  // an early end: products in flight still read shared memory and write TMEM
+      if (lane == 0) mma_commit(&sh.drain);
+      __syncwarp();
+      mbar_wait(&sh.drain, 0);
+    }
+  } else if (warp < 8) {
+    // ---- softmax: thread = row ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    const int a = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row
+    const uint32_t s_t = tmem + lanes + a * 128, o_t = tmem + lanes + 256 + a * 128;
+    uint32_t s_round = 0, o_round = 0, tiles = 0;
+    const int tok_r = r / p.G, head_r = r - tok_r * p.G;
+    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
+      const Item it = load_item(p, i);
+      const int tok = it.t0 + a * p.tok_tile + tok_r;
+      const bool real = tok_r < p.tok_tile && a * p.tok_tile + tok_r < it.ntok;
+      const int limit = !real ? -1 : p.causal ? it.s.len - it.s.ntok + tok : it.s.len - 1;
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < it.steps[a]; ++j) {
+        ok = mbar_wait(&sh.s_full[a], s_round & 1);
+        if (!ok) break;
+        ++s_round;
+        tc_fence_after();
+        const int slot = (tiles + j) & (kInfoSlots - 1);
+        float x[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(x + 32 * c, s_t + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_wait_ld32(x + 32 * c);
+        if (sh.hi[slot] > limit) {
+#pragma unroll
+          for (int pg = 0; pg < 8; ++pg) {
+            const int first = sh.pos[slot][pg];
+#pragma unroll
+            for (int c = 0; c < kPage; ++c)
+              if (first + c > limit) x[16 * pg + c] = -INFINITY;
+          }
+        }
+        __syncwarp();
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(x[c], x[c + 4]);
+#pragma unroll
+        for (int c = 8; c < 128; c += 4)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[c + e]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        // move the reference only when it is 2^8 behind (or nothing was seen so far)
+        float f = 1.f;
+        const bool move = top > m + 8.f;  // from -inf: any finite maximum
+        if (move) {
+          f = tile_ex2(m - top);
+          m = top;
+          l *= f;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, move)) {
+          // S of this step is complete, so the product of the step before is too: O may be changed
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            uint32_t w[32];
+            tmem_ld32(o, o_t + 32 * c);
+            tmem_wait_ld32(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
+            tmem_st32(o_t + 32 * c, w);
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float a0 = tile_ex2(fmaf(x[64 * c + 2 * e], p.scale_log2, -ref));
+            const float a1 = tile_ex2(fmaf(x[64 * c + 2 * e + 1], p.scale_log2, -ref));
+            sum[(2 * e) & 3] += a0;
+            sum[(2 * e + 1) & 3] += a1;
+            // weights go to the tensor cores in the model type (half a step of it each); their sum stays unrounded
+            w[e] = tile_pack2<T>(a0, a1);
+          }
+          tmem_st32(s_t + 32 * c, w);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&sh.p_full[a]);
+      }
+      if (!ok) break;
+      tiles += max(it.steps[0], it.steps[1]);
+      const bool any = it.steps[a] > 0;
+      if (any) {
+        ok = mbar_wait(&sh.o_full[a], o_round & 1);
+        if (!ok) break;
+        ++o_round;
+        tc_fence_after();
+      }
+      const int64_t row = (int64_t)(it.s.tok0 + tok), head = it.kvh * p.G + head_r;
+      const int64_t part = it.s.pbase < 0 ? -1 : it.s.pbase + ((int64_t)it.chunk * it.s.ntok + tok) * p.Hq + head;
+      const bool write = real && (part < 0 || part < p.part_cap);
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float o[32];
+        __syncwarp();
+        if (any) {
+          tmem_ld32(o, o_t + 32 * c);
+          tmem_wait_ld32(o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (!write) continue;
+        if (part >= 0) {
+          if (l != 0.f) {
+            float4* to = reinterpret_cast<float4*>(p.part_acc + part * kD + 32 * c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) to[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        } else {
+          uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row * p.o_ts + head * kD + 32 * c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              w[k] = l != 0.f ? tile_pack2<T>(o[8 * e + 2 * k] * inv, o[8 * e + 2 * k + 1] * inv) : 0u;
+            to[e] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      if (write) {
+        if (part >= 0)
+          p.part_ml[part] = make_float2(m, l);
+        else if (p.lse)
+          p.lse[row * p.Hq + head] = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+      }
+    }
+  }
+  if (!ok && lane == 0) raise_flag(p.status, TWL_FLAG_WAIT_LIMIT);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn tensor_map_encoder() {
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+
+int tile_attention_launch(const AttnParams& p, int dtype, cudaStream_t st) {
+  const EncodeFn encode = tensor_map_encoder();
+  if (!encode) {
+    set_last_cuda_error(cudaErrorNotSupported);
+    return TWL_ERR_LAUNCH;
+  }
+  TileParams tp;
+  tp.a = p;
+  const CUtensorMapDataType type = dtype == TWL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const cuuint64_t kv_dims[2] = {(cuuint64_t)kD, (cuuint64_t)p.num_pages_total * p.Hkv * kPage};
+  const cuuint64_t kv_strides[1] = {kD * 2};
+  const cuuint32_t kv_box[2] = {64, (cuuint32_t)kPage};
+  const cuuint64_t q_dims[3] = {(cuuint64_t)kD, (cuuint64_t)p.Hq, (cuuint64_t)p.num_tokens};
+  const cuuint64_t q_strides[2] = {kD * 2, (cuuint64_t)p.q_ts * 2};
+  const cuuint32_t q_box[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.tok_tile};
+  bool ok = true;
+  for (int i = 0; i < 2; ++i)
+    ok = ok && encode(i ? &tp.tv : &tp.tk, type, 2, const_cast<void*>(i ? p.v_pages : p.k_pages), kv_dims, kv_strides, kv_box,
+                      ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  ok = ok && encode(&tp.tq, type, 3, const_cast<void*>(p.q), q_dims, q_strides, q_box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  if (!ok) {
+    set_last_cuda_error(cudaErrorInvalidValue);
+    return TWL_ERR_LAUNCH;
+  }
+  auto* kernel = dtype == TWL_F16 ? prompt_tile_kernel<__half> : prompt_tile_kernel<__nv_bfloat16>;
+  TWL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem));
+  TWL_CUDA_TRY(launch_chain(kernel, dim3((unsigned)num_sms()), dim3(kTileThreads), kTileSmem, st, tp));
+  return TWL_OK;
+}
+
+}  // namespace twl

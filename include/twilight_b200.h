@@ -346,7 +346,7 @@ TWL_API int twl_append_kv(const void* new_k, const void* new_v, int dtype, void*
  * may be q itself), rotated K and V rows to the pages, and, unless null, the INT4 slabs (the
  * arithmetic of twl_quantize_k_pages) and the page metadata (a page whose first row is new starts
  * afresh, others fold).  A page that gets new tokens must not belong to a second sequence.
- * Rotation of channels 0..rotary_dim (a multiple of 8 up to 128; 0 = none): pair i turns by
+ * Rotation of channels 0..rotary_dim (a multiple of 16, interleaved of 8, up to 128; 0 = none): pair i turns by
  * position * freqs[i] (freqs: double [rotary_dim/2], radians per position), its channels are i and
  * i + rotary_dim/2, or 2i and 2i+1 with `interleaved`; cos and sin are multiplied by
  * attention_scale.  positions: int32 or int64 [T], or null for the cache positions.
@@ -360,7 +360,7 @@ TWL_API int twl_rope_append_kv(const void* q, const void* k, const void* v, int 
                                int64_t out_token_stride, int64_t out_head_stride,
                                const void* positions, int32_t positions_are_64bit,
                                const double* freqs, int32_t rotary_dim, int32_t interleaved,
-                               float attention_scale, void* k_pages, void* v_pages,
+                               double attention_scale, void* k_pages, void* v_pages,
                                uint8_t* k4_pages, void* kmeta, const int32_t* qo_indptr,
                                const int32_t* kv_indptr, const int32_t* kv_indices,
                                const int32_t* kv_last_page_len, int32_t num_tokens, int32_t batch,

@@ -100,6 +100,6 @@ def _rope_c(**kw):
 
 def test_rope_append_status_codes():
     assert _rope_c(q=None) == _rope_c(t=0) == _rope_c(hq=3) == _rope_c(freqs=None) == _rope_c(rot=-8) == -1
-    assert _rope_c(rot=12) == _rope_c(rot=136) == _rope_c(dtype=5) == -3
+    assert _rope_c(rot=12) == _rope_c(rot=8) == _rope_c(rot=136) == _rope_c(dtype=5) == -3
     assert _rope_c(q=260) == _rope_c(s=(510, 128, 256, 128, 256, 128)) == _rope_c(kp=264) == _rope_c(meta=8) == -2
-    assert _rope_c(hq=2 * 65535 * 8, hkv=2) == -5
+    assert _rope_c(hq=65536, hkv=65536) == -5

@@ -10,7 +10,7 @@ from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent / "lib" / "libtwilight_b200.so"
 
-i32, i64, f32, u32 = C.c_int32, C.c_int64, C.c_float, C.c_uint32
+i32, i64, f32, f64, u32 = C.c_int32, C.c_int64, C.c_float, C.c_double, C.c_uint32
 ptr, sz = C.c_void_p, C.c_size_t
 
 # name -> (restype, argtypes); must list every symbol of include/twilight_b200.h
@@ -51,7 +51,7 @@ SIGNATURES = {
                                                i32, i32, i32, i32, f32, ptr, f32, i32, i32, i32, ptr, ptr, sz,
                                                ptr, ptr]),
     "twl_rope_append_kv": (C.c_int, [ptr, ptr, ptr, C.c_int, i64, i64, i64, i64, i64, i64, ptr, i64, i64, ptr, i32, ptr,
-                                     i32, i32, f32, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, i32, i32, i32, i32, i32,
+                                     i32, i32, f64, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, i32, i32, i32, i32, i32,
                                      ptr, ptr]),
     "twl_dequantize_k_pages": (C.c_int, [ptr, ptr, i64, ptr, C.c_int, i32, i32, ptr, ptr]),
     "twl_prompt_attn_workspace_bytes": (sz, [i32] * 6),

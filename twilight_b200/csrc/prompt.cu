@@ -54,123 +54,154 @@ __device__ __forceinline__ int tok_tiles(const AttnParams& p, int ntok) {
   return whole * ((p.query_block + t - 1) / t) + (rest + t - 1) / t;
 }
 
-__device__ __forceinline__ long long block_sum(long long v, long long* s) {
+// Sums of N values over the block; every thread gets them.  One barrier before, one after the read.
+template <int N>
+__device__ __forceinline__ void block_sums(long long (&v)[N], long long (*s)[4]) {
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[threadIdx.x >> 5][k] = v[k];
   __syncthreads();
-  long long t = 0;
-  for (int i = 0; i < kPlanThreads / 32; ++i) t += s[i];
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = lane < warps ? s[lane][k] : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
   __syncthreads();
-  return t;
+}
+
+// pages of a chunk: enough chunks to give every tile slot about one, but not more than that many items
+__device__ __forceinline__ int chunk_size(long long tiles, long long work, int target, int least, int step) {
+  if (tiles >= target) return 0x3fffffff;  // every tile has a slot's worth of company
+  // a tile of w pages becomes ceil(w/c) items, on average w/c + 1/2
+  const long long room = max(1LL, target - tiles / 2);
+  const long long c = max((long long)least, (work + room - 1) / room);
+  return (int)min((long long)0x3fffffff, (c + step - 1) / step * step);
 }
 
 __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnParams p) {
-  __shared__ long long sums[kPlanThreads / 32];
-  __shared__ int wsum[66];
+  __shared__ long long sums[kPlanThreads / 32][4];
+  __shared__ int scan[kPlanThreads / 32][3];
   pdl_wait();
   pdl_release();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_thr = blockDim.x, n_warps = n_thr >> 5;
   const int n_seg = p.n_first + p.n_second;
-  long long ru = 0, rw = 0, tu = 0, tw = 0;  // tiles and pages x tiles of the row kernel, of the tile kernel
-  for (int i = tid; i < n_seg; i += kPlanThreads) {
+  const auto pages_of = [&](const Segment& s) { return p.block_pages ? min(s.npages, p.max_k) : s.npages; };
+  // tiles and tiles x pages of the row kernel and of the tile kernel
+  long long v[4] = {0, 0, 0, 0};
+  Segment mine;  // this thread's segment of the first round
+  mine.ntok = 0;
+  for (int i = tid; i < n_seg; i += n_thr) {
     const Segment s = load_segment(p, i);
-    const int pages = p.block_pages ? min(s.npages, p.max_k) : s.npages;
-    if (s.ntok * p.G <= p.few_rows) {
-      const int n = row_tiles(p, s.ntok);
-      ru += n;
-      rw += (long long)n * pages;
-    } else {
-      const int n = tok_tiles(p, s.ntok);
-      tu += n;
-      tw += (long long)n * pages;
+    if (i == tid) mine = s;
+    const bool few = s.ntok * p.G <= p.few_rows;
+    const int n = few ? row_tiles(p, s.ntok) : tok_tiles(p, s.ntok);
+    v[few ? 0 : 2] += n;
+    v[few ? 1 : 3] += (long long)n * pages_of(s);
+  }
+  block_sums<4>(v, sums);
+  const int rc = chunk_size(v[0] * p.Hkv, v[1] * p.Hkv, p.row_target, kRowChunkMin, 1);
+  int tc = chunk_size(v[2] * p.Hkv, v[3] * p.Hkv, p.tile_target, kTileChunkMin, 8);  // whole key tiles
+  // one wave of tiles should stay one wave: count, and make the chunks longer by what is too much
+  if (tc < 0x3fffffff) {
+    for (int round = 0; round < 3; ++round) {
+      long long items[1] = {0};
+      for (int i = tid; i < n_seg; i += n_thr) {
+        const Segment s = i == tid ? mine : load_segment(p, i);
+        if (s.ntok * p.G > p.few_rows) items[0] += (long long)tok_tiles(p, s.ntok) * max(1, (pages_of(s) + tc - 1) / tc);
+      }
+      block_sums<1>(items, sums);
+      const long long n = items[0] * p.Hkv;
+      if (n <= p.tile_target) break;
+      tc = (int)(((long long)tc * n / p.tile_target + 8) & ~7LL);
     }
   }
-  ru = block_sum(ru, sums) * p.Hkv;
-  rw = block_sum(rw, sums) * p.Hkv;
-  tu = block_sum(tu, sums) * p.Hkv;
-  tw = block_sum(tw, sums) * p.Hkv;
-  // With u < target tiles, chunks of w/target pages give fewer than u + target < 2*target items.
-  int rc = 0x3fffffff, tc = 0x3fffffff;
-  if (ru < p.row_target) rc = max((long long)kRowChunkMin, (rw + p.row_target - 1) / p.row_target);
-  if (tu < p.tile_target) tc = max((long long)kTileChunkMin, (tw + p.tile_target - 1) / p.tile_target);
-  if (tc < 0x3fffffff) tc = (tc + 7) & ~7;  // whole key tiles
 
-  int row_base = 0, tile_base = 0;
-  long long part_base = 0;
-  int split = 0;
-  for (int i0 = 0; i0 < n_seg; i0 += kPlanThreads) {
+  int row_base = 0, tile_base = 0, part_base = 0, split = 0;
+  for (int i0 = 0; i0 < n_seg; i0 += n_thr) {
     const int i = i0 + tid;
     Segment s;
     s.ntok = 0;
-    int rows = 0, tiles = 0;
-    long long parts = 0;
+    s.chunks = 1;
+    int cnt[3] = {0, 0, 0};  // row items, tile items, partial rows
     if (i < n_seg) {
-      s = load_segment(p, i);
-      const int pages = p.block_pages ? min(s.npages, p.max_k) : s.npages;
+      s = i0 == 0 ? mine : load_segment(p, i);
       const bool few = s.ntok * p.G <= p.few_rows;
       s.chunk_pages = few ? rc : tc;
-      s.chunks = max(1, (pages + s.chunk_pages - 1) / s.chunk_pages);
-      if (few)
-        rows = row_tiles(p, s.ntok) * s.chunks;
-      else
-        tiles = tok_tiles(p, s.ntok) * s.chunks;
-      if (s.chunks > 1 || p.always_partial) parts = (long long)s.chunks * s.ntok * p.Hq;
+      s.chunks = max(1, (pages_of(s) + s.chunk_pages - 1) / s.chunk_pages);
+      cnt[few ? 0 : 1] = (few ? row_tiles(p, s.ntok) : tok_tiles(p, s.ntok)) * s.chunks;
+      if (s.chunks > 1 || p.always_partial) cnt[2] = s.chunks * s.ntok * p.Hq;
       split |= s.chunks > 1;
     }
-    // segment bases: items in 32 bits, partial rows in 64
-    int er, et, tr, tt;
-    block_excl_scan2<kPlanThreads>(rows, tiles, &er, &et, &tr, &tt, wsum);
-    long long inc = parts;
+    // exclusive sums over the segments
+    int inc[3] = {cnt[0], cnt[1], cnt[2]};
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += x;
-    }
-    if (lane == 31) sums[warp] = inc;
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        const int x = __shfl_up_sync(0xffffffffu, inc[k], o);
+        if (lane >= o) inc[k] += x;
+      }
+    if (lane == 31)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) scan[warp][k] = inc[k];
     __syncthreads();
-    long long before = 0, total = 0;
-    for (int w = 0; w < kPlanThreads / 32; ++w) {
-      if (w < warp) before += sums[w];
-      total += sums[w];
+    int at[3], total[3];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const int w = lane < n_warps ? scan[lane][k] : 0;
+      const int before = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
+      total[k] = __reduce_add_sync(0xffffffffu, w);
+      at[k] = before + inc[k] - cnt[k];
     }
     __syncthreads();
     if (i < n_seg) {
-      s.pbase = (s.chunks > 1 || p.always_partial) ? part_base + before + inc - parts : -1;
+      s.pbase = cnt[2] > 0 ? (int64_t)part_base + at[2] : -1;
       p.segs[i] = s;
     }
-    // the items: a warp writes one segment's at a time
-    for (int l = 0; l < 32; ++l) {
-      const int seg = i0 + warp * 32 + l;
-      if (seg >= n_seg) break;
-      const int ntok = __shfl_sync(0xffffffffu, s.ntok, l), chunks = __shfl_sync(0xffffffffu, s.chunks, l);
-      const int nr = __shfl_sync(0xffffffffu, rows, l), nt = __shfl_sync(0xffffffffu, tiles, l);
-      const int rb = row_base + __shfl_sync(0xffffffffu, er, l), tb = tile_base + __shfl_sync(0xffffffffu, et, l);
-      for (int k = lane; k < nr; k += 32) {
-        const int tile = k / chunks, chunk = k - tile * chunks;
-        int r0 = tile * p.row_tile, end = ntok * p.G;
-        if (p.block_pages) {
-          const int per = (p.query_block * p.G + p.row_tile - 1) / p.row_tile, blk = tile / per;
-          r0 = blk * p.query_block * p.G + (tile - blk * per) * p.row_tile;
-          end = min(end, (blk + 1) * p.query_block * p.G);
-        }
-        if (rb + k < p.row_cap) p.row_list[rb + k] = make_int4(seg, r0, min(p.row_tile, end - r0), chunk);
+    // a few items: their thread writes them; many: the warp does, segment by segment
+    constexpr int kSelf = 4;
+    const auto row_item = [&](int seg, int ntok, int chunks, int k, int to) {
+      const int tile = k / chunks;
+      int r0 = tile * p.row_tile, end = ntok * p.G;
+      if (p.block_pages) {
+        const int per = (p.query_block * p.G + p.row_tile - 1) / p.row_tile, blk = tile / per;
+        r0 = blk * p.query_block * p.G + (tile - blk * per) * p.row_tile;
+        end = min(end, (blk + 1) * p.query_block * p.G);
       }
-      for (int k = lane; k < nt; k += 32) {
-        // the last tiles of a causal segment see most keys: first in the list
-        const int tile = nt / chunks - 1 - k / chunks, chunk = k % chunks;
-        int t0 = tile * 2 * p.tok_tile, end = ntok;
-        if (p.block_pages) {
-          const int per = (p.query_block + 2 * p.tok_tile - 1) / (2 * p.tok_tile), blk = tile / per;
-          t0 = blk * p.query_block + (tile - blk * per) * 2 * p.tok_tile;
-          end = min(end, (blk + 1) * p.query_block);
-        }
-        if (tb + k < p.tile_cap) p.tile_list[tb + k] = make_int4(seg, t0, min(2 * p.tok_tile, end - t0), chunk);
+      if (to < p.row_cap) p.row_list[to] = make_int4(seg, r0, min(p.row_tile, end - r0), k - tile * chunks);
+    };
+    const auto tile_item = [&](int seg, int ntok, int chunks, int n, int k, int to) {
+      const int tile = n / chunks - 1 - k / chunks;  // the last tiles of a causal segment see most keys: first in the list
+      int t0 = tile * 2 * p.tok_tile, end = ntok;
+      if (p.block_pages) {
+        const int per = (p.query_block + 2 * p.tok_tile - 1) / (2 * p.tok_tile), blk = tile / per;
+        t0 = blk * p.query_block + (tile - blk * per) * 2 * p.tok_tile;
+        end = min(end, (blk + 1) * p.query_block);
       }
+      if (to < p.tile_cap) p.tile_list[to] = make_int4(seg, t0, min(2 * p.tok_tile, end - t0), k % chunks);
+    };
+    const bool many = cnt[0] + cnt[1] > kSelf;
+    if (!many) {
+      for (int k = 0; k < cnt[0]; ++k) row_item(i, s.ntok, s.chunks, k, row_base + at[0] + k);
+      for (int k = 0; k < cnt[1]; ++k) tile_item(i, s.ntok, s.chunks, cnt[1], k, tile_base + at[1] + k);
     }
-    row_base += tr;
-    tile_base += tt;
-    part_base += total;
+    for (uint32_t left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
+      const int l = __ffs(left) - 1, seg = i0 + warp * 32 + l;
+      const int ntok = __shfl_sync(0xffffffffu, s.ntok, l), chunks = __shfl_sync(0xffffffffu, s.chunks, l);
+      const int nr = __shfl_sync(0xffffffffu, cnt[0], l), nt = __shfl_sync(0xffffffffu, cnt[1], l);
+      const int rb = row_base + __shfl_sync(0xffffffffu, at[0], l), tb = tile_base + __shfl_sync(0xffffffffu, at[1], l);
+      for (int k = lane; k < nr; k += 32) row_item(seg, ntok, chunks, k, rb + k);
+      for (int k = lane; k < nt; k += 32) tile_item(seg, ntok, chunks, nt, k, tb + k);
+    }
+    row_base += total[0];
+    tile_base += total[1];
+    part_base += total[2];
   }
   split = __syncthreads_or(split);
   if (tid == 0) {
@@ -485,19 +516,38 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const AttnParams p) {
       if (tok < s.tok0 || tok >= s.tok0 + s.ntok) continue;
       if (s.pbase < 0) continue;
       found = true;
-      for (int c = 0; c < s.chunks; ++c) {
-        const int64_t slot = s.pbase + ((int64_t)c * s.ntok + (tok - s.tok0)) * p.Hq + head;
-        if (slot >= p.part_cap) break;
-        const float2 v = p.part_ml[slot];
-        if (v.y == 0.f) continue;  // (a NaN goes on)
-        const float4 x = *reinterpret_cast<const float4*>(p.part_acc + slot * kD + 4 * lane);
-        const float mn = fmaxf(m, v.x), f0 = ex2(m - mn), f1 = ex2(v.x - mn);
-        l = l * f0 + v.y * f1;
-        a.x = a.x * f0 + x.x * f1;
-        a.y = a.y * f0 + x.y * f1;
-        a.z = a.z * f0 + x.z * f1;
-        a.w = a.w * f0 + x.w * f1;
+      // a lane takes a chunk's maximum and sum; the accumulators follow, four in flight
+      const int64_t slot0 = s.pbase + (int64_t)(tok - s.tok0) * p.Hq + head, step = (int64_t)s.ntok * p.Hq;
+      for (int c0 = 0; c0 < s.chunks; c0 += 32) {
+        const int n = min(32, s.chunks - c0);
+        float2 v = make_float2(-INFINITY, 0.f);
+        if (lane < n && slot0 + (c0 + lane) * step < p.part_cap) v = p.part_ml[slot0 + (c0 + lane) * step];
+        const float mn = fmaxf(m, warp_max(v.x)), ref = mn == -INFINITY ? 0.f : mn;
+        const float f0 = ex2(m - ref);
+        const float w = v.y == 0.f ? 0.f : ex2(v.x - ref);  // (a NaN sum goes on)
+        l = l * f0 + warp_sum(v.y * w);
+        a.x *= f0;
+        a.y *= f0;
+        a.z *= f0;
+        a.w *= f0;
         m = mn;
+        const uint32_t has = __ballot_sync(0xffffffffu, v.y != 0.f);  // the others' accumulators were not written
+        for (int c = 0; c < n; c += 4) {
+          float4 x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if ((has >> (c + k)) & 1) x[k] = *reinterpret_cast<const float4*>(p.part_acc + (slot0 + (c0 + c + k) * step) * kD + 4 * lane);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float f = __shfl_sync(0xffffffffu, w, (c + k) & 31);
+            if ((has >> (c + k)) & 1) {
+              a.x += x[k].x * f;
+              a.y += x[k].y * f;
+              a.z += x[k].z * f;
+              a.w += x[k].w * f;
+            }
+          }
+        }
       }
     }
     if (!found) continue;
@@ -570,7 +620,8 @@ static void place_workspace(AttnParams& p, const WorkspaceLayout& w, void* works
 
 template <typename T>
 static int run_attention(const AttnParams& p, int dtype, bool need_merge, cudaStream_t st) {
-  TWL_CUDA_TRY(launch_chain(prompt_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p));
+  const int plan_threads = p.n_first + p.n_second <= 256 ? 256 : kPlanThreads;
+  TWL_CUDA_TRY(launch_chain(prompt_plan_kernel, dim3(1), dim3(plan_threads), 0, st, p));
   const dim3 rows_grid((unsigned)(num_sms() * kRowBlocksPerSm));
   if (p.row_tile == 8) {
     TWL_CUDA_TRY(cudaFuncSetAttribute(prompt_rows_kernel<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem));

@@ -4,8 +4,8 @@
 // Rotation of a head's first R channels at position p, with the angle a_i = p * f_i of pair i < R/2:
 //   x'_u = x_u cos a_i - x_v sin a_i,  x'_v = x_v cos a_i + x_u sin a_i,
 // (u, v) = (i, i + R/2), or (2i, 2i + 1) when interleaved.  cos and sin carry attention_scale.  Angles are formed
-// and reduced to a fraction of a turn in 64 bits (at position 10^5 a 32-bit product is off by 0.004 rad), the
-// sine and cosine of the fraction are 32-bit; the rotation is 32-bit and rounded once to the model type.
+// and reduced to a fraction of a turn in 64 bits (at position 10^5 a 32-bit product is off by 0.004 rad), and so are
+// its sine and cosine, once per page and pair; the rotation is 32-bit and rounded once to the model type.
 //
 // Bound: HBM.  Every row is read once and written once; the INT4 slab and the metadata of a page are made from
 // the rows while they are in registers.  The decode form (one token per sequence) is bound by the latency of a
@@ -24,68 +24,121 @@ struct RopeParams {
   uint8_t* k4;
   const int32_t *qo_indptr, *indptr, *indices, *last_len;
   int32_t* status;
-  int32_t batch, Hq, Hkv, num_tokens, num_pages_total, rotary, interleaved, pos64, tasks_per_block;
-  float attn_scale;
+  int32_t batch, Hq, Hkv, num_tokens, num_pages_total, rotary, pos64, heads_per_block, wide;
+  double attn_scale;
 };
 
 constexpr int kRopeWarps = 8;
+
+// Rows of the caller's tensors: 16-byte pieces, or two of 8 bytes where a base or stride asks for it.
+template <typename T>
+__device__ __forceinline__ uint4 load_row16(const T* p, int wide) {
+  if (wide) return ldg_stream_u4(p);
+  const uint2 a = ldg_stream_u2(p), b = ldg_stream_u2(p + 4);
+  return make_uint4(a.x, a.y, b.x, b.y);
+}
+template <typename T>
+__device__ __forceinline__ void store_row16(T* p, const uint4& v, int wide) {
+  if (wide) {
+    *reinterpret_cast<uint4*>(p) = v;
+  } else {
+    reinterpret_cast<uint2*>(p)[0] = make_uint2(v.x, v.y);
+    reinterpret_cast<uint2*>(p)[1] = make_uint2(v.z, v.w);
+  }
+}
+static_assert(kRopeWarps * 2 == kPage, "a half-warp for every token of a page");
 
 template <typename T>
 __device__ __forceinline__ float rope_rnd(float x) {
   return Elem<T>::to_f(Elem<T>::from_f(x));
 }
-
 template <typename T>
-__device__ __forceinline__ uint2 pack4(const float (&x)[4]) {
-  using T2 = typename Elem<T>::T2;
-  T2 a, b;
-  a.x = Elem<T>::from_f(x[0]);
-  a.y = Elem<T>::from_f(x[1]);
-  b.x = Elem<T>::from_f(x[2]);
-  b.y = Elem<T>::from_f(x[3]);
-  return make_uint2(*reinterpret_cast<uint32_t*>(&a), *reinterpret_cast<uint32_t*>(&b));
-}
-
-// Rotates one row held four channels to a lane (channels 4*lane ..).  table: this token's R/2 {cos, sin}.
-// Every lane of the warp takes part in the shuffles; lanes past R keep their channels.
-__device__ __forceinline__ void rotate_row(float (&x)[4], const float2* table, int rotary, bool inter, int lane) {
-  const int c = 4 * lane;
-  if (inter) {
-    if (c < rotary) {
-      const float4 t = reinterpret_cast<const float4*>(table)[lane];  // {cos, sin} of pairs 2*lane, 2*lane+1
-      const float a = x[0], b = x[2];
-      x[0] = a * t.x - x[1] * t.y;
-      x[1] = x[1] * t.x + a * t.y;
-      x[2] = b * t.z - x[3] * t.w;
-      x[3] = x[3] * t.z + b * t.w;
-    }
-  } else {
-    const int half = rotary >> 1, hl = half >> 2;  // half is a multiple of 4
-    const bool lowside = c < half, in = c < rotary;
-    const int peer = lowside ? lane + hl : lane - hl;
-    float y[4];
+__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) y[j] = __shfl_sync(0xffffffffu, x[j], in ? peer : lane);
-    if (in) {
-      const float4* t = reinterpret_cast<const float4*>(table + (lowside ? c : c - half));
-      const float4 t0 = t[0], t1 = t[1];
-      const float cs[4] = {t0.x, t0.z, t1.x, t1.z};
-      const float sn[4] = {t0.y, t0.w, t1.y, t1.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = lowside ? x[j] * cs[j] - y[j] * sn[j] : x[j] * cs[j] + y[j] * sn[j];
-    }
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = Elem<T>::to_f2(w[k]);
+    x[2 * k] = f.x;
+    x[2 * k + 1] = f.y;
   }
 }
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    typename Elem<T>::T2 v;
+    v.x = Elem<T>::from_f(x[2 * k]);
+    v.y = Elem<T>::from_f(x[2 * k + 1]);
+    w[k] = *reinterpret_cast<uint32_t*>(&v);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
-// Block = (a page that gets new tokens, a run of tasks); a task is one head's rows of that page: K of a KV head
-// (rotated, written, quantised, folded into the metadata), V of a KV head (copied), or one query head (rotated).
-// A warp takes a task whole, eight rows of 256 bytes in flight, so the metadata needs no exchange between warps;
-// the block shares the sines of the page's 16 positions.
+// cos and sin for the eight channels of a lane (8 * (lane & 15) ..): channel j of a half turns with pair j, of
+// interleaved channels 2k and 2k+1 with pair k.
+template <bool INTER>
+struct Angles {
+  static constexpr int N = INTER ? 4 : 8;
+  float c[N], s[N];
+  __device__ __forceinline__ void read(const float* cos_row, const float* sin_row, int ch, int rotary) {
+    const int at = INTER ? ch >> 1 : ch >= (rotary >> 1) ? ch - (rotary >> 1) : ch;
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(cos_row + at + k);
+      const float4 y = *reinterpret_cast<const float4*>(sin_row + at + k);
+      c[k] = x.x; c[k + 1] = x.y; c[k + 2] = x.z; c[k + 3] = x.w;
+      s[k] = y.x; s[k + 1] = y.y; s[k + 2] = y.z; s[k + 3] = y.w;
+    }
+  }
+};
+
+// Rotates the row that a half-warp holds eight channels to a lane.  Every lane takes part in the exchange of halves;
+// lanes behind `rotary` keep their channels.  Both products are rounded (not fused into the sum), so that the stored K
+// and with it the 4-bit codes do not depend on which of them a compiler would fuse.
+template <typename T, bool INTER>
+__device__ __forceinline__ uint4 rotate8(const uint4& u, const Angles<INTER>& g, int ch, int rotary) {
+  float x[8];
+  unpack8<T>(u, x);
+  if (INTER) {
+    if (ch >= rotary) return u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float a = x[2 * k], b = x[2 * k + 1];
+      x[2 * k] = __fsub_rn(__fmul_rn(a, g.c[k % Angles<INTER>::N]), __fmul_rn(b, g.s[k % Angles<INTER>::N]));
+      x[2 * k + 1] = __fadd_rn(__fmul_rn(b, g.c[k % Angles<INTER>::N]), __fmul_rn(a, g.s[k % Angles<INTER>::N]));
+    }
+    return pack8<T>(x);
+  }
+  const int half = rotary >> 1, away = half >> 3;  // half is a multiple of 8
+  const bool low = ch < half;
+  const int lane = threadIdx.x & 31, peer = ch >= rotary ? lane : low ? lane + away : lane - away;
+  uint4 v;
+  v.x = __shfl_sync(0xffffffffu, u.x, peer);
+  v.y = __shfl_sync(0xffffffffu, u.y, peer);
+  v.z = __shfl_sync(0xffffffffu, u.z, peer);
+  v.w = __shfl_sync(0xffffffffu, u.w, peer);
+  if (ch >= rotary) return u;
+  float y[8];
+  unpack8<T>(v, y);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float sn = low ? -g.s[k % Angles<INTER>::N] : g.s[k % Angles<INTER>::N];
+    x[k] = __fadd_rn(__fmul_rn(x[k], g.c[k % Angles<INTER>::N]), __fmul_rn(y[k], sn));
+  }
+  return pack8<T>(x);
+}
+
+// Block = (a page that gets new tokens, a run of KV heads with their query heads).  The block computes the sines of the
+// page's positions once; then K (a warp takes a head, half a warp a token, so that the metadata is folded in
+// registers), V (copied) and q (half a warp takes a token and walks the heads with its sines in registers; where the
+// page has fewer new tokens, several half-warps share a token).  Rows move in 16-byte pieces, four to eight of
+// them in flight per lane.
 // Pages are found without a scan: sequence b owns the block slots from qo_indptr[b]/16 + 2b on, always as many as
 // the pages its new tokens can touch; a slot beyond them has nothing to do.
-template <typename T>
-__global__ void __launch_bounds__(kRopeWarps * 32) rope_append_kernel(const RopeParams p) {
-  __shared__ alignas(16) float2 table[kPage][kD / 2];
+template <typename T, bool INTER>
+__global__ void __launch_bounds__(kRopeWarps * 32, 3) rope_append_kernel(const RopeParams p) {
+  __shared__ alignas(16) float cos_s[kPage][kD / 2], sin_s[kPage][kD / 2];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slot = blockIdx.x;
@@ -114,8 +167,8 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_append_kernel(const Rope
   const int lp = (start >> 4) + (slot - ((row0 >> 4) + 2 * b));
   if (lp >= n_pages) return;
   const int t0 = max(start, lp * kPage), t1 = min(len, lp * kPage + kPage);
-  const int n = t1 - t0;                 // new tokens of this page, 1..16
-  const int row = row0 + (t0 - start);   // row of the first of them in q, k, v
+  const int n = t1 - t0;                // new tokens of this page, 1..16
+  const int row = row0 + (t0 - start);  // row of the first of them in q, k, v
   const int first_slot = t0 & (kPage - 1);
   const int phys = __ldg(p.indices + pbase + lp);
   const bool page_ok = phys >= 0 && phys < p.num_pages_total;
@@ -132,76 +185,72 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_append_kernel(const Rope
     else
       pos = (double)__ldg(static_cast<const int*>(p.positions) + row + tok);
     const double turns = pos * __ldg(p.freqs + f) * 0.15915494309189533577;  // 1 / (2 pi)
-    float s, c;
-    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-    table[tok][f] = make_float2(c * p.attn_scale, s * p.attn_scale);
+    double s, c;
+    sincospi(2. * (turns - rint(turns)), &s, &c);
+    cos_s[tok][f] = (float)(c * p.attn_scale);
+    sin_s[tok][f] = (float)(s * p.attn_scale);
   }
   __syncthreads();
 
-  const int tasks = 2 * p.Hkv + p.Hq;
-  const int task_end = min(tasks, (int)(blockIdx.y + 1) * p.tasks_per_block);
-  for (int task = blockIdx.y * p.tasks_per_block + warp; task < task_end; task += kRopeWarps) {
-    const bool is_k = task < p.Hkv, is_v = !is_k && task < 2 * p.Hkv;
-    const int head = is_k ? task : is_v ? task - p.Hkv : task - 2 * p.Hkv;
-    if ((is_k || is_v) && !page_ok) continue;
-    const T* src;
-    int64_t ts;
-    T* dst;
-    int64_t dts;
-    const size_t slab = (size_t)max(phys, 0) * p.Hkv + head;
-    if (is_k) {
-      src = static_cast<const T*>(p.k) + row * p.k_ts + head * p.k_hs;
-      ts = p.k_ts;
-      dst = static_cast<T*>(p.k_pages) + slab * (kPage * kD) + first_slot * kD;
-      dts = kD;
-    } else if (is_v) {
-      src = static_cast<const T*>(p.v) + row * p.v_ts + head * p.v_hs;
-      ts = p.v_ts;
-      dst = static_cast<T*>(p.v_pages) + slab * (kPage * kD) + first_slot * kD;
-      dts = kD;
-    } else {
-      src = static_cast<const T*>(p.q) + row * p.q_ts + head * p.q_hs;
-      ts = p.q_ts;
-      dst = static_cast<T*>(p.q_out) + row * p.o_ts + head * p.o_hs;
-      dts = p.o_ts;
-    }
-    float mn[4] = {INFINITY, INFINITY, INFINITY, INFINITY}, mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    const bool meta = is_k && p.kmeta != nullptr;
-    T* mrow = static_cast<T*>(p.kmeta) + slab * 2 * kD;
-    if (meta && first_slot != 0) {  // the page holds older tokens: fold into what it says
-      const uint2 a = reinterpret_cast<const uint2*>(mrow)[lane], z = reinterpret_cast<const uint2*>(mrow + kD)[lane];
-      const float2 a0 = Elem<T>::to_f2(a.x), a1 = Elem<T>::to_f2(a.y);
-      const float2 z0 = Elem<T>::to_f2(z.x), z1 = Elem<T>::to_f2(z.y);
-      mn[0] = a0.x; mn[1] = a0.y; mn[2] = a1.x; mn[3] = a1.y;
-      mx[0] = z0.x; mx[1] = z0.y; mx[2] = z1.x; mx[3] = z1.y;
-    }
-    for (int r0 = 0; r0 < n; r0 += 8) {
-      uint2 u[8];
+  const int G = p.Hq / p.Hkv;
+  const int kv0 = blockIdx.y * p.heads_per_block, kv1 = min(p.Hkv, kv0 + p.heads_per_block);
+  const int hw = lane >> 4, ch = 8 * (lane & 15);  // this lane's half of the warp, its channels
+  Angles<INTER> ang;
+
+  if (page_ok) {
+    for (int task = warp; task < 2 * (kv1 - kv0); task += kRopeWarps) {
+      const bool is_k = task < kv1 - kv0;
+      const int head = kv0 + (is_k ? task : task - (kv1 - kv0));
+      const size_t slab = (size_t)phys * p.Hkv + head;
+      const int64_t ts = is_k ? p.k_ts : p.v_ts;
+      const T* src = static_cast<const T*>(is_k ? p.k : p.v) + row * ts + head * (is_k ? p.k_hs : p.v_hs) + ch;
+      T* dst = static_cast<T*>(is_k ? p.k_pages : p.v_pages) + slab * (kPage * kD) + first_slot * kD + ch;
+      float mn[8], mx[8];
+      const bool meta = is_k && p.kmeta != nullptr;
+      T* mrow = static_cast<T*>(p.kmeta) + slab * 2 * kD + ch;
+      if (meta && first_slot != 0) {  // the page holds older tokens: fold into what it says
+        unpack8<T>(*reinterpret_cast<const uint4*>(mrow), mn);
+        unpack8<T>(*reinterpret_cast<const uint4*>(mrow + kD), mx);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (r0 + i < n) u[i] = ldg_stream_u2(src + (r0 + i) * ts + 4 * lane);
+        for (int j = 0; j < 8; ++j) {
+          mn[j] = INFINITY;
+          mx[j] = -INFINITY;
+        }
+      }
+      for (int r0 = 0; r0 < n; r0 += 8) {
+        uint4 u[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = r0 + i;
-        if (r >= n) break;
-        if (!is_v) {
-          const float2 a = Elem<T>::to_f2(u[i].x), c = Elem<T>::to_f2(u[i].y);
-          float x[4] = {a.x, a.y, c.x, c.y};
-          if (p.rotary > 0) rotate_row(x, table[r], p.rotary, p.interleaved != 0, lane);
-          u[i] = pack4<T>(x);
+        for (int i = 0; i < 4; ++i)
+          if (r0 + 2 * i + hw < n) u[i] = load_row16(src + (r0 + 2 * i + hw) * ts, p.wide);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = r0 + 2 * i + hw;
+          if (r0 + 2 * i >= n) break;  // (both halves)
+          const bool mine = r < n;
           if (is_k) {
-            const float2 y0 = Elem<T>::to_f2(u[i].x), y1 = Elem<T>::to_f2(u[i].y);  // as the cache holds them
-            const float y[4] = {y0.x, y0.y, y1.x, y1.y};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              mn[j] = fminf(mn[j], y[j]);
-              mx[j] = fmaxf(mx[j], y[j]);
+            if (p.rotary > 0) {
+              ang.read(cos_s[mine ? r : 0], sin_s[mine ? r : 0], ch < p.rotary ? ch : 0, p.rotary);
+              u[i] = rotate8<T, INTER>(u[i], ang, ch, p.rotary);
             }
-            if (p.k4 != nullptr) {  // groups of 32 channels = eight lanes; the arithmetic of quantize_k_pages
-              float gx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-              float gn = fminf(fminf(y[0], y[1]), fminf(y[2], y[3]));
+            float y[8];
+            unpack8<T>(u[i], y);  // as the cache holds them
+            if (mine) {
 #pragma unroll
-              for (int o = 4; o > 0; o >>= 1) {
+              for (int j = 0; j < 8; ++j) {
+                mn[j] = fminf(mn[j], y[j]);
+                mx[j] = fmaxf(mx[j], y[j]);
+              }
+            }
+            if (p.k4 != nullptr) {  // groups of 32 channels = four lanes; the arithmetic of quantize_k_pages
+              float gx = y[0], gn = y[0];
+#pragma unroll
+              for (int j = 1; j < 8; ++j) {
+                gx = fmaxf(gx, y[j]);
+                gn = fminf(gn, y[j]);
+              }
+#pragma unroll
+              for (int o = 2; o > 0; o >>= 1) {
                 gx = fmaxf(gx, __shfl_xor_sync(0xffffffffu, gx, o));
                 gn = fminf(gn, __shfl_xor_sync(0xffffffffu, gn, o));
               }
@@ -209,27 +258,57 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_append_kernel(const Rope
               const float scale = rope_rnd<T>(__fdiv_rn(range, 15.f));
               uint32_t word = 0;
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
+              for (int j = 0; j < 8; ++j) {
                 const float t = rope_rnd<T>(y[j] - gn);
                 float w = (scale > 0.f) ? rope_rnd<T>(__fdiv_rn(t, scale)) : 0.f;
                 w = fminf(fmaxf(rintf(w), 0.f), 15.f);
                 word |= (uint32_t)(int)w << (4 * j);
               }
-              uint8_t* q4 = p.k4 + slab * kSlab;
-              const int tok = first_slot + r;
-              *reinterpret_cast<uint16_t*>(q4 + tok * 64 + 2 * lane) = (uint16_t)word;
-              if ((lane & 7) == 0)
-                *reinterpret_cast<__half2*>(q4 + kSlabCodes + tok * 16 + (lane >> 3) * 4) =
-                    __halves2half2(__float2half_rn(scale), __float2half_rn(gn));
+              if (mine) {
+                uint8_t* q4 = p.k4 + slab * kSlab;
+                const int tok = first_slot + r;
+                *reinterpret_cast<uint32_t*>(q4 + tok * 64 + (ch >> 1)) = word;
+                if ((lane & 3) == 0)
+                  *reinterpret_cast<__half2*>(q4 + kSlabCodes + tok * 16 + (ch >> 5) * 4) =
+                      __halves2half2(__float2half_rn(scale), __float2half_rn(gn));
+              }
             }
           }
+          if (mine) *reinterpret_cast<uint4*>(dst + r * kD) = u[i];
         }
-        *reinterpret_cast<uint2*>(dst + r * dts + 4 * lane) = u[i];
+      }
+      if (meta) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          mn[j] = fminf(mn[j], __shfl_xor_sync(0xffffffffu, mn[j], 16));
+          mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 16));
+        }
+        *reinterpret_cast<uint4*>(mrow + hw * kD) = pack8<T>(hw ? mx : mn);
       }
     }
-    if (meta) {
-      reinterpret_cast<uint2*>(mrow)[lane] = pack4<T>(mn);
-      reinterpret_cast<uint2*>(mrow + kD)[lane] = pack4<T>(mx);
+  }
+
+  // q: 16 half-warps over the tokens (rounded up to a power of two), the rest of them over the heads
+  const int width = n > 8 ? 16 : n > 4 ? 8 : n > 2 ? 4 : n, unit = 2 * warp + hw;
+  const int tok = unit & (width - 1), h_step = kPage / width, h_end = kv1 * G;
+  const bool mine = tok < n;
+  if (p.rotary > 0) ang.read(cos_s[mine ? tok : 0], sin_s[mine ? tok : 0], ch < p.rotary ? ch : 0, p.rotary);
+  const T* src = static_cast<const T*>(p.q) + (int64_t)(row + (mine ? tok : 0)) * p.q_ts + ch;
+  T* dst = static_cast<T*>(p.q_out) + (int64_t)(row + (mine ? tok : 0)) * p.o_ts + ch;
+  const int h_off = unit / width, rounds = (h_end - kv0 * G + h_step - 1) / h_step;  // rounds: the same for every lane
+  for (int i0 = 0; i0 < rounds; i0 += 4) {
+    uint4 u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int h = kv0 * G + h_off + (i0 + i) * h_step;
+      if (mine && h < h_end) u[i] = load_row16(src + h * p.q_hs, p.wide);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int h = kv0 * G + h_off + (i0 + i) * h_step;
+      if (i0 + i >= rounds) break;
+      if (p.rotary > 0) u[i] = rotate8<T, INTER>(u[i], ang, ch, p.rotary);
+      if (mine && h < h_end) store_row16(dst + h * p.o_hs, u[i], p.wide);
     }
   }
 }
@@ -256,14 +335,10 @@ __global__ void __launch_bounds__(256) dequantize_k_pages_kernel(const DequantPa
     const uint32_t code = ldg_stream_u32(slab + tok * 64 + w * 4);
     const uint32_t sz = ldg_stream_u32(slab + kSlabCodes + tok * 16 + (w >> 2) * 4);
     const float2 f = Elem<__half>::to_f2(sz);
-    float a[4], b[4];
+    float x[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      a[j] = (float)((code >> (4 * j)) & 15u) * f.x + f.y;
-      b[j] = (float)((code >> (4 * j + 16)) & 15u) * f.x + f.y;
-    }
-    const uint2 x = pack4<T>(a), y = pack4<T>(b);
-    r = make_uint4(x.x, x.y, y.x, y.y);
+    for (int j = 0; j < 8; ++j) x[j] = (float)((code >> (4 * j)) & 15u) * f.x + f.y;
+    r = pack8<T>(x);
   } else if (threadIdx.x == 0) {
     raise_flag(p.status, TWL_FLAG_BAD_INDEX);
   }
@@ -281,7 +356,7 @@ extern "C" int twl_rope_append_kv(const void* q, const void* k, const void* v, i
                                   int64_t v_token_stride, int64_t v_head_stride, void* q_out,
                                   int64_t out_token_stride, int64_t out_head_stride, const void* positions,
                                   int32_t positions_are_64bit, const double* freqs, int32_t rotary_dim,
-                                  int32_t interleaved, float attention_scale, void* k_pages, void* v_pages,
+                                  int32_t interleaved, double attention_scale, void* k_pages, void* v_pages,
                                   uint8_t* k4_pages, void* kmeta, const int32_t* qo_indptr, const int32_t* kv_indptr,
                                   const int32_t* kv_indices, const int32_t* kv_last_page_len, int32_t num_tokens,
                                   int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t num_pages_total,
@@ -294,7 +369,7 @@ extern "C" int twl_rope_append_kv(const void* q, const void* k, const void* v, i
       num_q_heads % num_kv_heads != 0)
     return TWL_ERR_BAD_ARG;
   if (rotary_dim < 0 || (rotary_dim > 0 && !freqs)) return TWL_ERR_BAD_ARG;
-  if (rotary_dim > kD || rotary_dim % 8 != 0) return TWL_ERR_UNSUPPORTED;
+  if (rotary_dim > kD || rotary_dim % (interleaved ? 8 : 16) != 0) return TWL_ERR_UNSUPPORTED;
   if (!strides_ok(q, q_token_stride, q_head_stride) || !strides_ok(k, k_token_stride, k_head_stride) ||
       !strides_ok(v, v_token_stride, v_head_stride) || !strides_ok(q_out, out_token_stride, out_head_stride) ||
       !aligned(k_pages, 16) || !aligned(v_pages, 16) || (k4_pages && !aligned(k4_pages, 16)) ||
@@ -302,28 +377,33 @@ extern "C" int twl_rope_append_kv(const void* q, const void* k, const void* v, i
     return TWL_ERR_MISALIGNED;
   if (dtype != TWL_F16 && dtype != TWL_BF16) return TWL_ERR_UNSUPPORTED;
   const int64_t slots = (int64_t)num_tokens / kPage + 2 * (int64_t)batch;
-  const int64_t tasks = 2 * (int64_t)num_kv_heads + num_q_heads;
-  if (slots > 0x7fffffffLL || tasks > 65535LL * kRopeWarps) return TWL_ERR_TOO_LARGE;
+  if (slots > 0x7fffffffLL || num_kv_heads > 65535) return TWL_ERR_TOO_LARGE;
   RopeParams p;
   p.q = q; p.k = k; p.v = v; p.q_out = q_out;
   p.q_ts = q_token_stride; p.q_hs = q_head_stride; p.k_ts = k_token_stride; p.k_hs = k_head_stride;
   p.v_ts = v_token_stride; p.v_hs = v_head_stride; p.o_ts = out_token_stride; p.o_hs = out_head_stride;
   p.positions = positions; p.pos64 = positions_are_64bit; p.freqs = freqs; p.rotary = rotary_dim;
-  p.interleaved = interleaved; p.attn_scale = attention_scale;
+  p.attn_scale = attention_scale;
   p.k_pages = k_pages; p.v_pages = v_pages; p.k4 = k4_pages; p.kmeta = kmeta;
   p.qo_indptr = qo_indptr; p.indptr = kv_indptr; p.indices = kv_indices; p.last_len = kv_last_page_len;
   p.status = status; p.batch = batch; p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.num_tokens = num_tokens;
   p.num_pages_total = num_pages_total;
-  // One task per warp while that leaves every block resident at once (decode: latency), two where there is
-  // work for several waves (the sines of a page are then computed half as often).
-  const int64_t fine = (tasks + kRopeWarps - 1) / kRopeWarps;
-  p.tasks_per_block = slots * fine <= (int64_t)num_sms() * 6 ? kRopeWarps : 2 * kRopeWarps;
-  const dim3 grid((unsigned)slots, (unsigned)((tasks + p.tasks_per_block - 1) / p.tasks_per_block));
+  const auto wide = [](const void* x, int64_t ts, int64_t hs) { return aligned(x, 16) && ts % 8 == 0 && hs % 8 == 0; };
+  p.wide = wide(q, q_token_stride, q_head_stride) && wide(k, k_token_stride, k_head_stride) &&
+           wide(v, v_token_stride, v_head_stride) && wide(q_out, out_token_stride, out_head_stride);
+  // One KV head (with its query heads) a block while there are fewer blocks than eight per SM (decode: latency), then
+  // more, up to eight: the sines of a page are computed once per block.
+  const int64_t room = (int64_t)num_sms() * 8;
+  int64_t heads = (slots * num_kv_heads + room - 1) / room;
+  heads = heads < 1 ? 1 : heads > kRopeWarps ? kRopeWarps : heads;
+  p.heads_per_block = (int32_t)(heads < num_kv_heads ? heads : num_kv_heads);
+  const dim3 grid((unsigned)slots, (unsigned)((num_kv_heads + p.heads_per_block - 1) / p.heads_per_block));
+  const dim3 block(kRopeWarps * 32);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == TWL_F16)
-    TWL_CUDA_TRY(launch_chain(rope_append_kernel<__half>, grid, dim3(kRopeWarps * 32), 0, st, p));
-  else
-    TWL_CUDA_TRY(launch_chain(rope_append_kernel<__nv_bfloat16>, grid, dim3(kRopeWarps * 32), 0, st, p));
+  auto* kernel = dtype == TWL_F16 ? (interleaved ? rope_append_kernel<__half, true> : rope_append_kernel<__half, false>)
+                                  : (interleaved ? rope_append_kernel<__nv_bfloat16, true>
+                                                 : rope_append_kernel<__nv_bfloat16, false>);
+  TWL_CUDA_TRY(launch_chain(kernel, grid, block, 0, st, p));
   return TWL_OK;
 }
 

@@ -7,15 +7,17 @@
 //   P = 2^(S c - m)    one softmax thread per row: S from TMEM, running maximum and sum in registers, P back to TMEM
 //   O += P V           tcgen05.mma, P from TMEM, V in shared memory as it lies in the cache (keys x channels)
 // The two subtiles share K and V and alternate on the tensor cores: while one subtile's weights are computed, the
-// other's products run.  TMEM (512 columns): S of both subtiles (P takes the place of S once it is read), O of both.
+// other's products run.  An item of one subtile takes both places: they take its key tiles in turn, and their results
+// are joined at the end.  TMEM (512 columns): S of both (P takes the place of S once it is read), O of both.
 // The reference maximum m of a row is only moved when the true one has grown by more than 2^8, so O is rescaled a
 // few times per row; weights then stay below 2^8, which fp16 and the fp32 sums hold without loss.
 //
-// Warps: 0-3 and 4-7 softmax of subtile 0 and 1, 8 page loads (TMA: a page is two boxes of 16 rows x 128 bytes, issued by
-// sixteen lanes), 9 tensor-core issue (10 and 11 only complete the warpgroup).  K and V tiles share a ring of five 32 KiB stages.
+// Warps: 0-3 and 4-7 softmax, 8 page loads (TMA: a page is two boxes of 16 rows x 128 bytes, issued by sixteen lanes),
+// 9 tensor-core issue, 10 work items (taken from a counter, two ahead).  K and V tiles share a ring of five 32 KiB stages.
 //
 // Bound: two products of 128 x 128 x 128 (512 clocks each at the tensor peak) and 128 x 128 exponentials per subtile and
-// step; with few rows per KV head, reading K and V.
+// step (1024 clocks of the special-function units, were they to do all of them); with few rows per KV head, reading
+// K and V.
 #include <cuda.h>
 
 #include <type_traits>
@@ -31,6 +33,7 @@ constexpr int kStages = 5;
 constexpr int kStageBytes = 128 * kD * 2;      // 128 keys (or 128 query rows)
 constexpr int kHalfBytes = kStageBytes / 2;    // 64 channels of 128 rows
 constexpr int kInfoSlots = 8;                  // key tiles whose positions are kept
+constexpr int kPolyOf = 8, kPolyTake = 2;        // of eight pairs of exponentials, how many take the polynomial
 constexpr uint32_t kWaitLimit = 1u << 31;      // clocks (about a second)
 
 struct alignas(64) TileParams {
@@ -38,14 +41,32 @@ struct alignas(64) TileParams {
   AttnParams a;
 };
 
+// One work item as every role of the block sees it; n_tiles < 0 ends the block.
+struct Item {
+  const int32_t* indices;  // the segment's part of its page table
+  const int32_t* list;     // block list from the item's first page on, or null
+  int64_t part0;           // partial row of its first token and query head 0, or -1
+  int32_t tok0, ntok, kvh; // first token
+  int32_t page0;           // first page (without a list)
+  int32_t npages, len;     // of the segment
+  int32_t limit0;          // last position the first token sees (all tokens, when not causal)
+  int32_t n_pages;
+  int32_t n_tiles;         // key tiles of the item
+  int32_t steps[2];        // and of its two subtiles
+  int32_t pair;            // one subtile in both places: key tile 2j + a is step j of place a
+};
+
 struct TileShared {
-  uint64_t q_full, q_free, kv_full[kStages], kv_empty[kStages], s_full[2], p_full[2], o_full[2], drain;
+  uint64_t item_full[2], item_empty[2];
+  uint64_t q_full, q_free, kv_full[kStages], kv_empty[kStages], s_full[2], p_half[2], p_full[2], o_full[2], pair[2], drain;
+  Item items[2];
   uint32_t tmem;
   int32_t hi[kInfoSlots];      // largest position of the tile's keys, INT_MAX when a page is missing
   int32_t tail[kInfoSlots];    // which of its pages the sequence ends in, -1 for none
   int32_t pos[kInfoSlots][8];  // position of every page's first key
+  float2 ml[2][128];           // results of the two places of a pair
 };
-constexpr int kTileSmem = 2 * kStageBytes + kStages * kStageBytes + 1024 + (int)sizeof(TileShared);
+constexpr int kTileSmem = 2 * kStageBytes + kStages * kStageBytes + (int)sizeof(TileShared);
 static_assert(kTileSmem <= 232448, "shared memory of a block");
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -154,57 +175,105 @@ __device__ __forceinline__ float tile_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-template <typename T>
-__device__ __forceinline__ uint32_t tile_pack2(float a, float b) {
-  typename Elem<T>::T2 v;
-  v.x = Elem<T>::from_f(a);
-  v.y = Elem<T>::from_f(b);
-  return *reinterpret_cast<uint32_t*>(&v);
+__device__ __forceinline__ uint32_t tile_pack2(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t tile_pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// two fp32 values to an instruction
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void f2_split(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// (a NaN goes on: the row's reference, and with it the row, becomes NaN)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two values on the multiply-add pipes: x = n + f with n the nearest integer (left in the low bits by adding
+// 1.5 * 2^23), 2^f on [-1/2, 1/2] by the degree-4 polynomial of least largest relative error (2.7e-6, Remez exchange),
+// n added to the exponent.  Results below 2^-126 become 2^-126.
+__device__ __forceinline__ void exp2_poly(uint64_t x, float& a, float& b) {
+  float x0, x1;
+  f2_split(x, x0, x1);
+  x = f2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+  const uint64_t big = f2(12582912.f, 12582912.f), minus_big = f2(-12582912.f, -12582912.f);
+  const uint64_t n = add2(x, big);
+  const uint64_t f = fma2(add2(n, minus_big), f2(-1.f, -1.f), x);
+  uint64_t y = f2(9.570102207362652e-3f, 9.570102207362652e-3f);
+  y = fma2(y, f, f2(5.591785907745361e-2f, 5.591785907745361e-2f));
+  y = fma2(y, f, f2(0.240247443318367f, 0.240247443318367f));
+  y = fma2(y, f, f2(0.6931217908859253f, 0.6931217908859253f));
+  y = fma2(y, f, f2(0.9999992847442627f, 0.9999992847442627f));
+  float y0, y1, n0, n1;
+  f2_split(y, y0, y1);
+  f2_split(n, n0, n1);
+  a = __int_as_float(__float_as_int(y0) + (__float_as_int(n0) << 23));
+  b = __int_as_float(__float_as_int(y1) + (__float_as_int(n1) << 23));
 }
 
-// One work item as every role of the block sees it.
-struct Item {
-  Segment s;
-  const int32_t* list;  // block list, or null
-  int t0, ntok, chunk, kvh;
-  int first, n_pages;   // its pages: numbers first .. first + n_pages of the segment's (or of the list)
-  int steps[2];         // key tiles of the two subtiles
-};
 __device__ __forceinline__ Item load_item(const AttnParams& p, int i) {
   Item it;
   const int4 w = p.tile_list[i / p.Hkv];
   it.kvh = i % p.Hkv;
-  it.s = p.segs[w.x];
-  it.t0 = w.y;
+  const Segment s = p.segs[w.x];
+  it.indices = (s.second ? p.indices2 : p.indices1) + s.kvbase;
+  it.tok0 = s.tok0 + w.y;
   it.ntok = w.z;
-  it.chunk = w.w;
+  it.page0 = w.w * s.chunk_pages;  // (a chunk that is everything: number 0)
+  it.npages = s.npages;
+  it.len = s.len;
+  it.limit0 = p.causal ? s.len - s.ntok + w.y : s.len - 1;
+  it.part0 = s.pbase < 0 ? -1 : s.pbase + ((int64_t)w.w * s.ntok + w.y) * p.Hq;
   it.list = nullptr;
   int avail = 0;
   if (p.block_pages) {
-    const int64_t slot = (int64_t)(it.s.tok0 / p.query_block + w.x + it.t0 / p.query_block) * p.Hkv + it.kvh;
-    it.list = p.block_pages + slot * p.max_k;
+    const int64_t slot = (int64_t)(s.tok0 / p.query_block + w.x + w.y / p.query_block) * p.Hkv + it.kvh;
+    it.list = p.block_pages + slot * p.max_k + it.page0;
     avail = min(max(p.block_npages[slot], 0), p.max_k);
   }
-  it.first = it.chunk * it.s.chunk_pages;
   it.n_pages = 0;
 #pragma unroll
   for (int a = 0; a < 2; ++a) {
     const int n = min(it.ntok - a * p.tok_tile, p.tok_tile);
     int pages = 0;
     if (n > 0) {
-      if (!it.list) avail = pages_seen(it.s, it.t0 + a * p.tok_tile + n - 1, p.causal);
-      pages = max(0, min(avail - it.first, it.s.chunk_pages));
+      if (!it.list) avail = pages_seen(s, w.y + a * p.tok_tile + n - 1, p.causal);
+      pages = max(0, min(avail - it.page0, s.chunk_pages));
     }
     it.steps[a] = (pages + 7) >> 3;
     it.n_pages = max(it.n_pages, pages);
+  }
+  it.n_tiles = max(it.steps[0], it.steps[1]);
+  it.pair = it.ntok <= p.tok_tile && it.n_tiles > 1;
+  if (it.pair) {
+    it.steps[0] = (it.n_tiles + 1) >> 1;
+    it.steps[1] = it.n_tiles >> 1;
   }
   return it;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __grid_constant__ TileParams tp) {
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t smem[];  // swizzle atoms of 1024 bytes
   uint8_t* q_s = smem;
   uint8_t* kv_s = smem + 2 * kStageBytes;
   TileShared& sh = *reinterpret_cast<TileShared*>(smem + (2 + kStages) * kStageBytes);
@@ -219,9 +288,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       mbar_init(&sh.kv_empty[i], 1);
     }
     for (int a = 0; a < 2; ++a) {
+      mbar_init(&sh.item_full[a], 1);
+      mbar_init(&sh.item_empty[a], 10);  // loads, tensor cores, eight softmax warps
       mbar_init(&sh.s_full[a], 1);
+      mbar_init(&sh.p_half[a], 128);
       mbar_init(&sh.p_full[a], 128);
       mbar_init(&sh.o_full[a], 1);
+      mbar_init(&sh.pair[a], 256);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -235,20 +308,50 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   pdl_wait();
-  const int n_items = p.hdr->tile_items * p.Hkv;
   bool ok = true;
+  uint32_t n_item = 0;  // items so far: slot n_item & 1 of the two
+  // The next item, copied out of its slot; false at the end (or when a wait ran out: ok is false then).
+  const auto next_item = [&](Item& it) {
+    const int s = n_item & 1;
+    ok = mbar_wait(&sh.item_full[s], (n_item >> 1) & 1);
+    if (!ok) return false;
+    it = sh.items[s];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.item_empty[s]);
+    ++n_item;
+    return it.n_tiles >= 0;
+  };
   if (warp >= 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
 
-  if (warp == 8) {
-    // ---- loads ----
+  if (warp == 10) {
+    // ---- work items ----
+    const int n_items = p.hdr->tile_items * p.Hkv;
+    for (int i = blockIdx.x;; ++n_item) {
+      Item it;
+      if (i < n_items)
+        it = load_item(p, i);
+      else
+        it.n_tiles = -1;
+      const int s = n_item & 1;
+      ok = mbar_wait(&sh.item_empty[s], ((n_item >> 1) & 1) ^ 1);
+      if (!ok) break;
+      if (lane == 0) {
+        sh.items[s] = it;
+        mbar_arrive(&sh.item_full[s]);
+      }
+      __syncwarp();
+      if (i >= n_items) break;
+      if (lane == 0) i = gridDim.x + atomicAdd(&p.hdr->next_tile, 1);
+      i = __shfl_sync(0xffffffffu, i, 0);
+    }
+  } else if (warp == 8) {
+    // ---- loads: K of the first tile (of the first two of a pair), then V of tile t and K of the tile that follows ----
     uint32_t stage = 0, round = 0, q_round = 0;
     uint32_t tiles = 0;  // key tiles so far, over all items
-    uint32_t used = 0;  // stages filled so far, at most kStages: what an early end has to wait for
+    uint32_t used = 0;   // stages filled so far, at most kStages: what an early end has to wait for
     const int page_of_lane = (lane & 15) >> 1, half = lane & 1;
     const int gone = p.num_pages_total * p.Hkv * kPage;  // a row behind the pool: reads as zeros
-    auto put = [&](const CUtensorMap* map, int row) {
-      ok = mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1);
-      if (!ok) return;
+    const auto put = [&](const CUtensorMap* map, int row) {
       if (lane == 0) mbar_expect(&sh.kv_full[stage], kStageBytes);
       __syncwarp();
       if (lane < 16)
@@ -260,12 +363,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
         ++round;
       }
     };
-    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
-      const Item it = load_item(p, i);
-      const int32_t* indices = (it.s.second ? p.indices2 : p.indices1) + it.s.kvbase;
-      const int steps = max(it.steps[0], it.steps[1]);
-      if (steps == 0) continue;
-      const int subs = it.steps[1] > 0 ? 2 : 1;
+    Item it;
+    while (next_item(it)) {
+      if (it.n_tiles == 0) continue;
+      const int subs = it.ntok > p.tok_tile ? 2 : 1;
       ok = mbar_wait(&sh.q_free, (q_round & 1) ^ 1);
       if (!ok) break;
       ++q_round;
@@ -273,151 +374,198 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
         mbar_expect(&sh.q_full, (uint32_t)(subs * 2 * 64 * 2 * p.G * p.tok_tile));
         for (int a = 0; a < subs; ++a)
           for (int h = 0; h < 2; ++h)
-            tma_3d(smem_u32(q_s) + a * kStageBytes + h * kHalfBytes, &tp.tq, h * 64, it.kvh * p.G,
-                   it.s.tok0 + it.t0 + a * p.tok_tile, &sh.q_full);
+            tma_3d(smem_u32(q_s) + a * kStageBytes + h * kHalfBytes, &tp.tq, h * 64, it.kvh * p.G, it.tok0 + a * p.tok_tile,
+                   &sh.q_full);
       }
       __syncwarp();
-      auto look_up = [&](int j, int& lp, int& phys) {
+      const auto look_up = [&](int j, int& lp, int& phys) {
         const int at = 8 * j + page_of_lane;
         lp = -1;
         phys = -1;
-        if (j < steps && at < it.n_pages) {
-          lp = it.list ? it.list[it.first + at] : it.first + at;
-          if (lp >= 0 && lp < it.s.npages) phys = indices[lp];
+        if (at < it.n_pages) {
+          lp = it.list ? it.list[at] : it.page0 + at;
+          if (lp >= 0 && lp < it.npages) phys = it.indices[lp];
           if (phys < 0 || phys >= p.num_pages_total) {
             phys = -1;
             raise_flag(p.status, TWL_FLAG_BAD_INDEX);
           }
         }
       };
-      int lp, phys, lp_next, phys_next;
+      const int lead = it.pair ? 2 : 1;
+      int rows[3];  // pool rows of this lane's page of tiles whose K is loaded and V is not: the oldest first
+      int lp, phys;
       look_up(0, lp, phys);
-      for (int j = 0; j < steps && ok; ++j) {
-        look_up(j + 1, lp_next, phys_next);
-        const int row = phys < 0 ? gone : (phys * p.Hkv + it.kvh) * kPage;
-        const int pos = phys < 0 ? 0x3fffffff : lp * kPage;
-        const int hi = __reduce_max_sync(0xffffffffu, phys < 0 ? 0x7fffffff : pos + kPage - 1);
-        const bool last = phys >= 0 && lp == it.s.npages - 1 && (it.s.len & (kPage - 1)) != 0;
-        const uint32_t tail = __ballot_sync(0xffffffffu, last);
-        // Room for K means that V of three tiles ago has been used, so every reader of the info of that tile and of
-        // those before it is done: of the eight slots three are still in use.
-        ok = mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1);
-        if (!ok) break;
-        const int slot = tiles++ & (kInfoSlots - 1);
-        if (lane < 16 && half == 0) sh.pos[slot][page_of_lane] = pos;
-        if (lane == 0) {
-          sh.hi[slot] = hi;
-          sh.tail[slot] = tail ? (__ffs(tail) - 1) >> 1 : -1;
+      for (int k = 0; k < it.n_tiles + lead && ok; ++k) {
+        if (k < it.n_tiles) {  // K of tile k
+          const int row = phys < 0 ? gone : (phys * p.Hkv + it.kvh) * kPage;
+          const int pos = phys < 0 ? 0x3fffffff : lp * kPage;
+          const int hi = __reduce_max_sync(0xffffffffu, phys < 0 ? 0x7fffffff : pos + kPage - 1);
+          const bool last = phys >= 0 && lp == it.npages - 1 && (it.len & (kPage - 1)) != 0;
+          const uint32_t tail = __ballot_sync(0xffffffffu, last);
+          look_up(k + 1, lp, phys);
+          // Room for K means that V of at least three tiles ago has been used, so every reader of the info of that tile
+          // and of those before it is done: of the eight slots four are still in use.
+          ok = mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1);
+          if (!ok) break;
+          const int slot = tiles++ & (kInfoSlots - 1);
+          if (lane < 16 && half == 0) sh.pos[slot][page_of_lane] = pos;
+          if (lane == 0) {
+            sh.hi[slot] = hi;
+            sh.tail[slot] = tail ? (__ffs(tail) - 1) >> 1 : -1;
+          }
+          __syncwarp();
+          put(&tp.tk, row);
+          rows[2] = row;
         }
-        __syncwarp();
-        put(&tp.tk, row);
-        if (ok) put(&tp.tv, row);
-        lp = lp_next;
-        phys = phys_next;
+        if (k + 1 >= lead && k + 1 - lead < it.n_tiles) {  // V of tile k + 1 - lead
+          ok = mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1);
+          if (!ok) break;
+          put(&tp.tv, it.pair ? rows[1] : rows[2]);
+        }
+        rows[0] = rows[1];
+        rows[1] = rows[2];
       }
     }
     if (!ok) {  // an early end: the copies in flight still write to shared memory
       for (uint32_t s = 0; s < used; ++s) mbar_wait(&sh.kv_full[s], (s < stage ? round : round - 1) & 1);
       if (q_round) mbar_wait(&sh.q_full, (q_round - 1) & 1);
+      ok = false;
     }
   } else if (warp == 9) {
     // ---- tensor cores ----
-    uint32_t stage = 0, round = 0, q_round = 0, p_round[2] = {0, 0}, tiles = 0;
+    uint32_t stage = 0, round = 0, q_round = 0, p_rounds = 0, tiles = 0;  // p_rounds: bit a is place a's parity
     const uint32_t kS = mma_desc<T>(false), kO = mma_desc<T>(true);
     const uint32_t q_a = smem_u32(q_s), kv_a = smem_u32(kv_s);
-    auto next = [&]() {
+    const auto next = [&]() {
       if (++stage == kStages) {
         stage = 0;
         ++round;
       }
     };
-    auto scores = [&](int a, uint32_t k_stage) {  // S = Q K^T
+    const auto scores = [&](int a, uint32_t q_at) {  // S = Q K^T with the K of the current stage
       if (lane == 0) {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const uint32_t off = (ks >> 2) * kHalfBytes + (ks & 3) * 32;
-          mma_ss(tmem + a * 128, smem_desc(q_a + a * kStageBytes + off, 16, 1024),
-                 smem_desc(kv_a + k_stage * kStageBytes + off, 16, 1024), kS, ks > 0);
+          mma_ss(tmem + a * 128, smem_desc(q_at + off, 16, 1024), smem_desc(kv_a + stage * kStageBytes + off, 16, 1024), kS,
+                 ks > 0);
         }
         mma_commit(&sh.s_full[a]);
       }
       __syncwarp();
     };
-    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
-      const Item it = load_item(p, i);
-      const int steps = max(it.steps[0], it.steps[1]);
-      if (steps == 0) continue;
+    const auto commit = [&](uint64_t* bar) {
+      if (lane == 0) mma_commit(bar);
+      __syncwarp();
+    };
+    // O += P V in two halves of 64 keys: the first starts while the softmax works on the second
+    const auto values = [&](int a, uint32_t v_stage, bool add) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        ok = mbar_wait(h ? &sh.p_full[a] : &sh.p_half[a], (p_rounds >> a) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        if (lane == 0) {
+#pragma unroll
+          for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
+            mma_ts(tmem + 256 + a * 128, tmem + a * 128 + ks * 8,
+                   smem_desc(kv_a + v_stage * kStageBytes + ks * 2048, kHalfBytes, 1024), kO, add || ks > 0);
+        }
+        __syncwarp();
+      }
+      p_rounds ^= 1u << a;
+    };
+    const auto wait_kv = [&]() {
+      ok = mbar_wait(&sh.kv_full[stage], round & 1);
+      tc_fence_after();
+      return ok;
+    };
+    const auto clean_tail = [&](const Item& it, uint32_t v_stage) {
+      const int tail = sh.tail[tiles++ & (kInfoSlots - 1)];
+      if (tail < 0) return;
+      // rows behind the sequence's end may hold anything, and 0 x NaN is not 0
+      const int r0 = it.len & (kPage - 1);
+      uint4* page = reinterpret_cast<uint4*>(kv_s + v_stage * kStageBytes + tail * 2048);
+      for (int c = r0 * 8 + lane; c < kPage * 8; c += 32) {
+        page[c] = make_uint4(0, 0, 0, 0);
+        page[kHalfBytes / 16 + c] = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    };
+    Item it;
+    while (next_item(it)) {
+      if (it.n_tiles == 0) continue;
       ok = mbar_wait(&sh.q_full, q_round & 1);
       if (!ok) break;
       ++q_round;
-      ok = mbar_wait(&sh.kv_full[stage], round & 1);
-      if (!ok) break;
-      tc_fence_after();
-      if (it.steps[0] > 0) scores(0, stage);
-      if (it.steps[1] > 0) scores(1, stage);
-      if (lane == 0) {
-        mma_commit(&sh.kv_empty[stage]);
-        if (steps == 1) mma_commit(&sh.q_free);
-      }
-      __syncwarp();
-      next();
-      for (int j = 0; j < steps && ok; ++j) {
-        const uint32_t v_stage = stage;
-        ok = mbar_wait(&sh.kv_full[v_stage], round & 1);
-        if (!ok) break;
+      if (!wait_kv()) break;
+      if (it.pair) {
+        scores(0, q_a);
+        commit(&sh.kv_empty[stage]);
         next();
-        const int tail = sh.tail[tiles++ & (kInfoSlots - 1)];
-        if (tail >= 0) {
-          // rows behind the sequence's end may hold anything, and 0 x NaN is not 0
-          const int r0 = it.s.len & (kPage - 1);
-          uint4* page = reinterpret_cast<uint4*>(kv_s + v_stage * kStageBytes + tail * 2048);
-          for (int c = r0 * 8 + lane; c < kPage * 8; c += 32) {
-            page[c] = make_uint4(0, 0, 0, 0);
-            page[kHalfBytes / 16 + c] = make_uint4(0, 0, 0, 0);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-        }
-        bool k_here = false;
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          if (j >= it.steps[a]) continue;
-          ok = mbar_wait(&sh.p_full[a], p_round[a] & 1);
+        if (!wait_kv()) break;
+        scores(1, q_a);
+        commit(&sh.kv_empty[stage]);
+        if (it.n_tiles == 2) commit(&sh.q_free);
+        next();
+        for (int t = 0; t < it.n_tiles && ok; ++t) {
+          const int a = t & 1;
+          if (!wait_kv()) break;
+          const uint32_t v_stage = stage;
+          next();
+          clean_tail(it, v_stage);
+          values(a, v_stage, t > 1);
           if (!ok) break;
-          ++p_round[a];
-          tc_fence_after();
-          if (lane == 0) {
+          commit(&sh.kv_empty[v_stage]);
+          if (t + 2 < it.n_tiles) {
+            if (!wait_kv()) break;
+            scores(a, q_a);
+            commit(&sh.kv_empty[stage]);
+            next();
+            if (t + 3 == it.n_tiles) commit(&sh.q_free);  // the last product with Q has been issued
+          } else {
+            commit(&sh.o_full[a]);
+          }
+        }
+      } else {
+        if (it.steps[0] > 0) scores(0, q_a);
+        if (it.steps[1] > 0) scores(1, q_a + kStageBytes);
+        commit(&sh.kv_empty[stage]);
+        if (it.n_tiles == 1) commit(&sh.q_free);
+        next();
+        for (int j = 0; j < it.n_tiles && ok; ++j) {
+          if (!wait_kv()) break;
+          const uint32_t v_stage = stage;
+          next();
+          clean_tail(it, v_stage);
+          const int last = j < it.steps[1] ? 1 : 0;  // the subtile that uses this V last
+          bool k_here = false;
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-              mma_ts(tmem + 256 + a * 128, tmem + a * 128 + ks * 8,
-                     smem_desc(kv_a + v_stage * kStageBytes + ks * 2048, kHalfBytes, 1024), kO, j > 0 || ks > 0);
-          }
-          __syncwarp();
-          if (j + 1 < it.steps[a]) {
-            if (!k_here) {
-              ok = mbar_wait(&sh.kv_full[stage], round & 1);
-              if (!ok) break;
+          for (int a = 0; a < 2; ++a) {
+            if (j >= it.steps[a]) continue;
+            values(a, v_stage, j > 0);
+            if (!ok) break;
+            if (a == last) commit(&sh.kv_empty[v_stage]);
+            if (j + 1 < it.steps[a]) {
+              if (!k_here && !wait_kv()) break;
               k_here = true;
-              tc_fence_after();
+              scores(a, q_a + a * kStageBytes);
+            } else {
+              commit(&sh.o_full[a]);
             }
-            scores(a, stage);
-          } else if (lane == 0) {
-            mma_commit(&sh.o_full[a]);
+          }
+          if (!ok) break;
+          if (k_here) {
+            commit(&sh.kv_empty[stage]);
+            if (j + 2 == it.n_tiles) commit(&sh.q_free);  // the last product with Q has been issued
+            next();
           }
         }
-        if (!ok) break;
-        if (lane == 0) {
-          mma_commit(&sh.kv_empty[v_stage]);
-          if (k_here) mma_commit(&sh.kv_empty[stage]);
-          if (j + 2 == steps) mma_commit(&sh.q_free);  // the last product with Q has been issued
-        }
-        __syncwarp();
-        if (k_here) next();
       }
     }
     if (!ok) {  // an early end: products in flight still read shared memory and write TMEM
-      if (lane == 0) mma_commit(&sh.drain);
-      __syncwarp();
+      commit(&sh.drain);
       mbar_wait(&sh.drain, 0);
     }
   } else if (warp < 8) {
@@ -426,52 +574,58 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
     const int a = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane of the warp's first row
     const uint32_t s_t = tmem + lanes + a * 128, o_t = tmem + lanes + 256 + a * 128;
-    uint32_t s_round = 0, o_round = 0, tiles = 0;
+    uint32_t s_round = 0, o_own = 0, o_other = 0, tiles = 0, pairs = 0;
     const int tok_r = r / p.G, head_r = r - tok_r * p.G;
-    for (int i = blockIdx.x; i < n_items && ok; i += gridDim.x) {
-      const Item it = load_item(p, i);
-      const int tok = it.t0 + a * p.tok_tile + tok_r;
-      const bool real = tok_r < p.tok_tile && a * p.tok_tile + tok_r < it.ntok;
-      const int limit = !real ? -1 : p.causal ? it.s.len - it.s.ntok + tok : it.s.len - 1;
+    const float scale = p.scale_log2;
+    for (;; ++n_item) {
+      // (read in place and given back at the end: a copy would hold registers that a row of scores needs)
+      const Item& it = sh.items[n_item & 1];
+      ok = mbar_wait(&sh.item_full[n_item & 1], (n_item >> 1) & 1);
+      if (!ok || it.n_tiles < 0) break;
+      const int pair = it.pair;
+      const int tok = (pair ? 0 : a * p.tok_tile) + tok_r;  // of the item
+      const bool real = tok_r < p.tok_tile && tok < it.ntok;
+      const int limit = !real ? -1 : p.causal ? it.limit0 + tok : it.limit0;
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < it.steps[a]; ++j) {
+      const int steps = a ? it.steps[1] : it.steps[0], steps_other = a ? it.steps[0] : it.steps[1];
+      for (int j = 0; j < steps; ++j) {
         ok = mbar_wait(&sh.s_full[a], s_round & 1);
         if (!ok) break;
         ++s_round;
         tc_fence_after();
-        const int slot = (tiles + j) & (kInfoSlots - 1);
+        const int slot = (tiles + (pair ? 2 * j + a : j)) & (kInfoSlots - 1);
         float x[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(x + 32 * c, s_t + 32 * c);
+        const bool masked = __any_sync(0xffffffffu, real && sh.hi[slot] > limit);
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_wait_ld32(x + 32 * c);
-        if (sh.hi[slot] > limit) {
+        if (masked) {
 #pragma unroll
           for (int pg = 0; pg < 8; ++pg) {
-            const int first = sh.pos[slot][pg];
+            const int n = limit - sh.pos[slot][pg];  // keys 0..n of the page are seen
 #pragma unroll
             for (int c = 0; c < kPage; ++c)
-              if (first + c > limit) x[16 * pg + c] = -INFINITY;
+              if (c > n) x[16 * pg + c] = -INFINITY;
           }
         }
-        __syncwarp();
-        float mx[4];
+        float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(x[c], x[c + 4]);
+        for (int c = 4; c < 124; c += 8)
 #pragma unroll
-        for (int c = 8; c < 128; c += 4)
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[c + e], x[c + 4 + e]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], x[c + e]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        for (int e = 0; e < 4; e += 2) mx[e] = max3(max3(mx[e], mx[e + 1], x[124 + e]), x[125 + e], mx[e]);
+        const float top = max3(mx[0], mx[2], mx[2]) * scale;
         // move the reference only when it is 2^8 behind (or nothing was seen so far)
         float f = 1.f;
-        const bool move = top > m + 8.f;  // from -inf: any finite maximum
+        const bool move = !(top <= m + 8.f);  // from -inf: any finite maximum
         if (move) {
           f = tile_ex2(m - top);
           m = top;
           l *= f;
         }
-        if (j > 0 && __any_sync(0xffffffffu, move)) {
+        if (__any_sync(0xffffffffu, move) && j > 0) {
           // S of this step is complete, so the product of the step before is too: O may be changed
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -485,41 +639,68 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
           }
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = f2(scale, scale), ref2 = f2(-ref, -ref);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t w[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            const float a0 = tile_ex2(fmaf(x[64 * c + 2 * e], p.scale_log2, -ref));
-            const float a1 = tile_ex2(fmaf(x[64 * c + 2 * e + 1], p.scale_log2, -ref));
-            sum[(2 * e) & 3] += a0;
-            sum[(2 * e + 1) & 3] += a1;
+            const uint64_t y = fma2(f2(x[64 * c + 2 * e], x[64 * c + 2 * e + 1]), scale2, ref2);
+            float a0, a1;
+            if (e % kPolyOf < kPolyTake && !masked) {
+              exp2_poly(y, a0, a1);
+            } else {
+              f2_split(y, a0, a1);
+              a0 = tile_ex2(a0);
+              a1 = tile_ex2(a1);
+            }
+            sum[e & 1] = add2(sum[e & 1], f2(a0, a1));
             // weights go to the tensor cores in the model type (half a step of it each); their sum stays unrounded
-            w[e] = tile_pack2<T>(a0, a1);
+            w[e] = tile_pack2(a0, a1, T());
           }
           tmem_st32(s_t + 32 * c, w);
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(c ? &sh.p_full[a] : &sh.p_half[a]);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(&sh.p_full[a]);
+        float s0, s1;
+        f2_split(add2(sum[0], sum[1]), s0, s1);
+        l += s0 + s1;
       }
       if (!ok) break;
-      tiles += max(it.steps[0], it.steps[1]);
-      const bool any = it.steps[a] > 0;
-      if (any) {
-        ok = mbar_wait(&sh.o_full[a], o_round & 1);
+      tiles += it.n_tiles;
+      // ---- the item's rows: columns c0 .. of O, of both places of a pair ----
+      const bool any = steps > 0;
+      float f_own = 1.f, f_other = 0.f;
+      if (pair) {
+        sh.ml[a][r] = make_float2(m, l);
+        mbar_arrive(&sh.pair[0]);
+        ok = mbar_wait(&sh.pair[0], pairs & 1);
         if (!ok) break;
-        ++o_round;
-        tc_fence_after();
+        const float2 v = sh.ml[a ^ 1][r];
+        const float mm = fmaxf(m, v.x), ref = mm == -INFINITY ? 0.f : mm;
+        f_own = tile_ex2(m - ref);
+        f_other = tile_ex2(v.x - ref);
+        l = a ? v.y * f_other + l * f_own : l * f_own + v.y * f_other;  // the same sum in both places
+        m = mm;
+        ok = mbar_wait(&sh.o_full[a ^ 1], o_other & 1);
+        if (!ok) break;
       }
-      const int64_t row = (int64_t)(it.s.tok0 + tok), head = it.kvh * p.G + head_r;
-      const int64_t part = it.s.pbase < 0 ? -1 : it.s.pbase + ((int64_t)it.chunk * it.s.ntok + tok) * p.Hq + head;
+      if (any) {
+        ok = mbar_wait(&sh.o_full[a], o_own & 1);
+        if (!ok) break;
+      }
+      o_own += any;
+      o_other += steps_other > 0;
+      tc_fence_after();
+      const int64_t row = (int64_t)it.tok0 + tok, head = it.kvh * p.G + head_r;
+      const int64_t part = it.part0 < 0 ? -1 : it.part0 + (int64_t)tok * p.Hq + head;
       const bool write = real && (part < 0 || part < p.part_cap);
       const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
+        if (pair && (c >> 1) != a) continue;  // each place writes half of the channels
         float o[32];
         __syncwarp();
         if (any) {
@@ -528,6 +709,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
         } else {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (pair) {
+          float z[32];
+          tmem_ld32(z, tmem + lanes + 256 + (a ^ 1) * 128 + 32 * c);
+          tmem_wait_ld32(z);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = o[e] * f_own + z[e] * f_other;
         }
         if (!write) continue;
         if (part >= 0) {
@@ -543,17 +731,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              w[k] = l != 0.f ? tile_pack2<T>(o[8 * e + 2 * k] * inv, o[8 * e + 2 * k + 1] * inv) : 0u;
+              w[k] = l != 0.f ? tile_pack2(o[8 * e + 2 * k] * inv, o[8 * e + 2 * k + 1] * inv, T()) : 0u;
             to[e] = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
       }
-      if (write) {
+      if (write && !(pair && a)) {
         if (part >= 0)
           p.part_ml[part] = make_float2(m, l);
         else if (p.lse)
           p.lse[row * p.Hq + head] = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
       }
+      // a pair's places have read each other's O (and ml): only then may the next item's products replace it
+      tc_fence_before();
+      if (pair) {
+        mbar_arrive(&sh.pair[1]);
+        ok = mbar_wait(&sh.pair[1], pairs++ & 1);
+        if (!ok) break;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.item_empty[n_item & 1]);
     }
   }
   if (!ok && lane == 0) raise_flag(p.status, TWL_FLAG_WAIT_LIMIT);

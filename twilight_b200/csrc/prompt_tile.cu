@@ -33,8 +33,8 @@ constexpr int kStages = 5;
 constexpr int kStageBytes = 128 * kD * 2;      // 128 keys (or 128 query rows)
 constexpr int kHalfBytes = kStageBytes / 2;    // 64 channels of 128 rows
 constexpr int kInfoSlots = 8;                  // key tiles whose positions are kept
-constexpr int kPolyOf = 8, kPolyTake = 2;        // of eight pairs of exponentials, how many take the polynomial
-constexpr uint32_t kWaitLimit = 1u << 31;      // clocks (about a second)
+constexpr int kPolyTake = 2;                   // of eight pairs of exponentials, how many take the polynomial
+constexpr uint32_t kWaitTries = 2000, kWaitNs = 500000;  // a wait gives up after about a second
 
 struct alignas(64) TileParams {
   CUtensorMap tq, tk, tv;
@@ -53,6 +53,7 @@ struct Item {
   int32_t n_pages;
   int32_t n_tiles;         // key tiles of the item
   int32_t steps[2];        // and of its two subtiles
+  int32_t tail_page;       // page of the last key tile in which the sequence ends inside the page, or -1
   int32_t pair;            // one subtile in both places: key tile 2j + a is step j of place a
 };
 
@@ -62,7 +63,6 @@ struct TileShared {
   Item items[2];
   uint32_t tmem;
   int32_t hi[kInfoSlots];      // largest position of the tile's keys, INT_MAX when a page is missing
-  int32_t tail[kInfoSlots];    // which of its pages the sequence ends in, -1 for none
   int32_t pos[kInfoSlots][8];  // position of every page's first key
   float2 ml[2][128];           // results of the two places of a pair
 };
@@ -79,23 +79,21 @@ __device__ __forceinline__ void mbar_expect(uint64_t* b, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint64_t* b) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
 }
-__device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
+// Bounded wait for the completion of the phase with this parity; false when the limit ran out.  A thread that was refused
+// goes on (with data that is not there yet) to the next all_ok of its warp, so that the warps stay together.
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-      : "=r"(ok) : "r"(smem_u32(b)), "r"(parity) : "memory");
+      "{ .reg .pred p; .reg .u32 n; mov.u32 n, %3;\n"
+      "W: mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n"
+      "@p bra D;\n"
+      "sub.u32 n, n, 1; setp.ne.u32 p, n, 0;\n"
+      "@p bra W;\n"
+      "D: selp.u32 %0, 1, 0, p; }"
+      : "=r"(ok) : "r"(smem_u32(b)), "r"(parity), "n"(kWaitTries), "n"(kWaitNs) : "memory");
   return ok != 0;
 }
-// Bounded wait of a whole warp for the completion of the phase with this parity; false when the limit ran out.
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity) {
-  bool ok = mbar_try(b, parity);
-  if (!ok) {
-    const long long t0 = clock64();
-    do ok = mbar_try(b, parity);
-    while (!ok && clock64() - t0 <= (long long)kWaitLimit);
-  }
-  return __all_sync(0xffffffffu, ok);
-}
+__device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, uint64_t* bar) {
   asm volatile(
@@ -134,6 +132,13 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a),
       "l"(b), "r"(idesc), "r"((uint32_t)add)
       : "memory");
+}
+// One lane of the warp (always the same), in a form that the compiler knows to be a single thread: the operands of what
+// it issues then stay in uniform registers.
+__device__ __forceinline__ bool one_lane() {
+  uint32_t p;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+  return p != 0;
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -230,6 +235,26 @@ __device__ __forceinline__ void exp2_poly(uint64_t x, float& a, float& b) {
   b = __int_as_float(__float_as_int(y1) + (__float_as_int(n1) << 23));
 }
 
+// 64 weights 2^(x scale - ref) of a row: their sum in 32 bits, and themselves rounded to the model type (half a step each),
+// in which they go to the tensor cores.  POLY of eight pairs take the polynomial (never masked ones: it has no zero).
+template <typename T, int POLY>
+__device__ __forceinline__ void weights(const float* x, uint64_t scale, uint64_t ref, uint64_t (&sum)[2], uint32_t (&w)[32]) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) {
+    const uint64_t y = fma2(f2(x[2 * e], x[2 * e + 1]), scale, ref);
+    float a, b;
+    if (e % 8 < POLY) {
+      exp2_poly(y, a, b);
+    } else {
+      f2_split(y, a, b);
+      a = tile_ex2(a);
+      b = tile_ex2(b);
+    }
+    sum[e & 1] = add2(sum[e & 1], f2(a, b));
+    w[e] = tile_pack2(a, b, T());
+  }
+}
+
 __device__ __forceinline__ Item load_item(const AttnParams& p, int i) {
   Item it;
   const int4 w = p.tile_list[i / p.Hkv];
@@ -263,6 +288,10 @@ __device__ __forceinline__ Item load_item(const AttnParams& p, int i) {
     it.n_pages = max(it.n_pages, pages);
   }
   it.n_tiles = max(it.steps[0], it.steps[1]);
+  it.tail_page = -1;
+  if (it.n_pages > 0 && (s.len & (kPage - 1)) != 0 &&
+      (it.list ? it.list[it.n_pages - 1] : it.page0 + it.n_pages - 1) == s.npages - 1)
+    it.tail_page = (it.n_pages - 1) & 7;
   it.pair = it.ntok <= p.tok_tile && it.n_tiles > 1;
   if (it.pair) {
     it.steps[0] = (it.n_tiles + 1) >> 1;
@@ -313,7 +342,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
   // The next item, copied out of its slot; false at the end (or when a wait ran out: ok is false then).
   const auto next_item = [&](Item& it) {
     const int s = n_item & 1;
-    ok = mbar_wait(&sh.item_full[s], (n_item >> 1) & 1);
+    ok = all_ok(mbar_wait(&sh.item_full[s], (n_item >> 1) & 1));
     if (!ok) return false;
     it = sh.items[s];
     __syncwarp();
@@ -333,7 +362,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       else
         it.n_tiles = -1;
       const int s = n_item & 1;
-      ok = mbar_wait(&sh.item_empty[s], ((n_item >> 1) & 1) ^ 1);
+      ok = all_ok(mbar_wait(&sh.item_empty[s], ((n_item >> 1) & 1) ^ 1));
       if (!ok) break;
       if (lane == 0) {
         sh.items[s] = it;
@@ -367,7 +396,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
     while (next_item(it)) {
       if (it.n_tiles == 0) continue;
       const int subs = it.ntok > p.tok_tile ? 2 : 1;
-      ok = mbar_wait(&sh.q_free, (q_round & 1) ^ 1);
+      ok = all_ok(mbar_wait(&sh.q_free, (q_round & 1) ^ 1));
       if (!ok) break;
       ++q_round;
       if (lane == 0) {
@@ -400,25 +429,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
           const int row = phys < 0 ? gone : (phys * p.Hkv + it.kvh) * kPage;
           const int pos = phys < 0 ? 0x3fffffff : lp * kPage;
           const int hi = __reduce_max_sync(0xffffffffu, phys < 0 ? 0x7fffffff : pos + kPage - 1);
-          const bool last = phys >= 0 && lp == it.npages - 1 && (it.len & (kPage - 1)) != 0;
-          const uint32_t tail = __ballot_sync(0xffffffffu, last);
           look_up(k + 1, lp, phys);
           // Room for K means that V of at least three tiles ago has been used, so every reader of the info of that tile
           // and of those before it is done: of the eight slots four are still in use.
-          ok = mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1);
+          ok = all_ok(mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1));
           if (!ok) break;
           const int slot = tiles++ & (kInfoSlots - 1);
           if (lane < 16 && half == 0) sh.pos[slot][page_of_lane] = pos;
-          if (lane == 0) {
-            sh.hi[slot] = hi;
-            sh.tail[slot] = tail ? (__ffs(tail) - 1) >> 1 : -1;
-          }
+          if (lane == 0) sh.hi[slot] = hi;
           __syncwarp();
           put(&tp.tk, row);
           rows[2] = row;
         }
         if (k + 1 >= lead && k + 1 - lead < it.n_tiles) {  // V of tile k + 1 - lead
-          ok = mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1);
+          ok = all_ok(mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1));
           if (!ok) break;
           put(&tp.tv, it.pair ? rows[1] : rows[2]);
         }
@@ -433,9 +457,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
     }
   } else if (warp == 9) {
     // ---- tensor cores ----
-    uint32_t stage = 0, round = 0, q_round = 0, p_rounds = 0, tiles = 0;  // p_rounds: bit a is place a's parity
+    uint32_t stage = 0, round = 0, q_round = 0, p_rounds = 0;  // p_rounds: bit a is place a's parity
     const uint32_t kS = mma_desc<T>(false), kO = mma_desc<T>(true);
-    const uint32_t q_a = smem_u32(q_s), kv_a = smem_u32(kv_s);
+    // operand descriptors of the first query row, of the first stage as keys and as values (sixteen-byte units)
+    const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024), k_desc = smem_desc(smem_u32(kv_s), 16, 1024);
+    const uint64_t v_desc = smem_desc(smem_u32(kv_s), kHalfBytes, 1024);
     const auto next = [&]() {
       if (++stage == kStages) {
         stage = 0;
@@ -443,49 +469,44 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       }
     };
     const auto scores = [&](int a, uint32_t q_at) {  // S = Q K^T with the K of the current stage
-      if (lane == 0) {
+      const uint64_t qd = q_desc + (q_at >> 4), kd = k_desc + stage * (kStageBytes >> 4);
+      if (one_lane()) {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          const uint32_t off = (ks >> 2) * kHalfBytes + (ks & 3) * 32;
-          mma_ss(tmem + a * 128, smem_desc(q_at + off, 16, 1024), smem_desc(kv_a + stage * kStageBytes + off, 16, 1024), kS,
-                 ks > 0);
+          const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
+          mma_ss(tmem + a * 128, qd + off, kd + off, kS, ks > 0);
         }
         mma_commit(&sh.s_full[a]);
       }
       __syncwarp();
     };
     const auto commit = [&](uint64_t* bar) {
-      if (lane == 0) mma_commit(bar);
+      if (one_lane()) mma_commit(bar);
       __syncwarp();
     };
     // O += P V in two halves of 64 keys: the first starts while the softmax works on the second
     const auto values = [&](int a, uint32_t v_stage, bool add) {
+      const uint64_t vd = v_desc + v_stage * (kStageBytes >> 4);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        ok = mbar_wait(h ? &sh.p_full[a] : &sh.p_half[a], (p_rounds >> a) & 1);
-        if (!ok) return;
+        ok &= mbar_wait(h ? &sh.p_full[a] : &sh.p_half[a], (p_rounds >> a) & 1);
         tc_fence_after();
-        if (lane == 0) {
+        if (one_lane()) {
 #pragma unroll
           for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
-            mma_ts(tmem + 256 + a * 128, tmem + a * 128 + ks * 8,
-                   smem_desc(kv_a + v_stage * kStageBytes + ks * 2048, kHalfBytes, 1024), kO, add || ks > 0);
+            mma_ts(tmem + 256 + a * 128, tmem + a * 128 + ks * 8, vd + ks * (2048 >> 4), kO, add || ks > 0);
         }
         __syncwarp();
       }
       p_rounds ^= 1u << a;
     };
     const auto wait_kv = [&]() {
-      ok = mbar_wait(&sh.kv_full[stage], round & 1);
-      tc_fence_after();
-      return ok;
+      ok &= mbar_wait(&sh.kv_full[stage], round & 1);
     };
     const auto clean_tail = [&](const Item& it, uint32_t v_stage) {
-      const int tail = sh.tail[tiles++ & (kInfoSlots - 1)];
-      if (tail < 0) return;
       // rows behind the sequence's end may hold anything, and 0 x NaN is not 0
       const int r0 = it.len & (kPage - 1);
-      uint4* page = reinterpret_cast<uint4*>(kv_s + v_stage * kStageBytes + tail * 2048);
+      uint4* page = reinterpret_cast<uint4*>(kv_s + v_stage * kStageBytes + it.tail_page * 2048);
       for (int c = r0 * 8 + lane; c < kPage * 8; c += 32) {
         page[c] = make_uint4(0, 0, 0, 0);
         page[kHalfBytes / 16 + c] = make_uint4(0, 0, 0, 0);
@@ -496,73 +517,73 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
     Item it;
     while (next_item(it)) {
       if (it.n_tiles == 0) continue;
-      ok = mbar_wait(&sh.q_full, q_round & 1);
-      if (!ok) break;
+      ok &= mbar_wait(&sh.q_full, q_round & 1);
       ++q_round;
-      if (!wait_kv()) break;
+      wait_kv();
       if (it.pair) {
-        scores(0, q_a);
+        scores(0, 0);
         commit(&sh.kv_empty[stage]);
         next();
-        if (!wait_kv()) break;
-        scores(1, q_a);
+        wait_kv();
+        scores(1, 0);
         commit(&sh.kv_empty[stage]);
         if (it.n_tiles == 2) commit(&sh.q_free);
         next();
-        for (int t = 0; t < it.n_tiles && ok; ++t) {
+        for (int t = 0; t < it.n_tiles; ++t) {
           const int a = t & 1;
-          if (!wait_kv()) break;
+          wait_kv();
           const uint32_t v_stage = stage;
           next();
-          clean_tail(it, v_stage);
+          if (t + 1 == it.n_tiles && it.tail_page >= 0) clean_tail(it, v_stage);
           values(a, v_stage, t > 1);
-          if (!ok) break;
           commit(&sh.kv_empty[v_stage]);
           if (t + 2 < it.n_tiles) {
-            if (!wait_kv()) break;
-            scores(a, q_a);
+            wait_kv();
+            scores(a, 0);
             commit(&sh.kv_empty[stage]);
             next();
             if (t + 3 == it.n_tiles) commit(&sh.q_free);  // the last product with Q has been issued
           } else {
             commit(&sh.o_full[a]);
           }
+          ok = all_ok(ok);
+          if (!ok) break;
         }
       } else {
-        if (it.steps[0] > 0) scores(0, q_a);
-        if (it.steps[1] > 0) scores(1, q_a + kStageBytes);
+        if (it.steps[0] > 0) scores(0, 0);
+        if (it.steps[1] > 0) scores(1, kStageBytes);
         commit(&sh.kv_empty[stage]);
         if (it.n_tiles == 1) commit(&sh.q_free);
         next();
-        for (int j = 0; j < it.n_tiles && ok; ++j) {
-          if (!wait_kv()) break;
+        for (int j = 0; j < it.n_tiles; ++j) {
+          wait_kv();
           const uint32_t v_stage = stage;
           next();
-          clean_tail(it, v_stage);
+          if (j + 1 == it.n_tiles && it.tail_page >= 0) clean_tail(it, v_stage);
           const int last = j < it.steps[1] ? 1 : 0;  // the subtile that uses this V last
-          bool k_here = false;
+          const bool more = j + 1 < it.n_tiles;
+          if (more) wait_kv();
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
             if (j >= it.steps[a]) continue;
             values(a, v_stage, j > 0);
-            if (!ok) break;
             if (a == last) commit(&sh.kv_empty[v_stage]);
-            if (j + 1 < it.steps[a]) {
-              if (!k_here && !wait_kv()) break;
-              k_here = true;
-              scores(a, q_a + a * kStageBytes);
-            } else {
+            if (j + 1 < it.steps[a])
+              scores(a, a * kStageBytes);
+            else
               commit(&sh.o_full[a]);
-            }
           }
-          if (!ok) break;
-          if (k_here) {
+          if (more) {
             commit(&sh.kv_empty[stage]);
             if (j + 2 == it.n_tiles) commit(&sh.q_free);  // the last product with Q has been issued
             next();
           }
+          ok = all_ok(ok);
+          if (!ok) break;
         }
       }
+      ok = all_ok(ok);
+      if (!ok) break;
     }
     if (!ok) {  // an early end: products in flight still read shared memory and write TMEM
       commit(&sh.drain);
@@ -580,7 +601,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
     for (;; ++n_item) {
       // (read in place and given back at the end: a copy would hold registers that a row of scores needs)
       const Item& it = sh.items[n_item & 1];
-      ok = mbar_wait(&sh.item_full[n_item & 1], (n_item >> 1) & 1);
+      ok = all_ok(mbar_wait(&sh.item_full[n_item & 1], (n_item >> 1) & 1));
       if (!ok || it.n_tiles < 0) break;
       const int pair = it.pair;
       const int tok = (pair ? 0 : a * p.tok_tile) + tok_r;  // of the item
@@ -590,13 +611,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       const int steps = a ? it.steps[1] : it.steps[0], steps_other = a ? it.steps[0] : it.steps[1];
       for (int j = 0; j < steps; ++j) {
         ok = mbar_wait(&sh.s_full[a], s_round & 1);
-        if (!ok) break;
         ++s_round;
         tc_fence_after();
         const int slot = (tiles + (pair ? 2 * j + a : j)) & (kInfoSlots - 1);
         float x[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(x + 32 * c, s_t + 32 * c);
+        if (!all_ok(ok)) break;
         const bool masked = __any_sync(0xffffffffu, real && sh.hi[slot] > limit);
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_wait_ld32(x + 32 * c);
@@ -644,21 +665,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t w[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const uint64_t y = fma2(f2(x[64 * c + 2 * e], x[64 * c + 2 * e + 1]), scale2, ref2);
-            float a0, a1;
-            if (e % kPolyOf < kPolyTake && !masked) {
-              exp2_poly(y, a0, a1);
-            } else {
-              f2_split(y, a0, a1);
-              a0 = tile_ex2(a0);
-              a1 = tile_ex2(a1);
-            }
-            sum[e & 1] = add2(sum[e & 1], f2(a0, a1));
-            // weights go to the tensor cores in the model type (half a step of it each); their sum stays unrounded
-            w[e] = tile_pack2(a0, a1, T());
-          }
+          // (one branch around each whole loop: the elements of a loop without branches overlap)
+          if (masked)
+            weights<T, 0>(x + 64 * c, scale2, ref2, sum, w);
+          else
+            weights<T, kPolyTake>(x + 64 * c, scale2, ref2, sum, w);
+          __syncwarp();
           tmem_st32(s_t + 32 * c, w);
           tmem_wait_st();
           tc_fence_before();
@@ -668,6 +680,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
         f2_split(add2(sum[0], sum[1]), s0, s1);
         l += s0 + s1;
       }
+      ok = all_ok(ok);
       if (!ok) break;
       tiles += it.n_tiles;
       // ---- the item's rows: columns c0 .. of O, of both places of a pair ----
@@ -676,7 +689,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       if (pair) {
         sh.ml[a][r] = make_float2(m, l);
         mbar_arrive(&sh.pair[0]);
-        ok = mbar_wait(&sh.pair[0], pairs & 1);
+        ok = all_ok(mbar_wait(&sh.pair[0], pairs & 1));
         if (!ok) break;
         const float2 v = sh.ml[a ^ 1][r];
         const float mm = fmaxf(m, v.x), ref = mm == -INFINITY ? 0.f : mm;
@@ -684,11 +697,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
         f_other = tile_ex2(v.x - ref);
         l = a ? v.y * f_other + l * f_own : l * f_own + v.y * f_other;  // the same sum in both places
         m = mm;
-        ok = mbar_wait(&sh.o_full[a ^ 1], o_other & 1);
+        ok = all_ok(mbar_wait(&sh.o_full[a ^ 1], o_other & 1));
         if (!ok) break;
       }
       if (any) {
-        ok = mbar_wait(&sh.o_full[a], o_own & 1);
+        ok = all_ok(mbar_wait(&sh.o_full[a], o_own & 1));
         if (!ok) break;
       }
       o_own += any;
@@ -746,7 +759,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       tc_fence_before();
       if (pair) {
         mbar_arrive(&sh.pair[1]);
-        ok = mbar_wait(&sh.pair[1], pairs++ & 1);
+        ok = all_ok(mbar_wait(&sh.pair[1], pairs++ & 1));
         if (!ok) break;
       }
       __syncwarp();

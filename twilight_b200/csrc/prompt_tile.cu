@@ -12,8 +12,10 @@
 // The reference maximum m of a row is only moved when the true one has grown by more than 2^8, so O is rescaled a
 // few times per row; weights then stay below 2^8, which fp16 and the fp32 sums hold without loss.
 //
-// Warps: 0-3 and 4-7 softmax, 8 page loads (TMA: a page is two boxes of 16 rows x 128 bytes, issued by sixteen lanes),
-// 9 tensor-core issue, 10 work items (taken from a counter, two ahead).  K and V tiles share a ring of five 32 KiB stages.
+// Warps: 0-3 and 4-7 softmax, 8 K pages, 11 V pages, 9 tensor-core issue, 10 work items (taken from a counter, two ahead).
+// K has three 32 KiB stages, V two.  A page is ONE copy: seen as [groups of 8 rows][halves of 64 channels][8 rows][64] it
+// lands as four swizzle atoms, equal halves 2 KiB apart for both operands.  (As two boxes per page, issued by one warp, the
+// copies took 2700 clocks a step of K and V, more than its products: each costs its warp about 85.)
 //
 // Bound: two products of 128 x 128 x 128 (512 clocks each at the tensor peak) and 128 x 128 exponentials per subtile and
 // step (1024 clocks of the special-function units, were they to do all of them); with few rows per KV head, reading
@@ -29,9 +31,10 @@ namespace twl {
 constexpr int kTileThreads = 384;  // three warpgroups, the unit of the register split
 constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "registers of the launch: 168 a thread at 384 threads");
-constexpr int kStages = 5;
+constexpr int kKStages = 3, kVStages = 2, kStages = kKStages + kVStages;
 constexpr int kStageBytes = 128 * kD * 2;      // 128 keys (or 128 query rows)
-constexpr int kHalfBytes = kStageBytes / 2;    // 64 channels of 128 rows
+constexpr int kHalfBytes = kStageBytes / 2;    // 64 channels of 128 query rows
+constexpr int kPageBytes = kPage * kD * 2, kAtom = 1024;
 constexpr int kInfoSlots = 8;                  // key tiles whose positions are kept
 constexpr int kPolyTake = 2;                   // of eight pairs of exponentials, how many take the polynomial
 constexpr uint32_t kWaitTries = 2000, kWaitNs = 500000;  // a wait gives up after about a second
@@ -59,7 +62,7 @@ struct Item {
 
 struct TileShared {
   uint64_t item_full[2], item_empty[2];
-  uint64_t q_full, q_free, kv_full[kStages], kv_empty[kStages], s_full[2], p_half[2], p_full[2], o_full[2], pair[2], drain;
+  uint64_t q_full, q_free, k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages], s_full[2], p_half[2], p_full[2], o_full[2], pair[2], drain;
   Item items[2];
   uint32_t tmem;
   int32_t hi[kInfoSlots];      // largest position of the tile's keys, INT_MAX when a page is missing
@@ -95,10 +98,11 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity) {
 }
 __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
 
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* m, int x, int y, uint64_t* bar) {
+__device__ __forceinline__ void tma_page(uint32_t dst, const CUtensorMap* m, int group, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(m), "r"(x), "r"(y), "r"(smem_u32(bar))
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %2, %2, %3}], [%4];" ::"r"(
+          dst),
+      "l"(m), "r"(0), "r"(group), "r"(smem_u32(bar))
       : "memory");
 }
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* m, int x, int y, int z, uint64_t* bar) {
@@ -235,6 +239,16 @@ __device__ __forceinline__ void exp2_poly(uint64_t x, float& a, float& b) {
   b = __int_as_float(__float_as_int(y1) + (__float_as_int(n1) << 23));
 }
 
+__device__ __forceinline__ float max64(const float* x) {
+  float m[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+  for (int c = 4; c < 60; c += 8)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = max3(m[e], x[c + e], x[c + 4 + e]);
+  m[0] = max3(m[0], x[60], x[61]);
+  m[1] = max3(m[1], x[62], x[63]);
+  return max3(max3(m[0], m[1], m[2]), m[3], m[3]);
+}
 // 64 weights 2^(x scale - ref) of a row: their sum in 32 bits, and themselves rounded to the model type (half a step each),
 // in which they go to the tensor cores.  POLY of eight pairs take the polynomial (never masked ones: it has no zero).
 template <typename T, int POLY>
@@ -312,13 +326,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_free, 1);
     mbar_init(&sh.drain, 1);
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&sh.kv_full[i], 1);
-      mbar_init(&sh.kv_empty[i], 1);
+    for (int i = 0; i < kKStages; ++i) {
+      mbar_init(&sh.k_full[i], 1);
+      mbar_init(&sh.k_empty[i], 1);
+    }
+    for (int i = 0; i < kVStages; ++i) {
+      mbar_init(&sh.v_full[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&sh.item_full[a], 1);
-      mbar_init(&sh.item_empty[a], 10);  // loads, tensor cores, eight softmax warps
+      mbar_init(&sh.item_empty[a], 11);  // two of loads, tensor cores, eight softmax warps
       mbar_init(&sh.s_full[a], 1);
       mbar_init(&sh.p_half[a], 128);
       mbar_init(&sh.p_full[a], 128);
@@ -373,108 +391,105 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       if (lane == 0) i = gridDim.x + atomicAdd(&p.hdr->next_tile, 1);
       i = __shfl_sync(0xffffffffu, i, 0);
     }
-  } else if (warp == 8) {
-    // ---- loads: K of the first tile (of the first two of a pair), then V of tile t and K of the tile that follows ----
+  } else if (warp == 8 || warp == 11) {
+    // ---- loads: warp 8 Q and K, warp 11 V; lane l takes page l of a key tile ----
+    const bool is_k = warp == 8;
+    const int n_stages = is_k ? kKStages : kVStages;
+    uint64_t* const full = is_k ? sh.k_full : sh.v_full;
+    uint64_t* const empty = is_k ? sh.k_empty : sh.v_empty;
+    uint8_t* const base = kv_s + (is_k ? 0 : kKStages * kStageBytes);
+    const CUtensorMap* const map = is_k ? &tp.tk : &tp.tv;
     uint32_t stage = 0, round = 0, q_round = 0;
     uint32_t tiles = 0;  // key tiles so far, over all items
-    uint32_t used = 0;   // stages filled so far, at most kStages: what an early end has to wait for
-    const int page_of_lane = (lane & 15) >> 1, half = lane & 1;
-    const int gone = p.num_pages_total * p.Hkv * kPage;  // a row behind the pool: reads as zeros
-    const auto put = [&](const CUtensorMap* map, int row) {
-      if (lane == 0) mbar_expect(&sh.kv_full[stage], kStageBytes);
-      __syncwarp();
-      if (lane < 16)
-        tma_2d(smem_u32(kv_s + stage * kStageBytes) + half * kHalfBytes + page_of_lane * 2048, map, half * 64, row,
-               &sh.kv_full[stage]);
-      used = max(used, stage + 1);
-      if (++stage == kStages) {
-        stage = 0;
-        ++round;
-      }
-    };
+    const int gone = p.num_pages_total * p.Hkv * 2;  // a group of rows behind the pool: reads as zeros
     Item it;
     while (next_item(it)) {
       if (it.n_tiles == 0) continue;
-      const int subs = it.ntok > p.tok_tile ? 2 : 1;
-      ok = all_ok(mbar_wait(&sh.q_free, (q_round & 1) ^ 1));
-      if (!ok) break;
-      ++q_round;
-      if (lane == 0) {
-        mbar_expect(&sh.q_full, (uint32_t)(subs * 2 * 64 * 2 * p.G * p.tok_tile));
-        for (int a = 0; a < subs; ++a)
-          for (int h = 0; h < 2; ++h)
-            tma_3d(smem_u32(q_s) + a * kStageBytes + h * kHalfBytes, &tp.tq, h * 64, it.kvh * p.G, it.tok0 + a * p.tok_tile,
-                   &sh.q_full);
+      if (is_k) {
+        const int subs = it.ntok > p.tok_tile ? 2 : 1;
+        ok = all_ok(mbar_wait(&sh.q_free, (q_round & 1) ^ 1));
+        if (!ok) break;
+        ++q_round;
+        if (lane == 0) {
+          mbar_expect(&sh.q_full, (uint32_t)(subs * 2 * 64 * 2 * p.G * p.tok_tile));
+          for (int a = 0; a < subs; ++a)
+            for (int h = 0; h < 2; ++h)
+              tma_3d(smem_u32(q_s) + a * kStageBytes + h * kHalfBytes, &tp.tq, h * 64, it.kvh * p.G,
+                     it.tok0 + a * p.tok_tile, &sh.q_full);
+        }
+        __syncwarp();
       }
-      __syncwarp();
       const auto look_up = [&](int j, int& lp, int& phys) {
-        const int at = 8 * j + page_of_lane;
+        const int at = 8 * j + lane;
         lp = -1;
         phys = -1;
-        if (at < it.n_pages) {
+        if (lane < 8 && at < it.n_pages) {
           lp = it.list ? it.list[at] : it.page0 + at;
           if (lp >= 0 && lp < it.npages) phys = it.indices[lp];
           if (phys < 0 || phys >= p.num_pages_total) {
             phys = -1;
-            raise_flag(p.status, TWL_FLAG_BAD_INDEX);
+            if (is_k) raise_flag(p.status, TWL_FLAG_BAD_INDEX);
           }
         }
       };
-      const int lead = it.pair ? 2 : 1;
-      int rows[3];  // pool rows of this lane's page of tiles whose K is loaded and V is not: the oldest first
       int lp, phys;
       look_up(0, lp, phys);
-      for (int k = 0; k < it.n_tiles + lead && ok; ++k) {
-        if (k < it.n_tiles) {  // K of tile k
-          const int row = phys < 0 ? gone : (phys * p.Hkv + it.kvh) * kPage;
-          const int pos = phys < 0 ? 0x3fffffff : lp * kPage;
-          const int hi = __reduce_max_sync(0xffffffffu, phys < 0 ? 0x7fffffff : pos + kPage - 1);
-          look_up(k + 1, lp, phys);
-          // Room for K means that V of at least three tiles ago has been used, so every reader of the info of that tile
-          // and of those before it is done: of the eight slots four are still in use.
-          ok = all_ok(mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1));
-          if (!ok) break;
+      for (int t = 0; t < it.n_tiles; ++t) {
+        const int group = phys < 0 ? gone : (phys * p.Hkv + it.kvh) * 2;
+        const int pos = phys < 0 ? 0x3fffffff : lp * kPage;
+        const int hi = __reduce_max_sync(0xffffffffu, lane >= 8 ? -1 : phys < 0 ? 0x7fffffff : pos + kPage - 1);
+        look_up(t + 1, lp, phys);
+        ok = all_ok(mbar_wait(&empty[stage], (round & 1) ^ 1));
+        if (!ok) break;
+        if (is_k) {
+          // Room for K means that the scores of three tiles ago are done, and they were begun after the weights of at the
+          // latest five tiles ago: of the eight slots of the info at most five are still read.
           const int slot = tiles++ & (kInfoSlots - 1);
-          if (lane < 16 && half == 0) sh.pos[slot][page_of_lane] = pos;
+          if (lane < 8) sh.pos[slot][lane] = pos;
           if (lane == 0) sh.hi[slot] = hi;
-          __syncwarp();
-          put(&tp.tk, row);
-          rows[2] = row;
         }
-        if (k + 1 >= lead && k + 1 - lead < it.n_tiles) {  // V of tile k + 1 - lead
-          ok = all_ok(mbar_wait(&sh.kv_empty[stage], (round & 1) ^ 1));
-          if (!ok) break;
-          put(&tp.tv, it.pair ? rows[1] : rows[2]);
+        if (lane == 0) mbar_expect(&full[stage], kStageBytes);
+        __syncwarp();
+        if (lane < 8) tma_page(smem_u32(base + stage * kStageBytes) + lane * kPageBytes, map, group, &full[stage]);
+        __syncwarp();
+        if (++stage == (uint32_t)n_stages) {
+          stage = 0;
+          ++round;
         }
-        rows[0] = rows[1];
-        rows[1] = rows[2];
       }
+      if (!ok) break;
     }
     if (!ok) {  // an early end: the copies in flight still write to shared memory
-      for (uint32_t s = 0; s < used; ++s) mbar_wait(&sh.kv_full[s], (s < stage ? round : round - 1) & 1);
+      for (uint32_t s = 0; s < (uint32_t)n_stages; ++s)
+        if (round > 0 || s < stage) mbar_wait(&full[s], (s < stage ? round : round - 1) & 1);
       if (q_round) mbar_wait(&sh.q_full, (q_round - 1) & 1);
-      ok = false;
     }
   } else if (warp == 9) {
     // ---- tensor cores ----
-    uint32_t stage = 0, round = 0, q_round = 0, p_rounds = 0;  // p_rounds: bit a is place a's parity
+    uint32_t k_stage = 0, k_round = 0, v_stage = 0, v_round = 0, q_round = 0, p_rounds = 0;  // p_rounds: bit a is place a's parity
     const uint32_t kS = mma_desc<T>(false), kO = mma_desc<T>(true);
-    // operand descriptors of the first query row, of the first stage as keys and as values (sixteen-byte units)
-    const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, 1024), k_desc = smem_desc(smem_u32(kv_s), 16, 1024);
-    const uint64_t v_desc = smem_desc(smem_u32(kv_s), kHalfBytes, 1024);
-    const auto next = [&]() {
-      if (++stage == kStages) {
-        stage = 0;
-        ++round;
+    // operand descriptors of the first query row, of the first stages (sixteen-byte units)
+    const uint64_t q_desc = smem_desc(smem_u32(q_s), 16, kAtom), k_desc = smem_desc(smem_u32(kv_s), 16, 2 * kAtom);
+    const uint64_t v_desc = smem_desc(smem_u32(kv_s + kKStages * kStageBytes), kAtom, 2 * kAtom);
+    const auto next_k = [&]() {
+      if (++k_stage == kKStages) {
+        k_stage = 0;
+        ++k_round;
+      }
+    };
+    const auto next_v = [&]() {
+      if (++v_stage == kVStages) {
+        v_stage = 0;
+        ++v_round;
       }
     };
     const auto scores = [&](int a, uint32_t q_at) {  // S = Q K^T with the K of the current stage
-      const uint64_t qd = q_desc + (q_at >> 4), kd = k_desc + stage * (kStageBytes >> 4);
+      const uint64_t qd = q_desc + (q_at >> 4), kd = k_desc + k_stage * (kStageBytes >> 4);
       if (one_lane()) {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          const uint32_t off = ((ks >> 2) * kHalfBytes + (ks & 3) * 32) >> 4;
-          mma_ss(tmem + a * 128, qd + off, kd + off, kS, ks > 0);
+          const uint32_t q_off = (ks >> 2) * kHalfBytes + (ks & 3) * 32, k_off = (ks >> 2) * kAtom + (ks & 3) * 32;
+          mma_ss(tmem + a * 128, qd + (q_off >> 4), kd + (k_off >> 4), kS, ks > 0);
         }
         mma_commit(&sh.s_full[a]);
       }
@@ -485,7 +500,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       __syncwarp();
     };
     // O += P V in two halves of 64 keys: the first starts while the softmax works on the second
-    const auto values = [&](int a, uint32_t v_stage, bool add) {
+    const auto values = [&](int a, bool add) {
       const uint64_t vd = v_desc + v_stage * (kStageBytes >> 4);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -494,22 +509,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
         if (one_lane()) {
 #pragma unroll
           for (int ks = 4 * h; ks < 4 * h + 4; ++ks)
-            mma_ts(tmem + 256 + a * 128, tmem + a * 128 + ks * 8, vd + ks * (2048 >> 4), kO, add || ks > 0);
+            mma_ts(tmem + 256 + a * 128, tmem + a * 128 + ks * 8, vd + ks * (kPageBytes >> 4), kO, add || ks > 0);
         }
         __syncwarp();
       }
       p_rounds ^= 1u << a;
     };
-    const auto wait_kv = [&]() {
-      ok &= mbar_wait(&sh.kv_full[stage], round & 1);
-    };
-    const auto clean_tail = [&](const Item& it, uint32_t v_stage) {
+    const auto wait_k = [&]() { ok &= mbar_wait(&sh.k_full[k_stage], k_round & 1); };
+    const auto wait_v = [&]() { ok &= mbar_wait(&sh.v_full[v_stage], v_round & 1); };
+    const auto clean_tail = [&](const Item& it) {
       // rows behind the sequence's end may hold anything, and 0 x NaN is not 0
-      const int r0 = it.len & (kPage - 1);
-      uint4* page = reinterpret_cast<uint4*>(kv_s + v_stage * kStageBytes + it.tail_page * 2048);
-      for (int c = r0 * 8 + lane; c < kPage * 8; c += 32) {
-        page[c] = make_uint4(0, 0, 0, 0);
-        page[kHalfBytes / 16 + c] = make_uint4(0, 0, 0, 0);
+      uint8_t* page = kv_s + (kKStages + v_stage) * kStageBytes + it.tail_page * kPageBytes;
+      for (int c = (it.len & (kPage - 1)) * 16 + lane; c < kPage * 16; c += 32) {  // row, half, piece
+        const int r = c >> 4;
+        *reinterpret_cast<uint4*>(page + (r >> 3) * 2 * kAtom + ((c >> 3) & 1) * kAtom + (r & 7) * 128 + (c & 7) * 16) =
+            make_uint4(0, 0, 0, 0);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -519,29 +533,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       if (it.n_tiles == 0) continue;
       ok &= mbar_wait(&sh.q_full, q_round & 1);
       ++q_round;
-      wait_kv();
+      wait_k();
       if (it.pair) {
         scores(0, 0);
-        commit(&sh.kv_empty[stage]);
-        next();
-        wait_kv();
+        commit(&sh.k_empty[k_stage]);
+        next_k();
+        wait_k();
         scores(1, 0);
-        commit(&sh.kv_empty[stage]);
+        commit(&sh.k_empty[k_stage]);
         if (it.n_tiles == 2) commit(&sh.q_free);
-        next();
+        next_k();
         for (int t = 0; t < it.n_tiles; ++t) {
           const int a = t & 1;
-          wait_kv();
-          const uint32_t v_stage = stage;
-          next();
-          if (t + 1 == it.n_tiles && it.tail_page >= 0) clean_tail(it, v_stage);
-          values(a, v_stage, t > 1);
-          commit(&sh.kv_empty[v_stage]);
-          if (t + 2 < it.n_tiles) {
-            wait_kv();
+          const bool more = t + 2 < it.n_tiles;
+          wait_v();
+          if (more) wait_k();
+          if (t + 1 == it.n_tiles && it.tail_page >= 0) clean_tail(it);
+          values(a, t > 1);
+          commit(&sh.v_empty[v_stage]);
+          next_v();
+          if (more) {
             scores(a, 0);
-            commit(&sh.kv_empty[stage]);
-            next();
+            commit(&sh.k_empty[k_stage]);
+            next_k();
             if (t + 3 == it.n_tiles) commit(&sh.q_free);  // the last product with Q has been issued
           } else {
             commit(&sh.o_full[a]);
@@ -552,31 +566,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       } else {
         if (it.steps[0] > 0) scores(0, 0);
         if (it.steps[1] > 0) scores(1, kStageBytes);
-        commit(&sh.kv_empty[stage]);
+        commit(&sh.k_empty[k_stage]);
         if (it.n_tiles == 1) commit(&sh.q_free);
-        next();
+        next_k();
         for (int j = 0; j < it.n_tiles; ++j) {
-          wait_kv();
-          const uint32_t v_stage = stage;
-          next();
-          if (j + 1 == it.n_tiles && it.tail_page >= 0) clean_tail(it, v_stage);
-          const int last = j < it.steps[1] ? 1 : 0;  // the subtile that uses this V last
           const bool more = j + 1 < it.n_tiles;
-          if (more) wait_kv();
+          wait_v();
+          if (more) wait_k();
+          if (!more && it.tail_page >= 0) clean_tail(it);
+          const int last = j < it.steps[1] ? 1 : 0;  // the subtile that uses this V last
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
             if (j >= it.steps[a]) continue;
-            values(a, v_stage, j > 0);
-            if (a == last) commit(&sh.kv_empty[v_stage]);
+            values(a, j > 0);
+            if (a == last) commit(&sh.v_empty[v_stage]);
             if (j + 1 < it.steps[a])
               scores(a, a * kStageBytes);
             else
               commit(&sh.o_full[a]);
           }
+          next_v();
           if (more) {
-            commit(&sh.kv_empty[stage]);
+            commit(&sh.k_empty[k_stage]);
             if (j + 2 == it.n_tiles) commit(&sh.q_free);  // the last product with Q has been issued
-            next();
+            next_k();
           }
           ok = all_ok(ok);
           if (!ok) break;
@@ -608,6 +621,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       const bool real = tok_r < p.tok_tile && tok < it.ntok;
       const int limit = !real ? -1 : p.causal ? it.limit0 + tok : it.limit0;
       float m = -INFINITY, l = 0.f;
+      bool settled = false;  // every row of the warp has a reference
       const int steps = a ? it.steps[1] : it.steps[0], steps_other = a ? it.steps[0] : it.steps[1];
       for (int j = 0; j < steps; ++j) {
         ok = mbar_wait(&sh.s_full[a], s_round & 1);
@@ -615,67 +629,93 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
         tc_fence_after();
         const int slot = (tiles + (pair ? 2 * j + a : j)) & (kInfoSlots - 1);
         float x[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(x + 32 * c, s_t + 32 * c);
+        tmem_ld32(x, s_t);
+        tmem_ld32(x + 32, s_t + 32);
         if (!all_ok(ok)) break;
         const bool masked = __any_sync(0xffffffffu, real && sh.hi[slot] > limit);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_wait_ld32(x + 32 * c);
-        if (masked) {
-#pragma unroll
-          for (int pg = 0; pg < 8; ++pg) {
-            const int n = limit - sh.pos[slot][pg];  // keys 0..n of the page are seen
-#pragma unroll
-            for (int c = 0; c < kPage; ++c)
-              if (c > n) x[16 * pg + c] = -INFINITY;
-          }
-        }
-        float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int c = 4; c < 124; c += 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], x[c + e], x[c + 4 + e]);
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) mx[e] = max3(max3(mx[e], mx[e + 1], x[124 + e]), x[125 + e], mx[e]);
-        const float top = max3(mx[0], mx[2], mx[2]) * scale;
-        // move the reference only when it is 2^8 behind (or nothing was seen so far)
-        float f = 1.f;
-        const bool move = !(top <= m + 8.f);  // from -inf: any finite maximum
-        if (move) {
-          f = tile_ex2(m - top);
-          m = top;
-          l *= f;
-        }
-        if (__any_sync(0xffffffffu, move) && j > 0) {
-          // S of this step is complete, so the product of the step before is too: O may be changed
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float o[32];
-            uint32_t w[32];
-            tmem_ld32(o, o_t + 32 * c);
-            tmem_wait_ld32(o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
-            tmem_st32(o_t + 32 * c, w);
-          }
-        }
-        const float ref = m == -INFINITY ? 0.f : m;
-        const uint64_t scale2 = f2(scale, scale), ref2 = f2(-ref, -ref);
+        tmem_wait_ld32(x);
+        tmem_wait_ld32(x + 32);
+        tmem_ld32(x + 64, s_t + 64);
+        tmem_ld32(x + 96, s_t + 96);
+        const uint64_t scale2 = f2(scale, scale);
         uint64_t sum[2] = {0, 0};
+        uint32_t w[32];
+        float top;
+        bool first_done = false;
+        if (settled && !masked) {
+          // The reference hardly ever moves: the first weights are computed with it while the maximum is found.
+          const float ref = m;
+          weights<T, kPolyTake>(x, scale2, f2(-ref, -ref), sum, w);
+          top = max64(x);
+          tmem_wait_ld32(x + 64);
+          tmem_wait_ld32(x + 96);
+          top = max3(top, max64(x + 64), top) * scale;
+          first_done = !__any_sync(0xffffffffu, !(top <= m + 8.f));
+          if (!first_done) {  // it does: take them again
+            sum[0] = sum[1] = 0;
+            tmem_ld32(x, s_t);
+            tmem_ld32(x + 32, s_t + 32);
+            tmem_wait_ld32(x);
+            tmem_wait_ld32(x + 32);
+          }
+        } else {
+          tmem_wait_ld32(x + 64);
+          tmem_wait_ld32(x + 96);
+          if (masked) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t w[32];
-          // (one branch around each whole loop: the elements of a loop without branches overlap)
-          if (masked)
-            weights<T, 0>(x + 64 * c, scale2, ref2, sum, w);
-          else
-            weights<T, kPolyTake>(x + 64 * c, scale2, ref2, sum, w);
-          __syncwarp();
-          tmem_st32(s_t + 32 * c, w);
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(c ? &sh.p_full[a] : &sh.p_half[a]);
+            for (int pg = 0; pg < 8; ++pg) {
+              const int n = limit - sh.pos[slot][pg];  // keys 0..n of the page are seen
+#pragma unroll
+              for (int c = 0; c < kPage; ++c)
+                if (c > n) x[16 * pg + c] = -INFINITY;
+            }
+            __syncwarp();
+          }
+          top = max3(max64(x), max64(x + 64), -INFINITY) * scale;
         }
+        if (!first_done) {
+          // move the reference only when it is 2^8 behind (or nothing was seen so far)
+          float f = 1.f;
+          const bool move = !(top <= m + 8.f);  // from -inf: any finite maximum; a NaN moves it too
+          if (move) {
+            f = tile_ex2(m - top);
+            m = top;
+            l *= f;
+          }
+          if (__any_sync(0xffffffffu, move) && j > 0) {
+            // S of this step is complete, so the product of the step before is too: O may be changed
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float o[32];
+              tmem_ld32(o, o_t + 32 * c);
+              tmem_wait_ld32(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
+              tmem_st32(o_t + 32 * c, w);
+            }
+          }
+          settled = !__any_sync(0xffffffffu, real && m == -INFINITY);
+          const float ref = m == -INFINITY ? 0.f : m;
+          if (masked)
+            weights<T, 0>(x, scale2, f2(-ref, -ref), sum, w);
+          else
+            weights<T, kPolyTake>(x, scale2, f2(-ref, -ref), sum, w);
+          __syncwarp();
+        }
+        tmem_st32(s_t, w);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&sh.p_half[a]);
+        const float ref = m == -INFINITY ? 0.f : m;
+        if (masked)
+          weights<T, 0>(x + 64, scale2, f2(-ref, -ref), sum, w);
+        else
+          weights<T, kPolyTake>(x + 64, scale2, f2(-ref, -ref), sum, w);
+        __syncwarp();
+        tmem_st32(s_t + 32, w);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&sh.p_full[a]);
         float s0, s1;
         f2_split(add2(sum[0], sum[1]), s0, s1);
         l += s0 + s1;
@@ -800,16 +840,16 @@ int tile_attention_launch(const AttnParams& p, int dtype, cudaStream_t st) {
   TileParams tp;
   tp.a = p;
   const CUtensorMapDataType type = dtype == TWL_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const cuuint32_t ones[3] = {1, 1, 1};
-  const cuuint64_t kv_dims[2] = {(cuuint64_t)kD, (cuuint64_t)p.num_pages_total * p.Hkv * kPage};
-  const cuuint64_t kv_strides[1] = {kD * 2};
-  const cuuint32_t kv_box[2] = {64, (cuuint32_t)kPage};
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const cuuint64_t kv_dims[4] = {64, 8, 2, (cuuint64_t)p.num_pages_total * p.Hkv * 2};
+  const cuuint64_t kv_strides[3] = {kD * 2, 128, 8 * kD * 2};
+  const cuuint32_t kv_box[4] = {64, 8, 2, 2};
   const cuuint64_t q_dims[3] = {(cuuint64_t)kD, (cuuint64_t)p.Hq, (cuuint64_t)p.num_tokens};
   const cuuint64_t q_strides[2] = {kD * 2, (cuuint64_t)p.q_ts * 2};
   const cuuint32_t q_box[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.tok_tile};
   bool ok = true;
   for (int i = 0; i < 2; ++i)
-    ok = ok && encode(i ? &tp.tv : &tp.tk, type, 2, const_cast<void*>(i ? p.v_pages : p.k_pages), kv_dims, kv_strides, kv_box,
+    ok = ok && encode(i ? &tp.tv : &tp.tk, type, 4, const_cast<void*>(i ? p.v_pages : p.k_pages), kv_dims, kv_strides, kv_box,
                       ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
   ok = ok && encode(&tp.tq, type, 3, const_cast<void*>(p.q), q_dims, q_strides, q_box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,

@@ -9,10 +9,11 @@
 namespace twl {
 
 // ---- plan -------------------------------------------------------------------------------------------
-// One block: lengths and work of every segment, the chunk sizes, and the two lists of work items.  A separate
-// launch, so that the lengths stay on the device and the other kernels find their work with one load.
+// One block: lengths and work of every segment, the run of a warp of the row kernel, the key chunks and the list of the
+// tile kernel.  A separate launch, so that the lengths stay on the device and the other kernels find their work with one
+// load.
 constexpr int kPlanThreads = 1024;
-constexpr int kRowChunkMin = 16;   // pages: four a warp; shorter chunks cost more in the merge than they balance
+constexpr int kRowRunMin = 4;      // pages: shorter runs cost more in the merge than they balance
 constexpr int kTileChunkMin = 32;  // pages: four key tiles, for the same reason
 
 __device__ __forceinline__ Segment load_segment(const AttnParams& p, int i) {
@@ -27,8 +28,10 @@ __device__ __forceinline__ Segment load_segment(const AttnParams& p, int i) {
   s.npages = indptr[j + 1] - s.kvbase;
   const int last = (second ? p.last2 : p.last1)[j];
   s.second = second;
+  s.units = 0;
   s.chunks = 1;
-  s.chunk_pages = 0;
+  s.chunk_pages = 0x3fffffff;
+  s.start = 0;
   s.pbase = -1;
   const bool bad = s.tok0 < 0 || s.ntok < 0 || s.tok0 + s.ntok > p.num_tokens || s.npages < 0 ||
                    (s.npages > 0 && (last < 1 || last > kPage));
@@ -38,15 +41,11 @@ __device__ __forceinline__ Segment load_segment(const AttnParams& p, int i) {
   }
   if (s.npages <= 0 || bad) s.npages = 0;
   s.len = s.npages ? (s.npages - 1) * kPage + last : 0;
+  s.few = s.ntok * p.G <= kFewRows;
   return s;
 }
 
-// row tiles of a segment (per KV head); a tile stays within one query block when there are block lists
-__device__ __forceinline__ int row_tiles(const AttnParams& p, int ntok) {
-  if (p.block_pages == nullptr) return (ntok * p.G + p.row_tile - 1) / p.row_tile;
-  const int whole = ntok / p.query_block, rest = ntok - whole * p.query_block;
-  return whole * ((p.query_block * p.G + p.row_tile - 1) / p.row_tile) + (rest * p.G + p.row_tile - 1) / p.row_tile;
-}
+// tiles of the tile kernel (per KV head); a tile stays within one query block when there are block lists
 __device__ __forceinline__ int tok_tiles(const AttnParams& p, int ntok) {
   const int t = 2 * p.tok_tile;
   if (p.block_pages == nullptr) return (ntok + t - 1) / t;
@@ -75,108 +74,104 @@ __device__ __forceinline__ void block_sums(long long (&v)[N], long long (*s)[4])
   __syncthreads();
 }
 
-// pages of a chunk: enough chunks to give every tile slot about one, but not more than that many items
-__device__ __forceinline__ int chunk_size(long long tiles, long long work, int target, int least, int step) {
-  if (tiles >= target) return 0x3fffffff;  // every tile has a slot's worth of company
-  // a tile of w pages becomes ceil(w/c) items, on average w/c + 1/2
-  const long long room = max(1LL, target - tiles / 2);
-  const long long c = max((long long)least, (work + room - 1) / room);
-  return (int)min((long long)0x3fffffff, (c + step - 1) / step * step);
-}
-
 __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnParams p) {
   __shared__ long long sums[kPlanThreads / 32][4];
-  __shared__ int scan[kPlanThreads / 32][3];
+  __shared__ long long scan[kPlanThreads / 32][3];
   pdl_wait();
   pdl_release();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_thr = blockDim.x, n_warps = n_thr >> 5;
   const int n_seg = p.n_first + p.n_second;
   const auto pages_of = [&](const Segment& s) { return p.block_pages ? min(s.npages, p.max_k) : s.npages; };
-  // tiles and tiles x pages of the row kernel and of the tile kernel
-  long long v[4] = {0, 0, 0, 0};
+  // units of the row kernel; tiles and tiles x pages of the tile kernel
+  long long v[3] = {0, 0, 0};
   Segment mine;  // this thread's segment of the first round
   mine.ntok = 0;
   for (int i = tid; i < n_seg; i += n_thr) {
     const Segment s = load_segment(p, i);
     if (i == tid) mine = s;
-    const bool few = s.ntok * p.G <= p.few_rows;
-    const int n = few ? row_tiles(p, s.ntok) : tok_tiles(p, s.ntok);
-    v[few ? 0 : 2] += n;
-    v[few ? 1 : 3] += (long long)n * pages_of(s);
-  }
-  block_sums<4>(v, sums);
-  const int rc = chunk_size(v[0] * p.Hkv, v[1] * p.Hkv, p.row_target, kRowChunkMin, 1);
-  int tc = chunk_size(v[2] * p.Hkv, v[3] * p.Hkv, p.tile_target, kTileChunkMin, 8);  // whole key tiles
-  // one wave of tiles should stay one wave: count, and make the chunks longer by what is too much
-  if (tc < 0x3fffffff) {
-    for (int round = 0; round < 3; ++round) {
-      long long items[1] = {0};
-      for (int i = tid; i < n_seg; i += n_thr) {
-        const Segment s = i == tid ? mine : load_segment(p, i);
-        if (s.ntok * p.G > p.few_rows) items[0] += (long long)tok_tiles(p, s.ntok) * max(1, (pages_of(s) + tc - 1) / tc);
-      }
-      block_sums<1>(items, sums);
-      const long long n = items[0] * p.Hkv;
-      if (n <= p.tile_target) break;
-      tc = (int)(((long long)tc * n / p.tile_target + 8) & ~7LL);
+    if (s.few) {
+      v[0] += (long long)few_tiles(p, s.ntok) * p.Hkv * pages_of(s);
+    } else {
+      const int n = tok_tiles(p, s.ntok) * p.Hkv;
+      v[1] += n;
+      v[2] += (long long)n * pages_of(s);
     }
   }
+  block_sums<3>(v, sums);
+  const int per_warp = (int)max((long long)kRowRunMin, (v[0] + p.row_warps - 1) / p.row_warps);
+  // Key chunks.  Little work (up to 24 key tiles a block): one wave of equal chunks, a tile of w pages giving ceil(w/c)
+  // items, on average w/c + 1/2.  More work: chunks of a third of a block's share, so that the counter can balance them.
+  const long long share = (v[2] + p.tile_target - 1) / p.tile_target;
+  const bool wave = share <= 24 * 8 && v[1] < p.tile_target;
+  long long tc = wave ? (v[2] + p.tile_target - v[1] / 2 - 1) / (p.tile_target - v[1] / 2) : (share + 2) / 3;
+  tc = (max(tc, (long long)(wave ? kTileChunkMin : 16 * 8)) + 7) & ~7LL;  // whole key tiles
+  for (int round = 0; wave && round < 3; ++round) {  // one wave should stay one: count, and lengthen by what is too much
+    long long items[1] = {0};
+    for (int i = tid; i < n_seg; i += n_thr) {
+      const Segment s = i == tid ? mine : load_segment(p, i);
+      if (!s.few) items[0] += (long long)tok_tiles(p, s.ntok) * p.Hkv * max(1LL, (pages_of(s) + tc - 1) / tc);
+    }
+    block_sums<1>(items, sums);
+    if (items[0] <= p.tile_target) break;
+    tc = (tc * items[0] / p.tile_target + 8) & ~7LL;
+  }
 
-  int row_base = 0, tile_base = 0, part_base = 0, split = 0;
+  long long base[3] = {0, 0, 0};  // units, tile items, partial rows so far
+  int merge = 0;
   for (int i0 = 0; i0 < n_seg; i0 += n_thr) {
     const int i = i0 + tid;
     Segment s;
     s.ntok = 0;
     s.chunks = 1;
-    int cnt[3] = {0, 0, 0};  // row items, tile items, partial rows
+    long long cnt[3] = {0, 0, 0};
     if (i < n_seg) {
       s = i0 == 0 ? mine : load_segment(p, i);
-      const bool few = s.ntok * p.G <= p.few_rows;
-      s.chunk_pages = few ? rc : tc;
-      s.chunks = max(1, (pages_of(s) + s.chunk_pages - 1) / s.chunk_pages);
-      cnt[few ? 0 : 1] = (few ? row_tiles(p, s.ntok) : tok_tiles(p, s.ntok)) * s.chunks;
-      if (s.chunks > 1 || p.always_partial) cnt[2] = s.chunks * s.ntok * p.Hq;
-      split |= s.chunks > 1;
+      const int pages = pages_of(s);
+      if (s.few) {
+        s.units = pages;
+        cnt[0] = (long long)few_tiles(p, s.ntok) * p.Hkv * pages;
+        // a run of `pages` units touches at most so many warps
+        cnt[2] = (long long)s.ntok * p.Hq * ((pages + per_warp - 1) / per_warp + 1);
+      } else {
+        s.chunks = (int)max(1LL, (pages + tc - 1) / tc);
+        s.chunk_pages = s.chunks == 1 ? 0x3fffffff : ((pages + s.chunks - 1) / s.chunks + 7) & ~7;  // equal ones
+        cnt[1] = tok_tiles(p, s.ntok) * s.chunks;
+        if (s.chunks > 1 || p.always_partial) cnt[2] = (long long)s.chunks * s.ntok * p.Hq;
+      }
+      merge |= cnt[2] > 0;
     }
     // exclusive sums over the segments
-    int inc[3] = {cnt[0], cnt[1], cnt[2]};
+    long long inc[3] = {cnt[0], cnt[1], cnt[2]};
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1)
 #pragma unroll
       for (int k = 0; k < 3; ++k) {
-        const int x = __shfl_up_sync(0xffffffffu, inc[k], o);
+        const long long x = __shfl_up_sync(0xffffffffu, inc[k], o);
         if (lane >= o) inc[k] += x;
       }
     if (lane == 31)
 #pragma unroll
       for (int k = 0; k < 3; ++k) scan[warp][k] = inc[k];
     __syncthreads();
-    int at[3], total[3];
+    long long at[3];
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-      const int w = lane < n_warps ? scan[lane][k] : 0;
-      const int before = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0);
-      total[k] = __reduce_add_sync(0xffffffffu, w);
-      at[k] = before + inc[k] - cnt[k];
+      long long before = 0, total = 0;
+      for (int w = 0; w < n_warps; ++w) {
+        if (w < warp) before += scan[w][k];
+        total += scan[w][k];
+      }
+      at[k] = base[k] + before + inc[k] - cnt[k];
+      base[k] += total;
     }
     __syncthreads();
     if (i < n_seg) {
-      s.pbase = cnt[2] > 0 ? (int64_t)part_base + at[2] : -1;
+      s.start = at[0];
+      if (cnt[2] > 0) s.pbase = at[2];
       p.segs[i] = s;
     }
     // a few items: their thread writes them; many: the warp does, segment by segment
-    constexpr int kSelf = 4;
-    const auto row_item = [&](int seg, int ntok, int chunks, int k, int to) {
-      const int tile = k / chunks;
-      int r0 = tile * p.row_tile, end = ntok * p.G;
-      if (p.block_pages) {
-        const int per = (p.query_block * p.G + p.row_tile - 1) / p.row_tile, blk = tile / per;
-        r0 = blk * p.query_block * p.G + (tile - blk * per) * p.row_tile;
-        end = min(end, (blk + 1) * p.query_block * p.G);
-      }
-      if (to < p.row_cap) p.row_list[to] = make_int4(seg, r0, min(p.row_tile, end - r0), k - tile * chunks);
-    };
-    const auto tile_item = [&](int seg, int ntok, int chunks, int n, int k, int to) {
+    const auto tile_item = [&](int seg, int ntok, int chunks, int n, int k, long long to) {
       const int tile = n / chunks - 1 - k / chunks;  // the last tiles of a causal segment see most keys: first in the list
       int t0 = tile * 2 * p.tok_tile, end = ntok;
       if (p.block_pages) {
@@ -186,42 +181,46 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnPar
       }
       if (to < p.tile_cap) p.tile_list[to] = make_int4(seg, t0, min(2 * p.tok_tile, end - t0), k % chunks);
     };
-    const bool many = cnt[0] + cnt[1] > kSelf;
-    if (!many) {
-      for (int k = 0; k < cnt[0]; ++k) row_item(i, s.ntok, s.chunks, k, row_base + at[0] + k);
-      for (int k = 0; k < cnt[1]; ++k) tile_item(i, s.ntok, s.chunks, cnt[1], k, tile_base + at[1] + k);
-    }
+    const bool many = cnt[1] > 4;
+    if (!many)
+      for (int k = 0; k < (int)cnt[1]; ++k) tile_item(i, s.ntok, s.chunks, (int)cnt[1], k, at[1] + k);
     for (uint32_t left = __ballot_sync(0xffffffffu, many); left; left &= left - 1) {
       const int l = __ffs(left) - 1, seg = i0 + warp * 32 + l;
       const int ntok = __shfl_sync(0xffffffffu, s.ntok, l), chunks = __shfl_sync(0xffffffffu, s.chunks, l);
-      const int nr = __shfl_sync(0xffffffffu, cnt[0], l), nt = __shfl_sync(0xffffffffu, cnt[1], l);
-      const int rb = row_base + __shfl_sync(0xffffffffu, at[0], l), tb = tile_base + __shfl_sync(0xffffffffu, at[1], l);
-      for (int k = lane; k < nr; k += 32) row_item(seg, ntok, chunks, k, rb + k);
+      const int nt = __shfl_sync(0xffffffffu, (int)cnt[1], l);
+      const long long tb = __shfl_sync(0xffffffffu, at[1], l);
       for (int k = lane; k < nt; k += 32) tile_item(seg, ntok, chunks, nt, k, tb + k);
     }
-    row_base += total[0];
-    tile_base += total[1];
-    part_base += total[2];
   }
-  split = __syncthreads_or(split);
+  merge = __syncthreads_or(merge);
   if (tid == 0) {
-    p.hdr->row_items = min(row_base, p.row_cap);
-    p.hdr->tile_items = min(tile_base, p.tile_cap);
-    p.hdr->split = split;
+    p.hdr->units = base[0];
+    p.hdr->per_warp = per_warp;
+    p.hdr->tile_items = (int)min(base[1], (long long)p.tile_cap);
+    p.hdr->merge = merge;
     p.hdr->next_tile = 0;
   }
 }
 
 // ---- row kernel -----------------------------------------------------------------------------------
-// Block = one item: up to 8*NT rows of a segment for one KV head, over one chunk of its pages.  Its four warps take
-// the pages in turn, each through a ring of its own (three pages of K and V, 16-byte async copies, rows 256 bytes
-// with the 16-byte pieces rotated by the row so that ldmatrix is free of bank conflicts), and meet once at the end.
+// A warp works on its own: per_warp consecutive units of the line, a unit being one page for one tile of up to 8*NT rows of a
+// segment and one KV head (the order is segment, tile, KV head, page).  Pages come through a ring of the warp's own (three
+// pages of K and V, 16-byte async copies, rows of 256 bytes with the 16-byte pieces rotated by the row so that
+// ldmatrix is free of bank conflicts), and the copies run two pages ahead across the ends of (tile, KV head) pieces, the
+// next piece's query rows with its first page: reading does not pause where a piece ends.
 //   S[row][token] = Q K^T   m16n8k16, rows the M side (rows 8-15 are zero for NT = 1), K rows the B operand
 //   O^T[channel][row] += V^T P^T: P as the B operand has the layout of the S accumulators.
+// Each piece leaves a partial result per row; a (tile, KV head) that several warps share has one from each.
 // Bound by reading K and V.
-constexpr int kRowWarps = 4, kRowStages = 3;
-constexpr int kRowStageBytes = 2 * kPage * kD * 2;  // K page, V page: 8 KiB
-constexpr int kRowSmem = kRowWarps * kRowStages * kRowStageBytes;
+constexpr int kRowStages = 3;
+constexpr int kPageKV = 2 * kPage * kD * 2;  // K page, V page: 8 KiB
+template <int NT>
+struct RowShape {
+  static constexpr int kWarps = NT == 1 ? 8 : 7;  // what 227 KiB hold
+  static constexpr int kQBytes = 8 * NT * kD * 2;
+  static constexpr int kWarpBytes = kRowStages * kPageKV + 2 * kQBytes;
+  static constexpr int kSmem = kWarps * kWarpBytes;
+};
 
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
   const int n = real ? 16 : 0;
@@ -248,239 +247,279 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// A position in a warp's run: a piece is the part of one (tile, KV head) that the run covers.
+struct RowCursor {
+  int seg, tile, kvh;
+  int page, end;  // unit of the (tile, KV head), and where the piece ends
+  int left;       // units of the run from this one on
+  Segment s;
+
+  // the segment that holds unit x of the line
+  __device__ __forceinline__ void start(const AttnParams& p, long long x, int n) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = p.n_first + p.n_second;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) >> 5, c = lo + lane * step;
+      const int cnt = __popc(__ballot_sync(0xffffffffu, c < hi && p.segs[c].start <= x));
+      lo += (cnt > 0 ? cnt - 1 : 0) * step;
+      hi = min(hi, lo + step);
+    }
+    seg = lo;  // the last that starts at or before x; those after the last unit's start behind it
+    s = p.segs[seg];
+    const long long in = x - s.start;
+    const int piece = (int)(in / s.units);
+    tile = piece / p.Hkv;
+    kvh = piece - tile * p.Hkv;
+    page = (int)(in - (long long)piece * s.units);
+    left = n;
+    end = min(s.units, page + left);
+  }
+  // to the next unit; true when it is in another piece (or the run is over: left == 0)
+  __device__ __forceinline__ bool step(const AttnParams& p) {
+    --left;
+    if (++page < end) return false;
+    if (left > 0) {
+      page = 0;
+      if (++kvh == p.Hkv) {
+        kvh = 0;
+        if (++tile == few_tiles(p, s.ntok)) {
+          tile = 0;
+          do s = p.segs[++seg];
+          while (s.units == 0 || s.ntok == 0);
+        }
+      }
+      end = min(s.units, left);
+    }
+    return true;
+  }
+};
+
 template <typename T, int NT>
-__global__ void __launch_bounds__(kRowWarps * 32) prompt_rows_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(const AttnParams p) {
+  using Shape = RowShape<NT>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 ml_s[kRowWarps][8 * NT];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int n_items = p.hdr->row_items * p.Hkv;
-  uint8_t* ring = smem + warp * (kRowStages * kRowStageBytes);
-  const uint32_t ring_a = (uint32_t)__cvta_generic_to_shared(ring);
-  for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-    const int4 it = p.row_list[item / p.Hkv];
-    const int kvh = item % p.Hkv;
-    const Segment s = p.segs[it.x];
-    const int32_t* indices = (s.second ? p.indices2 : p.indices1) + s.kvbase;
-    const int tok_first = it.y / p.G, tok_last = (it.y + it.z - 1) / p.G;
-    // the pages: a run of the segment's, or of the block's list
+  const int per = p.hdr->per_warp;
+  const long long w_id = (long long)blockIdx.x * Shape::kWarps + warp, x0 = w_id * per, units = p.hdr->units;
+  if (x0 >= units) return;
+  const uint32_t ring_a = (uint32_t)__cvta_generic_to_shared(smem + warp * Shape::kWarpBytes);
+  const uint32_t q_a = ring_a + kRowStages * kPageKV;
+
+  RowCursor f, c;  // where the copies are, and the arithmetic
+  f.start(p, x0, (int)min((long long)per, units - x0));
+  c = f;
+  // lane j holds number 32*(page/32) + j of the piece's pages: logical page and physical id (or "none")
+  constexpr int kNone = 0x3fffff;  // a logical page behind every limit
+  int my_lp = kNone, my_phys = -1, window = -1, window_seg = -1;
+  const auto look_up = [&]() {
+    const int w = f.page >> 5;
+    if (w == window && f.seg == window_seg && !p.block_pages) return;  // another KV head of the same pages
+    window = w;
+    window_seg = f.seg;
+    int n = f.s.npages;
     const int32_t* list = nullptr;
-    int n_avail = pages_seen(s, tok_last, p.causal);
     if (p.block_pages) {
-      const int64_t slot = (int64_t)(s.tok0 / p.query_block + it.x + tok_first / p.query_block) * p.Hkv + kvh;
+      const int tok = f.tile * p.row_tile / p.G;
+      const int64_t slot = (int64_t)(f.s.tok0 / p.query_block + f.seg + tok / p.query_block) * p.Hkv + f.kvh;
+      n = min(max(p.block_npages[slot], 0), p.max_k);
       list = p.block_pages + slot * p.max_k;
-      n_avail = min(max(p.block_npages[slot], 0), p.max_k);
     }
-    const int first = it.w * s.chunk_pages;  // chunk_pages can be "all": the product is only used for chunk 0 then
-    const int n_pg = max(0, min(n_avail - first, s.chunk_pages));
-    // rows g and g + 8 of the tile: query row, and the last position it sees
-    uint32_t qa[8][2 * NT];
-    int limit[NT];
-#pragma unroll
-    for (int h = 0; h < NT; ++h) {
-      const int r = g + 8 * h;
-      const bool ok = r < it.z;
-      const int row = it.y + (ok ? r : 0), tok = row / p.G, head = kvh * p.G + row % p.G;
-      limit[h] = !ok ? -1 : p.causal ? s.len - s.ntok + tok : s.len - 1;
-      const T* src = static_cast<const T*>(p.q) + (int64_t)(s.tok0 + tok) * p.q_ts + head * kD;
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        qa[ks][h] = ok ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 2 * t) : 0u;
-        qa[ks][NT + h] = ok ? *reinterpret_cast<const uint32_t*>(src + 16 * ks + 8 + 2 * t) : 0u;
+    const int at = 32 * w + lane;
+    my_lp = kNone;
+    my_phys = -1;
+    if (at < n) {
+      my_lp = list ? list[at] : at;
+      if (my_lp >= 0 && my_lp < f.s.npages) my_phys = ((f.s.second ? p.indices2 : p.indices1) + f.s.kvbase)[my_lp];
+      if (my_phys < 0 || my_phys >= p.num_pages_total) {
+        raise_flag(p.status, TWL_FLAG_BAD_INDEX);
+        my_phys = -1;
+        my_lp = kNone;
       }
     }
-    const int sure = p.causal ? s.len - s.ntok + tok_first : s.len - 1;  // every row sees positions up to here
-    float o[8][NT][4], m[NT], l[NT];
+  };
+  int f_unit = 0, f_piece = 0;  // units and pieces whose copies were issued
+  bool f_first = true;
+  // the next page (and, before a piece's first, its query rows) into the ring; returns the logical page
+  const auto fetch = [&]() -> int {
+    int lp = kNone;
+    if (f.left > 0) {
+      if (f_first || (f.page & 31) == 0) look_up();
+      if (f_first) {
+        const uint32_t dst = q_a + (f_piece & 1) * Shape::kQBytes;
+        const int r0 = f.tile * p.row_tile, n = min(p.row_tile, f.s.ntok * p.G - r0);
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
-#pragma unroll
-      for (int h = 0; h < NT; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[c][h][e] = 0.f;
-#pragma unroll
-    for (int h = 0; h < NT; ++h) {
-      m[h] = -INFINITY;
-      l[h] = 0.f;
-    }
-    // this warp's pages are first + warp + 4*i; lane j holds number 32*k + j of them: logical page and physical id
-    const int mine = (n_pg - warp + kRowWarps - 1) / kRowWarps;
-    int my_lp = 0, my_phys = -1;
-    auto look_up = [&](int k) {
-      const int i = 32 * k + lane;
-      my_lp = 0x3fffff;
-      my_phys = -1;
-      if (i < mine) {
-        const int at = first + warp + kRowWarps * i;
-        my_lp = list ? list[at] : at;
-        if (my_lp >= 0 && my_lp < s.npages) my_phys = indices[my_lp];
-        if (my_phys < 0 || my_phys >= p.num_pages_total) {
-          raise_flag(p.status, TWL_FLAG_BAD_INDEX);
-          my_phys = -1;
-          my_lp = 0x3fffff;  // behind every limit
+        for (int j = 0; j < 4 * NT; ++j) {
+          const int piece = 32 * j + lane, r = piece >> 4, cc = piece & 15;
+          const int row = r0 + (r < n ? r : 0), tok = row / p.G;
+          cp_async16_or_zero(dst + r * 256 + ((cc ^ (r & 7)) << 4),
+                             static_cast<const T*>(p.q) + (int64_t)(f.s.tok0 + tok) * p.q_ts +
+                                 (f.kvh * p.G + row - tok * p.G) * kD + cc * 8,
+                             r < n);
         }
+        ++f_piece;
       }
-    };
-    auto fetch = [&](int i, int lp, int phys) {
-      const uint32_t dst = ring_a + (i % kRowStages) * kRowStageBytes;
+      lp = __shfl_sync(0xffffffffu, my_lp, f.page & 31);
+      const int phys = __shfl_sync(0xffffffffu, my_phys, f.page & 31);
+      const uint32_t dst = ring_a + (f_unit % kRowStages) * kPageKV;
       const bool ok = phys >= 0;
-      const size_t slab = ((size_t)(ok ? phys : 0) * p.Hkv + kvh) * (kPage * kD);
+      const size_t slab = ((size_t)(ok ? phys : 0) * p.Hkv + f.kvh) * (kPage * kD);
       const T* ksrc = static_cast<const T*>(p.k_pages) + slab;
       const T* vsrc = static_cast<const T*>(p.v_pages) + slab;
-      const int valid = ok ? min(kPage, s.len - lp * kPage) : 0;  // rows behind the sequence read as zero
+      const int valid = ok ? min(kPage, f.s.len - lp * kPage) : 0;  // rows behind the sequence read as zero
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int piece = 32 * j + lane, row = piece >> 4, c = piece & 15;
-        const uint32_t to = dst + row * 256 + ((c ^ (row & 7)) << 4);
+        const int piece = 32 * j + lane, row = piece >> 4, cc = piece & 15;
+        const uint32_t to = dst + row * 256 + ((cc ^ (row & 7)) << 4);
         cp_async16_or_zero(to, ksrc + piece * 8, row < valid);
         cp_async16_or_zero(to + kPage * kD * 2, vsrc + piece * 8, row < valid);
       }
-    };
-    look_up(0);
-    int next_lp, next_phys;
-#pragma unroll
-    for (int i = 0; i < kRowStages - 1; ++i) {
-      next_lp = __shfl_sync(0xffffffffu, my_lp, i);
-      next_phys = __shfl_sync(0xffffffffu, my_phys, i);
-      if (i < mine) fetch(i, next_lp, next_phys);
-      cp_async_commit();
+      ++f_unit;
+      f_first = f.step(p);
     }
-    int lp_ring[kRowStages - 1];  // logical pages of the stages in flight
+    cp_async_commit();
+    return lp;
+  };
+
+  uint32_t qa[8][2 * NT];
+  int limit[NT], sure = 0;
+  float o[8][NT][4], m[NT], l[NT];
+  bool first = true;
+  int unit = 0, piece = 0;
+  int lp_ring[kRowStages - 1];  // logical pages of the stages in flight
 #pragma unroll
-    for (int i = 0; i < kRowStages - 1; ++i) lp_ring[i] = __shfl_sync(0xffffffffu, my_lp, i);
-    for (int i = 0; i < mine; ++i) {
-      const int ahead = i + kRowStages - 1;
-      if ((ahead & 31) == 0) look_up(ahead >> 5);
-      next_lp = __shfl_sync(0xffffffffu, my_lp, ahead & 31);
-      next_phys = __shfl_sync(0xffffffffu, my_phys, ahead & 31);
-      if (ahead < mine) fetch(ahead, next_lp, next_phys);
-      cp_async_commit();
-      cp_async_wait<kRowStages - 1>();
-      __syncwarp();
-      const int lp = lp_ring[0];
-#pragma unroll
-      for (int j = 0; j + 1 < kRowStages - 1; ++j) lp_ring[j] = lp_ring[j + 1];
-      lp_ring[kRowStages - 2] = next_lp;
-      const uint32_t base = ring_a + (i % kRowStages) * kRowStageBytes;
-      const int fr = (lane & 7) + ((lane >> 4) << 3), fc = (lane >> 3) & 1;  // ldmatrix row and piece of this lane
-      float sc[2][4] = {};
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        uint32_t b[4];
-        ldsm4(b, base + fr * 256 + (((2 * ks + fc) ^ (fr & 7)) << 4));
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-          MmaTile<T>::run(sc[n], qa[ks][0], NT == 2 ? qa[ks][1] : 0u, qa[ks][NT], NT == 2 ? qa[ks][NT + 1] : 0u,
-                          b[2 * n], b[2 * n + 1]);
-      }
-      uint32_t pb[NT][2];
-      float f[NT];
-      bool moved = false;
-      const int pos = lp * kPage + 2 * t;
+  for (int i = 0; i < kRowStages - 1; ++i) lp_ring[i] = fetch();
+  const int fr = (lane & 7) + ((lane >> 4) << 3), fc = (lane >> 3) & 1;  // ldmatrix row and piece of this lane
+  while (c.left > 0) {
+    cp_async_wait<kRowStages - 2>();
+    __syncwarp();
+    if (first) {
+      const uint32_t src = q_a + (piece & 1) * Shape::kQBytes;
+      const int r0 = c.tile * p.row_tile, n = min(p.row_tile, c.s.ntok * p.G - r0);
 #pragma unroll
       for (int h = 0; h < NT; ++h) {
-        float x[4] = {sc[0][2 * h] * p.scale_log2, sc[0][2 * h + 1] * p.scale_log2, sc[1][2 * h] * p.scale_log2,
-                      sc[1][2 * h + 1] * p.scale_log2};
-        if (lp * kPage + kPage - 1 > sure) {
-          if (pos > limit[h]) x[0] = -INFINITY;
-          if (pos + 1 > limit[h]) x[1] = -INFINITY;
-          if (pos + 8 > limit[h]) x[2] = -INFINITY;
-          if (pos + 9 > limit[h]) x[3] = -INFINITY;
-        }
-        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[h], mx);
-        const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far: every weight is 2^-inf = 0
-        f[h] = ex2(m[h] - ref);
-        moved |= mn != m[h];
-        m[h] = mn;
+        const int r = g + 8 * h;
+        limit[h] = r >= n ? -1 : p.causal ? c.s.len - c.s.ntok + (r0 + r) / p.G : c.s.len - 1;
+        m[h] = -INFINITY;
+        l[h] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = ex2(x[e] - ref);
-        l[h] = l[h] * f[h] + (x[0] + x[1]) + (x[2] + x[3]);
-        // weights go to the tensor cores in the model type (half a step of it each); their sum stays unrounded
-        pb[h][0] = pack2<T>(x[0], x[1]);
-        pb[h][1] = pack2<T>(x[2], x[3]);
+        for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            asm volatile("ld.shared.u32 %0, [%1];"
+                         : "=r"(qa[ks][e * NT + h])
+                         : "r"(src + r * 256 + (((2 * ks + e) ^ g) << 4) + 4 * t));
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[k][h][e] = 0.f;
       }
-      if (__any_sync(0xffffffffu, moved)) {
+      sure = p.causal ? c.s.len - c.s.ntok + r0 / p.G : c.s.len - 1;  // every row sees positions up to here
+      ++piece;
+      __syncwarp();  // before the slot is filled again
+    }
+    const int lp = lp_ring[0];
 #pragma unroll
-        for (int h = 0; h < NT; ++h) {  // accumulator columns are rows 2t and 2t+1 of the half
-          const float f0 = __shfl_sync(0xffffffffu, f[h], 8 * t), f1 = __shfl_sync(0xffffffffu, f[h], 8 * t + 4);
+    for (int j = 0; j + 1 < kRowStages - 1; ++j) lp_ring[j] = lp_ring[j + 1];
+    lp_ring[kRowStages - 2] = fetch();
+
+    const uint32_t base = ring_a + (unit % kRowStages) * kPageKV;
+    float sc[2][4] = {};
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            o[c][h][0] *= f0;
-            o[c][h][1] *= f1;
-            o[c][h][2] *= f0;
-            o[c][h][3] *= f1;
+    for (int ks = 0; ks < 8; ++ks) {
+      uint32_t b[4];
+      ldsm4(b, base + fr * 256 + (((2 * ks + fc) ^ (fr & 7)) << 4));
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+        MmaTile<T>::run(sc[n], qa[ks][0], NT == 2 ? qa[ks][1] : 0u, qa[ks][NT], NT == 2 ? qa[ks][NT + 1] : 0u, b[2 * n],
+                        b[2 * n + 1]);
+    }
+    uint32_t pb[NT][2];
+    float fac[NT];
+    bool moved = false;
+    const int pos = lp * kPage + 2 * t;
+#pragma unroll
+    for (int h = 0; h < NT; ++h) {
+      float x[4] = {sc[0][2 * h] * p.scale_log2, sc[0][2 * h + 1] * p.scale_log2, sc[1][2 * h] * p.scale_log2,
+                    sc[1][2 * h + 1] * p.scale_log2};
+      if (lp * kPage + kPage - 1 > sure) {
+        if (pos > limit[h]) x[0] = -INFINITY;
+        if (pos + 1 > limit[h]) x[1] = -INFINITY;
+        if (pos + 8 > limit[h]) x[2] = -INFINITY;
+        if (pos + 9 > limit[h]) x[3] = -INFINITY;
+      }
+      float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[h], mx);
+      const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far: every weight is 2^-inf = 0
+      fac[h] = ex2(m[h] - ref);
+      moved |= mn != m[h];
+      m[h] = mn;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = ex2(x[e] - ref);
+      l[h] = l[h] * fac[h] + (x[0] + x[1]) + (x[2] + x[3]);
+      // weights go to the tensor cores in the model type (half a step of it each); their sum stays unrounded
+      pb[h][0] = pack2<T>(x[0], x[1]);
+      pb[h][1] = pack2<T>(x[2], x[3]);
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int h = 0; h < NT; ++h) {  // accumulator columns are rows 2t and 2t+1 of the half
+        const float f0 = __shfl_sync(0xffffffffu, fac[h], 8 * t), f1 = __shfl_sync(0xffffffffu, fac[h], 8 * t + 4);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          o[k][h][0] *= f0;
+          o[k][h][1] *= f1;
+          o[k][h][2] *= f0;
+          o[k][h][3] *= f1;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint32_t a[4];
+      ldsm4t(a, base + kPage * kD * 2 + fr * 256 + (((2 * k + fc) ^ (fr & 7)) << 4));
+#pragma unroll
+      for (int h = 0; h < NT; ++h) MmaTile<T>::run(o[k][h], a[0], a[1], a[2], a[3], pb[h][0], pb[h][1]);
+    }
+    ++unit;
+    if (c.page + 1 == c.end) {  // the piece's results: one for each row
+      const int r0 = c.tile * p.row_tile, n = min(p.row_tile, c.s.ntok * p.G - r0);
+      const long long first_unit = c.s.start + ((long long)c.tile * p.Hkv + c.kvh) * c.s.units;
+      const int64_t slot0 = c.s.pbase + (w_id - first_unit / per) * c.s.ntok * p.Hq + c.kvh * p.G;
+      const auto slot_of = [&](int r) {
+        const int row = r0 + r, tok = row / p.G;
+        return slot0 + (int64_t)tok * p.Hq + (row - tok * p.G);
+      };
+#pragma unroll
+      for (int h = 0; h < NT; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        if (t == 0 && g + 8 * h < n) {
+          const int64_t slot = slot_of(g + 8 * h);
+          if (slot < p.part_cap) p.part_ml[slot] = make_float2(m[h], l[h]);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 8 * h + 2 * t + e;
+          if (r >= n) continue;
+          const int64_t slot = slot_of(r);
+          if (slot >= p.part_cap) continue;
+          float* to = p.part_acc + slot * kD + g;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            to[16 * k] = o[k][h][e];
+            to[16 * k + 8] = o[k][h][2 + e];
           }
         }
       }
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint32_t a[4];
-        ldsm4t(a, base + kPage * kD * 2 + fr * 256 + (((2 * c + fc) ^ (fr & 7)) << 4));
-#pragma unroll
-        for (int h = 0; h < NT; ++h) MmaTile<T>::run(o[c][h], a[0], a[1], a[2], a[3], pb[h][0], pb[h][1]);
-      }
-      __syncwarp();  // the stage is refilled in the next round
     }
-    cp_async_wait<0>();
-    // the four warps' results meet in shared memory: [warp][row][channel], a padded row per warp
-#pragma unroll
-    for (int h = 0; h < NT; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      if (t == 0) ml_s[warp][g + 8 * h] = make_float2(m[h], l[h]);
-    }
-    __syncthreads();  // every warp is done with its ring
-    float* acc_s = reinterpret_cast<float*>(smem);
-    constexpr int kRowPitch = kD + 4;
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-#pragma unroll
-      for (int h = 0; h < NT; ++h) {
-        float* to = acc_s + (warp * 8 * NT + 8 * h + 2 * t) * kRowPitch + 16 * c + g;
-        to[0] = o[c][h][0];
-        to[kRowPitch] = o[c][h][1];
-        to[8] = o[c][h][2];
-        to[kRowPitch + 8] = o[c][h][3];
-      }
-    __syncthreads();
-    for (int r = warp; r < it.z; r += kRowWarps) {
-      float mm = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) mm = fmaxf(mm, ml_s[w][r].x);
-      const float ref = mm == -INFINITY ? 0.f : mm;
-      float ll = 0.f;
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) {
-        const float2 v = ml_s[w][r];
-        const float fw = ex2(v.x - ref);
-        ll += v.y * fw;
-        const float4 x = *reinterpret_cast<const float4*>(acc_s + (w * 8 * NT + r) * kRowPitch + 4 * lane);
-        a.x += x.x * fw;
-        a.y += x.y * fw;
-        a.z += x.z * fw;
-        a.w += x.w * fw;
-      }
-      const int row = it.y + r, tok = row / p.G, head = kvh * p.G + row % p.G;
-      if (s.pbase >= 0) {
-        const int64_t slot = s.pbase + ((int64_t)it.w * s.ntok + tok) * p.Hq + head;
-        if (slot < p.part_cap) {
-          if (ll != 0.f) *reinterpret_cast<float4*>(p.part_acc + slot * kD + 4 * lane) = a;
-          if (lane == 0) p.part_ml[slot] = make_float2(mm, ll);
-        }
-      } else {
-        const float inv = ll != 0.f ? 1.f / ll : 0.f;
-        T* to = static_cast<T*>(p.out) + (int64_t)(s.tok0 + tok) * p.o_ts + head * kD + 4 * lane;
-        *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
-        if (p.lse && lane == 0)
-          p.lse[(int64_t)(s.tok0 + tok) * p.Hq + head] = ll != 0.f ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
-      }
-    }
-    __syncthreads();  // before the next item's copies
+    first = c.step(p);
+    __syncwarp();  // the stage is refilled in the next round
   }
+  cp_async_wait<0>();
 }
 
 // ---- merge -----------------------------------------------------------------------------------------
@@ -488,7 +527,8 @@ __global__ void __launch_bounds__(kRowWarps * 32) prompt_rows_kernel(const AttnP
 template <typename T>
 __global__ void __launch_bounds__(256) prompt_merge_kernel(const AttnParams p) {
   pdl_wait();
-  if (!p.always_partial && p.hdr->split == 0) return;
+  if (p.hdr->merge == 0) return;
+  const int per = p.hdr->per_warp;
   const int lane = threadIdx.x & 31;
   const int64_t rows = (int64_t)p.num_tokens * p.Hq;
   for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += (int64_t)gridDim.x * 8) {
@@ -518,8 +558,14 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const AttnParams p) {
       found = true;
       // a lane takes a chunk's maximum and sum; the accumulators follow, four in flight
       const int64_t slot0 = s.pbase + (int64_t)(tok - s.tok0) * p.Hq + head, step = (int64_t)s.ntok * p.Hq;
-      for (int c0 = 0; c0 < s.chunks; c0 += 32) {
-        const int n = min(32, s.chunks - c0);
+      int chunks = s.chunks;
+      if (s.few) {  // the warps whose runs touch the row's (tile, KV head)
+        const int kvh = head / p.G, tile = ((tok - s.tok0) * p.G + head - kvh * p.G) / p.row_tile;
+        const long long u = s.start + ((long long)tile * p.Hkv + kvh) * s.units;
+        chunks = s.units ? (int)((u + s.units - 1) / per - u / per) + 1 : 0;
+      }
+      for (int c0 = 0; c0 < chunks; c0 += 32) {
+        const int n = min(32, chunks - c0);
         float2 v = make_float2(-INFINITY, 0.f);
         if (lane < n && slot0 + (c0 + lane) * step < p.part_cap) v = p.part_ml[slot0 + (c0 + lane) * step];
         const float mn = fmaxf(m, warp_max(v.x)), ref = mn == -INFINITY ? 0.f : mn;
@@ -560,39 +606,39 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const AttnParams p) {
 
 // ---- host ------------------------------------------------------------------------------------------
 struct WorkspaceLayout {
-  size_t hdr, segs, row_list, tile_list, acc, ml, total;
+  size_t hdr, segs, tile_list, acc, ml, total;
   int64_t rows;
-  int32_t row_cap, tile_cap;
+  int32_t tile_cap;
 };
 
 static inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-constexpr int kTilesPerSm = 1;
-constexpr int kRowBlocksPerSm = 2;
-
-// `tokens` query tokens in n_seg segments; prefix: every row has partial results of both its segments.
+// Query tokens in n_seg segments; prefix: every row has partial results of both its segments.
 static WorkspaceLayout workspace_layout(int64_t tokens, int64_t n_seg, int64_t Hq, int64_t Hkv, int64_t max_pages,
                                         int64_t query_block, bool prefix) {
   WorkspaceLayout w;
-  const int64_t G = Hq / Hkv, row_target = (int64_t)num_sms() * kRowBlocksPerSm * 2, tile_target = num_sms() * kTilesPerSm;
-  const int64_t tt = kPage * 8 / G;  // tokens of a 128-row tile
-  const int64_t blocks = query_block > 0 ? tokens / query_block + n_seg : n_seg;  // runs that are cut into tiles
-  // items per KV head without key chunks, and at most two targets more where keys are split
-  const int64_t row_u = n_seg * (kFewRows / 8);  // at most 16 rows a segment, in tiles of 8 or 16
-  const int64_t tile_u = tokens / (2 * tt) + blocks;
-  w.row_cap = (int32_t)(row_u + 2 * row_target + 1);
-  w.tile_cap = (int32_t)(tile_u + 2 * tile_target + 1);
-  const int64_t chunks = (max_pages + kRowChunkMin - 1) / kRowChunkMin;
-  const int64_t most = tokens * Hq * (prefix ? 2 * chunks : chunks);
-  const int64_t split = 2 * row_target * 16 + 2 * tile_target * 2 * tt * G + (prefix ? 2 * tokens * Hq : 0);
-  w.rows = !prefix && chunks <= 1 ? 0 : most < split ? most : split;
+  const int64_t G = Hq / Hkv, warps = (int64_t)num_sms() * RowShape<1>::kWarps, blocks = num_sms();
+  const int64_t tt = 128 / G;  // tokens of a 128-row tile
+  const int64_t runs = query_block > 0 ? tokens / query_block + n_seg : n_seg;  // tokens that are cut into tiles together
+  const auto least = [](int64_t a, int64_t b) { return a < b ? a : b; };
+  // tiles per KV head without key chunks, and at most six times the blocks more where keys are split: those of one wave, or of
+  // more work the items longer than a third of a block's share, each cut into fewer pieces than it has thirds plus one
+  w.tile_cap = (int32_t)(tokens / (2 * tt) + runs + 6 * blocks + 1);
+  // partial rows of the row kernel: at most 16 rows a segment and KV head, one result from each warp that touches them,
+  // which are the warps and one or two more for each
+  const int64_t few = least(tokens * Hq * (prefix ? 2 : 1), n_seg * kFewRows * Hkv);
+  const int64_t row_parts = least(few * ((max_pages + kRowRunMin - 1) / kRowRunMin + 1), few * 2 + warps * kFewRows);
+  // and of the tile kernel
+  const int64_t whole = tokens * Hq * ((max_pages + kTileChunkMin - 1) / kTileChunkMin);
+  const int64_t tile_parts = tokens * G <= kFewRows ? 0
+                             : !prefix && max_pages <= kTileChunkMin ? 0
+                                                                     : least(whole, 6 * blocks * 2 * tt * G + (prefix ? tokens * Hq : 0));
+  w.rows = row_parts + tile_parts;
   size_t at = 0;
   w.hdr = at;
   at = up256(at + sizeof(PlanHeader));
   w.segs = at;
   at = up256(at + sizeof(Segment) * n_seg);
-  w.row_list = at;
-  at = up256(at + sizeof(int4) * w.row_cap);
   w.tile_list = at;
   at = up256(at + sizeof(int4) * w.tile_cap);
   w.ml = at;
@@ -607,37 +653,33 @@ static void place_workspace(AttnParams& p, const WorkspaceLayout& w, void* works
   uint8_t* base = static_cast<uint8_t*>(workspace);
   p.hdr = reinterpret_cast<PlanHeader*>(base + w.hdr);
   p.segs = reinterpret_cast<Segment*>(base + w.segs);
-  p.row_list = reinterpret_cast<int4*>(base + w.row_list);
   p.tile_list = reinterpret_cast<int4*>(base + w.tile_list);
   p.part_ml = reinterpret_cast<float2*>(base + w.ml);
   p.part_acc = reinterpret_cast<float*>(base + w.acc);
   p.part_cap = w.rows;
-  p.row_cap = w.row_cap;
   p.tile_cap = w.tile_cap;
-  p.row_target = num_sms() * kRowBlocksPerSm * 2;
-  p.tile_target = num_sms() * kTilesPerSm;
+  p.row_warps = num_sms() * (p.row_tile == 8 ? RowShape<1>::kWarps : RowShape<2>::kWarps);
+  p.tile_target = num_sms();
+}
+
+template <typename T, int NT>
+static int launch_rows(const AttnParams& p, cudaStream_t st) {
+  TWL_CUDA_TRY(cudaFuncSetAttribute(prompt_rows_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    RowShape<NT>::kSmem));
+  TWL_CUDA_TRY(launch_chain(prompt_rows_kernel<T, NT>, dim3((unsigned)num_sms()), dim3(RowShape<NT>::kWarps * 32),
+                            RowShape<NT>::kSmem, st, p));
+  return TWL_OK;
 }
 
 template <typename T>
-static int run_attention(const AttnParams& p, int dtype, bool need_merge, cudaStream_t st) {
+static int run_attention(const AttnParams& p, int dtype, cudaStream_t st) {
   const int plan_threads = p.n_first + p.n_second <= 256 ? 256 : kPlanThreads;
   TWL_CUDA_TRY(launch_chain(prompt_plan_kernel, dim3(1), dim3(plan_threads), 0, st, p));
-  const dim3 rows_grid((unsigned)(num_sms() * kRowBlocksPerSm));
-  if (p.row_tile == 8) {
-    TWL_CUDA_TRY(cudaFuncSetAttribute(prompt_rows_kernel<T, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem));
-    TWL_CUDA_TRY(launch_chain(prompt_rows_kernel<T, 1>, rows_grid, dim3(kRowWarps * 32), kRowSmem, st, p));
-  } else {
-    TWL_CUDA_TRY(cudaFuncSetAttribute(prompt_rows_kernel<T, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSmem));
-    TWL_CUDA_TRY(launch_chain(prompt_rows_kernel<T, 2>, rows_grid, dim3(kRowWarps * 32), kRowSmem, st, p));
-  }
-  if ((int64_t)p.num_tokens * p.G > p.few_rows) {
-    const int bad = tile_attention_launch(p, dtype, st);
-    if (bad != TWL_OK) return bad;
-  }
-  if (need_merge) {
-    const int64_t blocks = ((int64_t)p.num_tokens * p.Hq + 7) / 8, most = (int64_t)num_sms() * 8;
-    TWL_CUDA_TRY(launch_chain(prompt_merge_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, p));
-  }
+  int bad = p.row_tile == 8 ? launch_rows<T, 1>(p, st) : launch_rows<T, 2>(p, st);
+  if (bad == TWL_OK && (int64_t)p.num_tokens * p.G > kFewRows) bad = tile_attention_launch(p, dtype, st);
+  if (bad != TWL_OK) return bad;
+  const int64_t blocks = ((int64_t)p.num_tokens * p.Hq + 7) / 8, most = (int64_t)num_sms() * 8;
+  TWL_CUDA_TRY(launch_chain(prompt_merge_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, p));
   return TWL_OK;
 }
 
@@ -690,13 +732,12 @@ extern "C" int twl_prompt_attn(const void* q, int dtype, int64_t q_token_stride,
   p.block_pages = block_pages; p.block_npages = block_npages; p.max_k = max_k;
   p.query_block = query_block > 0 ? query_block : 1;
   p.num_tokens = num_tokens; p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = num_q_heads / num_kv_heads;
-  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; p.row_tile = 16; p.few_rows = kFewRows;
+  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; p.row_tile = 16;
   p.scale_log2 = sm_scale * 1.44269504088896341f;
   p.status = status;
   place_workspace(p, w, workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == TWL_F16 ? run_attention<__half>(p, dtype, w.rows > 0, st)
-                          : run_attention<__nv_bfloat16>(p, dtype, w.rows > 0, st);
+  return dtype == TWL_F16 ? run_attention<__half>(p, dtype, st) : run_attention<__nv_bfloat16>(p, dtype, st);
 }
 
 extern "C" size_t twl_shared_prefix_workspace_bytes(int32_t batch, int32_t num_groups, int32_t num_q_heads,
@@ -734,10 +775,10 @@ extern "C" int twl_shared_prefix_attn(const void* q, int dtype, int64_t q_token_
   p.qo2 = group_indptr; p.indptr2 = prefix_indptr; p.indices2 = prefix_indices; p.last2 = prefix_last_page_len;
   p.n_second = num_groups; p.always_partial = 1; p.query_block = 1;
   p.num_tokens = batch; p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = num_q_heads / num_kv_heads;
-  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; p.row_tile = p.G <= 8 ? 8 : 16; p.few_rows = kFewRows;
+  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; p.row_tile = p.G <= 8 ? 8 : 16;
   p.scale_log2 = sm_scale * 1.44269504088896341f;
   p.status = status;
   place_workspace(p, w, workspace);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == TWL_F16 ? run_attention<__half>(p, dtype, true, st) : run_attention<__nv_bfloat16>(p, dtype, true, st);
+  return dtype == TWL_F16 ? run_attention<__half>(p, dtype, st) : run_attention<__nv_bfloat16>(p, dtype, st);
 }

@@ -4,10 +4,11 @@
 // A call is a list of SEGMENTS: a run of consecutive query tokens that attend to the same pages.  prompt_attn has
 // one per sequence (causal); shared_prefix_attn one per sequence (its own pages) and one per group (the prefix, no
 // mask).  With G query heads per KV head, the rows of a segment for one KV head are its tokens x G, packed, so a
-// K/V page is read once for all of them.  A segment with at most kFewRows rows is cut into tiles of 8 or 16 rows for
-// the row kernel (warp-level tensor-core tiles: bound by reading K and V); longer ones into tiles of up to 256 rows
-// for the tile kernel.  Where there are fewer tiles than the GPU runs at once, the keys are cut into chunks too and
-// the partial (maximum, sum, accumulator) triples are joined by the merge kernel.
+// K/V page is read once for all of them.
+// Segments of at most kFewRows rows go to the row kernel (warp-level tensor-core tiles of 8 or 16 rows; bound by reading
+// K and V): all their (row tile, KV head, page) units in one line, cut into equal runs, one per warp of the GPU.  Longer
+// segments go to the tile kernel in tiles of up to 256 rows; where there are fewer of those than the GPU runs at once,
+// the keys are cut into chunks too.  Partial (maximum, sum, accumulator) triples are joined by the merge kernel.
 #pragma once
 #include "common.cuh"
 
@@ -19,16 +20,21 @@ struct Segment {
   int32_t tok0, ntok;     // query tokens
   int32_t kvbase, npages; // its part of kv_indices (or of the prefix's)
   int32_t len;            // tokens of the pages
-  int32_t chunks;         // key chunks of every tile
-  int32_t chunk_pages;    // pages of a chunk
+  int32_t units;          // row kernel: pages of a (row tile, KV head); 0 for the tile kernel's segments
+  int32_t chunks;         // tile kernel: key chunks of every tile
+  int32_t chunk_pages;    // and their pages
   int32_t second;         // 1: pages of the prefix table
+  int32_t few;            // 1: the row kernel's
+  int64_t start;          // row kernel: its first unit in the line
   int64_t pbase;          // first partial row, or -1 where tiles write the output themselves
 };
 
 struct PlanHeader {
-  int32_t row_items, tile_items;  // per KV head
-  int32_t split;                  // some output row is joined from partial results
-  int32_t next_tile;              // work counter of the tile kernel
+  int64_t units;         // of the row kernel
+  int32_t per_warp;      // units of a warp
+  int32_t tile_items;    // per KV head
+  int32_t merge;         // some output row is joined from partial results
+  int32_t next_tile;     // work counter of the tile kernel
 };
 
 struct AttnParams {
@@ -44,14 +50,13 @@ struct AttnParams {
   const int32_t *block_pages, *block_npages;
   int32_t max_k, query_block;
   int32_t num_tokens, Hq, Hkv, G, num_pages_total, tok_tile;
-  int32_t row_target, tile_target, row_tile, few_rows;
+  int32_t row_warps, tile_target, row_tile;
   float scale_log2;
   // workspace
   PlanHeader* hdr;
   Segment* segs;
-  int4* row_list;   // {segment, first packed row, rows, chunk}
   int4* tile_list;  // {segment, first token, tokens, chunk}
-  int32_t row_cap, tile_cap;
+  int32_t tile_cap;
   float* part_acc;  // [rows][128]
   float2* part_ml;  // [rows] {maximum in log2 units, sum}
   int64_t part_cap;
@@ -64,6 +69,9 @@ __device__ __forceinline__ int pages_seen(const Segment& s, int tok, int causal)
   const int pos = s.len - s.ntok + tok;
   return pos < 0 ? 0 : min(s.npages, (pos >> 4) + 1);
 }
+
+// row tiles of a segment of the row kernel
+__device__ __forceinline__ int few_tiles(const AttnParams& p, int ntok) { return (ntok * p.G + p.row_tile - 1) / p.row_tile; }
 
 int tile_attention_launch(const AttnParams& p, int dtype, cudaStream_t st);
 

@@ -248,6 +248,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // A position in a warp's run: a piece is the part of one (tile, KV head) that the run covers.
+template <int ROWS>
 struct RowCursor {
   int seg, tile, kvh;
   int page, end;  // unit of the (tile, KV head), and where the piece ends
@@ -282,7 +283,7 @@ struct RowCursor {
       page = 0;
       if (++kvh == p.Hkv) {
         kvh = 0;
-        if (++tile == few_tiles(p, s.ntok)) {
+        if (++tile * ROWS >= s.ntok * p.G) {
           tile = 0;
           do s = p.segs[++seg];
           while (s.units == 0 || s.ntok == 0);
@@ -307,9 +308,18 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
   const uint32_t ring_a = (uint32_t)__cvta_generic_to_shared(smem + warp * Shape::kWarpBytes);
   const uint32_t q_a = ring_a + kRowStages * kPageKV;
 
-  RowCursor f, c;  // where the copies are, and the arithmetic
+  constexpr int kRows = 8 * NT;
+  RowCursor<kRows> f, c;  // where the copies are, and the arithmetic
   f.start(p, x0, (int)min((long long)per, units - x0));
   c = f;
+  // Of the warps that share the first piece this is number `chunk`; every other piece begins in this run.
+  int chunk = (int)(w_id - (c.s.start + ((long long)c.tile * p.Hkv + c.kvh) * c.s.units) / per);
+  const uint32_t inv_g = 65536u / p.G + 1;  // row / G of the at most kFewRows rows of a segment
+  const auto tok_of = [&](int row) { return (int)((row * inv_g) >> 16); };
+  // where this lane's pieces of a page go: rows 2j + lane/16, piece lane%16 rotated by the row; j mod 4 decides the rotation
+  uint32_t to_off[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) to_off[j] = (2 * j + (lane >> 4)) * 256 + (((lane & 15) ^ (2 * j + (lane >> 4))) << 4);
   // lane j holds number 32*(page/32) + j of the piece's pages: logical page and physical id (or "none")
   constexpr int kNone = 0x3fffff;  // a logical page behind every limit
   int my_lp = kNone, my_phys = -1, window = -1, window_seg = -1;
@@ -321,7 +331,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
     int n = f.s.npages;
     const int32_t* list = nullptr;
     if (p.block_pages) {
-      const int tok = f.tile * p.row_tile / p.G;
+      const int tok = tok_of(f.tile * kRows);
       const int64_t slot = (int64_t)(f.s.tok0 / p.query_block + f.seg + tok / p.query_block) * p.Hkv + f.kvh;
       n = min(max(p.block_npages[slot], 0), p.max_k);
       list = p.block_pages + slot * p.max_k;
@@ -339,7 +349,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
       }
     }
   };
-  int f_unit = 0, f_piece = 0;  // units and pieces whose copies were issued
+  int f_stage = 0, f_piece = 0;  // stage of the next copies, pieces begun
   bool f_first = true;
   // the next page (and, before a piece's first, its query rows) into the ring; returns the logical page
   const auto fetch = [&]() -> int {
@@ -348,34 +358,38 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
       if (f_first || (f.page & 31) == 0) look_up();
       if (f_first) {
         const uint32_t dst = q_a + (f_piece & 1) * Shape::kQBytes;
-        const int r0 = f.tile * p.row_tile, n = min(p.row_tile, f.s.ntok * p.G - r0);
+        const int r0 = f.tile * kRows, n = min(kRows, f.s.ntok * p.G - r0);
+        const T* src = static_cast<const T*>(p.q) + (int64_t)f.s.tok0 * p.q_ts + f.kvh * p.G * kD + (lane & 15) * 8;
 #pragma unroll
         for (int j = 0; j < 4 * NT; ++j) {
-          const int piece = 32 * j + lane, r = piece >> 4, cc = piece & 15;
-          const int row = r0 + (r < n ? r : 0), tok = row / p.G;
-          cp_async16_or_zero(dst + r * 256 + ((cc ^ (r & 7)) << 4),
-                             static_cast<const T*>(p.q) + (int64_t)(f.s.tok0 + tok) * p.q_ts +
-                                 (f.kvh * p.G + row - tok * p.G) * kD + cc * 8,
-                             r < n);
+          const int r = 2 * j + (lane >> 4), row = r0 + (r < n ? r : 0), tok = tok_of(row);
+          cp_async16_or_zero(dst + to_off[j & 3] + (j >> 2) * 2048, src + tok * p.q_ts + (row - tok * p.G) * kD, r < n);
         }
         ++f_piece;
       }
       lp = __shfl_sync(0xffffffffu, my_lp, f.page & 31);
       const int phys = __shfl_sync(0xffffffffu, my_phys, f.page & 31);
-      const uint32_t dst = ring_a + (f_unit % kRowStages) * kPageKV;
-      const bool ok = phys >= 0;
-      const size_t slab = ((size_t)(ok ? phys : 0) * p.Hkv + f.kvh) * (kPage * kD);
-      const T* ksrc = static_cast<const T*>(p.k_pages) + slab;
-      const T* vsrc = static_cast<const T*>(p.v_pages) + slab;
-      const int valid = ok ? min(kPage, f.s.len - lp * kPage) : 0;  // rows behind the sequence read as zero
+      const uint32_t dst = ring_a + f_stage * kPageKV;
+      const size_t at = ((size_t)max(phys, 0) * p.Hkv + f.kvh) * (kPage * kD) + lane * 8;
+      const T* ksrc = static_cast<const T*>(p.k_pages) + at;
+      const T* vsrc = static_cast<const T*>(p.v_pages) + at;
+      if (phys >= 0 && f.s.len - lp * kPage >= kPage) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int piece = 32 * j + lane, row = piece >> 4, cc = piece & 15;
-        const uint32_t to = dst + row * 256 + ((cc ^ (row & 7)) << 4);
-        cp_async16_or_zero(to, ksrc + piece * 8, row < valid);
-        cp_async16_or_zero(to + kPage * kD * 2, vsrc + piece * 8, row < valid);
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t to = dst + to_off[j & 3] + (j >> 2) * 2048;
+          cp_async16(to, ksrc + j * 256);
+          cp_async16(to + kPage * kD * 2, vsrc + j * 256);
+        }
+      } else {  // rows behind the sequence (or of a page that is not there) read as zero
+        const int valid = phys >= 0 ? f.s.len - lp * kPage : 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t to = dst + to_off[j & 3] + (j >> 2) * 2048;
+          cp_async16_or_zero(to, ksrc + j * 256, 2 * j + (lane >> 4) < valid);
+          cp_async16_or_zero(to + kPage * kD * 2, vsrc + j * 256, 2 * j + (lane >> 4) < valid);
+        }
       }
-      ++f_unit;
+      if (++f_stage == kRowStages) f_stage = 0;
       f_first = f.step(p);
     }
     cp_async_commit();
@@ -386,7 +400,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
   int limit[NT], sure = 0;
   float o[8][NT][4], m[NT], l[NT];
   bool first = true;
-  int unit = 0, piece = 0;
+  int stage = 0, piece = 0;
   int lp_ring[kRowStages - 1];  // logical pages of the stages in flight
 #pragma unroll
   for (int i = 0; i < kRowStages - 1; ++i) lp_ring[i] = fetch();
@@ -396,11 +410,11 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
     __syncwarp();
     if (first) {
       const uint32_t src = q_a + (piece & 1) * Shape::kQBytes;
-      const int r0 = c.tile * p.row_tile, n = min(p.row_tile, c.s.ntok * p.G - r0);
+      const int r0 = c.tile * kRows, n = min(kRows, c.s.ntok * p.G - r0);
 #pragma unroll
       for (int h = 0; h < NT; ++h) {
         const int r = g + 8 * h;
-        limit[h] = r >= n ? -1 : p.causal ? c.s.len - c.s.ntok + (r0 + r) / p.G : c.s.len - 1;
+        limit[h] = r >= n ? -1 : p.causal ? c.s.len - c.s.ntok + tok_of(r0 + r) : c.s.len - 1;
         m[h] = -INFINITY;
         l[h] = 0.f;
 #pragma unroll
@@ -415,7 +429,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[k][h][e] = 0.f;
       }
-      sure = p.causal ? c.s.len - c.s.ntok + r0 / p.G : c.s.len - 1;  // every row sees positions up to here
+      sure = p.causal ? c.s.len - c.s.ntok + tok_of(r0) : c.s.len - 1;  // every row sees positions up to here
       ++piece;
       __syncwarp();  // before the slot is filled again
     }
@@ -424,7 +438,8 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
     for (int j = 0; j + 1 < kRowStages - 1; ++j) lp_ring[j] = lp_ring[j + 1];
     lp_ring[kRowStages - 2] = fetch();
 
-    const uint32_t base = ring_a + (unit % kRowStages) * kPageKV;
+    const uint32_t base = ring_a + stage * kPageKV;
+    if (++stage == kRowStages) stage = 0;
     float sc[2][4] = {};
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
@@ -484,14 +499,13 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
 #pragma unroll
       for (int h = 0; h < NT; ++h) MmaTile<T>::run(o[k][h], a[0], a[1], a[2], a[3], pb[h][0], pb[h][1]);
     }
-    ++unit;
     if (c.page + 1 == c.end) {  // the piece's results: one for each row
-      const int r0 = c.tile * p.row_tile, n = min(p.row_tile, c.s.ntok * p.G - r0);
-      const long long first_unit = c.s.start + ((long long)c.tile * p.Hkv + c.kvh) * c.s.units;
-      const int64_t slot0 = c.s.pbase + (w_id - first_unit / per) * c.s.ntok * p.Hq + c.kvh * p.G;
+      const int r0 = c.tile * kRows, n = min(kRows, c.s.ntok * p.G - r0);
+      const int64_t slot0 = c.s.pbase + (int64_t)chunk * c.s.ntok * p.Hq + c.kvh * p.G;
+      chunk = 0;
       const auto slot_of = [&](int r) {
-        const int row = r0 + r, tok = row / p.G;
-        return slot0 + (int64_t)tok * p.Hq + (row - tok * p.G);
+        const int tok = tok_of(r0 + r);
+        return slot0 + tok * p.Hq + (r0 + r - tok * p.G);
       };
 #pragma unroll
       for (int h = 0; h < NT; ++h) {

@@ -57,12 +57,12 @@ def _append_args(t=4, hq=4, hkv=2, dtype=torch.float16):
 
 @pytest.mark.parametrize("change, match", [
     (dict(q=torch.zeros(4, 4, 64, dtype=torch.float16)), "q must be"),
-    (dict(k=torch.zeros(4, 1, 128, dtype=torch.float16)), "k has 1 heads"),
-    (dict(v=torch.zeros(5, 2, 128, dtype=torch.float16)), "same tokens"),
-    (dict(k=torch.zeros(4, 2, 128, dtype=torch.bfloat16)), "same tokens and type"),
+    (dict(k=torch.zeros(4, 1, 128, dtype=torch.float16)), "cache's 2 heads"),
+    (dict(v=torch.zeros(5, 2, 128, dtype=torch.float16)), "q's tokens"),
+    (dict(k=torch.zeros(4, 2, 128, dtype=torch.bfloat16)), "tokens and type"),
     (dict(q=torch.zeros(4, 3, 128, dtype=torch.float16)), "multiple of KV heads"),
     (dict(kmeta=torch.zeros(3, 2, 2, 128, dtype=torch.bfloat16)), "kmeta is"),
-    (dict(v_pages=torch.zeros(4, 2, 16, 128, dtype=torch.float16)), "same pages"),
+    (dict(v_pages=torch.zeros(4, 2, 16, 128, dtype=torch.float16)), "pages and heads of k_pages"),
     (dict(k4_pages=torch.zeros(3, 2, 1024, dtype=torch.uint8)), "k4_pages"),
     (dict(kv_last_page_len=torch.zeros(3, dtype=torch.int32)), "kv_last_page_len must have 2"),
     (dict(kv_indices=torch.zeros(3, dtype=torch.int64)), "kv_indices must be"),
@@ -103,3 +103,100 @@ def test_rope_append_status_codes():
     assert _rope_c(rot=12) == _rope_c(rot=8) == _rope_c(rot=136) == _rope_c(dtype=5) == -3
     assert _rope_c(q=260) == _rope_c(s=(510, 128, 256, 128, 256, 128)) == _rope_c(kp=264) == _rope_c(meta=8) == -2
     assert _rope_c(hq=65536, hkv=65536) == -5
+
+
+def _prompt_args(t=40, hq=4, hkv=2, dtype=torch.bfloat16):
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    return dict(q=torch.zeros(t, hq, 128, dtype=dtype), k_pages=torch.zeros(3, hkv, 16, 128, dtype=dtype),
+                v_pages=torch.zeros(3, hkv, 16, 128, dtype=dtype), qo_indptr=i32([0, 1, t]), kv_indptr=i32([0, 1, 3]),
+                kv_indices=i32([0, 1, 2]), kv_last_page_len=i32([3, 4]), max_pages=2)
+
+
+@pytest.mark.parametrize("change, match", [
+    (dict(q=torch.zeros(40, 4, 64, dtype=torch.bfloat16)), "q must be"),
+    (dict(q=torch.zeros(4, 40, 128, dtype=torch.bfloat16).transpose(0, 1)), "heads of a token contiguous"),
+    (dict(q=torch.zeros(40, 3, 128, dtype=torch.bfloat16)), "multiple of KV heads"),
+    (dict(v_pages=torch.zeros(3, 2, 16, 128)), "v_pages is"),
+    (dict(k_pages=torch.zeros(3, 2, 128, 16, dtype=torch.bfloat16)), "k_pages must be"),
+    (dict(kv_indptr=torch.zeros(5, dtype=torch.int32)), "kv_indptr must have 3"),
+    (dict(qo_indptr=torch.zeros(3, dtype=torch.int64)), "qo_indptr must be"),
+    (dict(out=torch.zeros(40, 4, 128)), "out must be"),
+    (dict(lse=torch.zeros(40, 3)), "lse must be"),
+    (dict(block_pages=torch.zeros(2, 2, 4, dtype=torch.int32)), "go together"),
+    (dict(block_pages=torch.zeros(1, 2, 4, dtype=torch.int32), block_npages=torch.zeros(2, 2, dtype=torch.int32)),
+     "block_pages must be"),
+    ({}, "CUDA tensors only"),
+])
+def test_prompt_attn_refuses(change, match):
+    with pytest.raises(_lib.TwilightError, match=match):
+        ops.prompt_attn(**{**_prompt_args(), **change})
+
+
+@pytest.mark.parametrize("change, match", [
+    (dict(token_budget=0), "must be positive"),
+    (dict(query_block=40), "multiple of 16"),
+    (dict(kmeta=torch.zeros(3, 2, 2, 128)), "kmeta is"),
+    (dict(pooled=torch.zeros(2, 2, 128)), "pooled must be"),
+    (dict(block_pages=torch.zeros(2, 2, 1, dtype=torch.int32)), "at least 2"),
+    ({}, "CUDA tensors only"),
+])
+def test_quest_select_blocks_refuses(change, match):
+    a = _prompt_args()
+    a = {**{k: v for k, v in a.items() if k not in ("k_pages", "v_pages")}, "token_budget": 64, "query_block": 64,
+         "kmeta": torch.zeros(3, 2, 2, 128, dtype=torch.bfloat16), **change}
+    if "CUDA" not in match and "positive" not in match and "multiple of 16" not in match and "kmeta" not in match:
+        real, ops._cuda = ops._cuda, lambda t: None      # past the device check, to the scratch buffers' own
+        try:
+            with pytest.raises(_lib.TwilightError, match=match):
+                ops.quest_select_blocks(**a)
+        finally:
+            ops._cuda = real
+        return
+    with pytest.raises(_lib.TwilightError, match=match):
+        ops.quest_select_blocks(**a)
+
+
+@pytest.mark.parametrize("change, match", [
+    (dict(q=torch.zeros(3, 4, 2, 128, dtype=torch.bfloat16)), "q_len must be 1"),
+    (dict(group_indptr=torch.zeros(0, dtype=torch.int32), prefix_indptr=torch.zeros(0, dtype=torch.int32)), "at least two entries"),
+    (dict(prefix_last_page_len=torch.zeros(2, dtype=torch.int32)), "prefix_last_page_len must have 1"),
+    (dict(kv_indices=torch.zeros(2)), "kv_indices must be"),
+    (dict(workspace=torch.zeros(4)), "CUDA tensors only"),
+])
+def test_shared_prefix_refuses(change, match):
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    pools = torch.zeros(2, 3, 2, 16, 128, dtype=torch.bfloat16)
+    a = dict(q=torch.zeros(3, 4, 128, dtype=torch.bfloat16), k_pages=pools[0], v_pages=pools[1], group_indptr=i32([0, 3]),
+             prefix_indptr=i32([0, 1]), prefix_indices=i32([0]), prefix_last_page_len=i32([16]),
+             kv_indptr=i32([0, 1, 1, 2]), kv_indices=i32([1, 2]), kv_last_page_len=i32([1, 0, 2]))
+    with pytest.raises(_lib.TwilightError, match=match):
+        ops.shared_prefix_attn(**{**a, **change})
+
+
+def test_attention_status_codes():
+    lib = _lib.load()
+
+    def prompt(**kw):
+        a = dict(q=256, dtype=1, ts=512, k=256, v=256, qo=256, ip=256, idx=256, ll=256, t=4, b=2, hq=4, hkv=2, pages=3, mp=2,
+                 causal=1, bp=None, bn=None, mk=0, qb=0, scale=0.1, out=256, lse=None, ws=256, wb=1 << 40)
+        a.update(kw)
+        return lib.twl_prompt_attn(*a.values(), None, None)
+
+    assert prompt(q=None) == prompt(out=None) == prompt(hq=3) == prompt(mp=0) == prompt(bp=256) == prompt(scale=0.0) == -1
+    assert prompt(scale=float("nan")) == prompt(bp=256, bn=256, mk=0, qb=64) == -1
+    assert prompt(dtype=2) == prompt(hq=129 * 2) == prompt(bp=256, bn=256, mk=2, qb=40) == -3
+    assert prompt(q=264) == prompt(ts=516) == prompt(k=264) == prompt(out=8) == -2
+    assert prompt(ws=None) == prompt(wb=64) == prompt(ws=257) == -6
+    assert prompt(pages=1 << 30) == -5
+    need = lib.twl_prompt_attn_workspace_bytes(4, 2, 4, 2, 2, 0)
+    assert 0 < need < 1 << 20 and lib.twl_prompt_attn_workspace_bytes(4, 2, 3, 2, 2, 0) == 0
+    assert lib.twl_prompt_attn_workspace_bytes(32768, 1, 32, 8, 2048, 64) < 200 << 20
+    assert lib.twl_shared_prefix_workspace_bytes(4, 0, 4, 2, 2) == 0
+    assert lib.twl_shared_prefix_workspace_bytes(64, 1, 32, 8, 2048) < 200 << 20
+    assert lib.twl_shared_prefix_attn(None, 1, 512, 256, 256, 256, 256, 256, 256, 256, 256, 256, 4, 1, 4, 2, 3, 2, 0.1, 256,
+                                      None, 256, 1 << 40, None, None) == -1
+    select = lambda **kw: lib.twl_quest_select_blocks(*{**dict(  # noqa: E731
+        q=256, dtype=1, ts=512, meta=256, qo=256, ip=256, idx=256, ll=256, t=4, b=2, hq=4, hkv=2, pages=3, budget=64, qb=64,
+        mp=2, pooled=256, scores=256, bp=256, bn=256, mk=2), **kw}.values(), None, None)
+    assert select(budget=0) == select(pooled=None) == select(hq=5) == -1
+    assert select(qb=24) == select(dtype=9) == -3 and select(ts=510) == -2 and select(mp=60000) == -5

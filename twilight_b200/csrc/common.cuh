@@ -71,6 +71,20 @@ inline cudaError_t launch_chain(void (*kernel)(Params), dim3 grid, dim3 block, s
   return cudaLaunchKernelEx(&cfg, kernel, params);
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory on the current device; asked of the runtime once per kernel and device
+// (`done`: a zeroed array of the caller's for this kernel).
+constexpr int kSmemDevices = 64;
+template <typename Kernel>
+inline cudaError_t allow_smem(Kernel* kernel, int bytes, int8_t (&done)[kSmemDevices]) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 0 && dev < kSmemDevices && __atomic_load_n(&done[dev], __ATOMIC_ACQUIRE)) return cudaSuccess;
+  const cudaError_t s = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (s == cudaSuccess && dev >= 0 && dev < kSmemDevices) __atomic_store_n(&done[dev], (int8_t)1, __ATOMIC_RELEASE);
+  return s;
+}
+
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // ---- element type traits ---------------------------------------------------------------

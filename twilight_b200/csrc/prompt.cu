@@ -41,7 +41,8 @@ __device__ __forceinline__ Segment load_segment(const AttnParams& p, int i) {
   }
   if (s.npages <= 0 || bad) s.npages = 0;
   s.len = s.npages ? (s.npages - 1) * kPage + last : 0;
-  s.few = s.ntok * p.G <= kFewRows;
+  s.few = s.ntok * p.G <= p.row_tile;
+  if (s.few && s.ntok > 0) s.units = p.block_pages ? min(s.npages, p.max_k) : s.npages;
   return s;
 }
 
@@ -90,7 +91,7 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnPar
     const Segment s = load_segment(p, i);
     if (i == tid) mine = s;
     if (s.few) {
-      v[0] += (long long)few_tiles(p, s.ntok) * p.Hkv * pages_of(s);
+      v[0] += (long long)p.Hkv * s.units;
     } else {
       const int n = tok_tiles(p, s.ntok) * p.Hkv;
       v[1] += n;
@@ -99,22 +100,27 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnPar
   }
   block_sums<3>(v, sums);
   const int per_warp = (int)max((long long)kRowRunMin, (v[0] + p.row_warps - 1) / p.row_warps);
-  // Key chunks.  Little work (up to 24 key tiles a block): one wave of equal chunks, a tile of w pages giving ceil(w/c)
-  // items, on average w/c + 1/2.  More work: chunks of a third of a block's share, so that the counter can balance them.
+  // Key chunks.  With fewer tiles than blocks: one wave of equal chunks (a tile of w pages gives ceil(w/c) items, on average
+  // w/c + 1/2; count, and lengthen by what is too much), unless that leaves more than a fifth of the blocks' time unused.
+  // Otherwise chunks of a third of a block's share, so that the counter can balance them.
   const long long share = (v[2] + p.tile_target - 1) / p.tile_target;
-  const bool wave = share <= 24 * 8 && v[1] < p.tile_target;
-  long long tc = wave ? (v[2] + p.tile_target - v[1] / 2 - 1) / (p.tile_target - v[1] / 2) : (share + 2) / 3;
-  tc = (max(tc, (long long)(wave ? kTileChunkMin : 16 * 8)) + 7) & ~7LL;  // whole key tiles
-  for (int round = 0; wave && round < 3; ++round) {  // one wave should stay one: count, and lengthen by what is too much
-    long long items[1] = {0};
-    for (int i = tid; i < n_seg; i += n_thr) {
-      const Segment s = i == tid ? mine : load_segment(p, i);
-      if (!s.few) items[0] += (long long)tok_tiles(p, s.ntok) * p.Hkv * max(1LL, (pages_of(s) + tc - 1) / tc);
+  long long tc = 0;
+  if (v[1] < p.tile_target) {
+    const long long room = p.tile_target - v[1] / 2;
+    tc = (max((v[2] + room - 1) / room, (long long)kTileChunkMin) + 7) & ~7LL;  // whole key tiles
+    for (int round = 0; round < 3; ++round) {
+      long long items[1] = {0};
+      for (int i = tid; i < n_seg; i += n_thr) {
+        const Segment s = i == tid ? mine : load_segment(p, i);
+        if (!s.few) items[0] += (long long)tok_tiles(p, s.ntok) * p.Hkv * max(1LL, (pages_of(s) + tc - 1) / tc);
+      }
+      block_sums<1>(items, sums);
+      if (items[0] <= p.tile_target) break;
+      tc = (tc * items[0] / p.tile_target + 8) & ~7LL;
     }
-    block_sums<1>(items, sums);
-    if (items[0] <= p.tile_target) break;
-    tc = (tc * items[0] / p.tile_target + 8) & ~7LL;
+    if (share * 5 < tc * 4 && share > 24 * 8) tc = 0;
   }
+  if (tc == 0) tc = (max((share + 2) / 3, 16 * 8LL) + 7) & ~7LL;
 
   long long base[3] = {0, 0, 0};  // units, tile items, partial rows so far
   int merge = 0;
@@ -128,10 +134,9 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnPar
       s = i0 == 0 ? mine : load_segment(p, i);
       const int pages = pages_of(s);
       if (s.few) {
-        s.units = pages;
-        cnt[0] = (long long)few_tiles(p, s.ntok) * p.Hkv * pages;
-        // a run of `pages` units touches at most so many warps
-        cnt[2] = (long long)s.ntok * p.Hq * ((pages + per_warp - 1) / per_warp + 1);
+        cnt[0] = (long long)p.Hkv * s.units;
+        // so many units in a row touch at most so many warps
+        cnt[2] = (long long)s.ntok * p.Hq * ((s.units + per_warp - 1) / per_warp + 1);
       } else {
         s.chunks = (int)max(1LL, (pages + tc - 1) / tc);
         s.chunk_pages = s.chunks == 1 ? 0x3fffffff : ((pages + s.chunks - 1) / s.chunks + 7) & ~7;  // equal ones
@@ -155,14 +160,16 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnPar
     __syncthreads();
     long long at[3];
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      long long before = 0, total = 0;
-      for (int w = 0; w < n_warps; ++w) {
-        if (w < warp) before += scan[w][k];
-        total += scan[w][k];
+    for (int k = 0; k < 3; ++k) {  // every warp scans the warps' totals
+      long long w = lane < n_warps ? scan[lane][k] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += x;
       }
-      at[k] = base[k] + before + inc[k] - cnt[k];
-      base[k] += total;
+      const long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+      at[k] = base[k] + (warp ? before : 0) + inc[k] - cnt[k];
+      base[k] += __shfl_sync(0xffffffffu, w, 31);
     }
     __syncthreads();
     if (i < n_seg) {
@@ -203,14 +210,14 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnPar
 }
 
 // ---- row kernel -----------------------------------------------------------------------------------
-// A warp works on its own: per_warp consecutive units of the line, a unit being one page for one tile of up to 8*NT rows of a
-// segment and one KV head (the order is segment, tile, KV head, page).  Pages come through a ring of the warp's own (three
+// A warp works on its own: per_warp consecutive units of the line, a unit being one page for the up to 8*NT rows of a
+// segment and one KV head (the order is segment, KV head, page).  Pages come through a ring of the warp's own (three
 // pages of K and V, 16-byte async copies, rows of 256 bytes with the 16-byte pieces rotated by the row so that
-// ldmatrix is free of bank conflicts), and the copies run two pages ahead across the ends of (tile, KV head) pieces, the
+// ldmatrix is free of bank conflicts), and the copies run two pages ahead across the ends of pieces (a KV head's units), the
 // next piece's query rows with its first page: reading does not pause where a piece ends.
 //   S[row][token] = Q K^T   m16n8k16, rows the M side (rows 8-15 are zero for NT = 1), K rows the B operand
 //   O^T[channel][row] += V^T P^T: P as the B operand has the layout of the S accumulators.
-// Each piece leaves a partial result per row; a (tile, KV head) that several warps share has one from each.
+// Each piece leaves a partial result per row; a KV head that several warps share has one from each.
 // Bound by reading K and V.
 constexpr int kRowStages = 3;
 constexpr int kPageKV = 2 * kPage * kD * 2;  // K page, V page: 8 KiB
@@ -247,11 +254,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// A position in a warp's run: a piece is the part of one (tile, KV head) that the run covers.
-template <int ROWS>
+// A position in a warp's run: a piece is the part of one KV head's pages that the run covers.
 struct RowCursor {
-  int seg, tile, kvh;
-  int page, end;  // unit of the (tile, KV head), and where the piece ends
+  int seg, kvh;
+  int page, end;  // unit of the KV head, and where the piece ends
   int left;       // units of the run from this one on
   Segment s;
 
@@ -268,10 +274,8 @@ struct RowCursor {
     seg = lo;  // the last that starts at or before x; those after the last unit's start behind it
     s = p.segs[seg];
     const long long in = x - s.start;
-    const int piece = (int)(in / s.units);
-    tile = piece / p.Hkv;
-    kvh = piece - tile * p.Hkv;
-    page = (int)(in - (long long)piece * s.units);
+    kvh = (int)(in / s.units);
+    page = (int)(in - (long long)kvh * s.units);
     left = n;
     end = min(s.units, page + left);
   }
@@ -283,11 +287,8 @@ struct RowCursor {
       page = 0;
       if (++kvh == p.Hkv) {
         kvh = 0;
-        if (++tile * ROWS >= s.ntok * p.G) {
-          tile = 0;
-          do s = p.segs[++seg];
-          while (s.units == 0 || s.ntok == 0);
-        }
+        do s = p.segs[++seg];
+        while (s.units == 0);
       }
       end = min(s.units, left);
     }
@@ -300,6 +301,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
   using Shape = RowShape<NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_wait();
+  pdl_release();  // the plan is complete: the tile kernel, which needs no more than that, may move in where a block ends
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int per = p.hdr->per_warp;
@@ -308,13 +310,12 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
   const uint32_t ring_a = (uint32_t)__cvta_generic_to_shared(smem + warp * Shape::kWarpBytes);
   const uint32_t q_a = ring_a + kRowStages * kPageKV;
 
-  constexpr int kRows = 8 * NT;
-  RowCursor<kRows> f, c;  // where the copies are, and the arithmetic
+  RowCursor f, c;  // where the copies are, and the arithmetic
   f.start(p, x0, (int)min((long long)per, units - x0));
   c = f;
   // Of the warps that share the first piece this is number `chunk`; every other piece begins in this run.
-  int chunk = (int)(w_id - (c.s.start + ((long long)c.tile * p.Hkv + c.kvh) * c.s.units) / per);
-  const uint32_t inv_g = 65536u / p.G + 1;  // row / G of the at most kFewRows rows of a segment
+  int chunk = (int)(w_id - (c.s.start + (long long)c.kvh * c.s.units) / per);
+  const uint32_t inv_g = 65536u / p.G + 1;  // row / G of the at most sixteen rows of a segment
   const auto tok_of = [&](int row) { return (int)((row * inv_g) >> 16); };
   // where this lane's pieces of a page go: rows 2j + lane/16, piece lane%16 rotated by the row; j mod 4 decides the rotation
   uint32_t to_off[4];
@@ -331,8 +332,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
     int n = f.s.npages;
     const int32_t* list = nullptr;
     if (p.block_pages) {
-      const int tok = tok_of(f.tile * kRows);
-      const int64_t slot = (int64_t)(f.s.tok0 / p.query_block + f.seg + tok / p.query_block) * p.Hkv + f.kvh;
+      const int64_t slot = (int64_t)(f.s.tok0 / p.query_block + f.seg) * p.Hkv + f.kvh;  // (all in one query block)
       n = min(max(p.block_npages[slot], 0), p.max_k);
       list = p.block_pages + slot * p.max_k;
     }
@@ -358,11 +358,11 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
       if (f_first || (f.page & 31) == 0) look_up();
       if (f_first) {
         const uint32_t dst = q_a + (f_piece & 1) * Shape::kQBytes;
-        const int r0 = f.tile * kRows, n = min(kRows, f.s.ntok * p.G - r0);
+        const int n = f.s.ntok * p.G;
         const T* src = static_cast<const T*>(p.q) + (int64_t)f.s.tok0 * p.q_ts + f.kvh * p.G * kD + (lane & 15) * 8;
 #pragma unroll
         for (int j = 0; j < 4 * NT; ++j) {
-          const int r = 2 * j + (lane >> 4), row = r0 + (r < n ? r : 0), tok = tok_of(row);
+          const int r = 2 * j + (lane >> 4), row = r < n ? r : 0, tok = tok_of(row);
           cp_async16_or_zero(dst + to_off[j & 3] + (j >> 2) * 2048, src + tok * p.q_ts + (row - tok * p.G) * kD, r < n);
         }
         ++f_piece;
@@ -410,11 +410,11 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
     __syncwarp();
     if (first) {
       const uint32_t src = q_a + (piece & 1) * Shape::kQBytes;
-      const int r0 = c.tile * kRows, n = min(kRows, c.s.ntok * p.G - r0);
+      const int n = c.s.ntok * p.G;
 #pragma unroll
       for (int h = 0; h < NT; ++h) {
         const int r = g + 8 * h;
-        limit[h] = r >= n ? -1 : p.causal ? c.s.len - c.s.ntok + tok_of(r0 + r) : c.s.len - 1;
+        limit[h] = r >= n ? -1 : p.causal ? c.s.len - c.s.ntok + tok_of(r) : c.s.len - 1;
         m[h] = -INFINITY;
         l[h] = 0.f;
 #pragma unroll
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[k][h][e] = 0.f;
       }
-      sure = p.causal ? c.s.len - c.s.ntok + tok_of(r0) : c.s.len - 1;  // every row sees positions up to here
+      sure = p.causal ? c.s.len - c.s.ntok : c.s.len - 1;  // every row sees positions up to here
       ++piece;
       __syncwarp();  // before the slot is filled again
     }
@@ -500,12 +500,12 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
       for (int h = 0; h < NT; ++h) MmaTile<T>::run(o[k][h], a[0], a[1], a[2], a[3], pb[h][0], pb[h][1]);
     }
     if (c.page + 1 == c.end) {  // the piece's results: one for each row
-      const int r0 = c.tile * kRows, n = min(kRows, c.s.ntok * p.G - r0);
+      const int n = c.s.ntok * p.G;
       const int64_t slot0 = c.s.pbase + (int64_t)chunk * c.s.ntok * p.Hq + c.kvh * p.G;
       chunk = 0;
       const auto slot_of = [&](int r) {
-        const int tok = tok_of(r0 + r);
-        return slot0 + tok * p.Hq + (r0 + r - tok * p.G);
+        const int tok = tok_of(r);
+        return slot0 + tok * p.Hq + (r - tok * p.G);
       };
 #pragma unroll
       for (int h = 0; h < NT; ++h) {
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
 // ---- merge -----------------------------------------------------------------------------------------
 // Warp = one output row (token, query head): the partial results of its segment's chunks, and of its group's prefix.
 template <typename T>
-__global__ void __launch_bounds__(256) prompt_merge_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(256, 4) prompt_merge_kernel(const AttnParams p) {
   pdl_wait();
   if (p.hdr->merge == 0) return;
   const int per = p.hdr->per_warp;
@@ -547,66 +547,77 @@ __global__ void __launch_bounds__(256) prompt_merge_kernel(const AttnParams p) {
   const int64_t rows = (int64_t)p.num_tokens * p.Hq;
   for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += (int64_t)gridDim.x * 8) {
     const int tok = (int)(row / p.Hq), head = (int)(row - (int64_t)tok * p.Hq);
+    // the row's partial results: n[0] of its sequence's segment, n[1] of its group's, `step` slots apart
+    int n[2] = {0, 0};
+    int64_t slot0[2] = {0, 0}, step[2] = {0, 0};
+    bool found = false;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      const int segs = part ? p.n_second : p.n_first;
+      const int32_t* qo = part ? p.qo2 : p.qo1;
+      if (segs == 0) continue;
+      int at = tok;
+      if (qo) {  // last segment that starts at or before the token
+        int lo = 0, hi = segs;
+        while (hi - lo > 1) {
+          const int jump = (hi - lo + 31) >> 5, c = lo + lane * jump;
+          const int cnt = __popc(__ballot_sync(0xffffffffu, c < hi && qo[c] <= tok));
+          lo += (cnt > 0 ? cnt - 1 : 0) * jump;
+          hi = min(hi, lo + jump);
+        }
+        at = lo;
+      }
+      if (at >= segs) continue;
+      const Segment s = p.segs[(part ? p.n_first : 0) + at];
+      if (tok < s.tok0 || tok >= s.tok0 + s.ntok || s.pbase < 0) continue;
+      found = true;
+      slot0[part] = s.pbase + (int64_t)(tok - s.tok0) * p.Hq + head;
+      step[part] = (int64_t)s.ntok * p.Hq;
+      n[part] = s.chunks;
+      if (s.few) {  // the warps whose runs touch the KV head's units
+        const long long u = s.start + (long long)(head / p.G) * s.units;
+        n[part] = s.units ? (int)((u + s.units - 1) / per - u / per) + 1 : 0;
+      }
+    }
     float m = -INFINITY, l = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    bool found = false;
-    for (int part = 0; part < 2; ++part) {
-      const int n = part ? p.n_second : p.n_first;
-      const int32_t* qo = part ? p.qo2 : p.qo1;
-      if (n == 0) continue;
-      int sidx = tok;
-      if (qo) {  // last segment that starts at or before the token
-        int lo = 0, hi = n;
-        while (hi - lo > 1) {
-          const int step = (hi - lo + 31) >> 5, c = lo + lane * step;
-          const int cnt = __popc(__ballot_sync(0xffffffffu, c < hi && qo[c] <= tok));
-          lo += (cnt > 0 ? cnt - 1 : 0) * step;
-          hi = min(hi, lo + step);
+    // a lane takes a partial result's maximum and sum; the accumulators follow, four in flight
+    for (int c0 = 0; c0 < n[0] + n[1]; c0 += 32) {
+      const int c_mine = c0 + lane;
+      int64_t mine = p.part_cap;
+      if (c_mine < n[0])
+        mine = slot0[0] + c_mine * step[0];
+      else if (c_mine < n[0] + n[1])
+        mine = slot0[1] + (c_mine - n[0]) * step[1];
+      float2 v = make_float2(-INFINITY, 0.f);
+      if (mine < p.part_cap) v = p.part_ml[mine];
+      const float mn = fmaxf(m, warp_max(v.x)), ref = mn == -INFINITY ? 0.f : mn;
+      const float f0 = ex2(m - ref);
+      const float w = v.y == 0.f ? 0.f : ex2(v.x - ref);  // (a NaN sum goes on)
+      l = l * f0 + warp_sum(v.y * w);
+      a.x *= f0;
+      a.y *= f0;
+      a.z *= f0;
+      a.w *= f0;
+      m = mn;
+      for (uint32_t has = __ballot_sync(0xffffffffu, v.y != 0.f); has;) {  // the others' accumulators were not written
+        float4 x[4];
+        float f[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int c = has ? __ffs(has) - 1 : 0;
+          f[k] = has ? __shfl_sync(0xffffffffu, w, c) : 0.f;
+          const int64_t slot = __shfl_sync(0xffffffffu, mine, c);
+          x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (has) x[k] = *reinterpret_cast<const float4*>(p.part_acc + slot * kD + 4 * lane);
+          has &= has - 1;
         }
-        sidx = lo;
-      }
-      if (sidx >= n) continue;
-      const Segment s = p.segs[(part ? p.n_first : 0) + sidx];
-      if (tok < s.tok0 || tok >= s.tok0 + s.ntok) continue;
-      if (s.pbase < 0) continue;
-      found = true;
-      // a lane takes a chunk's maximum and sum; the accumulators follow, four in flight
-      const int64_t slot0 = s.pbase + (int64_t)(tok - s.tok0) * p.Hq + head, step = (int64_t)s.ntok * p.Hq;
-      int chunks = s.chunks;
-      if (s.few) {  // the warps whose runs touch the row's (tile, KV head)
-        const int kvh = head / p.G, tile = ((tok - s.tok0) * p.G + head - kvh * p.G) / p.row_tile;
-        const long long u = s.start + ((long long)tile * p.Hkv + kvh) * s.units;
-        chunks = s.units ? (int)((u + s.units - 1) / per - u / per) + 1 : 0;
-      }
-      for (int c0 = 0; c0 < chunks; c0 += 32) {
-        const int n = min(32, chunks - c0);
-        float2 v = make_float2(-INFINITY, 0.f);
-        if (lane < n && slot0 + (c0 + lane) * step < p.part_cap) v = p.part_ml[slot0 + (c0 + lane) * step];
-        const float mn = fmaxf(m, warp_max(v.x)), ref = mn == -INFINITY ? 0.f : mn;
-        const float f0 = ex2(m - ref);
-        const float w = v.y == 0.f ? 0.f : ex2(v.x - ref);  // (a NaN sum goes on)
-        l = l * f0 + warp_sum(v.y * w);
-        a.x *= f0;
-        a.y *= f0;
-        a.z *= f0;
-        a.w *= f0;
-        m = mn;
-        const uint32_t has = __ballot_sync(0xffffffffu, v.y != 0.f);  // the others' accumulators were not written
-        for (int c = 0; c < n; c += 4) {
-          float4 x[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if ((has >> (c + k)) & 1) x[k] = *reinterpret_cast<const float4*>(p.part_acc + (slot0 + (c0 + c + k) * step) * kD + 4 * lane);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float f = __shfl_sync(0xffffffffu, w, (c + k) & 31);
-            if ((has >> (c + k)) & 1) {
-              a.x += x[k].x * f;
-              a.y += x[k].y * f;
-              a.z += x[k].z * f;
-              a.w += x[k].w * f;
-            }
-          }
+        for (int k = 0; k < 4; ++k) {
+          a.x += x[k].x * f[k];
+          a.y += x[k].y * f[k];
+          a.z += x[k].z * f[k];
+          a.w += x[k].w * f[k];
         }
       }
     }
@@ -644,7 +655,7 @@ static WorkspaceLayout workspace_layout(int64_t tokens, int64_t n_seg, int64_t H
   const int64_t row_parts = least(few * ((max_pages + kRowRunMin - 1) / kRowRunMin + 1), few * 2 + warps * kFewRows);
   // and of the tile kernel
   const int64_t whole = tokens * Hq * ((max_pages + kTileChunkMin - 1) / kTileChunkMin);
-  const int64_t tile_parts = tokens * G <= kFewRows ? 0
+  const int64_t tile_parts = tokens * G <= 8 ? 0
                              : !prefix && max_pages <= kTileChunkMin ? 0
                                                                      : least(whole, 6 * blocks * 2 * tt * G + (prefix ? tokens * Hq : 0));
   w.rows = row_parts + tile_parts;
@@ -678,8 +689,8 @@ static void place_workspace(AttnParams& p, const WorkspaceLayout& w, void* works
 
 template <typename T, int NT>
 static int launch_rows(const AttnParams& p, cudaStream_t st) {
-  TWL_CUDA_TRY(cudaFuncSetAttribute(prompt_rows_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    RowShape<NT>::kSmem));
+  static int8_t done[kSmemDevices];
+  TWL_CUDA_TRY(allow_smem(prompt_rows_kernel<T, NT>, RowShape<NT>::kSmem, done));
   TWL_CUDA_TRY(launch_chain(prompt_rows_kernel<T, NT>, dim3((unsigned)num_sms()), dim3(RowShape<NT>::kWarps * 32),
                             RowShape<NT>::kSmem, st, p));
   return TWL_OK;
@@ -687,10 +698,10 @@ static int launch_rows(const AttnParams& p, cudaStream_t st) {
 
 template <typename T>
 static int run_attention(const AttnParams& p, int dtype, cudaStream_t st) {
-  const int plan_threads = p.n_first + p.n_second <= 256 ? 256 : kPlanThreads;
+  const int n_seg = p.n_first + p.n_second, plan_threads = n_seg <= 128 ? 128 : n_seg <= 512 ? 512 : kPlanThreads;
   TWL_CUDA_TRY(launch_chain(prompt_plan_kernel, dim3(1), dim3(plan_threads), 0, st, p));
   int bad = p.row_tile == 8 ? launch_rows<T, 1>(p, st) : launch_rows<T, 2>(p, st);
-  if (bad == TWL_OK && (int64_t)p.num_tokens * p.G > kFewRows) bad = tile_attention_launch(p, dtype, st);
+  if (bad == TWL_OK && (int64_t)p.num_tokens * p.G > p.row_tile) bad = tile_attention_launch(p, dtype, st);
   if (bad != TWL_OK) return bad;
   const int64_t blocks = ((int64_t)p.num_tokens * p.Hq + 7) / 8, most = (int64_t)num_sms() * 8;
   TWL_CUDA_TRY(launch_chain(prompt_merge_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, p));

@@ -5,8 +5,8 @@
 // one per sequence (causal); shared_prefix_attn one per sequence (its own pages) and one per group (the prefix, no
 // mask).  With G query heads per KV head, the rows of a segment for one KV head are its tokens x G, packed, so a
 // K/V page is read once for all of them.
-// Segments of at most kFewRows rows go to the row kernel (warp-level tensor-core tiles of 8 or 16 rows; bound by reading
-// K and V): all their (row tile, KV head, page) units in one line, cut into equal runs, one per warp of the GPU.  Longer
+// Segments of at most 8 (or 16) rows go to the row kernel (a warp-level tensor-core tile of as many rows; bound by reading
+// K and V): all their (KV head, page) units in one line, cut into equal runs, one per warp of the GPU.  Longer
 // segments go to the tile kernel in tiles of up to 256 rows; where there are fewer of those than the GPU runs at once,
 // the keys are cut into chunks too.  Partial (maximum, sum, accumulator) triples are joined by the merge kernel.
 #pragma once
@@ -14,13 +14,13 @@
 
 namespace twl {
 
-constexpr int kFewRows = 16;
+constexpr int kFewRows = 16;  // most rows of a segment of the row kernel
 
 struct Segment {
   int32_t tok0, ntok;     // query tokens
   int32_t kvbase, npages; // its part of kv_indices (or of the prefix's)
   int32_t len;            // tokens of the pages
-  int32_t units;          // row kernel: pages of a (row tile, KV head); 0 for the tile kernel's segments
+  int32_t units;          // row kernel: pages of a KV head; 0 for the tile kernel's segments
   int32_t chunks;         // tile kernel: key chunks of every tile
   int32_t chunk_pages;    // and their pages
   int32_t second;         // 1: pages of the prefix table
@@ -69,9 +69,6 @@ __device__ __forceinline__ int pages_seen(const Segment& s, int tok, int causal)
   const int pos = s.len - s.ntok + tok;
   return pos < 0 ? 0 : min(s.npages, (pos >> 4) + 1);
 }
-
-// row tiles of a segment of the row kernel
-__device__ __forceinline__ int few_tiles(const AttnParams& p, int ntok) { return (ntok * p.G + p.row_tile - 1) / p.row_tile; }
 
 int tile_attention_launch(const AttnParams& p, int dtype, cudaStream_t st);
 

@@ -354,7 +354,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  pdl_wait();
+  // No wait for the kernel before: that is the row kernel, which lets this one start once the plan is complete.  The two
+  // overlap; this one waits at its end, so that what follows it follows both.
   bool ok = true;
   uint32_t n_item = 0;  // items so far: slot n_item & 1 of the two
   // The next item, copied out of its slot; false at the end (or when a wait ran out: ok is false then).
@@ -807,6 +808,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
     }
   }
   if (!ok && lane == 0) raise_flag(p.status, TWL_FLAG_WAIT_LIMIT);
+  pdl_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {
@@ -859,8 +861,9 @@ int tile_attention_launch(const AttnParams& p, int dtype, cudaStream_t st) {
     set_last_cuda_error(cudaErrorInvalidValue);
     return TWL_ERR_LAUNCH;
   }
+  static int8_t done[2][kSmemDevices];
   auto* kernel = dtype == TWL_F16 ? prompt_tile_kernel<__half> : prompt_tile_kernel<__nv_bfloat16>;
-  TWL_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileSmem));
+  TWL_CUDA_TRY(allow_smem(kernel, kTileSmem, done[dtype == TWL_F16]));
   TWL_CUDA_TRY(launch_chain(kernel, dim3((unsigned)num_sms()), dim3(kTileThreads), kTileSmem, st, tp));
   return TWL_OK;
 }

@@ -739,6 +739,7 @@ __global__ void __launch_bounds__(256) pool_query_blocks_kernel(const BlockSelPa
 // block = 64 pages x 16 slots of one KV head; a thread owns one page and four slots.  Both operands are staged in
 // shared memory (metadata as it lies in HBM, rows padded by 8 bytes: conflict-free 8-byte reads).
 constexpr int kBlkPages = 64, kBlkSlots = 16, kBlkMetaPitch = 260;
+constexpr int kBlkKeys = 200 * 1024;  // shared memory for the keys of a row: 51200 pages
 constexpr int kBlkSmem = kBlkSlots * 256 * 4 + kBlkPages * kBlkMetaPitch * 2;
 template <typename T>
 __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelParams p) {
@@ -933,7 +934,7 @@ extern "C" int twl_quest_select_blocks(const void* q, int dtype, int64_t q_token
   const int64_t slots = (int64_t)num_tokens / query_block + batch;
   const size_t smem = (size_t)max_pages * 4;
   const int64_t slot_tiles = (slots + kBlkSlots - 1) / kBlkSlots;
-  if (smem > 200 * 1024 || slots > 0x7fffffffLL || slot_tiles > 65535 || num_kv_heads > 65535) return TWL_ERR_TOO_LARGE;
+  if (smem > (size_t)kBlkKeys || slots > 0x7fffffffLL || slot_tiles > 65535 || num_kv_heads > 65535) return TWL_ERR_TOO_LARGE;
   BlockSelParams p;
   p.q = q; p.kmeta = kmeta; p.q_ts = q_token_stride;
   p.qo_indptr = qo_indptr; p.indptr = kv_indptr; p.indices = kv_indices; p.last_len = kv_last_page_len;
@@ -947,16 +948,17 @@ extern "C" int twl_quest_select_blocks(const void* q, int dtype, int64_t q_token
   const dim3 tiles((unsigned)((max_pages + kBlkPages - 1) / kBlkPages), (unsigned)num_kv_heads, (unsigned)slot_tiles);
   if (dtype == TWL_F16) {
     TWL_CUDA_TRY(launch_chain(pool_query_blocks_kernel<__half>, per_slot, dim3(256), 0, st, p));
-    TWL_CUDA_TRY(cudaFuncSetAttribute(score_query_blocks_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      kBlkSmem));
+    static int8_t done[kSmemDevices];
+    TWL_CUDA_TRY(allow_smem(score_query_blocks_kernel<__half>, kBlkSmem, done));
     TWL_CUDA_TRY(launch_chain(score_query_blocks_kernel<__half>, tiles, dim3(256), kBlkSmem, st, p));
   } else {
     TWL_CUDA_TRY(launch_chain(pool_query_blocks_kernel<__nv_bfloat16>, per_slot, dim3(256), 0, st, p));
-    TWL_CUDA_TRY(cudaFuncSetAttribute(score_query_blocks_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      kBlkSmem));
+    static int8_t done[kSmemDevices];
+    TWL_CUDA_TRY(allow_smem(score_query_blocks_kernel<__nv_bfloat16>, kBlkSmem, done));
     TWL_CUDA_TRY(launch_chain(score_query_blocks_kernel<__nv_bfloat16>, tiles, dim3(256), kBlkSmem, st, p));
   }
-  TWL_CUDA_TRY(cudaFuncSetAttribute(select_query_blocks_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static int8_t done[kSmemDevices];
+  TWL_CUDA_TRY(allow_smem(select_query_blocks_kernel, kBlkKeys, done));
   TWL_CUDA_TRY(launch_chain(select_query_blocks_kernel, per_slot, dim3(kTopkThreads), smem, st, p));
   return TWL_OK;
 }

@@ -8,6 +8,7 @@ PyTorch or CPU fallback.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Tuple, Union
 
@@ -35,7 +36,9 @@ def _p(t: Optional[torch.Tensor]) -> Optional[int]:
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the raw handle (a Stream object costs 2 us a call on the host, what a small operator has to spare)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _same_device(dev: torch.device, **tensors: Optional[torch.Tensor]) -> None:
@@ -157,10 +160,16 @@ def _launch(name: str, on: torch.Tensor, *args, **same_device: Optional[torch.Te
     """Calls entry point ``twl_<name>`` with ``on``'s device current (the library launches on the
     current device); the keyword tensors are checked to live on that device.  Raises
     :class:`TwilightError` on a non-zero status."""
-    lib = _lib.load()
-    with _on(on, **same_device):
-        st = getattr(lib, "twl_" + name)(*args)
-    _lib.check(st, name)
+    fn = getattr(_lib.load(), "twl_" + name)
+    index = on.get_device()
+    if index < 0 or any(t is not None and t.get_device() != index for t in same_device.values()) \
+            or torch.cuda.current_device() != index:
+        with _on(on, **same_device):
+            st = fn(*args)
+    else:  # the usual case, without a context
+        st = fn(*args)
+    if st != 0:
+        _lib.check(st, name)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -542,32 +551,40 @@ def _cuda(t: torch.Tensor) -> None:
         raise _lib.TwilightError("the operators take CUDA tensors only (there is no CPU path)")
 
 
-def _rows(t: torch.Tensor, name: str, heads: Optional[int] = None) -> torch.Tensor:
-    if t.dim() != 3 or t.shape[-1] != HEAD_DIM or t.stride(-1) != 1:
+def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
+    if t.dim() != 3 or t.shape[2] != HEAD_DIM or t.stride(2) != 1:
         raise _lib.TwilightError(f"{name} must be [tokens, heads, {HEAD_DIM}] with contiguous heads")
-    if heads is not None and t.shape[1] != heads:
-        raise _lib.TwilightError(f"{name} has {t.shape[1]} heads, the cache {heads}")
     return t
 
 
-def _pages(dtype: torch.dtype, **pools: torch.Tensor) -> None:
-    """K/V pools (and metadata) of the queries' type, contiguous, with the layout's trailing dimensions."""
-    for name, t in pools.items():
-        want = (2, HEAD_DIM) if name == "kmeta" else (PAGE, HEAD_DIM)
-        if t.dim() != 4 or tuple(t.shape[2:]) != want or not t.is_contiguous():
-            raise _lib.TwilightError(f"{name} must be contiguous [pages, kv heads, {want[0]}, {want[1]}]")
-        if t.dtype != dtype:
-            raise _lib.TwilightError(f"{name} is {t.dtype}, q is {dtype}")
+# (These run on every call of operators that can take less than ten microseconds on the GPU: plain comparisons,
+# messages only where one fails.)
+def _pool(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
+    """A K/V pool (or its metadata): contiguous, of the queries' type and of the given shape."""
+    if t.dtype != dtype:
+        raise _lib.TwilightError(f"{name} is {t.dtype}, q is {dtype}")
+    if t.shape != shape or not t.is_contiguous():
+        raise _lib.TwilightError(f"{name} must be contiguous {list(shape)} (pages and heads of k_pages)")
 
 
-def _table(batch: int, **tables: torch.Tensor) -> None:
-    """Page-table tensors: int32, contiguous, ``*indptr`` of batch+1 and ``*last_page_len`` of batch entries."""
-    for name, t in tables.items():
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise _lib.TwilightError(f"{name} must be contiguous int32")
-        want = batch + 1 if name.endswith("indptr") else batch if name.endswith("last_page_len") else None
-        if want is not None and t.numel() != want:
-            raise _lib.TwilightError(f"{name} must have {want} entries")
+def _i32(t: torch.Tensor, name: str, entries: int = -1) -> None:
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise _lib.TwilightError(f"{name} must be contiguous int32")
+    if entries >= 0 and t.numel() != entries:
+        raise _lib.TwilightError(f"{name} must have {entries} entries")
+
+
+def _kv_pools(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor) -> Tuple[int, int]:
+    """Checks the K and V pools against the queries; ``(pages, KV heads)``."""
+    if k_pages.dim() != 4:
+        raise _lib.TwilightError(f"k_pages must be [pages, kv heads, {PAGE}, {HEAD_DIM}]")
+    pages, hkv = k_pages.shape[0], k_pages.shape[1]
+    shape = (pages, hkv, PAGE, HEAD_DIM)
+    _pool(k_pages, "k_pages", q.dtype, shape)
+    _pool(v_pages, "v_pages", q.dtype, shape)
+    if hkv == 0 or q.shape[1] % hkv:
+        raise _lib.TwilightError("query heads must be a multiple of KV heads")
+    return pages, hkv
 
 
 def rope_append_kv(q, k, v, freqs, k_pages, v_pages, k4_pages, kmeta, qo_indptr, kv_indptr, kv_indices,
@@ -581,21 +598,20 @@ def rope_append_kv(q, k, v, freqs, k_pages, v_pages, k4_pages, kmeta, qo_indptr,
     ``interleaved`` pairs; None rotates nothing.  ``positions`` (int32 or int64 ``[T]``) replaces the cache
     positions.  K and V rows, INT4 slabs (``k4_pages``) and page metadata (``kmeta``) are written in place; the
     last two may be None.  ``out`` may be q itself."""
-    q, k, v = _rows(q, "q"), _rows(k, "k", k_pages.shape[1]), _rows(v, "v", k_pages.shape[1])
-    t, hq, _ = q.shape
+    _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    t, hq = q.shape[0], q.shape[1]
     batch = qo_indptr.numel() - 1
-    if k.shape[0] != t or v.shape[0] != t or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise _lib.TwilightError("q, k and v must have the same tokens and type")
-    if hq % k_pages.shape[1]:
-        raise _lib.TwilightError("query heads must be a multiple of KV heads")
-    _pages(q.dtype, k_pages=k_pages, v_pages=v_pages, **({} if kmeta is None else {"kmeta": kmeta}))
-    if v_pages.shape != k_pages.shape or (kmeta is not None and kmeta.shape[:2] != k_pages.shape[:2]):
-        raise _lib.TwilightError("k_pages, v_pages and kmeta must have the same pages and heads")
-    if k4_pages is not None and (k4_pages.dtype != torch.uint8 or not k4_pages.is_contiguous()
-                                 or k4_pages.shape != (*k_pages.shape[:2], K4_SLAB_BYTES)):
-        raise _lib.TwilightError(f"k4_pages must be contiguous uint8 [pages, kv heads, {K4_SLAB_BYTES}]")
-    _table(batch, qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices,
-           kv_last_page_len=kv_last_page_len)
+    pages, hkv = _kv_pools(q, k_pages, v_pages)
+    if k.shape != (t, hkv, HEAD_DIM) or v.shape != (t, hkv, HEAD_DIM) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise _lib.TwilightError(f"k and v must have q's tokens and type and the cache's {hkv} heads")
+    if kmeta is not None:
+        _pool(kmeta, "kmeta", q.dtype, (pages, hkv, 2, HEAD_DIM))
+    if k4_pages is not None:
+        _pool(k4_pages, "k4_pages", torch.uint8, (pages, hkv, K4_SLAB_BYTES))
+    _i32(qo_indptr, "qo_indptr")
+    _i32(kv_indptr, "kv_indptr", batch + 1)
+    _i32(kv_indices, "kv_indices")
+    _i32(kv_last_page_len, "kv_last_page_len", batch)
     if freqs is not None and (freqs.dtype != torch.float64 or not freqs.is_contiguous()):
         raise _lib.TwilightError("freqs must be contiguous float64 (see rope_frequencies)")
     if positions is not None and (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (t,)
@@ -603,8 +619,8 @@ def rope_append_kv(q, k, v, freqs, k_pages, v_pages, k4_pages, kmeta, qo_indptr,
         raise _lib.TwilightError("positions must be contiguous int32 or int64, one for each token")
     if out is None:
         out = torch.empty(t, hq, HEAD_DIM, dtype=q.dtype, device=q.device)
-    elif _rows(out, "out").shape != q.shape or out.dtype != q.dtype:
-        raise _lib.TwilightError("out must have q's shape and type")
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise _lib.TwilightError("out must have q's shape and type, and contiguous heads")
     _cuda(q)
     if t == 0:
         return out
@@ -613,8 +629,7 @@ def rope_append_kv(q, k, v, freqs, k_pages, v_pages, k4_pages, kmeta, qo_indptr,
             _p(positions), int(positions is not None and positions.dtype == torch.int64), _p(freqs),
             0 if freqs is None else 2 * freqs.numel(), int(interleaved), float(attention_scale), k_pages.data_ptr(),
             v_pages.data_ptr(), _p(k4_pages), _p(kmeta), qo_indptr.data_ptr(), kv_indptr.data_ptr(),
-            kv_indices.data_ptr(), kv_last_page_len.data_ptr(), t, batch, hq, k_pages.shape[1], k_pages.shape[0],
-            _p(status), _stream(q.device), k=k, v=v, out=out, positions=positions, freqs=freqs, k_pages=k_pages,
+            kv_indices.data_ptr(), kv_last_page_len.data_ptr(), t, batch, hq, hkv, pages, _p(status), _stream(q.device), k=k, v=v, out=out, positions=positions, freqs=freqs, k_pages=k_pages,
             v_pages=v_pages, k4_pages=k4_pages, kmeta=kmeta, qo_indptr=qo_indptr, kv_indptr=kv_indptr,
             kv_indices=kv_indices, kv_last_page_len=kv_last_page_len, status=status)
     return out
@@ -644,22 +659,15 @@ def dequantize_k_pages(k4_pages, page_ids=None, *, dtype: torch.dtype, out=None,
 # ---------------------------------------------------------------------------------------------
 # attention of more than one token at a time
 # ---------------------------------------------------------------------------------------------
-def _queries(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor) -> torch.Tensor:
-    _rows(q, "q")
-    if q.shape[1] > 1 and q.stride(1) != HEAD_DIM:
-        raise _lib.TwilightError("the heads of a token of q must be contiguous")
-    _pages(q.dtype, k_pages=k_pages, v_pages=v_pages)
-    if k_pages.shape != v_pages.shape:
-        raise _lib.TwilightError("k_pages and v_pages must have the same shape")
-    if q.shape[1] % k_pages.shape[1]:
-        raise _lib.TwilightError("query heads must be a multiple of KV heads")
-    return q
+def _queries(q: torch.Tensor) -> None:
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.stride(2) != 1 or (q.stride(1) != HEAD_DIM and q.shape[1] > 1):
+        raise _lib.TwilightError(f"q must be [tokens, heads, {HEAD_DIM}], the heads of a token contiguous")
 
 
 def _result(q: torch.Tensor, out, lse) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Checked or fresh output, and the log-sum-exp buffer where one is wanted (``lse``: True or a tensor)."""
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise _lib.TwilightError("out must be contiguous, of q's shape and type")
     if lse is None or lse is False:
@@ -679,6 +687,7 @@ def _workspace(t: Optional[torch.Tensor], nbytes: int, device) -> torch.Tensor:
     return t
 
 
+@functools.lru_cache(maxsize=1024)
 def prompt_attn_workspace_bytes(num_tokens: int, batch: int, num_q_heads: int, num_kv_heads: int, max_pages: int,
                                 query_block: int = 0) -> int:
     """Bytes of :func:`prompt_attn`'s workspace; ``query_block`` is 0 without block lists."""
@@ -698,16 +707,21 @@ def prompt_attn(q, k_pages, v_pages, qo_indptr, kv_indptr, kv_indices, kv_last_p
     largest page count of a sequence.  Returns ``out [T,Hq,128]``, and with ``lse`` (True or a tensor) also the fp32
     ``[T,Hq]`` logarithms of the sums of exponentials.  ``workspace``: ``prompt_attn_workspace_bytes`` bytes, one for
     each call that may overlap with another."""
-    _queries(q, k_pages, v_pages)
-    t, hq, _ = q.shape
-    batch, hkv = qo_indptr.numel() - 1, k_pages.shape[1]
-    _table(batch, qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices, kv_last_page_len=kv_last_page_len)
+    _queries(q)
+    t, hq = q.shape[0], q.shape[1]
+    pages, hkv = _kv_pools(q, k_pages, v_pages)
+    batch = qo_indptr.numel() - 1
+    _i32(qo_indptr, "qo_indptr")
+    _i32(kv_indptr, "kv_indptr", batch + 1)
+    _i32(kv_indices, "kv_indices")
+    _i32(kv_last_page_len, "kv_last_page_len", batch)
     out, lse = _result(q, out, lse)
     if (block_pages is None) != (block_npages is None):
         raise _lib.TwilightError("block_pages and block_npages go together")
     max_k = 0
     if block_pages is not None:
-        _table(batch, block_pages=block_pages, block_npages=block_npages)
+        _i32(block_pages, "block_pages")
+        _i32(block_npages, "block_npages")
         slots, max_k = t // query_block + batch, block_pages.shape[-1]
         if block_pages.shape != (slots, hkv, max_k) or block_npages.shape != (slots, hkv):
             raise _lib.TwilightError(f"block_pages must be [{slots}, {hkv}, max_k], block_npages [{slots}, {hkv}]")
@@ -718,7 +732,7 @@ def prompt_attn(q, k_pages, v_pages, qo_indptr, kv_indptr, kv_indices, kv_last_p
         workspace = _workspace(workspace, prompt_attn_workspace_bytes(t, batch, hq, hkv, max_pages, query_block), q.device)
         _launch("prompt_attn", q, q.data_ptr(), _dtype_code(q), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
                 qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), t, batch,
-                hq, hkv, k_pages.shape[0], max_pages, int(causal), _p(block_pages), _p(block_npages), max_k, query_block,
+                hq, hkv, pages, max_pages, int(causal), _p(block_pages), _p(block_npages), max_k, query_block,
                 1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, out.data_ptr(), _p(lse),
                 workspace.data_ptr(), workspace.numel(), _p(status), _stream(q.device), k_pages=k_pages, v_pages=v_pages,
                 qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices, kv_last_page_len=kv_last_page_len,
@@ -735,16 +749,19 @@ def quest_select_blocks(q, kmeta, qo_indptr, kv_indptr, kv_indices, kv_last_page
 
     Returns ``(block_pages [slots,Hkv,max_k] int32 ascending, block_npages [slots,Hkv] int32)`` with
     ``slots = T//query_block + batch``; block j of sequence b is row ``qo_indptr[b]//query_block + b + j``."""
-    _rows(q, "q")
-    t, hq, _ = q.shape
-    if hq > 1 and q.stride(1) != HEAD_DIM:
-        raise _lib.TwilightError("the heads of a token of q must be contiguous")
+    _queries(q)
+    t, hq = q.shape[0], q.shape[1]
     batch = qo_indptr.numel() - 1
-    _pages(q.dtype, kmeta=kmeta)
+    if kmeta.dim() != 4:
+        raise _lib.TwilightError(f"kmeta must be [pages, kv heads, 2, {HEAD_DIM}]")
     hkv = kmeta.shape[1]
-    if hq % hkv:
+    _pool(kmeta, "kmeta", q.dtype, (kmeta.shape[0], hkv, 2, HEAD_DIM))
+    if hkv == 0 or hq % hkv:
         raise _lib.TwilightError("query heads must be a multiple of KV heads")
-    _table(batch, qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices, kv_last_page_len=kv_last_page_len)
+    _i32(qo_indptr, "qo_indptr")
+    _i32(kv_indptr, "kv_indptr", batch + 1)
+    _i32(kv_indices, "kv_indices")
+    _i32(kv_last_page_len, "kv_last_page_len", batch)
     if token_budget <= 0 or max_pages <= 0:
         raise _lib.TwilightError("token_budget and max_pages must be positive")
     if query_block < PAGE or query_block % PAGE:
@@ -762,7 +779,8 @@ def quest_select_blocks(q, kmeta, qo_indptr, kv_indptr, kv_indices, kv_last_page
         pooled = torch.empty(slots, hkv, 2 * HEAD_DIM, dtype=torch.float32, device=dev)
     if page_scores is None:
         page_scores = torch.empty(slots, hkv, max_pages, dtype=torch.float32, device=dev)
-    _table(batch, block_pages=block_pages, block_npages=block_npages)
+    _i32(block_pages, "block_pages")
+    _i32(block_npages, "block_npages")
     if block_pages.dim() != 3 or block_pages.shape[:2] != (slots, hkv) or block_pages.shape[2] < max_k \
             or block_npages.shape != (slots, hkv):
         raise _lib.TwilightError(f"block_pages must be [{slots}, {hkv}, at least {max_k}], block_npages [{slots}, {hkv}]")
@@ -780,6 +798,7 @@ def quest_select_blocks(q, kmeta, qo_indptr, kv_indptr, kv_indices, kv_last_page
     return block_pages, block_npages
 
 
+@functools.lru_cache(maxsize=1024)
 def shared_prefix_workspace_bytes(batch: int, num_groups: int, num_q_heads: int, num_kv_heads: int, max_pages: int) -> int:
     return int(_lib.load().twl_shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads, max_pages))
 
@@ -799,12 +818,17 @@ def shared_prefix_attn(q, k_pages, v_pages, group_indptr, prefix_indptr, prefix_
         if q.shape[2] != 1:
             raise _lib.TwilightError("decode step only: q_len must be 1")
         q = q[:, :, 0, :]
-    _queries(q, k_pages, v_pages)
-    b, hq, _ = q.shape
-    groups, hkv = group_indptr.numel() - 1, k_pages.shape[1]
-    _table(groups, group_indptr=group_indptr, prefix_indptr=prefix_indptr, prefix_indices=prefix_indices,
-           prefix_last_page_len=prefix_last_page_len)
-    _table(b, kv_indptr=kv_indptr, kv_indices=kv_indices, kv_last_page_len=kv_last_page_len)
+    _queries(q)
+    b, hq = q.shape[0], q.shape[1]
+    pages, hkv = _kv_pools(q, k_pages, v_pages)
+    groups = group_indptr.numel() - 1
+    _i32(group_indptr, "group_indptr")
+    _i32(prefix_indptr, "prefix_indptr", groups + 1)
+    _i32(prefix_indices, "prefix_indices")
+    _i32(prefix_last_page_len, "prefix_last_page_len", groups)
+    _i32(kv_indptr, "kv_indptr", b + 1)
+    _i32(kv_indices, "kv_indices")
+    _i32(kv_last_page_len, "kv_last_page_len", b)
     if groups < 1:
         raise _lib.TwilightError("group_indptr must have at least two entries")
     out, lse = _result(q, out, lse)
@@ -816,7 +840,7 @@ def shared_prefix_attn(q, k_pages, v_pages, group_indptr, prefix_indptr, prefix_
         _launch("shared_prefix_attn", q, q.data_ptr(), _dtype_code(q), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
                 group_indptr.data_ptr(), prefix_indptr.data_ptr(), prefix_indices.data_ptr(),
                 prefix_last_page_len.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(),
-                b, groups, hq, hkv, k_pages.shape[0], max_pages,
+                b, groups, hq, hkv, pages, max_pages,
                 1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, out.data_ptr(), _p(lse),
                 workspace.data_ptr(), workspace.numel(), _p(status), _stream(q.device), k_pages=k_pages, v_pages=v_pages,
                 group_indptr=group_indptr, prefix_indptr=prefix_indptr, prefix_indices=prefix_indices,

@@ -29,14 +29,13 @@
 namespace twl {
 
 constexpr int kTileThreads = 384;  // three warpgroups, the unit of the register split
-constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // (200: 4 % slower, 192: spills, 40 % slower)
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "registers of the launch: 168 a thread at 384 threads");
 constexpr int kKStages = 3, kVStages = 2, kStages = kKStages + kVStages;
 constexpr int kStageBytes = 128 * kD * 2;      // 128 keys (or 128 query rows)
 constexpr int kHalfBytes = kStageBytes / 2;    // 64 channels of 128 query rows
 constexpr int kPageBytes = kPage * kD * 2, kAtom = 1024;
 constexpr int kInfoSlots = 8;                  // key tiles whose positions are kept
-constexpr int kPolyTake = 2;                   // of eight pairs of exponentials, how many take the polynomial
 constexpr uint32_t kWaitTries = 2000, kWaitNs = 500000;  // a wait gives up after about a second
 
 struct alignas(64) TileParams {
@@ -217,28 +216,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of two values on the multiply-add pipes: x = n + f with n the nearest integer (left in the low bits by adding
-// 1.5 * 2^23), 2^f on [-1/2, 1/2] by the degree-4 polynomial of least largest relative error (2.7e-6, Remez exchange),
-// n added to the exponent.  Results below 2^-126 become 2^-126.
-__device__ __forceinline__ void exp2_poly(uint64_t x, float& a, float& b) {
-  float x0, x1;
-  f2_split(x, x0, x1);
-  x = f2(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-  const uint64_t big = f2(12582912.f, 12582912.f), minus_big = f2(-12582912.f, -12582912.f);
-  const uint64_t n = add2(x, big);
-  const uint64_t f = fma2(add2(n, minus_big), f2(-1.f, -1.f), x);
-  uint64_t y = f2(9.570102207362652e-3f, 9.570102207362652e-3f);
-  y = fma2(y, f, f2(5.591785907745361e-2f, 5.591785907745361e-2f));
-  y = fma2(y, f, f2(0.240247443318367f, 0.240247443318367f));
-  y = fma2(y, f, f2(0.6931217908859253f, 0.6931217908859253f));
-  y = fma2(y, f, f2(0.9999992847442627f, 0.9999992847442627f));
-  float y0, y1, n0, n1;
-  f2_split(y, y0, y1);
-  f2_split(n, n0, n1);
-  a = __int_as_float(__float_as_int(y0) + (__float_as_int(n0) << 23));
-  b = __int_as_float(__float_as_int(y1) + (__float_as_int(n1) << 23));
-}
-
 __device__ __forceinline__ float max64(const float* x) {
   float m[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
@@ -250,20 +227,16 @@ __device__ __forceinline__ float max64(const float* x) {
   return max3(max3(m[0], m[1], m[2]), m[3], m[3]);
 }
 // 64 weights 2^(x scale - ref) of a row: their sum in 32 bits, and themselves rounded to the model type (half a step each),
-// in which they go to the tensor cores.  POLY of eight pairs take the polynomial (never masked ones: it has no zero).
-template <typename T, int POLY>
+// in which they go to the tensor cores.  All on the special-function unit: with a quarter of them by a polynomial on the
+// multiply-add pipes, 8K x 8K with 32/8 heads took 907 instead of 879 us, with half of them 944 us.
+template <typename T>
 __device__ __forceinline__ void weights(const float* x, uint64_t scale, uint64_t ref, uint64_t (&sum)[2], uint32_t (&w)[32]) {
 #pragma unroll
   for (int e = 0; e < 32; ++e) {
-    const uint64_t y = fma2(f2(x[2 * e], x[2 * e + 1]), scale, ref);
     float a, b;
-    if (e % 8 < POLY) {
-      exp2_poly(y, a, b);
-    } else {
-      f2_split(y, a, b);
-      a = tile_ex2(a);
-      b = tile_ex2(b);
-    }
+    f2_split(fma2(f2(x[2 * e], x[2 * e + 1]), scale, ref), a, b);
+    a = tile_ex2(a);
+    b = tile_ex2(b);
     sum[e & 1] = add2(sum[e & 1], f2(a, b));
     w[e] = tile_pack2(a, b, T());
   }
@@ -622,7 +595,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       const bool real = tok_r < p.tok_tile && tok < it.ntok;
       const int limit = !real ? -1 : p.causal ? it.limit0 + tok : it.limit0;
       float m = -INFINITY, l = 0.f;
-      bool settled = false;  // every row of the warp has a reference
       const int steps = a ? it.steps[1] : it.steps[0], steps_other = a ? it.steps[0] : it.steps[1];
       for (int j = 0; j < steps; ++j) {
         ok = mbar_wait(&sh.s_full[a], s_round & 1);
@@ -638,81 +610,52 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
         tmem_wait_ld32(x + 32);
         tmem_ld32(x + 64, s_t + 64);
         tmem_ld32(x + 96, s_t + 96);
-        const uint64_t scale2 = f2(scale, scale);
-        uint64_t sum[2] = {0, 0};
-        uint32_t w[32];
-        float top;
-        bool first_done = false;
-        if (settled && !masked) {
-          // The reference hardly ever moves: the first weights are computed with it while the maximum is found.
-          const float ref = m;
-          weights<T, kPolyTake>(x, scale2, f2(-ref, -ref), sum, w);
-          top = max64(x);
-          tmem_wait_ld32(x + 64);
-          tmem_wait_ld32(x + 96);
-          top = max3(top, max64(x + 64), top) * scale;
-          first_done = !__any_sync(0xffffffffu, !(top <= m + 8.f));
-          if (!first_done) {  // it does: take them again
-            sum[0] = sum[1] = 0;
-            tmem_ld32(x, s_t);
-            tmem_ld32(x + 32, s_t + 32);
-            tmem_wait_ld32(x);
-            tmem_wait_ld32(x + 32);
-          }
-        } else {
-          tmem_wait_ld32(x + 64);
-          tmem_wait_ld32(x + 96);
-          if (masked) {
+        tmem_wait_ld32(x + 64);
+        tmem_wait_ld32(x + 96);
+        if (masked) {
 #pragma unroll
-            for (int pg = 0; pg < 8; ++pg) {
-              const int n = limit - sh.pos[slot][pg];  // keys 0..n of the page are seen
+          for (int pg = 0; pg < 8; ++pg) {
+            const int n = limit - sh.pos[slot][pg];  // keys 0..n of the page are seen
 #pragma unroll
-              for (int c = 0; c < kPage; ++c)
-                if (c > n) x[16 * pg + c] = -INFINITY;
-            }
-            __syncwarp();
+            for (int c = 0; c < kPage; ++c)
+              if (c > n) x[16 * pg + c] = -INFINITY;
           }
-          top = max3(max64(x), max64(x + 64), -INFINITY) * scale;
-        }
-        if (!first_done) {
-          // move the reference only when it is 2^8 behind (or nothing was seen so far)
-          float f = 1.f;
-          const bool move = !(top <= m + 8.f);  // from -inf: any finite maximum; a NaN moves it too
-          if (move) {
-            f = tile_ex2(m - top);
-            m = top;
-            l *= f;
-          }
-          if (__any_sync(0xffffffffu, move) && j > 0) {
-            // S of this step is complete, so the product of the step before is too: O may be changed
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float o[32];
-              tmem_ld32(o, o_t + 32 * c);
-              tmem_wait_ld32(o);
-#pragma unroll
-              for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
-              tmem_st32(o_t + 32 * c, w);
-            }
-          }
-          settled = !__any_sync(0xffffffffu, real && m == -INFINITY);
-          const float ref = m == -INFINITY ? 0.f : m;
-          if (masked)
-            weights<T, 0>(x, scale2, f2(-ref, -ref), sum, w);
-          else
-            weights<T, kPolyTake>(x, scale2, f2(-ref, -ref), sum, w);
           __syncwarp();
         }
+        const float top = max3(max64(x), max64(x + 64), -INFINITY) * scale;
+        // Move the reference only when it is 2^8 behind (or nothing was seen so far).  (Computing the first weights with the
+        // standing reference while the maximum is found was 2 % slower.)
+        float f = 1.f;
+        const bool move = !(top <= m + 8.f);  // from -inf: any finite maximum; a NaN moves it too
+        if (move) {
+          f = tile_ex2(m - top);
+          m = top;
+          l *= f;
+        }
+        if (__any_sync(0xffffffffu, move) && j > 0) {
+          // S of this step is complete, so the product of the step before is too: O may be changed.  (Not unrolled: this is
+          // rare, and its registers would push those of the loop into local memory.)
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            uint32_t w[32];
+            tmem_ld32(o, o_t + 32 * c);
+            tmem_wait_ld32(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(o[e] * f);
+            tmem_st32(o_t + 32 * c, w);
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        const uint64_t scale2 = f2(scale, scale), ref2 = f2(-ref, -ref);
+        uint64_t sum[2] = {0, 0};
+        uint32_t w[32];
+        weights<T>(x, scale2, ref2, sum, w);
         tmem_st32(s_t, w);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&sh.p_half[a]);
-        const float ref = m == -INFINITY ? 0.f : m;
-        if (masked)
-          weights<T, 0>(x + 64, scale2, f2(-ref, -ref), sum, w);
-        else
-          weights<T, kPolyTake>(x + 64, scale2, f2(-ref, -ref), sum, w);
-        __syncwarp();
+        weights<T>(x + 64, scale2, ref2, sum, w);
         tmem_st32(s_t + 32, w);
         tmem_wait_st();
         tc_fence_before();
@@ -752,7 +695,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       const int64_t part = it.part0 < 0 ? -1 : it.part0 + (int64_t)tok * p.Hq + head;
       const bool write = real && (part < 0 || part < p.part_cap);
       const float inv = l != 0.f ? 1.f / l : 0.f;
-#pragma unroll
+#pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         if (pair && (c >> 1) != a) continue;  // each place writes half of the channels
         float o[32];

@@ -52,6 +52,64 @@ template <typename T>
 __device__ __forceinline__ float rope_rnd(float x) {
   return Elem<T>::to_f(Elem<T>::from_f(x));
 }
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_pair(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// minimum and maximum of two pairs of values of the type, a NaN giving way to a number
+template <typename T>
+__device__ __forceinline__ uint32_t min_pair(uint32_t a, uint32_t b) {
+  using T2 = typename Elem<T>::T2;
+  const T2 r = __hmin2(*reinterpret_cast<T2*>(&a), *reinterpret_cast<T2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+  using T2 = typename Elem<T>::T2;
+  const T2 r = __hmax2(*reinterpret_cast<T2*>(&a), *reinterpret_cast<T2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// The 4-bit codes of a lane's eight values of a group of 32 (four lanes), with the results of quantize_k_pages, which
+// rounds every step to the type: code = rint(rnd(rnd(x - min) / scale)).  The quotients are correctly rounded from the
+// reciprocal by one correction of the remainder, q + (t - q s) / s (Markstein 1990): both fused steps are exact here, t and
+// s having at most 11 bits.
+template <typename T>
+__device__ __forceinline__ uint32_t codes8(const uint32_t (&u)[4], float* scale_out, float* min_out) {
+  uint32_t lo = min_pair<T>(min_pair<T>(u[0], u[1]), min_pair<T>(u[2], u[3]));
+  uint32_t hi = max_pair<T>(max_pair<T>(u[0], u[1]), max_pair<T>(u[2], u[3]));
+#pragma unroll
+  for (int o = 2; o > 0; o >>= 1) {
+    lo = min_pair<T>(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_pair<T>(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  const float2 l2 = Elem<T>::to_f2(lo), h2 = Elem<T>::to_f2(hi);
+  const float mn = fminf(l2.x, l2.y), mx = fmaxf(h2.x, h2.y);
+  const float range = fmaxf(rope_rnd<T>(mx - mn), rope_rnd<T>(1e-9f));
+  const float scale = rope_rnd<T>(__fdiv_rn(range, 15.f));
+  const float inv = scale > 0.f ? __frcp_rn(scale) : 0.f;  // a group without a range: every code is 0
+  uint32_t word = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 x = Elem<T>::to_f2(u[k]);
+    const float2 d = Elem<T>::to_f2(pack_pair(x.x - mn, x.y - mn, T()));
+    float q0 = d.x * inv, q1 = d.y * inv;
+    q0 = fmaf(fmaf(-q0, scale, d.x), inv, q0);
+    q1 = fmaf(fmaf(-q1, scale, d.y), inv, q1);
+    const float2 r = Elem<T>::to_f2(pack_pair(q0, q1, T()));
+    // adding 1.5 * 2^23 rounds to the nearest integer (even on ties), which is then in the low bits
+    const uint32_t c0 = __float_as_uint(fminf(fmaxf(r.x, 0.f), 15.f) + 12582912.f) & 15u;
+    const uint32_t c1 = __float_as_uint(fminf(fmaxf(r.y, 0.f), 15.f) + 12582912.f) & 15u;
+    word |= (c0 | (c1 << 4)) << (8 * k);
+  }
+  *scale_out = scale;
+  *min_out = mn;
+  return word;
+}
 template <typename T>
 __device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
@@ -142,21 +200,33 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 3) rope_append_kernel(const R
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slot = blockIdx.x;
-  // largest b with qo_indptr[b]/16 + 2b <= slot, 32 candidates a round
-  int lo = 0, hi = p.batch;  // answer in [lo, hi)
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) >> 5;
-    const int b = lo + lane * step;
-    const bool ok = b < hi && (__ldg(p.qo_indptr + b) >> 4) + 2 * b <= slot;
+  // largest b with qo_indptr[b]/16 + 2b <= slot, 32 candidates a round; the last round's lanes hold the candidates' entries
+  int lo = 0, hi = p.batch, step;  // answer in [lo, hi)
+  int row0, n_new, pbase, n_pages, ll;
+  do {
+    step = (hi - lo + 31) >> 5;
+    const int b = min(lo + lane * step, p.batch - 1);
+    row0 = __ldg(p.qo_indptr + b);
+    if (step == 1) {
+      n_new = __ldg(p.qo_indptr + b + 1) - row0;
+      pbase = __ldg(p.indptr + b);
+      n_pages = __ldg(p.indptr + b + 1) - pbase;
+      ll = __ldg(p.last_len + b);
+    }
+    const bool ok = lo + lane * step < hi && (row0 >> 4) + 2 * b <= slot;
     const int n = __popc(__ballot_sync(0xffffffffu, ok));  // lane 0's candidate always fits
-    const int nlo = lo + (n > 0 ? n - 1 : 0) * step;
-    hi = min(hi, nlo + step);
-    lo = nlo;
-  }
+    const int at = n > 0 ? n - 1 : 0;
+    if (step == 1) {
+      row0 = __shfl_sync(0xffffffffu, row0, at);
+      n_new = __shfl_sync(0xffffffffu, n_new, at);
+      pbase = __shfl_sync(0xffffffffu, pbase, at);
+      n_pages = __shfl_sync(0xffffffffu, n_pages, at);
+      ll = __shfl_sync(0xffffffffu, ll, at);
+    }
+    lo += at * step;
+    hi = min(hi, lo + step);
+  } while (step > 1);
   const int b = lo;
-  const int row0 = __ldg(p.qo_indptr + b), n_new = __ldg(p.qo_indptr + b + 1) - row0;
-  const int pbase = __ldg(p.indptr + b), n_pages = __ldg(p.indptr + b + 1) - pbase;
-  const int ll = __ldg(p.last_len + b);
   if (n_new <= 0) return;
   const int len = (n_pages - 1) * kPage + ll;
   if (n_pages <= 0 || ll < 1 || ll > kPage || n_new > len || row0 < 0 || row0 + n_new > p.num_tokens) {
@@ -205,17 +275,18 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 3) rope_append_kernel(const R
       const int64_t ts = is_k ? p.k_ts : p.v_ts;
       const T* src = static_cast<const T*>(is_k ? p.k : p.v) + row * ts + head * (is_k ? p.k_hs : p.v_hs) + ch;
       T* dst = static_cast<T*>(is_k ? p.k_pages : p.v_pages) + slab * (kPage * kD) + first_slot * kD + ch;
-      float mn[8], mx[8];
+      uint32_t mn[4], mx[4];
       const bool meta = is_k && p.kmeta != nullptr;
       T* mrow = static_cast<T*>(p.kmeta) + slab * 2 * kD + ch;
       if (meta && first_slot != 0) {  // the page holds older tokens: fold into what it says
-        unpack8<T>(*reinterpret_cast<const uint4*>(mrow), mn);
-        unpack8<T>(*reinterpret_cast<const uint4*>(mrow + kD), mx);
+        const uint4 a = *reinterpret_cast<const uint4*>(mrow), z = *reinterpret_cast<const uint4*>(mrow + kD);
+        mn[0] = a.x; mn[1] = a.y; mn[2] = a.z; mn[3] = a.w;
+        mx[0] = z.x; mx[1] = z.y; mx[2] = z.z; mx[3] = z.w;
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          mn[j] = INFINITY;
-          mx[j] = -INFINITY;
+        for (int j = 0; j < 4; ++j) {
+          mn[j] = pack_pair(INFINITY, INFINITY, T());
+          mx[j] = pack_pair(-INFINITY, -INFINITY, T());
         }
       }
       for (int r0 = 0; r0 < n; r0 += 8) {
@@ -233,37 +304,17 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 3) rope_append_kernel(const R
               ang.read(cos_s[mine ? r : 0], sin_s[mine ? r : 0], ch < p.rotary ? ch : 0, p.rotary);
               u[i] = rotate8<T, INTER>(u[i], ang, ch, p.rotary);
             }
-            float y[8];
-            unpack8<T>(u[i], y);  // as the cache holds them
+            const uint32_t y[4] = {u[i].x, u[i].y, u[i].z, u[i].w};  // as the cache holds them
             if (mine) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                mn[j] = fminf(mn[j], y[j]);
-                mx[j] = fmaxf(mx[j], y[j]);
+              for (int j = 0; j < 4; ++j) {
+                mn[j] = min_pair<T>(mn[j], y[j]);
+                mx[j] = max_pair<T>(mx[j], y[j]);
               }
             }
-            if (p.k4 != nullptr) {  // groups of 32 channels = four lanes; the arithmetic of quantize_k_pages
-              float gx = y[0], gn = y[0];
-#pragma unroll
-              for (int j = 1; j < 8; ++j) {
-                gx = fmaxf(gx, y[j]);
-                gn = fminf(gn, y[j]);
-              }
-#pragma unroll
-              for (int o = 2; o > 0; o >>= 1) {
-                gx = fmaxf(gx, __shfl_xor_sync(0xffffffffu, gx, o));
-                gn = fminf(gn, __shfl_xor_sync(0xffffffffu, gn, o));
-              }
-              const float range = fmaxf(rope_rnd<T>(gx - gn), rope_rnd<T>(1e-9f));
-              const float scale = rope_rnd<T>(__fdiv_rn(range, 15.f));
-              uint32_t word = 0;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float t = rope_rnd<T>(y[j] - gn);
-                float w = (scale > 0.f) ? rope_rnd<T>(__fdiv_rn(t, scale)) : 0.f;
-                w = fminf(fmaxf(rintf(w), 0.f), 15.f);
-                word |= (uint32_t)(int)w << (4 * j);
-              }
+            if (p.k4 != nullptr) {
+              float scale, gn;
+              const uint32_t word = codes8<T>(y, &scale, &gn);
               if (mine) {
                 uint8_t* q4 = p.k4 + slab * kSlab;
                 const int tok = first_slot + r;
@@ -279,11 +330,12 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 3) rope_append_kernel(const R
       }
       if (meta) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          mn[j] = fminf(mn[j], __shfl_xor_sync(0xffffffffu, mn[j], 16));
-          mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 16));
+        for (int j = 0; j < 4; ++j) {
+          mn[j] = min_pair<T>(mn[j], __shfl_xor_sync(0xffffffffu, mn[j], 16));
+          mx[j] = max_pair<T>(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], 16));
         }
-        *reinterpret_cast<uint4*>(mrow + hw * kD) = pack8<T>(hw ? mx : mn);
+        *reinterpret_cast<uint4*>(mrow + hw * kD) =
+            hw ? make_uint4(mx[0], mx[1], mx[2], mx[3]) : make_uint4(mn[0], mn[1], mn[2], mn[3]);
       }
     }
   }
@@ -296,15 +348,15 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 3) rope_append_kernel(const R
   const T* src = static_cast<const T*>(p.q) + (int64_t)(row + (mine ? tok : 0)) * p.q_ts + ch;
   T* dst = static_cast<T*>(p.q_out) + (int64_t)(row + (mine ? tok : 0)) * p.o_ts + ch;
   const int h_off = unit / width, rounds = (h_end - kv0 * G + h_step - 1) / h_step;  // rounds: the same for every lane
-  for (int i0 = 0; i0 < rounds; i0 += 4) {
-    uint4 u[4];
+  for (int i0 = 0; i0 < rounds; i0 += 8) {
+    uint4 u[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const int h = kv0 * G + h_off + (i0 + i) * h_step;
       if (mine && h < h_end) u[i] = load_row16(src + h * p.q_hs, p.wide);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const int h = kv0 * G + h_off + (i0 + i) * h_step;
       if (i0 + i >= rounds) break;
       if (p.rotary > 0) u[i] = rotate8<T, INTER>(u[i], ang, ch, p.rotary);
@@ -391,9 +443,10 @@ extern "C" int twl_rope_append_kv(const void* q, const void* k, const void* v, i
   const auto wide = [](const void* x, int64_t ts, int64_t hs) { return aligned(x, 16) && ts % 8 == 0 && hs % 8 == 0; };
   p.wide = wide(q, q_token_stride, q_head_stride) && wide(k, k_token_stride, k_head_stride) &&
            wide(v, v_token_stride, v_head_stride) && wide(q_out, out_token_stride, out_head_stride);
-  // One KV head (with its query heads) a block while there are fewer blocks than eight per SM (decode: latency), then
-  // more, up to eight: the sines of a page are computed once per block.
-  const int64_t room = (int64_t)num_sms() * 8;
+  // One KV head (with its query heads) a block while there are fewer blocks than four per SM (decode: latency), then more,
+  // up to eight: a block's look-up of its page and the sines are worth more rows (prompts of 21K tokens, 32/8 heads: 108 us,
+  // with three times the blocks 160 us).
+  const int64_t room = (int64_t)num_sms() * 4;
   int64_t heads = (slots * num_kv_heads + room - 1) / room;
   heads = heads < 1 ? 1 : heads > kRopeWarps ? kRopeWarps : heads;
   p.heads_per_block = (int32_t)(heads < num_kv_heads ? heads : num_kv_heads);

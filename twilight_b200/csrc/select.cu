@@ -657,7 +657,7 @@ static int launch_scores_g(const ScoreParams& p, cudaStream_t st) {
 // its rows, which is linear in the metadata,
 //   sum_r sum_d max(q_rd kmax_d, q_rd kmin_d) = sum_d (sum_r min(q_rd, 0)) kmin_d + (sum_r max(q_rd, 0)) kmax_d,
 // so a block is pooled once into 256 numbers and a page costs it 256 multiply-adds whatever its rows.  All of it
-// in 32 bits.  Three launches: pool, scores, selection.
+// in 32 bits (or as good).  Three launches: pool, scores, selection.
 // Slots: query block j of sequence b is slot qo_indptr[b]/query_block + b + j.
 struct BlockSelParams {
   const void *q, *kmeta;
@@ -671,28 +671,52 @@ struct QueryBlock {
   int b, row0, rows, first, last, pages;  // sequence, first query row, tokens, positions of the first and last, its pages
 };
 
-// The query block of a slot, found by the warp; rows = 0 where there is none.
-__device__ __forceinline__ QueryBlock query_block_of(const BlockSelParams& p, int slot) {
+// The query blocks of consecutive slots, found by the warp together: lane i gets that of slot + i (i < 16; more than
+// sixteen slots can span more sequences than a warp looks at); rows = 0 where there is none.
+__device__ __forceinline__ QueryBlock query_blocks_from(const BlockSelParams& p, int slot) {
   const int lane = threadIdx.x & 31;
-  int lo = 0, hi = p.batch;
+  int lo = 0, hi = p.batch;  // the sequence that slot belongs to, 32 candidates a round
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) >> 5, c = lo + lane * step;
     const int n = __popc(__ballot_sync(0xffffffffu, c < hi && p.qo_indptr[c] / p.query_block + c <= slot));
     lo += (n > 0 ? n - 1 : 0) * step;
     hi = min(hi, lo + step);
   }
-  QueryBlock r;
-  r.b = lo;
-  const int t0 = p.qo_indptr[lo], n_new = p.qo_indptr[lo + 1] - t0;
-  const int at = (slot - (t0 / p.query_block + lo)) * p.query_block;
-  const int n_pages = p.indptr[lo + 1] - p.indptr[lo], ll = p.last_len[lo];
+  // lane j has the entries of sequence lo + j; every sequence has a slot at least
+  const int b = min(lo + lane, p.batch - 1);
+  const int t0 = p.qo_indptr[b], n_new = p.qo_indptr[b + 1] - t0;
+  const int n_pages = p.indptr[b + 1] - p.indptr[b], ll = p.last_len[b];
   const bool bad = t0 < 0 || t0 + n_new > p.num_tokens || (n_pages > 0 && (ll < 1 || ll > kPage));
   const int len = n_pages > 0 && !bad ? (n_pages - 1) * kPage + ll : 0;
-  r.row0 = t0 + at;
-  r.rows = bad || at >= n_new ? 0 : min(p.query_block, n_new - at);
-  r.first = len - n_new + at;
+  const int first_slot = lo + lane < p.batch ? t0 / p.query_block + b : 0x7fffffff;
+  int mine = 0;  // of the sequences looked at, which has this lane's slot
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int n = __popc(__ballot_sync(0xffffffffu, first_slot <= slot + i));
+    if (lane == i) mine = max(n - 1, 0);
+  }
+  QueryBlock r;
+  r.b = lo + mine;
+  const int s_t0 = __shfl_sync(0xffffffffu, t0, mine), s_new = __shfl_sync(0xffffffffu, n_new, mine);
+  const int s_len = __shfl_sync(0xffffffffu, len, mine), s_pages = __shfl_sync(0xffffffffu, n_pages, mine);
+  const int s_bad = __shfl_sync(0xffffffffu, (int)bad, mine), s_slot = __shfl_sync(0xffffffffu, first_slot, mine);
+  const int at = (slot + lane - s_slot) * p.query_block;
+  r.row0 = s_t0 + at;
+  r.rows = s_bad || at < 0 || at >= s_new ? 0 : min(p.query_block, s_new - at);
+  r.first = s_len - s_new + at;
   r.last = r.first + r.rows - 1;
-  r.pages = min(max(n_pages, 0), p.max_pages);
+  r.pages = min(max(s_pages, 0), p.max_pages);
+  return r;
+}
+// The query block of one slot, for every lane of the warp.
+__device__ __forceinline__ QueryBlock query_block_of(const BlockSelParams& p, int slot) {
+  QueryBlock r = query_blocks_from(p, slot);
+  r.b = __shfl_sync(0xffffffffu, r.b, 0);
+  r.row0 = __shfl_sync(0xffffffffu, r.row0, 0);
+  r.rows = __shfl_sync(0xffffffffu, r.rows, 0);
+  r.first = __shfl_sync(0xffffffffu, r.first, 0);
+  r.last = __shfl_sync(0xffffffffu, r.last, 0);
+  r.pages = __shfl_sync(0xffffffffu, r.pages, 0);
   return r;
 }
 // pages wholly before the block's first position: the ones it chooses from
@@ -710,18 +734,28 @@ __global__ void __launch_bounds__(256) pool_query_blocks_kernel(const BlockSelPa
   if (history_pages(qb) == 0) return;
   const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
   float lo[8] = {}, hi[8] = {};
-  for (int r = r0; r < qb.rows * G; r += 16) {
-    const int tok = r / G;
-    const T* src = static_cast<const T*>(p.q) + (int64_t)(qb.row0 + tok) * p.q_ts + (kvh * G + r - tok * G) * kD;
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + c);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  const int rows = qb.rows * G;
+  for (int r4 = r0; r4 < rows; r4 += 128) {
+    uint4 v[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 f = Elem<T>::to_f2(u[k]);
-      lo[2 * k] += fminf(f.x, 0.f);
-      hi[2 * k] += fmaxf(f.x, 0.f);
-      lo[2 * k + 1] += fminf(f.y, 0.f);
-      hi[2 * k + 1] += fmaxf(f.y, 0.f);
+    for (int i = 0; i < 8; ++i) {  // eight rows in flight
+      const int r = r4 + 16 * i, tok = r / G;
+      v[i] = make_uint4(0, 0, 0, 0);  // (a row of zeros adds nothing)
+      if (r < rows)
+        v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (int64_t)(qb.row0 + tok) * p.q_ts +
+                                                    (kvh * G + r - tok * G) * kD) + c);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = Elem<T>::to_f2(u[k]);
+        lo[2 * k] += fminf(f.x, 0.f);
+        hi[2 * k] += fmaxf(f.x, 0.f);
+        lo[2 * k + 1] += fminf(f.y, 0.f);
+        hi[2 * k + 1] += fmaxf(f.y, 0.f);
+      }
     }
   }
 #pragma unroll
@@ -736,81 +770,99 @@ __global__ void __launch_bounds__(256) pool_query_blocks_kernel(const BlockSelPa
   p.pooled[((size_t)slot * p.Hkv + kvh) * 256 + threadIdx.x] = s;
 }
 
-// block = 64 pages x 16 slots of one KV head; a thread owns one page and four slots.  Both operands are staged in
-// shared memory (metadata as it lies in HBM, rows padded by 8 bytes: conflict-free 8-byte reads).
-constexpr int kBlkPages = 64, kBlkSlots = 16, kBlkMetaPitch = 260;
-constexpr int kBlkKeys = 200 * 1024;  // shared memory for the keys of a row: 51200 pages
-constexpr int kBlkSmem = kBlkSlots * 256 * 4 + kBlkPages * kBlkMetaPitch * 2;
+// block = 128 pages x 16 slots of one KV head on tensor cores: a warp's 16 pages are the A rows, taken from memory in
+// 16-byte pieces straight into the fragments as in quest_page_scores_mma_kernel, eight slots the columns.  The pooled
+// vectors are split into three bf16 (two fp16) numbers, each the rounded rest of the one before: 24 (22) bits, so the
+// products and their fp32 sums are as good as 32-bit ones.  They are scaled by a power of two near 1 / rows first,
+// which keeps fp16 in range.
+constexpr int kBlkSlots = 16, kBlkPitch = 288;  // elements of a row of pooled numbers: 32 more than it holds, for the banks
+template <typename T>
+struct BlkTerms {
+  static constexpr int kN = 2;
+};
+template <>
+struct BlkTerms<__nv_bfloat16> {
+  static constexpr int kN = 3;
+};
 template <typename T>
 __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelParams p) {
-  extern __shared__ __align__(16) uint8_t blk_smem[];
-  float (*pooled)[256] = reinterpret_cast<float (*)[256]>(blk_smem);
-  T* meta = reinterpret_cast<T*>(blk_smem + kBlkSlots * 256 * sizeof(float));
+  constexpr int N = BlkTerms<T>::kN;
+  __shared__ alignas(16) T pooled[N][kBlkSlots][kBlkPitch];
   __shared__ int hist_s[kBlkSlots], seq_s[kBlkSlots];
+  __shared__ float unscale_s[kBlkSlots];
   pdl_wait();
-  const int slot0 = blockIdx.z * kBlkSlots, kvh = blockIdx.y, page0 = blockIdx.x * kBlkPages;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = warp; i < kBlkSlots; i += 8) {
-    QueryBlock qb;
-    qb.rows = 0;
-    qb.b = -1;
-    if (slot0 + i < p.slots) qb = query_block_of(p, slot0 + i);
-    if (lane == 0) {
-      hist_s[i] = history_pages(qb);
-      seq_s[i] = qb.b;
+  const int slot0 = blockIdx.z * kBlkSlots, kvh = blockIdx.y, block_page = blockIdx.x * 128;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  __shared__ int rows_s[kBlkSlots];
+  if (warp == 0) {
+    const QueryBlock qb = query_blocks_from(p, slot0);
+    if (lane < kBlkSlots) {
+      const bool there = slot0 + lane < p.slots;
+      hist_s[lane] = there ? history_pages(qb) : 0;
+      seq_s[lane] = there ? qb.b : -1;
+      rows_s[lane] = qb.rows;
     }
   }
   __syncthreads();
-  bool any = false;
-  for (int i = 0; i < kBlkSlots; ++i) any |= hist_s[i] > page0;
-  if (!any) return;
-  for (int i = threadIdx.x; i < kBlkSlots * 64; i += 256) {
-    const int s = i >> 6;
-    if (hist_s[s] > page0)
-      reinterpret_cast<float4*>(pooled[s])[i & 63] =
-          reinterpret_cast<const float4*>(p.pooled + ((size_t)(slot0 + s) * p.Hkv + kvh) * 256)[i & 63];
+  for (int i = warp; i < kBlkSlots; i += 8) {
+    const int hist = hist_s[i];
+    const int rows = max(1, rows_s[i] * (p.Hq / p.Hkv)), shift = 32 - __clz(rows);
+    if (lane == 0) unscale_s[i] = (float)(1u << shift);
+    if (hist > block_page) {
+      const float scale = 1.f / (float)(1u << shift);
+      const float* src = p.pooled + ((size_t)(slot0 + i) * p.Hkv + kvh) * 256;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float x = src[32 * k + lane] * scale;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const T y = Elem<T>::from_f(x);
+          pooled[n][i][32 * k + lane] = y;
+          x -= Elem<T>::to_f(y);
+        }
+      }
+    }
   }
-  const int page = threadIdx.x & 63, sg = threadIdx.x >> 6;
+  __syncthreads();
+  const int page0 = block_page + warp * 16;
   for (int i0 = 0; i0 < kBlkSlots;) {  // the slots of one sequence at a time
     const int b = seq_s[i0];
-    int i1 = i0 + 1, n = hist_s[i0];
-    while (i1 < kBlkSlots && seq_s[i1] == b) n = max(n, hist_s[i1++]);
-    n = min(n - page0, kBlkPages);
-    if (n > 0) {
-      __syncthreads();  // the metadata of the sequence before has been used
+    int i1 = i0 + 1, n_pages = hist_s[i0];
+    while (i1 < kBlkSlots && seq_s[i1] == b) n_pages = max(n_pages, hist_s[i1++]);
+    if (n_pages > page0) {
       const int32_t* idx = p.indices + p.indptr[b] + page0;
-      for (int i = threadIdx.x; i < n * 32; i += 256) {
-        const int pg = i >> 5;
-        const int phys = idx[pg];
-        const bool ok = phys >= 0 && phys < p.num_pages_total;
-        if (!ok && (i & 31) == 0) raise_flag(p.status, TWL_FLAG_BAD_INDEX);
-        const uint4 v = ldg_stream_u4(static_cast<const T*>(p.kmeta) + ((size_t)(ok ? phys : 0) * p.Hkv + kvh) * 2 * kD +
-                                      8 * (i & 31));
-        uint2* to = reinterpret_cast<uint2*>(meta + pg * kBlkMetaPitch + 8 * (i & 31));
-        to[0] = make_uint2(v.x, v.y);
-        to[1] = make_uint2(v.z, v.w);
-      }
-      __syncthreads();
-      float acc[4] = {};
-      if (page < n) {
-        const uint2* m = reinterpret_cast<const uint2*>(meta + page * kBlkMetaPitch);
-#pragma unroll 4
-        for (int d = 0; d < 64; ++d) {
-          const uint2 u = m[d];
-          const float2 x = Elem<T>::to_f2(u.x), y = Elem<T>::to_f2(u.y);
+      const int here = min(16, n_pages - page0);
+      int phys[2];
+      uint4 v[2][8];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 w = reinterpret_cast<const float4*>(pooled[4 * sg + j])[d];
-            acc[j] += (x.x * w.x + x.y * w.y) + (y.x * w.z + y.y * w.w);
-          }
+      for (int h = 0; h < 2; ++h) {
+        phys[h] = g + 8 * h < here ? idx[g + 8 * h] : 0;
+        if (phys[h] < 0 || phys[h] >= p.num_pages_total) {
+          if (t == 0) raise_flag(p.status, TWL_FLAG_BAD_INDEX);
+          phys[h] = -1;
         }
-        const int phys = idx[page];
-        const bool ok = phys >= 0 && phys < p.num_pages_total;
+        const T* src = static_cast<const T*>(p.kmeta) + ((size_t)max(phys[h], 0) * p.Hkv + kvh) * 2 * kD + 8 * t;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int s = 4 * sg + j;
-          if (s >= i0 && s < i1 && page0 + page < hist_s[s])
-            p.scores[((size_t)(slot0 + s) * p.Hkv + kvh) * p.max_pages + page0 + page] = ok ? acc[j] : -INFINITY;
+        for (int c = 0; c < 8; ++c) v[h][c] = ldg_stream_u4(src + 32 * c);
+      }
+#pragma unroll
+      for (int n8 = 0; n8 < kBlkSlots; n8 += 8) {
+        if (n8 + 8 <= i0 || n8 >= i1) continue;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = N - 1; n >= 0; --n)  // the small terms first
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(&pooled[n][n8 + g][32 * c + 8 * t]);
+            MmaTile<T>::run(acc, v[0][c].x, v[1][c].x, v[0][c].y, v[1][c].y, w.x, w.y);
+            MmaTile<T>::run(acc, v[0][c].z, v[1][c].z, v[0][c].w, v[1][c].w, w.z, w.w);
+          }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int s = n8 + 2 * t + (e & 1), page = page0 + g + 8 * (e >> 1);
+          if (s >= i0 && s < i1 && page < hist_s[s])
+            p.scores[((size_t)(slot0 + s) * p.Hkv + kvh) * p.max_pages + page] =
+                phys[e >> 1] >= 0 ? acc[e] * unscale_s[s] : -INFINITY;
         }
       }
     }
@@ -818,6 +870,7 @@ __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelP
   }
 }
 
+constexpr int kBlkKeys = 200 * 1024;  // shared memory for the keys of a row: 51200 pages
 // block = (slot, KV head): the budget's best of the pages before the block, then the pages it lies in
 __global__ void __launch_bounds__(kTopkThreads) select_query_blocks_kernel(const BlockSelParams p) {
   extern __shared__ __align__(16) uint32_t keys[];
@@ -945,17 +998,13 @@ extern "C" int twl_quest_select_blocks(const void* q, int dtype, int64_t q_token
   p.slots = (int32_t)slots;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const dim3 per_slot((unsigned)slots, (unsigned)num_kv_heads);
-  const dim3 tiles((unsigned)((max_pages + kBlkPages - 1) / kBlkPages), (unsigned)num_kv_heads, (unsigned)slot_tiles);
+  const dim3 tiles((unsigned)((max_pages + 127) / 128), (unsigned)num_kv_heads, (unsigned)slot_tiles);
   if (dtype == TWL_F16) {
     TWL_CUDA_TRY(launch_chain(pool_query_blocks_kernel<__half>, per_slot, dim3(256), 0, st, p));
-    static int8_t done[kSmemDevices];
-    TWL_CUDA_TRY(allow_smem(score_query_blocks_kernel<__half>, kBlkSmem, done));
-    TWL_CUDA_TRY(launch_chain(score_query_blocks_kernel<__half>, tiles, dim3(256), kBlkSmem, st, p));
+    TWL_CUDA_TRY(launch_chain(score_query_blocks_kernel<__half>, tiles, dim3(256), 0, st, p));
   } else {
     TWL_CUDA_TRY(launch_chain(pool_query_blocks_kernel<__nv_bfloat16>, per_slot, dim3(256), 0, st, p));
-    static int8_t done[kSmemDevices];
-    TWL_CUDA_TRY(allow_smem(score_query_blocks_kernel<__nv_bfloat16>, kBlkSmem, done));
-    TWL_CUDA_TRY(launch_chain(score_query_blocks_kernel<__nv_bfloat16>, tiles, dim3(256), kBlkSmem, st, p));
+    TWL_CUDA_TRY(launch_chain(score_query_blocks_kernel<__nv_bfloat16>, tiles, dim3(256), 0, st, p));
   }
   static int8_t done[kSmemDevices];
   TWL_CUDA_TRY(allow_smem(select_query_blocks_kernel, kBlkKeys, done));

@@ -383,7 +383,8 @@ TWL_API int twl_dequantize_k_pages(const uint8_t* k4_pages, const int32_t* page_
  * out [T][H_q][128]; lse (nullable) fp32 [T][H_q], natural logarithm of the sum of exponentials, -inf
  * for a row without keys.  Rows of q behind qo_indptr[batch] are left as they were.
  * Softmax statistics and accumulators are fp32; weights are rounded to `dtype` for the product with V.
- * max_pages = the largest page count of a sequence (sizes the workspace).  workspace: at least
+ * max_pages = the largest page count of a sequence (sizes the workspace; where it is smaller than one, results
+ * can be left out, flagged with TWL_FLAG_BAD_INDEX).  workspace: at least
  * twl_prompt_attn_workspace_bytes(...) bytes, 256-byte aligned, contents irrelevant; calls that can
  * overlap on the GPU need one each.  V rows of tokens that a query does not see must be finite where they
  * share a tile of keys with tokens that it sees (rows behind a sequence's end may hold anything).

@@ -369,3 +369,183 @@ def test_a_prompts_whole_way_through_the_operators():
     kk, vv = (dense(x, ptr, idx, 0, n, 0) for x in (k, v))
     ref, _, p = attend64(qd[1, :4].double(), kk, vv, torch.ones(4, n, dtype=torch.bool, device=DEV))
     assert ((got[1, :4].double() - ref).abs() <= tol_of(dtype, p, vv, ref)).all()
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_prompt_fuzz(seed):
+    """Random batches: head groupings, lengths around the tiles' and chunks' borders, both masks, lists or none."""
+    r = torch.Generator().manual_seed(100 + seed)
+    pick = lambda xs: xs[int(torch.randint(len(xs), (1,), generator=r))]  # noqa: E731
+    for _ in range(5):
+        hkv, g = pick([(1, 1), (2, 1), (1, 2), (2, 3), (1, 4), (2, 5), (1, 7), (2, 8), (1, 12), (1, 33)])
+        dtype = pick([torch.float16, torch.bfloat16])
+        n = pick([1, 1, 2, 5])
+        new = [pick([0, 1, 2, 15, 16, 17, 31, 63, 64, 65, 127, 128, 129, 257, 300]) for _ in range(n)]
+        old = [pick([0, 0, 1, 15, 16, 100, 111, 112, 127, 128, 500, 1024, 1500, 3000]) for _ in range(n)]
+        if sum(new) == 0 or sum(a + b for a, b in zip(new, old)) == 0:
+            continue
+        q, k, v, qo, tab, lens = make_prompt(new, old, g * hkv, hkv, dtype, seed=seed)
+        most = max(1, max((x + 15) // 16 for x in lens))
+        block = pick([16, 32, 64, 128])
+        sparse, causal = pick([False, True]), pick([True, True, False])
+        kw, pages_of = {}, None
+        if sparse:
+            meta = ops.build_page_meta(k, *tab, max_pages=most)
+            pages, count = ops.quest_select_blocks(q, meta, qo, *tab, pick([16, 100, 640]), max_pages=most, query_block=block)
+            kw = dict(block_pages=pages, block_npages=count, query_block=block)
+
+            def pages_of(b, j, h, pages=pages, count=count, qo=qo, block=block):
+                s = int(qo[b]) // block + b + j
+                return pages[s, h, : int(count[s, h])]
+        poison_tails(k, v, tab[0], tab[1], lens)
+        status = torch.zeros(1, **I32)
+        out, lse = ops.prompt_attn(q, k, v, qo, *tab, max_pages=most, causal=causal, lse=True, status=status, **kw)
+        assert int(status) == 0
+        k, v = torch.nan_to_num(k, 0, 0, 0), torch.nan_to_num(v, 0, 0, 0)
+        check_prompt(q, k, v, qo, tab, lens, out, lse, causal, pages_of, block)
+
+
+@pytest.mark.parametrize("case", [
+    # a few tokens over a long context: runs and chunks of the keys, joined; and many tiles over one
+    ([1], [40000], 8, 1, torch.bfloat16),
+    ([4], [30011], 8, 2, torch.float16),
+    ([20], [30000], 8, 2, torch.bfloat16),
+    ([130], [20000], 2, 2, torch.float16),
+    ([700], [9000], 4, 1, torch.bfloat16),
+    ([40, 1, 3], [12000, 9000, 0], 16, 2, torch.bfloat16),
+])
+def test_prompt_long_contexts(case):
+    new, old, hq, hkv, dtype = case
+    q, k, v, qo, tab, lens = make_prompt(new, old, hq, hkv, dtype, seed=13)
+    out, lse = ops.prompt_attn(q, k, v, qo, *tab, max_pages=max((n + 15) // 16 for n in lens), lse=True)
+    check_prompt(q, k, v, qo, tab, lens, out, lse)
+    again = ops.prompt_attn(q, k, v, qo, *tab, max_pages=max((n + 15) // 16 for n in lens))
+    assert torch.equal(out, again)                              # the order of the work does not show
+
+
+def test_pages_behind_32_bit_offsets():
+    """Pools of more than 2^32 elements, the pages in use at their end: append, selection, attention of both kinds."""
+    hq, hkv, n, dtype = 16, 8, 200, torch.bfloat16
+    pages = 2 ** 32 // (hkv * PAGE * D) + 64
+    k, v = (torch.empty(pages, hkv, PAGE, D, dtype=dtype, device=DEV) for _ in range(2))
+    meta = torch.empty(pages, hkv, 2, D, dtype=dtype, device=DEV)
+    idx = (pages - 1 - torch.randperm(13)).to(**I32)
+    tab = (torch.tensor([0, 13], **I32), idx, torch.tensor([8], **I32))
+    g = torch.Generator(device=DEV).manual_seed(1)
+    proj = torch.randn(n, hq + 2 * hkv, D, generator=g, device=DEV).to(dtype)
+    qo = torch.tensor([0, n], **I32)
+    q = ops.rope_append_kv(proj[:, :hq], proj[:, hq: hq + hkv], proj[:, hq + hkv:], None, k, v, None, meta, qo, *tab)
+    kk = k[idx.long()].transpose(0, 1).reshape(hkv, -1, D)[:, :n]
+    assert torch.equal(kk, proj[:, hq: hq + hkv].transpose(0, 1))
+    lens = [n]
+    sel = ops.quest_select_blocks(q, meta, qo, *tab, 64, max_pages=13, query_block=32)
+    out, lse = ops.prompt_attn(q, k, v, qo, *tab, max_pages=13, block_pages=sel[0], block_npages=sel[1], query_block=32, lse=True)
+    # (sequence 0's query block j is slot j)
+    check_prompt(q, k, v, qo, tab, lens, out, lse, True, lambda b, j, h: sel[0][j, h, : int(sel[1][j, h])], 32)
+    none = torch.zeros(4, **I32), torch.zeros(0, **I32), torch.zeros(3, **I32)
+    got = ops.shared_prefix_attn(q[:3], k, v, torch.tensor([0, 3], **I32), *tab, *none)
+    want = ops.prompt_attn(q[:3], k, v, torch.tensor([0, 3], **I32), *tab, max_pages=13, causal=False)
+    assert (got.float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+
+
+def test_a_nan_or_infinity_of_a_visible_key_shows_and_a_masked_one_does_not():
+    for new, old in (([3], [60]), ([100], [60])):
+        q, k, v, qo, tab, lens = make_prompt(new, old, 4, 2, torch.bfloat16, seed=4)
+        clean = ops.prompt_attn(q, k, v, qo, *tab, max_pages=10)
+        bad = k.clone()
+        page, row = int(tab[1][(lens[0] - 1) // PAGE]), (lens[0] - 1) % PAGE
+        bad[page, 0, row] = float("nan")                        # the last token's K: only the last query sees it
+        got = ops.prompt_attn(q, bad, v, qo, *tab, max_pages=10)
+        assert torch.isnan(got[-1, :2].float()).all()
+        assert torch.equal(got[:-1], clean[:-1]) and torch.equal(got[-1, 2:], clean[-1, 2:])
+        bad = k.clone()
+        bad[int(tab[1][0]), 1, 5] = float("nan")                # a token that every query sees
+        got = ops.prompt_attn(q, bad, v, qo, *tab, max_pages=10)
+        assert torch.isnan(got[:, 2:].float()).all() and torch.equal(got[:, :2], clean[:, :2])
+
+
+def test_calls_on_two_streams_and_two_graphs_with_their_own_workspaces():
+    a = make_prompt([500, 3], [100, 4000], 8, 2, torch.bfloat16, seed=21)
+    b = make_prompt([90], [2000], 8, 2, torch.bfloat16, seed=22)
+    calls = [lambda ws=None, out=None, x=x: ops.prompt_attn(*x[:4], *x[4], max_pages=260, workspace=ws, out=out) for x in (a, b)]
+    want = [f() for f in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(calls[i]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+    graphs, outs = [], []
+    for i, f in enumerate(calls):
+        x = (a, b)[i]
+        n = ops.prompt_attn_workspace_bytes(x[0].shape[0], len(x[5]), 8, 2, 260)
+        ws, out = torch.empty(n, dtype=torch.uint8, device=DEV), torch.zeros_like(want[i])
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            f(ws, out)
+        graphs.append(gr)
+        outs.append((out, ws))
+    torch.cuda.synchronize()
+    for s, gr in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            for _ in range(3):
+                gr.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(outs[i][0], want[i])
+
+
+def test_too_small_max_pages_is_flagged_and_stays_in_its_workspace():
+    q, k, v, qo, tab, lens = make_prompt([2] * 40, [3000] * 40, 8, 2, torch.bfloat16, seed=6)
+    n = ops.prompt_attn_workspace_bytes(80, 40, 8, 2, 1)
+    ws = torch.full((n + 4096,), 173, dtype=torch.uint8, device=DEV)
+    status = torch.zeros(1, **I32)
+    ops.prompt_attn(q, k, v, qo, *tab, max_pages=1, workspace=ws[:n], status=status)
+    assert int(status) & ops.FLAG_BAD_INDEX and (ws[n:] == 173).all()
+
+
+def test_one_token_of_a_batch_with_a_foreign_stride_and_no_pages():
+    q, k, v, qo, tab, lens = make_prompt([1], [50], 4, 2, torch.float16, seed=8)
+    odd = torch.as_strided(q, q.shape, (13, D, 1))              # one token: its stride means nothing
+    assert torch.equal(ops.prompt_attn(odd, k, v, qo, *tab, max_pages=4), ops.prompt_attn(q, k, v, qo, *tab, max_pages=4))
+    empty = torch.zeros(2, **I32), torch.zeros(0, **I32), torch.zeros(1, **I32)
+    out, lse = ops.prompt_attn(q, k, v, qo, *empty, max_pages=1, lse=True)
+    assert not out.any() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_shared_prefix_fuzz(seed):
+    r = torch.Generator().manual_seed(300 + seed)
+    pick = lambda xs: xs[int(torch.randint(len(xs), (1,), generator=r))]  # noqa: E731
+    for _ in range(3):
+        hkv, gq = pick([(1, 1), (2, 4), (1, 8), (2, 5), (1, 16), (1, 9)])
+        dtype = pick([torch.float16, torch.bfloat16])
+        sizes = [pick([0, 1, 2, 3, 9, 16, 17, 60]) for _ in range(pick([1, 2, 4]))]
+        n = sum(sizes)
+        if n == 0:
+            continue
+        prefix = [pick([0, 1, 16, 127, 128, 129, 500, 2049]) for _ in sizes]
+        own = [pick([0, 0, 1, 15, 16, 17, 200, 700]) for _ in range(n)]
+        total = max(1, sum((x + 15) // 16 for x in prefix + own))
+        ptr, idx, last = table(own, 4, 0, total)
+        pptr, pidx, plast = table(prefix, 4, idx.numel(), total)
+        k, v, lean, g = pool(total, hkv, dtype, seed)
+        q = (torch.randn(n, hkv, gq, D, generator=g, device=DEV) + 0.3 * lean).reshape(n, hkv * gq, D).to(dtype)
+        poison_tails(k, v, ptr, idx, own)
+        poison_tails(k, v, pptr, pidx, prefix)
+        group = torch.tensor([0] + torch.tensor(sizes).cumsum(0).tolist(), **I32)
+        out = ops.shared_prefix_attn(q, k, v, group, pptr, pidx, plast, ptr, idx, last)
+        k, v = torch.nan_to_num(k, 0, 0, 0), torch.nan_to_num(v, 0, 0, 0)
+        for i in range(len(sizes)):
+            for b in range(int(group[i]), int(group[i + 1])):
+                for h in range(hkv):
+                    kk = torch.cat([dense(k, pptr, pidx, i, prefix[i], h), dense(k, ptr, idx, b, own[b], h)])
+                    vv = torch.cat([dense(v, pptr, pidx, i, prefix[i], h), dense(v, ptr, idx, b, own[b], h)])
+                    ref, _, p = attend64(q[b, h * gq: (h + 1) * gq].double(), kk, vv,
+                                         torch.ones(gq, kk.shape[0], dtype=torch.bool, device=DEV))
+                    got = out[b, h * gq: (h + 1) * gq].double()
+                    assert ((got - ref).abs() <= tol_of(dtype, p, vv, ref)).all(), (sizes, prefix, i, b, h)

@@ -201,6 +201,8 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnPar
   }
   merge = __syncthreads_or(merge);
   if (tid == 0) {
+    // (more work than the workspace is sized for: max_pages was smaller than a page count; what does not fit is left out)
+    if (base[1] > p.tile_cap || base[2] > p.part_cap) raise_flag(p.status, TWL_FLAG_BAD_INDEX);
     p.hdr->units = base[0];
     p.hdr->per_warp = per_warp;
     p.hdr->tile_items = (int)min(base[1], (long long)p.tile_cap);
@@ -736,12 +738,13 @@ extern "C" int twl_prompt_attn(const void* q, int dtype, int64_t q_token_stride,
                                void* out, float* lse, void* workspace, size_t workspace_bytes, int32_t* status,
                                void* stream) {
   using namespace twl;
-  if (!q || !k_pages || !v_pages || !qo_indptr || !kv_indptr || !kv_indices || !kv_last_page_len || !out)
-    return TWL_ERR_BAD_ARG;
+  // (the index list may be null where no sequence has pages)
+  if (!q || !k_pages || !v_pages || !qo_indptr || !kv_indptr || !kv_last_page_len || !out) return TWL_ERR_BAD_ARG;
   if ((block_pages == nullptr) != (block_npages == nullptr)) return TWL_ERR_BAD_ARG;
   if (block_pages && (max_k <= 0 || query_block <= 0)) return TWL_ERR_BAD_ARG;
   const int bad = check_attention(dtype, num_tokens, batch, num_q_heads, num_kv_heads, num_pages_total, max_pages);
   if (bad != TWL_OK) return bad;
+  if (num_tokens == 1) q_token_stride = (int64_t)num_q_heads * kD;  // one token: its stride says nothing
   if (block_pages && query_block % kPage != 0) return TWL_ERR_UNSUPPORTED;
   if (!(sm_scale > 0.f)) return TWL_ERR_BAD_ARG;  // the running maximum is that of the scaled products
   if (!aligned(q, 16) || q_token_stride % 8 != 0 || !aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(out, 16))
@@ -751,7 +754,8 @@ extern "C" int twl_prompt_attn(const void* q, int dtype, int64_t q_token_stride,
   if (!workspace || workspace_bytes < w.total || !aligned(workspace, 256)) return TWL_ERR_WORKSPACE;
   AttnParams p = {};
   p.q = q; p.k_pages = k_pages; p.v_pages = v_pages; p.out = out; p.lse = lse;
-  p.q_ts = q_token_stride; p.o_ts = (int64_t)num_q_heads * kD;
+  p.q_ts = q_token_stride;
+  p.o_ts = (int64_t)num_q_heads * kD;
   p.qo1 = qo_indptr; p.indptr1 = kv_indptr; p.indices1 = kv_indices; p.last1 = kv_last_page_len;
   p.n_first = batch; p.causal = causal != 0;
   p.block_pages = block_pages; p.block_npages = block_npages; p.max_k = max_k;
@@ -787,6 +791,7 @@ extern "C" int twl_shared_prefix_attn(const void* q, int dtype, int64_t q_token_
     return TWL_ERR_BAD_ARG;
   const int bad = check_attention(dtype, batch, batch, num_q_heads, num_kv_heads, num_pages_total, max_pages);
   if (bad != TWL_OK) return bad;
+  if (batch == 1) q_token_stride = (int64_t)num_q_heads * kD;  // one token: its stride says nothing
   if (!(sm_scale > 0.f)) return TWL_ERR_BAD_ARG;
   if (!aligned(q, 16) || q_token_stride % 8 != 0 || !aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(out, 16))
     return TWL_ERR_MISALIGNED;
@@ -795,7 +800,8 @@ extern "C" int twl_shared_prefix_attn(const void* q, int dtype, int64_t q_token_
   if (!workspace || workspace_bytes < w.total || !aligned(workspace, 256)) return TWL_ERR_WORKSPACE;
   AttnParams p = {};
   p.q = q; p.k_pages = k_pages; p.v_pages = v_pages; p.out = out; p.lse = lse;
-  p.q_ts = q_token_stride; p.o_ts = (int64_t)num_q_heads * kD;
+  p.q_ts = q_token_stride;
+  p.o_ts = (int64_t)num_q_heads * kD;
   p.indptr1 = kv_indptr; p.indices1 = kv_indices; p.last1 = kv_last_page_len; p.n_first = batch;
   p.qo2 = group_indptr; p.indptr2 = prefix_indptr; p.indices2 = prefix_indices; p.last2 = prefix_last_page_len;
   p.n_second = num_groups; p.always_partial = 1; p.query_block = 1;

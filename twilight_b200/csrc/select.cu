@@ -770,12 +770,12 @@ __global__ void __launch_bounds__(256) pool_query_blocks_kernel(const BlockSelPa
   p.pooled[((size_t)slot * p.Hkv + kvh) * 256 + threadIdx.x] = s;
 }
 
-// block = 128 pages x 16 slots of one KV head on tensor cores: a warp's 16 pages are the A rows, taken from memory in
+// block = 256 pages x 16 slots of one KV head on tensor cores: 16 pages at a time are a warp's A rows, taken from memory in
 // 16-byte pieces straight into the fragments as in quest_page_scores_mma_kernel, eight slots the columns.  The pooled
 // vectors are split into three bf16 (two fp16) numbers, each the rounded rest of the one before: 24 (22) bits, so the
 // products and their fp32 sums are as good as 32-bit ones.  They are scaled by a power of two near 1 / rows first,
 // which keeps fp16 in range.
-constexpr int kBlkSlots = 16, kBlkPitch = 288;  // elements of a row of pooled numbers: 32 more than it holds, for the banks
+constexpr int kBlkPages = 256, kBlkSlots = 16, kBlkPitch = 288;  // elements of a row of pooled numbers: 32 more than it holds, for the banks
 template <typename T>
 struct BlkTerms {
   static constexpr int kN = 2;
@@ -791,7 +791,7 @@ __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelP
   __shared__ int hist_s[kBlkSlots], seq_s[kBlkSlots];
   __shared__ float unscale_s[kBlkSlots];
   pdl_wait();
-  const int slot0 = blockIdx.z * kBlkSlots, kvh = blockIdx.y, block_page = blockIdx.x * 128;
+  const int slot0 = blockIdx.z * kBlkSlots, kvh = blockIdx.y, block_page = blockIdx.x * kBlkPages;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   __shared__ int rows_s[kBlkSlots];
   if (warp == 0) {
@@ -824,49 +824,50 @@ __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelP
     }
   }
   __syncthreads();
-  const int page0 = block_page + warp * 16;
-  for (int i0 = 0; i0 < kBlkSlots;) {  // the slots of one sequence at a time
-    const int b = seq_s[i0];
-    int i1 = i0 + 1, n_pages = hist_s[i0];
-    while (i1 < kBlkSlots && seq_s[i1] == b) n_pages = max(n_pages, hist_s[i1++]);
-    if (n_pages > page0) {
-      const int32_t* idx = p.indices + p.indptr[b] + page0;
-      const int here = min(16, n_pages - page0);
-      int phys[2];
-      uint4 v[2][8];
+  for (int page0 = block_page + warp * 16; page0 < block_page + kBlkPages; page0 += 128) {
+    for (int i0 = 0; i0 < kBlkSlots;) {  // the slots of one sequence at a time
+      const int b = seq_s[i0];
+      int i1 = i0 + 1, n_pages = hist_s[i0];
+      while (i1 < kBlkSlots && seq_s[i1] == b) n_pages = max(n_pages, hist_s[i1++]);
+      if (n_pages > page0) {
+        const int32_t* idx = p.indices + p.indptr[b] + page0;
+        const int here = min(16, n_pages - page0);
+        int phys[2];
+        uint4 v[2][8];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        phys[h] = g + 8 * h < here ? idx[g + 8 * h] : 0;
-        if (phys[h] < 0 || phys[h] >= p.num_pages_total) {
-          if (t == 0) raise_flag(p.status, TWL_FLAG_BAD_INDEX);
-          phys[h] = -1;
-        }
-        const T* src = static_cast<const T*>(p.kmeta) + ((size_t)max(phys[h], 0) * p.Hkv + kvh) * 2 * kD + 8 * t;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[h][c] = ldg_stream_u4(src + 32 * c);
-      }
-#pragma unroll
-      for (int n8 = 0; n8 < kBlkSlots; n8 += 8) {
-        if (n8 + 8 <= i0 || n8 >= i1) continue;
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int n = N - 1; n >= 0; --n)  // the small terms first
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const uint4 w = *reinterpret_cast<const uint4*>(&pooled[n][n8 + g][32 * c + 8 * t]);
-            MmaTile<T>::run(acc, v[0][c].x, v[1][c].x, v[0][c].y, v[1][c].y, w.x, w.y);
-            MmaTile<T>::run(acc, v[0][c].z, v[1][c].z, v[0][c].w, v[1][c].w, w.z, w.w);
+        for (int h = 0; h < 2; ++h) {
+          phys[h] = g + 8 * h < here ? idx[g + 8 * h] : 0;
+          if (phys[h] < 0 || phys[h] >= p.num_pages_total) {
+            if (t == 0) raise_flag(p.status, TWL_FLAG_BAD_INDEX);
+            phys[h] = -1;
           }
+          const T* src = static_cast<const T*>(p.kmeta) + ((size_t)max(phys[h], 0) * p.Hkv + kvh) * 2 * kD + 8 * t;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int s = n8 + 2 * t + (e & 1), page = page0 + g + 8 * (e >> 1);
-          if (s >= i0 && s < i1 && page < hist_s[s])
-            p.scores[((size_t)(slot0 + s) * p.Hkv + kvh) * p.max_pages + page] =
-                phys[e >> 1] >= 0 ? acc[e] * unscale_s[s] : -INFINITY;
+          for (int c = 0; c < 8; ++c) v[h][c] = ldg_stream_u4(src + 32 * c);
+        }
+#pragma unroll
+        for (int n8 = 0; n8 < kBlkSlots; n8 += 8) {
+          if (n8 + 8 <= i0 || n8 >= i1) continue;
+          float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int n = N - 1; n >= 0; --n)  // the small terms first
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const uint4 w = *reinterpret_cast<const uint4*>(&pooled[n][n8 + g][32 * c + 8 * t]);
+              MmaTile<T>::run(acc, v[0][c].x, v[1][c].x, v[0][c].y, v[1][c].y, w.x, w.y);
+              MmaTile<T>::run(acc, v[0][c].z, v[1][c].z, v[0][c].w, v[1][c].w, w.z, w.w);
+            }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int s = n8 + 2 * t + (e & 1), page = page0 + g + 8 * (e >> 1);
+            if (s >= i0 && s < i1 && page < hist_s[s])
+              p.scores[((size_t)(slot0 + s) * p.Hkv + kvh) * p.max_pages + page] =
+                  phys[e >> 1] >= 0 ? acc[e] * unscale_s[s] : -INFINITY;
+          }
         }
       }
+      i0 = i1;
     }
-    i0 = i1;
   }
 }
 
@@ -982,6 +983,7 @@ extern "C" int twl_quest_select_blocks(const void* q, int dtype, int64_t q_token
     return TWL_ERR_BAD_ARG;
   if (query_block < kPage || query_block % kPage != 0) return TWL_ERR_UNSUPPORTED;
   if (dtype != TWL_F16 && dtype != TWL_BF16) return TWL_ERR_UNSUPPORTED;
+  if (num_tokens == 1) q_token_stride = (int64_t)num_q_heads * kD;  // one token: its stride says nothing
   if (!aligned(q, 16) || q_token_stride % 8 != 0 || !aligned(kmeta, 16) || !aligned(pooled, 16))
     return TWL_ERR_MISALIGNED;
   const int64_t slots = (int64_t)num_tokens / query_block + batch;
@@ -998,7 +1000,7 @@ extern "C" int twl_quest_select_blocks(const void* q, int dtype, int64_t q_token
   p.slots = (int32_t)slots;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const dim3 per_slot((unsigned)slots, (unsigned)num_kv_heads);
-  const dim3 tiles((unsigned)((max_pages + 127) / 128), (unsigned)num_kv_heads, (unsigned)slot_tiles);
+  const dim3 tiles((unsigned)((max_pages + kBlkPages - 1) / kBlkPages), (unsigned)num_kv_heads, (unsigned)slot_tiles);
   if (dtype == TWL_F16) {
     TWL_CUDA_TRY(launch_chain(pool_query_blocks_kernel<__half>, per_slot, dim3(256), 0, st, p));
     TWL_CUDA_TRY(launch_chain(score_query_blocks_kernel<__half>, tiles, dim3(256), 0, st, p));

@@ -806,7 +806,8 @@ extern "C" int twl_shared_prefix_attn(const void* q, int dtype, int64_t q_token_
   p.qo2 = group_indptr; p.indptr2 = prefix_indptr; p.indices2 = prefix_indices; p.last2 = prefix_last_page_len;
   p.n_second = num_groups; p.always_partial = 1; p.query_block = 1;
   p.num_tokens = batch; p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = num_q_heads / num_kv_heads;
-  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; p.row_tile = p.G <= 8 ? 8 : 16;
+  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; // (a batch of up to sixteen rows per KV head is one row tile, its prefixes' too)
+  p.row_tile = p.G <= 8 && batch * p.G > kFewRows ? 8 : 16;
   p.scale_log2 = sm_scale * 1.44269504088896341f;
   p.status = status;
   place_workspace(p, w, workspace);

@@ -21,6 +21,8 @@ HEAD_DIM = 128
 K4_SLAB_BYTES = 1280
 
 FLAG_ITER_CAP, FLAG_BAD_INDEX, FLAG_WAIT_LIMIT = 1, 2, 4
+_SM_SCALE = 1.0 / math.sqrt(HEAD_DIM)
+_INT32 = torch.int32
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -160,14 +162,25 @@ def _launch(name: str, on: torch.Tensor, *args, **same_device: Optional[torch.Te
     """Calls entry point ``twl_<name>`` with ``on``'s device current (the library launches on the
     current device); the keyword tensors are checked to live on that device.  Raises
     :class:`TwilightError` on a non-zero status."""
+    lib = _lib.load()
+    with _on(on, **same_device):
+        st = getattr(lib, "twl_" + name)(*args)
+    _lib.check(st, name)
+
+
+def _launch_small(name: str, index: int, tensors, args) -> None:
+    """:func:`_launch` for operators that can take less than ten microseconds on the GPU, where what the host does
+    between two calls is what counts: ``tensors`` (name, tensor, name, tensor ..) are compared by device index, and no
+    context is entered when the device is the current one."""
+    for t in tensors[1::2]:
+        if t is not None and t.get_device() != index:
+            _same_device(torch.device("cuda", index), **dict(zip(tensors[::2], tensors[1::2])))
     fn = getattr(_lib.load(), "twl_" + name)
-    index = on.get_device()
-    if index < 0 or any(t is not None and t.get_device() != index for t in same_device.values()) \
-            or torch.cuda.current_device() != index:
-        with _on(on, **same_device):
-            st = fn(*args)
-    else:  # the usual case, without a context
+    if torch._C._cuda_getDevice() == index:
         st = fn(*args)
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args)
     if st != 0:
         _lib.check(st, name)
 
@@ -567,21 +580,25 @@ def _pool(t: torch.Tensor, name: str, dtype: torch.dtype, shape) -> None:
         raise _lib.TwilightError(f"{name} must be contiguous {list(shape)} (pages and heads of k_pages)")
 
 
-def _i32(t: torch.Tensor, name: str, entries: int = -1) -> None:
-    if t.dtype != torch.int32 or not t.is_contiguous():
+def _i32(t: torch.Tensor, name: str, entries: int = -1) -> int:
+    """Checks a contiguous int32 tensor (of so many entries); its address."""
+    if t.dtype != _INT32 or not t.is_contiguous():
         raise _lib.TwilightError(f"{name} must be contiguous int32")
     if entries >= 0 and t.numel() != entries:
         raise _lib.TwilightError(f"{name} must have {entries} entries")
+    return t.data_ptr()
 
 
 def _kv_pools(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor) -> Tuple[int, int]:
     """Checks the K and V pools against the queries; ``(pages, KV heads)``."""
     if k_pages.dim() != 4:
         raise _lib.TwilightError(f"k_pages must be [pages, kv heads, {PAGE}, {HEAD_DIM}]")
-    pages, hkv = k_pages.shape[0], k_pages.shape[1]
-    shape = (pages, hkv, PAGE, HEAD_DIM)
-    _pool(k_pages, "k_pages", q.dtype, shape)
-    _pool(v_pages, "v_pages", q.dtype, shape)
+    pages, hkv, page, dim = k_pages.shape
+    dtype = q.dtype
+    if (page != PAGE or dim != HEAD_DIM or k_pages.dtype != dtype or not k_pages.is_contiguous() or v_pages.dtype != dtype
+            or v_pages.shape != k_pages.shape or not v_pages.is_contiguous()):
+        _pool(k_pages, "k_pages", dtype, (pages, hkv, PAGE, HEAD_DIM))  # (says which)
+        _pool(v_pages, "v_pages", dtype, (pages, hkv, PAGE, HEAD_DIM))
     if hkv == 0 or q.shape[1] % hkv:
         raise _lib.TwilightError("query heads must be a multiple of KV heads")
     return pages, hkv
@@ -608,10 +625,8 @@ def rope_append_kv(q, k, v, freqs, k_pages, v_pages, k4_pages, kmeta, qo_indptr,
         _pool(kmeta, "kmeta", q.dtype, (pages, hkv, 2, HEAD_DIM))
     if k4_pages is not None:
         _pool(k4_pages, "k4_pages", torch.uint8, (pages, hkv, K4_SLAB_BYTES))
-    _i32(qo_indptr, "qo_indptr")
-    _i32(kv_indptr, "kv_indptr", batch + 1)
-    _i32(kv_indices, "kv_indices")
-    _i32(kv_last_page_len, "kv_last_page_len", batch)
+    qo_p, ptr_p = _i32(qo_indptr, "qo_indptr"), _i32(kv_indptr, "kv_indptr", batch + 1)
+    idx_p, last_p = _i32(kv_indices, "kv_indices"), _i32(kv_last_page_len, "kv_last_page_len", batch)
     if freqs is not None and (freqs.dtype != torch.float64 or not freqs.is_contiguous()):
         raise _lib.TwilightError("freqs must be contiguous float64 (see rope_frequencies)")
     if positions is not None and (positions.dtype not in (torch.int32, torch.int64) or positions.shape != (t,)
@@ -624,14 +639,17 @@ def rope_append_kv(q, k, v, freqs, k_pages, v_pages, k4_pages, kmeta, qo_indptr,
     _cuda(q)
     if t == 0:
         return out
-    _launch("rope_append_kv", q, q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(q), q.stride(0), q.stride(1),
-            k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
-            _p(positions), int(positions is not None and positions.dtype == torch.int64), _p(freqs),
-            0 if freqs is None else 2 * freqs.numel(), int(interleaved), float(attention_scale), k_pages.data_ptr(),
-            v_pages.data_ptr(), _p(k4_pages), _p(kmeta), qo_indptr.data_ptr(), kv_indptr.data_ptr(),
-            kv_indices.data_ptr(), kv_last_page_len.data_ptr(), t, batch, hq, hkv, pages, _p(status), _stream(q.device), k=k, v=v, out=out, positions=positions, freqs=freqs, k_pages=k_pages,
-            v_pages=v_pages, k4_pages=k4_pages, kmeta=kmeta, qo_indptr=qo_indptr, kv_indptr=kv_indptr,
-            kv_indices=kv_indices, kv_last_page_len=kv_last_page_len, status=status)
+    index = q.get_device()
+    (q_ts, q_hs, _), (k_ts, k_hs, _), (v_ts, v_hs, _), (o_ts, o_hs, _) = q.stride(), k.stride(), v.stride(), out.stride()
+    _launch_small("rope_append_kv", index,
+                  ("k", k, "v", v, "out", out, "positions", positions, "freqs", freqs, "k_pages", k_pages, "v_pages", v_pages,
+                   "k4_pages", k4_pages, "kmeta", kmeta, "qo_indptr", qo_indptr, "kv_indptr", kv_indptr,
+                   "kv_indices", kv_indices, "kv_last_page_len", kv_last_page_len, "status", status),
+                  (q.data_ptr(), k.data_ptr(), v.data_ptr(), _dtype_code(q), q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, out.data_ptr(),
+                   o_ts, o_hs, _p(positions), 0 if positions is None else positions.dtype == torch.int64, _p(freqs),
+                   0 if freqs is None else 2 * freqs.numel(), interleaved, attention_scale, k_pages.data_ptr(),
+                   v_pages.data_ptr(), _p(k4_pages), _p(kmeta), qo_p, ptr_p, idx_p, last_p, t, batch, hq, hkv, pages,
+                   _p(status), torch._C._cuda_getCurrentRawStream(index)))
     return out
 
 
@@ -651,8 +669,10 @@ def dequantize_k_pages(k4_pages, page_ids=None, *, dtype: torch.dtype, out=None,
         raise _lib.TwilightError(f"out must be contiguous {dtype} [{n}, {hkv}, {PAGE}, {HEAD_DIM}]")
     if out.numel() == 0:
         return out
-    _launch("dequantize_k_pages", k4_pages, k4_pages.data_ptr(), _p(page_ids), n, out.data_ptr(), _dtype_code(out),
-            hkv, pages, _p(status), _stream(k4_pages.device), page_ids=page_ids, out=out, status=status)
+    index = k4_pages.get_device()
+    _launch_small("dequantize_k_pages", index, ("page_ids", page_ids, "out", out, "status", status),
+                  (k4_pages.data_ptr(), _p(page_ids), n, out.data_ptr(), _dtype_code(out), hkv, pages, _p(status),
+                   torch._C._cuda_getCurrentRawStream(index)))
     return out
 
 
@@ -711,10 +731,8 @@ def prompt_attn(q, k_pages, v_pages, qo_indptr, kv_indptr, kv_indices, kv_last_p
     t, hq = q.shape[0], q.shape[1]
     pages, hkv = _kv_pools(q, k_pages, v_pages)
     batch = qo_indptr.numel() - 1
-    _i32(qo_indptr, "qo_indptr")
-    _i32(kv_indptr, "kv_indptr", batch + 1)
-    _i32(kv_indices, "kv_indices")
-    _i32(kv_last_page_len, "kv_last_page_len", batch)
+    qo_p, ptr_p = _i32(qo_indptr, "qo_indptr"), _i32(kv_indptr, "kv_indptr", batch + 1)
+    idx_p, last_p = _i32(kv_indices, "kv_indices"), _i32(kv_last_page_len, "kv_last_page_len", batch)
     out, lse = _result(q, out, lse)
     if (block_pages is None) != (block_npages is None):
         raise _lib.TwilightError("block_pages and block_npages go together")
@@ -730,13 +748,15 @@ def prompt_attn(q, k_pages, v_pages, qo_indptr, kv_indptr, kv_indices, kv_last_p
     _cuda(q)
     if t > 0:
         workspace = _workspace(workspace, prompt_attn_workspace_bytes(t, batch, hq, hkv, max_pages, query_block), q.device)
-        _launch("prompt_attn", q, q.data_ptr(), _dtype_code(q), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
-                qo_indptr.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(), t, batch,
-                hq, hkv, pages, max_pages, int(causal), _p(block_pages), _p(block_npages), max_k, query_block,
-                1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, out.data_ptr(), _p(lse),
-                workspace.data_ptr(), workspace.numel(), _p(status), _stream(q.device), k_pages=k_pages, v_pages=v_pages,
-                qo_indptr=qo_indptr, kv_indptr=kv_indptr, kv_indices=kv_indices, kv_last_page_len=kv_last_page_len,
-                block_pages=block_pages, block_npages=block_npages, out=out, lse=lse, workspace=workspace, status=status)
+        index = q.get_device()
+        _launch_small("prompt_attn", index,
+                      ("k_pages", k_pages, "v_pages", v_pages, "qo_indptr", qo_indptr, "kv_indptr", kv_indptr,
+                       "kv_indices", kv_indices, "kv_last_page_len", kv_last_page_len, "block_pages", block_pages,
+                       "block_npages", block_npages, "out", out, "lse", lse, "workspace", workspace, "status", status),
+                      (q.data_ptr(), _dtype_code(q), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(), qo_p, ptr_p, idx_p,
+                       last_p, t, batch, hq, hkv, pages, max_pages, causal, _p(block_pages), _p(block_npages), max_k,
+                       query_block, _SM_SCALE if sm_scale is None else sm_scale, out.data_ptr(), _p(lse),
+                       workspace.data_ptr(), workspace.numel(), _p(status), torch._C._cuda_getCurrentRawStream(index)))
     return out if lse is None else (out, lse)
 
 
@@ -822,13 +842,11 @@ def shared_prefix_attn(q, k_pages, v_pages, group_indptr, prefix_indptr, prefix_
     b, hq = q.shape[0], q.shape[1]
     pages, hkv = _kv_pools(q, k_pages, v_pages)
     groups = group_indptr.numel() - 1
-    _i32(group_indptr, "group_indptr")
-    _i32(prefix_indptr, "prefix_indptr", groups + 1)
-    _i32(prefix_indices, "prefix_indices")
-    _i32(prefix_last_page_len, "prefix_last_page_len", groups)
-    _i32(kv_indptr, "kv_indptr", b + 1)
-    _i32(kv_indices, "kv_indices")
-    _i32(kv_last_page_len, "kv_last_page_len", b)
+    group_p, pptr_p = _i32(group_indptr, "group_indptr"), _i32(prefix_indptr, "prefix_indptr", groups + 1)
+    pidx_p = _i32(prefix_indices, "prefix_indices")
+    plast_p = _i32(prefix_last_page_len, "prefix_last_page_len", groups)
+    ptr_p, idx_p = _i32(kv_indptr, "kv_indptr", b + 1), _i32(kv_indices, "kv_indices")
+    last_p = _i32(kv_last_page_len, "kv_last_page_len", b)
     if groups < 1:
         raise _lib.TwilightError("group_indptr must have at least two entries")
     out, lse = _result(q, out, lse)
@@ -837,15 +855,16 @@ def shared_prefix_attn(q, k_pages, v_pages, group_indptr, prefix_indptr, prefix_
         if max_pages is None:
             max_pages = max(prefix_indices.numel(), kv_indices.numel(), 1)
         workspace = _workspace(workspace, shared_prefix_workspace_bytes(b, groups, hq, hkv, max_pages), q.device)
-        _launch("shared_prefix_attn", q, q.data_ptr(), _dtype_code(q), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(),
-                group_indptr.data_ptr(), prefix_indptr.data_ptr(), prefix_indices.data_ptr(),
-                prefix_last_page_len.data_ptr(), kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_last_page_len.data_ptr(),
-                b, groups, hq, hkv, pages, max_pages,
-                1.0 / math.sqrt(HEAD_DIM) if sm_scale is None else sm_scale, out.data_ptr(), _p(lse),
-                workspace.data_ptr(), workspace.numel(), _p(status), _stream(q.device), k_pages=k_pages, v_pages=v_pages,
-                group_indptr=group_indptr, prefix_indptr=prefix_indptr, prefix_indices=prefix_indices,
-                prefix_last_page_len=prefix_last_page_len, kv_indptr=kv_indptr, kv_indices=kv_indices,
-                kv_last_page_len=kv_last_page_len, out=out, lse=lse, workspace=workspace, status=status)
+        index = q.get_device()
+        _launch_small("shared_prefix_attn", index,
+                      ("k_pages", k_pages, "v_pages", v_pages, "group_indptr", group_indptr, "prefix_indptr", prefix_indptr,
+                       "prefix_indices", prefix_indices, "prefix_last_page_len", prefix_last_page_len, "kv_indptr", kv_indptr,
+                       "kv_indices", kv_indices, "kv_last_page_len", kv_last_page_len, "out", out, "lse", lse,
+                       "workspace", workspace, "status", status),
+                      (q.data_ptr(), _dtype_code(q), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(), group_p, pptr_p,
+                       pidx_p, plast_p, ptr_p, idx_p, last_p, b, groups, hq, hkv, pages, max_pages,
+                       _SM_SCALE if sm_scale is None else sm_scale, out.data_ptr(), _p(lse), workspace.data_ptr(),
+                       workspace.numel(), _p(status), torch._C._cuda_getCurrentRawStream(index)))
     return out if lse is None else (out, lse)
 
 

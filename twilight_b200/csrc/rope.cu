@@ -365,36 +365,48 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 3) rope_append_kernel(const R
   }
 }
 
-// INT4 slabs as values: thread = eight channels of a token (one code word, one 16-byte store), block = a slab.
+// INT4 slabs as values: thread = eight channels of a token (one code word, one 16-byte store), block = four slabs that
+// follow one another in the output (all four in flight; one slab a block: 14.8 instead of 12.7 us on 10.6K slabs, 57 MB).
 struct DequantParams {
   const uint8_t* k4;
   const int32_t* page_ids;  // null: every page
   void* out;
   int32_t* status;
+  int64_t items;
   int32_t Hkv, num_pages_total;
 };
+constexpr int kDequantSlabs = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_k_pages_kernel(const DequantParams p) {
   pdl_wait();
-  const int64_t item = blockIdx.x;
-  const int64_t i = item / p.Hkv;
-  const int head = (int)(item - i * p.Hkv);
-  const int64_t page = p.page_ids ? (int64_t)__ldg(p.page_ids + i) : i;
+  const int64_t item0 = (int64_t)blockIdx.x * kDequantSlabs;
   const int tok = threadIdx.x >> 4, w = threadIdx.x & 15;
-  uint4 r = make_uint4(0, 0, 0, 0);
-  if (page >= 0 && page < p.num_pages_total) {
-    const uint8_t* slab = p.k4 + ((size_t)page * p.Hkv + head) * kSlab;
-    const uint32_t code = ldg_stream_u32(slab + tok * 64 + w * 4);
-    const uint32_t sz = ldg_stream_u32(slab + kSlabCodes + tok * 16 + (w >> 2) * 4);
-    const float2 f = Elem<__half>::to_f2(sz);
+  uint32_t code[kDequantSlabs], sz[kDequantSlabs];
+#pragma unroll
+  for (int k = 0; k < kDequantSlabs; ++k) {
+    const int64_t item = item0 + k;
+    code[k] = sz[k] = 0;  // a page that is not there: zeros
+    if (item >= p.items) continue;
+    const int64_t i = item / p.Hkv;
+    const int head = (int)(item - i * p.Hkv);
+    const int64_t page = p.page_ids ? (int64_t)__ldg(p.page_ids + i) : i;
+    if (page >= 0 && page < p.num_pages_total) {
+      const uint8_t* slab = p.k4 + ((size_t)page * p.Hkv + head) * kSlab;
+      code[k] = ldg_stream_u32(slab + tok * 64 + w * 4);
+      sz[k] = ldg_stream_u32(slab + kSlabCodes + tok * 16 + (w >> 2) * 4);
+    } else if (threadIdx.x == 0) {
+      raise_flag(p.status, TWL_FLAG_BAD_INDEX);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kDequantSlabs; ++k) {
+    if (item0 + k >= p.items) break;
+    const float2 f = Elem<__half>::to_f2(sz[k]);
     float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)((code >> (4 * j)) & 15u) * f.x + f.y;
-    r = pack8<T>(x);
-  } else if (threadIdx.x == 0) {
-    raise_flag(p.status, TWL_FLAG_BAD_INDEX);
+    for (int j = 0; j < 8; ++j) x[j] = (float)((code[k] >> (4 * j)) & 15u) * f.x + f.y;
+    reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (item0 + k) * (kPage * kD))[threadIdx.x] = pack8<T>(x);
   }
-  reinterpret_cast<uint4*>(static_cast<T*>(p.out) + item * (kPage * kD))[threadIdx.x] = r;
 }
 
 static inline bool strides_ok(const void* p, int64_t ts, int64_t hs) {
@@ -471,12 +483,13 @@ extern "C" int twl_dequantize_k_pages(const uint8_t* k4_pages, const int32_t* pa
   const int64_t items = n_pages * num_kv_heads;
   if (items > 0x7fffffffLL) return TWL_ERR_TOO_LARGE;
   DequantParams p;
-  p.k4 = k4_pages; p.page_ids = page_ids; p.out = out; p.status = status; p.Hkv = num_kv_heads;
+  p.k4 = k4_pages; p.page_ids = page_ids; p.out = out; p.status = status; p.Hkv = num_kv_heads; p.items = items;
   p.num_pages_total = num_pages_total;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const dim3 grid((unsigned)((items + kDequantSlabs - 1) / kDequantSlabs));
   if (dtype == TWL_F16)
-    TWL_CUDA_TRY(launch_chain(dequantize_k_pages_kernel<__half>, dim3((unsigned)items), dim3(256), 0, st, p));
+    TWL_CUDA_TRY(launch_chain(dequantize_k_pages_kernel<__half>, grid, dim3(256), 0, st, p));
   else
-    TWL_CUDA_TRY(launch_chain(dequantize_k_pages_kernel<__nv_bfloat16>, dim3((unsigned)items), dim3(256), 0, st, p));
+    TWL_CUDA_TRY(launch_chain(dequantize_k_pages_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p));
   return TWL_OK;
 }

@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
 // ---- merge -----------------------------------------------------------------------------------------
 // Warp = one output row (token, query head): the partial results of its segment's chunks, and of its group's prefix.
 template <typename T>
-__global__ void __launch_bounds__(256, 4) prompt_merge_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(256, 3) prompt_merge_kernel(const AttnParams p) {
   pdl_wait();
   if (p.hdr->merge == 0) return;
   const int per = p.hdr->per_warp;
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(256, 4) prompt_merge_kernel(const AttnParams p
     }
     float m = -INFINITY, l = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    // a lane takes a partial result's maximum and sum; the accumulators follow, four in flight
+    // a lane takes a partial result's maximum and sum; the accumulators follow, eight in flight
     for (int c0 = 0; c0 < n[0] + n[1]; c0 += 32) {
       const int c_mine = c0 + lane;
       int64_t mine = p.part_cap;
@@ -603,10 +603,10 @@ __global__ void __launch_bounds__(256, 4) prompt_merge_kernel(const AttnParams p
       a.w *= f0;
       m = mn;
       for (uint32_t has = __ballot_sync(0xffffffffu, v.y != 0.f); has;) {  // the others' accumulators were not written
-        float4 x[4];
-        float f[4];
+        float4 x[8];
+        float f[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 8; ++k) {
           const int c = has ? __ffs(has) - 1 : 0;
           f[k] = has ? __shfl_sync(0xffffffffu, w, c) : 0.f;
           const int64_t slot = __shfl_sync(0xffffffffu, mine, c);
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(256, 4) prompt_merge_kernel(const AttnParams p
           has &= has - 1;
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 8; ++k) {
           a.x += x[k].x * f[k];
           a.y += x[k].y * f[k];
           a.z += x[k].z * f[k];

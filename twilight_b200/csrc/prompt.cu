@@ -78,6 +78,7 @@ __device__ __forceinline__ void block_sums(long long (&v)[N], long long (*s)[4])
 __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnParams p) {
   __shared__ long long sums[kPlanThreads / 32][4];
   __shared__ long long scan[kPlanThreads / 32][3];
+  __shared__ int longest;
   pdl_wait();
   pdl_release();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n_thr = blockDim.x, n_warps = n_thr >> 5;
@@ -110,15 +111,22 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnPar
     tc = (max((v[2] + room - 1) / room, (long long)kTileChunkMin) + 7) & ~7LL;  // whole key tiles
     for (int round = 0; round < 3; ++round) {
       long long items[1] = {0};
+      int long_chunk = 0;
       for (int i = tid; i < n_seg; i += n_thr) {
         const Segment s = i == tid ? mine : load_segment(p, i);
-        if (!s.few) items[0] += (long long)tok_tiles(p, s.ntok) * p.Hkv * max(1LL, (pages_of(s) + tc - 1) / tc);
+        if (s.few) continue;
+        const int pages = pages_of(s), n = (int)max(1LL, (pages + tc - 1) / tc);
+        items[0] += (long long)tok_tiles(p, s.ntok) * p.Hkv * n;
+        long_chunk = max(long_chunk, (pages + n - 1) / n);
       }
-      block_sums<1>(items, sums);
+      if (tid == 0) longest = 0;
+      __syncthreads();
+      atomicMax(&longest, long_chunk);
+      block_sums<1>(items, sums);  // (its barriers order the maximum too)
       if (items[0] <= p.tile_target) break;
       tc = (tc * items[0] / p.tile_target + 8) & ~7LL;
     }
-    if (share * 5 < tc * 4 && share > 24 * 8) tc = 0;
+    if (share * 5 < longest * 4LL && share > 24 * 8) tc = 0;
   }
   if (tc == 0) tc = (max((share + 2) / 3, 16 * 8LL) + 7) & ~7LL;
 

@@ -549,3 +549,43 @@ def test_shared_prefix_fuzz(seed):
                                          torch.ones(gq, kk.shape[0], dtype=torch.bool, device=DEV))
                     got = out[b, h * gq: (h + 1) * gq].double()
                     assert ((got - ref).abs() <= tol_of(dtype, p, vv, ref)).all(), (sizes, prefix, i, b, h)
+
+
+@pytest.mark.parametrize("case", [
+    # more tiles than blocks, by a few
+    ([5200], [1000], 8, 8, torch.bfloat16, 0),
+    ([5000], [3000], 32, 8, torch.float16, 0),
+    ([1300, 1301], [2000, 2500], 32, 8, torch.bfloat16, 512),
+    ([2400, 9], [4000, 0], 64, 8, torch.bfloat16, 640),
+])
+def test_partly_filled_waves_of_tiles(case):
+    new, old, hq, hkv, dtype, budget = case
+    q, k, v, qo, tab, lens = make_prompt(new, old, hq, hkv, dtype, seed=17)
+    most = max((n + 15) // 16 for n in lens)
+    kw, pages_of = {}, None
+    if budget:
+        meta = ops.build_page_meta(k, *tab, max_pages=most)
+        pages, count = ops.quest_select_blocks(q, meta, qo, *tab, budget, max_pages=most, query_block=64)
+        kw = dict(block_pages=pages, block_npages=count, query_block=64)
+
+        def pages_of(b, j, h):
+            s = int(qo[b]) // 64 + b + j
+            return pages[s, h, : int(count[s, h])]
+    for causal in (True, False):
+        status = torch.zeros(1, **I32)
+        out, lse = ops.prompt_attn(q, k, v, qo, *tab, max_pages=most, causal=causal, lse=True, status=status, **kw)
+        assert int(status) == 0
+        check_prompt(q, k, v, qo, tab, lens, out, lse, causal, pages_of, 64)
+
+
+def test_many_sequences_over_one_prefix():
+    n, hq, hkv, prefix = 640, 64, 8, 3000
+    ptr, idx, last = torch.zeros(n + 1, **I32), torch.zeros(0, **I32), torch.zeros(n, **I32)
+    pptr, pidx, plast = table([prefix], 1)
+    k, v, lean, g = pool(pidx.numel(), hkv, torch.bfloat16, 2)
+    q = (torch.randn(n, hkv, hq // hkv, D, generator=g, device=DEV) + 0.3 * lean).reshape(n, hq, D).to(torch.bfloat16)
+    status = torch.zeros(1, **I32)
+    out, lse = ops.shared_prefix_attn(q, k, v, torch.tensor([0, n], **I32), pptr, pidx, plast, ptr, idx, last, lse=True,
+                                      max_pages=(prefix + 15) // 16, status=status)
+    assert int(status) == 0
+    check_prompt(q, k, v, torch.tensor([0, n], **I32), (pptr, pidx, plast), [prefix], out, lse, causal=False)

@@ -547,16 +547,22 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
 }
 
 // ---- merge -----------------------------------------------------------------------------------------
-// Warp = one output row (token, query head): the partial results of its segment's chunks, and of its group's prefix.
-template <typename T>
+// L lanes = one output row (token, query head), 128/L channels to a lane: the partial results of its segment's chunks (or of
+// the warps that read its keys), and of its group's prefix.  Bound by the latency of three loads in a row (segment, maximum
+// and sum, accumulators), so everything that can be asked for at once is.  L = 16 where there are enough rows to fill the
+// GPU's warps twice (16K rows of 3 to 4 parts: 12.5 us, with L = 32 17.7), else 32 (2K rows of 18 parts: 7.1 us, 10.8).
+template <typename T, int L>
 __global__ void __launch_bounds__(256, 3) prompt_merge_kernel(const AttnParams p) {
   pdl_wait();
   if (p.hdr->merge == 0) return;
   const int per = p.hdr->per_warp;
-  const int lane = threadIdx.x & 31;
+  constexpr int W = kD / L, kFlight = 32 / W;  // channels of a lane, accumulators in flight
+  const int lane = threadIdx.x & 31, sub = lane & (L - 1);
   const int64_t rows = (int64_t)p.num_tokens * p.Hq;
-  for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < rows; row += (int64_t)gridDim.x * 8) {
-    const int tok = (int)(row / p.Hq), head = (int)(row - (int64_t)tok * p.Hq);
+  // (all of a warp makes the same number of rounds)
+  for (int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (32 / L); row0 < rows; row0 += (int64_t)gridDim.x * (256 / L)) {
+    const int64_t row = row0 + lane / L;
+    const int tok = row < rows ? (int)(row / p.Hq) : -1, head = (int)(row - (int64_t)tok * p.Hq);
     // the row's partial results: n[0] of its sequence's segment, n[1] of its group's, `step` slots apart
     int n[2] = {0, 0};
     int64_t slot0[2] = {0, 0}, step[2] = {0, 0};
@@ -565,77 +571,94 @@ __global__ void __launch_bounds__(256, 3) prompt_merge_kernel(const AttnParams p
     for (int part = 0; part < 2; ++part) {
       const int segs = part ? p.n_second : p.n_first;
       const int32_t* qo = part ? p.qo2 : p.qo1;
-      if (segs == 0) continue;
+      if (segs == 0 || tok < 0) continue;
       int at = tok;
       if (qo) {  // last segment that starts at or before the token
         int lo = 0, hi = segs;
         while (hi - lo > 1) {
-          const int jump = (hi - lo + 31) >> 5, c = lo + lane * jump;
-          const int cnt = __popc(__ballot_sync(0xffffffffu, c < hi && qo[c] <= tok));
-          lo += (cnt > 0 ? cnt - 1 : 0) * jump;
-          hi = min(hi, lo + jump);
+          const int mid = (lo + hi) >> 1;
+          if (qo[mid] <= tok)
+            lo = mid;
+          else
+            hi = mid;
         }
         at = lo;
       }
       if (at >= segs) continue;
-      const Segment s = p.segs[(part ? p.n_first : 0) + at];
-      if (tok < s.tok0 || tok >= s.tok0 + s.ntok || s.pbase < 0) continue;
+      const Segment& s = p.segs[(part ? p.n_first : 0) + at];
+      const int tok0 = s.tok0, ntok = s.ntok;
+      const int64_t pbase = s.pbase;
+      if (tok < tok0 || tok >= tok0 + ntok || pbase < 0) continue;
       found = true;
-      slot0[part] = s.pbase + (int64_t)(tok - s.tok0) * p.Hq + head;
-      step[part] = (int64_t)s.ntok * p.Hq;
+      slot0[part] = pbase + (int64_t)(tok - tok0) * p.Hq + head;
+      step[part] = (int64_t)ntok * p.Hq;
       n[part] = s.chunks;
       if (s.few) {  // the warps whose runs touch the KV head's units
-        const long long u = s.start + (long long)(head / p.G) * s.units;
-        n[part] = s.units ? (int)((u + s.units - 1) / per - u / per) + 1 : 0;
+        const int units = s.units;
+        const long long u = s.start + (long long)(head / p.G) * units;
+        n[part] = units ? (int)((u + units - 1) / per - u / per) + 1 : 0;
       }
     }
-    float m = -INFINITY, l = 0.f;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    // a lane takes a partial result's maximum and sum; the accumulators follow, eight in flight
-    for (int c0 = 0; c0 < n[0] + n[1]; c0 += 32) {
-      const int c_mine = c0 + lane;
+    float m = -INFINITY, l = 0.f, a[W] = {};
+    const int total = n[0] + n[1], most = __reduce_max_sync(0xffffffffu, total);
+    // a lane takes a partial result's maximum and sum; the accumulators follow, several in flight
+    for (int c0 = 0; c0 < most; c0 += L) {
+      const int c_mine = c0 + sub;
       int64_t mine = p.part_cap;
       if (c_mine < n[0])
         mine = slot0[0] + c_mine * step[0];
-      else if (c_mine < n[0] + n[1])
+      else if (c_mine < total)
         mine = slot0[1] + (c_mine - n[0]) * step[1];
       float2 v = make_float2(-INFINITY, 0.f);
       if (mine < p.part_cap) v = p.part_ml[mine];
-      const float mn = fmaxf(m, warp_max(v.x)), ref = mn == -INFINITY ? 0.f : mn;
+      float mn = v.x;
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mn = fmaxf(m, mn);
+      const float ref = mn == -INFINITY ? 0.f : mn;
       const float f0 = ex2(m - ref);
       const float w = v.y == 0.f ? 0.f : ex2(v.x - ref);  // (a NaN sum goes on)
-      l = l * f0 + warp_sum(v.y * w);
-      a.x *= f0;
-      a.y *= f0;
-      a.z *= f0;
-      a.w *= f0;
+      float sum = v.y * w;
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      l = l * f0 + sum;
+#pragma unroll
+      for (int e = 0; e < W; ++e) a[e] *= f0;
       m = mn;
-      for (uint32_t has = __ballot_sync(0xffffffffu, v.y != 0.f); has;) {  // the others' accumulators were not written
-        float4 x[8];
-        float f[8];
+      for (int c = 0; c < min(L, most - c0); c += kFlight) {
+        float4 x[kFlight][W / 4];
+        float f[kFlight];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int c = has ? __ffs(has) - 1 : 0;
-          f[k] = has ? __shfl_sync(0xffffffffu, w, c) : 0.f;
-          const int64_t slot = __shfl_sync(0xffffffffu, mine, c);
-          x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (has) x[k] = *reinterpret_cast<const float4*>(p.part_acc + slot * kD + 4 * lane);
-          has &= has - 1;
+        for (int k = 0; k < kFlight; ++k) {
+          f[k] = __shfl_sync(0xffffffffu, w, c + k, L);
+          const int64_t slot = __shfl_sync(0xffffffffu, mine, c + k, L);
+#pragma unroll
+          for (int e = 0; e < W / 4; ++e) {
+            x[k][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (f[k] != 0.f)  // (no weight: its accumulator may not have been written; a NaN goes on)
+              x[k][e] = reinterpret_cast<const float4*>(p.part_acc + slot * kD + W * sub)[e];
+          }
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          a.x += x[k].x * f[k];
-          a.y += x[k].y * f[k];
-          a.z += x[k].z * f[k];
-          a.w += x[k].w * f[k];
-        }
+        for (int k = 0; k < kFlight; ++k)
+#pragma unroll
+          for (int e = 0; e < W / 4; ++e) {
+            a[4 * e] += x[k][e].x * f[k];
+            a[4 * e + 1] += x[k][e].y * f[k];
+            a[4 * e + 2] += x[k][e].z * f[k];
+            a[4 * e + 3] += x[k][e].w * f[k];
+          }
       }
     }
-    if (!found) continue;
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    T* to = static_cast<T*>(p.out) + (int64_t)tok * p.o_ts + head * kD + 4 * lane;
-    *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv));
-    if (p.lse && lane == 0) p.lse[row] = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    if (found) {
+      const float inv = l != 0.f ? 1.f / l : 0.f;
+      T* to = static_cast<T*>(p.out) + (int64_t)tok * p.o_ts + head * kD + W * sub;
+#pragma unroll
+      for (int e = 0; e < W; e += 4)
+        *reinterpret_cast<uint2*>(to + e) =
+            make_uint2(pack2<T>(a[e] * inv, a[e + 1] * inv), pack2<T>(a[e + 2] * inv, a[e + 3] * inv));
+      if (p.lse && sub == 0) p.lse[row] = l != 0.f ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
+    }
   }
 }
 
@@ -713,8 +736,14 @@ static int run_attention(const AttnParams& p, int dtype, cudaStream_t st) {
   int bad = p.row_tile == 8 ? launch_rows<T, 1>(p, st) : launch_rows<T, 2>(p, st);
   if (bad == TWL_OK && (int64_t)p.num_tokens * p.G > p.row_tile) bad = tile_attention_launch(p, dtype, st);
   if (bad != TWL_OK) return bad;
-  const int64_t blocks = ((int64_t)p.num_tokens * p.Hq + 7) / 8, most = (int64_t)num_sms() * 8;
-  TWL_CUDA_TRY(launch_chain(prompt_merge_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, p));
+  const int64_t rows = (int64_t)p.num_tokens * p.Hq, most = (int64_t)num_sms() * 8;
+  const bool halves = rows >= (int64_t)num_sms() * 48;
+  const int64_t blocks = halves ? (rows + 15) / 16 : (rows + 7) / 8;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most));
+  if (halves)
+    TWL_CUDA_TRY(launch_chain(prompt_merge_kernel<T, 16>, grid, dim3(256), 0, st, p));
+  else
+    TWL_CUDA_TRY(launch_chain(prompt_merge_kernel<T, 32>, grid, dim3(256), 0, st, p));
   return TWL_OK;
 }
 

@@ -111,16 +111,6 @@ __device__ __forceinline__ uint32_t codes8(const uint32_t (&u)[4], float* scale_
   return word;
 }
 template <typename T>
-__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 f = Elem<T>::to_f2(w[k]);
-    x[2 * k] = f.x;
-    x[2 * k + 1] = f.y;
-  }
-}
-template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   uint32_t w[4];
 #pragma unroll
@@ -133,69 +123,68 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// cos and sin for the eight channels of a lane (8 * (lane & 15) ..): channel j of a half turns with pair j, of
-// interleaved channels 2k and 2k+1 with pair k.
+// cos and sin for the eight channels of a lane (8 * (lane & 15) ..), two channels to a 64-bit register, the sines signed:
+// channel j of a half turns with pair j, of interleaved channels 2k and 2k+1 with pair k.
 template <bool INTER>
 struct Angles {
-  static constexpr int N = INTER ? 4 : 8;
-  float c[N], s[N];
+  uint64_t c[4], s[4];
   __device__ __forceinline__ void read(const float* cos_row, const float* sin_row, int ch, int rotary) {
-    const int at = INTER ? ch >> 1 : ch >= (rotary >> 1) ? ch - (rotary >> 1) : ch;
+    if (INTER) {
+      const float4 x = *reinterpret_cast<const float4*>(cos_row + (ch >> 1));
+      const float4 y = *reinterpret_cast<const float4*>(sin_row + (ch >> 1));
+      c[0] = f2(x.x, x.x); c[1] = f2(x.y, x.y); c[2] = f2(x.z, x.z); c[3] = f2(x.w, x.w);
+      s[0] = f2(-y.x, y.x); s[1] = f2(-y.y, y.y); s[2] = f2(-y.z, y.z); s[3] = f2(-y.w, y.w);
+    } else {
+      const int half = rotary >> 1, at = ch >= half ? ch - half : ch;
+      const uint32_t sign = ch >= half ? 0u : 0x80000000u;  // the low half takes minus the sine
 #pragma unroll
-    for (int k = 0; k < N; k += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(cos_row + at + k);
-      const float4 y = *reinterpret_cast<const float4*>(sin_row + at + k);
-      c[k] = x.x; c[k + 1] = x.y; c[k + 2] = x.z; c[k + 3] = x.w;
-      s[k] = y.x; s[k + 1] = y.y; s[k + 2] = y.z; s[k + 3] = y.w;
+      for (int k = 0; k < 4; k += 2) {
+        const float4 x = *reinterpret_cast<const float4*>(cos_row + at + 2 * k);
+        const uint4 y = *reinterpret_cast<const uint4*>(sin_row + at + 2 * k);
+        c[k] = f2(x.x, x.y);
+        c[k + 1] = f2(x.z, x.w);
+        s[k] = f2(__uint_as_float(y.x ^ sign), __uint_as_float(y.y ^ sign));
+        s[k + 1] = f2(__uint_as_float(y.z ^ sign), __uint_as_float(y.w ^ sign));
+      }
     }
   }
 };
 
 // Rotates the row that a half-warp holds eight channels to a lane.  Every lane takes part in the exchange of halves;
-// lanes behind `rotary` keep their channels.  Both products are rounded (not fused into the sum), so that the stored K
-// and with it the 4-bit codes do not depend on which of them a compiler would fuse.
-template <typename T, bool INTER>
+// lanes behind `rotary` keep their channels.  EXACT (K): both products are rounded, not one fused into the sum, so that the
+// stored K and with it the 4-bit codes are those of the formula's 32-bit steps.
+template <typename T, bool INTER, bool EXACT>
 __device__ __forceinline__ uint4 rotate8(const uint4& u, const Angles<INTER>& g, int ch, int rotary) {
-  float x[8];
-  unpack8<T>(u, x);
-  if (INTER) {
-    if (ch >= rotary) return u;
+  uint32_t w[4] = {u.x, u.y, u.z, u.w}, v[4] = {u.x, u.y, u.z, u.w};
+  if (!INTER) {
+    const int half = rotary >> 1, away = half >> 3;  // half is a multiple of 8
+    const int lane = threadIdx.x & 31, peer = ch >= rotary ? lane : ch < half ? lane + away : lane - away;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float a = x[2 * k], b = x[2 * k + 1];
-      x[2 * k] = __fsub_rn(__fmul_rn(a, g.c[k % Angles<INTER>::N]), __fmul_rn(b, g.s[k % Angles<INTER>::N]));
-      x[2 * k + 1] = __fadd_rn(__fmul_rn(b, g.c[k % Angles<INTER>::N]), __fmul_rn(a, g.s[k % Angles<INTER>::N]));
-    }
-    return pack8<T>(x);
+    for (int k = 0; k < 4; ++k) v[k] = __shfl_sync(0xffffffffu, w[k], peer);
   }
-  const int half = rotary >> 1, away = half >> 3;  // half is a multiple of 8
-  const bool low = ch < half;
-  const int lane = threadIdx.x & 31, peer = ch >= rotary ? lane : low ? lane + away : lane - away;
-  uint4 v;
-  v.x = __shfl_sync(0xffffffffu, u.x, peer);
-  v.y = __shfl_sync(0xffffffffu, u.y, peer);
-  v.z = __shfl_sync(0xffffffffu, u.z, peer);
-  v.w = __shfl_sync(0xffffffffu, u.w, peer);
   if (ch >= rotary) return u;
-  float y[8];
-  unpack8<T>(v, y);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float sn = low ? -g.s[k % Angles<INTER>::N] : g.s[k % Angles<INTER>::N];
-    x[k] = __fadd_rn(__fmul_rn(x[k], g.c[k % Angles<INTER>::N]), __fmul_rn(y[k], sn));
+  for (int k = 0; k < 4; ++k) {
+    const float2 x = Elem<T>::to_f2(w[k]), y = Elem<T>::to_f2(v[k]);
+    const uint64_t xs = f2(x.x, x.y), ys = INTER ? f2(y.y, y.x) : f2(y.x, y.y);
+    const uint64_t r = EXACT ? add2(mul2(xs, g.c[k]), mul2(ys, g.s[k])) : fma2(xs, g.c[k], mul2(ys, g.s[k]));
+    float a, b;
+    f2_split(r, a, b);
+    w[k] = pack_pair(a, b, T());
   }
-  return pack8<T>(x);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Block = (a page that gets new tokens, a run of KV heads with their query heads).  The block computes the sines of the
 // page's positions once; then K (a warp takes a head, half a warp a token, so that the metadata is folded in
 // registers), V (copied) and q (half a warp takes a token and walks the heads with its sines in registers; where the
-// page has fewer new tokens, several half-warps share a token).  Rows move in 16-byte pieces, four to eight of
-// them in flight per lane.
+// page has fewer new tokens, several half-warps share a token).  Rows move in 16-byte pieces, two (K, V) or four (q) of
+// them in flight per lane and 32 warps on an SM: with twice as many in flight and three quarters of the warps one token
+// for each of 256 sequences (32 KV heads) took 16.3 instead of 14.4 us, 21K tokens of prompts the same 108.
 // Pages are found without a scan: sequence b owns the block slots from qo_indptr[b]/16 + 2b on, always as many as
 // the pages its new tokens can touch; a slot beyond them has nothing to do.
 template <typename T, bool INTER>
-__global__ void __launch_bounds__(kRopeWarps * 32, 3) rope_append_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeWarps * 32, 4) rope_append_kernel(const RopeParams p) {
   __shared__ alignas(16) float cos_s[kPage][kD / 2], sin_s[kPage][kD / 2];
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -289,20 +278,20 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 3) rope_append_kernel(const R
           mx[j] = pack_pair(-INFINITY, -INFINITY, T());
         }
       }
-      for (int r0 = 0; r0 < n; r0 += 8) {
-        uint4 u[4];
+      for (int r0 = 0; r0 < n; r0 += 4) {
+        uint4 u[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
           if (r0 + 2 * i + hw < n) u[i] = load_row16(src + (r0 + 2 * i + hw) * ts, p.wide);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           const int r = r0 + 2 * i + hw;
           if (r0 + 2 * i >= n) break;  // (both halves)
           const bool mine = r < n;
           if (is_k) {
             if (p.rotary > 0) {
               ang.read(cos_s[mine ? r : 0], sin_s[mine ? r : 0], ch < p.rotary ? ch : 0, p.rotary);
-              u[i] = rotate8<T, INTER>(u[i], ang, ch, p.rotary);
+              u[i] = rotate8<T, INTER, true>(u[i], ang, ch, p.rotary);
             }
             const uint32_t y[4] = {u[i].x, u[i].y, u[i].z, u[i].w};  // as the cache holds them
             if (mine) {
@@ -348,18 +337,18 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 3) rope_append_kernel(const R
   const T* src = static_cast<const T*>(p.q) + (int64_t)(row + (mine ? tok : 0)) * p.q_ts + ch;
   T* dst = static_cast<T*>(p.q_out) + (int64_t)(row + (mine ? tok : 0)) * p.o_ts + ch;
   const int h_off = unit / width, rounds = (h_end - kv0 * G + h_step - 1) / h_step;  // rounds: the same for every lane
-  for (int i0 = 0; i0 < rounds; i0 += 8) {
-    uint4 u[8];
+  for (int i0 = 0; i0 < rounds; i0 += 4) {
+    uint4 u[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int h = kv0 * G + h_off + (i0 + i) * h_step;
       if (mine && h < h_end) u[i] = load_row16(src + h * p.q_hs, p.wide);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
       const int h = kv0 * G + h_off + (i0 + i) * h_step;
       if (i0 + i >= rounds) break;
-      if (p.rotary > 0) u[i] = rotate8<T, INTER>(u[i], ang, ch, p.rotary);
+      if (p.rotary > 0) u[i] = rotate8<T, INTER, false>(u[i], ang, ch, p.rotary);
       if (mine && h < h_end) store_row16(dst + h * p.o_hs, u[i], p.wide);
     }
   }

@@ -166,10 +166,17 @@ __device__ __forceinline__ uint4 rotate8(const uint4& u, const Angles<INTER>& g,
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const float2 x = Elem<T>::to_f2(w[k]), y = Elem<T>::to_f2(v[k]);
-    const uint64_t xs = f2(x.x, x.y), ys = INTER ? f2(y.y, y.x) : f2(y.x, y.y);
-    const uint64_t r = EXACT ? add2(mul2(xs, g.c[k]), mul2(ys, g.s[k])) : fma2(xs, g.c[k], mul2(ys, g.s[k]));
     float a, b;
-    f2_split(r, a, b);
+    if (EXACT) {  // (the two-value instructions would be fused)
+      float c0, c1, s0, s1;
+      f2_split(g.c[k], c0, c1);
+      f2_split(g.s[k], s0, s1);
+      a = __fadd_rn(__fmul_rn(x.x, c0), __fmul_rn(INTER ? y.y : y.x, s0));
+      b = __fadd_rn(__fmul_rn(x.y, c1), __fmul_rn(INTER ? y.x : y.y, s1));
+    } else {
+      const uint64_t xs = f2(x.x, x.y), ys = INTER ? f2(y.y, y.x) : f2(y.x, y.y);
+      f2_split(fma2(xs, g.c[k], mul2(ys, g.s[k])), a, b);
+    }
     w[k] = pack_pair(a, b, T());
   }
   return make_uint4(w[0], w[1], w[2], w[3]);

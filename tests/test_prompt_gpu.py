@@ -589,3 +589,35 @@ def test_many_sequences_over_one_prefix():
                                       max_pages=(prefix + 15) // 16, status=status)
     assert int(status) == 0
     check_prompt(q, k, v, torch.tensor([0, n], **I32), (pptr, pidx, plast), [prefix], out, lse, causal=False)
+
+
+@pytest.mark.parametrize("lead", [1, 64, 161])
+def test_a_part_of_a_larger_batch(lead):
+    """Offsets that begin behind row 0: the results of the part alone, and rows of no sequence are left."""
+    new, old, hq, hkv = [70, 1, 130], [300, 900, 0], 8, 2
+    q, k, v, qo, tab, lens = make_prompt(new, old, hq, hkv, torch.bfloat16, seed=11)
+    meta = torch.stack([k.amin(2), k.amax(2)], 2).contiguous()
+    most = max((n + 15) // 16 for n in lens)
+    wide = torch.nn.functional.pad(q, (0, 0, 0, 0, lead, 9), value=3.0)
+    t = q.shape[0]
+    for block in (None, 32):
+        args, wargs = {}, {}
+        if block:
+            pages, counts = ops.quest_select_blocks(q, meta, qo, *tab, 128, max_pages=most, query_block=block)
+            args = dict(block_pages=pages, block_npages=counts, query_block=block)
+            wpages, wcounts = ops.quest_select_blocks(wide, meta, qo + lead, *tab, 128, max_pages=most, query_block=block)
+            wargs = dict(block_pages=wpages, block_npages=wcounts, query_block=block)
+            for b, n in enumerate(new):
+                for j in range((n + block - 1) // block):
+                    one = int(qo[b]) // block + b + j
+                    two = (int(qo[b]) + lead) // block + b + j
+                    assert torch.equal(counts[one], wcounts[two])
+                    for h in range(hkv):
+                        c = int(counts[one, h])
+                        assert torch.equal(pages[one, h, :c], wpages[two, h, :c])
+        want = ops.prompt_attn(q, k, v, qo, *tab, max_pages=most, **args)
+        out = torch.full_like(wide, 5.0)
+        status = torch.zeros(1, **I32)
+        ops.prompt_attn(wide, k, v, qo + lead, *tab, max_pages=most, out=out, status=status, **wargs)
+        assert int(status) == 0 and torch.equal(out[lead: lead + t], want)
+        assert (out[:lead] == 5).all() and (out[lead + t:] == 5).all()

@@ -190,3 +190,21 @@ def test_runs_under_graph_capture_and_on_a_side_stream():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.equal(kp, kw) and torch.equal(vp, vw)
+
+
+@pytest.mark.parametrize("lead", [1, 16, 100, 161])
+def test_rows_before_the_first_sequence_and_behind_the_last_are_left(lead):
+    """Offsets that begin behind row 0: a part of a larger batch."""
+    new, old = [4, 40, 1], [0, 3, 700]
+    (q, k, v), kp, vp, (qo, *table), _ = make(new, old, 4, 2, torch.bfloat16, strided=False)
+    freqs, _ = ops.rope_frequencies(128, device=DEV)
+    k_want, v_want = kp.clone(), vp.clone()
+    want = ops.rope_append_kv(q, k, v, freqs, k_want, v_want, None, None, qo, *table)
+    wide = [torch.nn.functional.pad(x, (0, 0, 0, 0, lead, 7), value=3.0) for x in (q, k, v)]
+    out = torch.full_like(wide[0], 5.0)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.rope_append_kv(*wide, freqs, kp, vp, None, None, qo + lead, *table, out=out, status=status)
+    t = q.shape[0]
+    assert int(status) == 0 and torch.equal(out[lead: lead + t], want)
+    assert torch.equal(kp, k_want) and torch.equal(vp, v_want)
+    assert (out[:lead] == 5).all() and (out[lead + t:] == 5).all()

@@ -230,8 +230,10 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 4) rope_append_kernel(const R
     return;
   }
   const int start = len - n_new;  // cache position of the first new token
-  const int lp = (start >> 4) + (slot - ((row0 >> 4) + 2 * b));
-  if (lp >= n_pages) return;
+  // (before the sequence's first slot: rows before the first sequence's, which belong to none, or offsets that go back)
+  const int nth = slot - ((row0 >> 4) + 2 * b);
+  const int lp = (start >> 4) + nth;
+  if (nth < 0 || lp >= n_pages) return;
   const int t0 = max(start, lp * kPage), t1 = min(len, lp * kPage + kPage);
   const int n = t1 - t0;                // new tokens of this page, 1..16
   const int row = row0 + (t0 - start);  // row of the first of them in q, k, v

@@ -45,6 +45,29 @@ def test_rope_frequencies_of_the_known_scalings():
             ops.rope_frequencies(bad, device="cpu")
 
 
+def test_rope_frequencies_refuses_what_it_would_get_wrong():
+    yarn = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096}
+    freq = lambda sc, dim=128, base=1e4: ops.rope_frequencies(dim, base, scaling=sc, device="cpu")
+    for sc, said in (({**yarn, "mscale": 1.0}, "mscale"), ({**yarn, "mscale_all_dim": 0.7}, "mscale_all_dim"),
+                     ({"rope_type": "yarn", "factor": 4.0}, "original_max"), ({"rope_type": "linear"}, "factor"),
+                     ({"rope_type": "llama3", "factor": 8.0, "original_max_position_embeddings": 8192}, "low_freq"),
+                     ({"rope_type": "dynamic", "factor": 2.0, "alpha": 8.0}, "lacks"),
+                     ({"rope_type": "linear", "factor": 2.0, "short_factor": [1.0]}, "short_factor"),
+                     ({**yarn, "rope_theta": 5e5}, "rope_theta"), ({**yarn, "partial_rotary_factor": 0.5}, "partial")):
+        with pytest.raises(_lib.TwilightError, match=said):
+            freq(sc)
+    # what does not matter, or says what the arguments say, is taken
+    assert torch.equal(freq({**yarn, "rope_theta": 10000.0, "partial_rotary_factor": 1.0, "beta_fast": None})[0], freq(yarn)[0])
+    f, s = freq({**yarn, "attention_factor": 1.2, "mscale": 1.0, "mscale_all_dim": 1.0})
+    assert s == 1.2 and torch.equal(f, freq(yarn)[0])
+    # fractional ends of the ramp
+    f, _ = freq({**yarn, "truncate": False})
+    base = freq(None)[0]
+    ends = [128 * math.log(4096 / (t * 2 * math.pi)) / (2 * math.log(1e4)) for t in (32.0, 1.0)]
+    ramp = ((torch.arange(64, dtype=torch.float64) - ends[0]) / (ends[1] - ends[0])).clamp(0, 1)
+    assert torch.allclose(f, base * (1 - ramp) + base / 4 * ramp, rtol=1e-12) and not torch.equal(f, freq(yarn)[0])
+
+
 def _append_args(t=4, hq=4, hkv=2, dtype=torch.float16):
     q, k, v = (torch.zeros(t, h, 128, dtype=dtype) for h in (hq, hkv, hkv))
     kp, vp = (torch.zeros(3, hkv, 16, 128, dtype=dtype) for _ in range(2))

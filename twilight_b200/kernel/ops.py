@@ -516,6 +516,17 @@ def append_kv(new_k, new_v, k_pages, v_pages, k4_pages, kmeta, kv_indptr, kv_ind
 # ---------------------------------------------------------------------------------------------
 # a prompt's way into the cache
 # ---------------------------------------------------------------------------------------------
+# rope_type: what its dictionary must hold, and what it may (those without an effect on the angles among them)
+_LIMIT = "original_max_position_embeddings"
+_ROPE_ENTRIES = {
+    "default": ((), (_LIMIT,)),
+    "linear": (("factor",), (_LIMIT,)),
+    "dynamic": (("factor", _LIMIT), ()),
+    "llama3": (("factor", _LIMIT, "low_freq_factor", "high_freq_factor"), ()),
+    "yarn": (("factor", _LIMIT), ("attention_factor", "beta_fast", "beta_slow", "truncate")),
+}
+
+
 def rope_frequencies(rotary_dim: int = HEAD_DIM, base: float = 10000.0, *, scaling: Optional[dict] = None,
                      seq_len: Optional[int] = None, device="cuda") -> Tuple[torch.Tensor, float]:
     """Angles per position of the ``rotary_dim/2`` rotary pairs (float64, for :func:`rope_append_kv`) and the
@@ -523,15 +534,35 @@ def rope_frequencies(rotary_dim: int = HEAD_DIM, base: float = 10000.0, *, scali
     (``rope_scaling``), by ``rope_type``: ``"default"``; ``"linear"`` (positions divided by ``factor``);
     ``"dynamic"`` (the base grows with ``seq_len`` beyond ``original_max_position_embeddings``); ``"llama3"``
     (long wavelengths divided by ``factor``, short ones kept, a ramp between) and ``"yarn"`` (the same in terms
-    of the pair's index, with an attention factor)."""
+    of the pair's index, with an attention factor; ``truncate: False`` keeps the ends of its ramp fractional).
+    Entries that would change the angles and are not known here are refused."""
     if rotary_dim % 8 or not 8 <= rotary_dim <= HEAD_DIM:
         raise _lib.TwilightError(f"rotary_dim must be a multiple of 8 from 8 to {HEAD_DIM}")
     kind = "default" if scaling is None else scaling.get("rope_type", scaling.get("type", "default"))
+    if kind not in _ROPE_ENTRIES:
+        raise _lib.TwilightError(f"unknown rope_type {kind!r}")
+    if scaling is not None:
+        needs, takes = _ROPE_ENTRIES[kind]
+        missing = [n for n in needs if scaling.get(n) is None]
+        if missing:
+            raise _lib.TwilightError(f"scaling of rope_type {kind!r} lacks {', '.join(missing)}")
+        known = {"rope_type", "type", "factor", "rope_theta", "partial_rotary_factor", *needs, *takes}
+        other = [n for n, x in scaling.items() if n not in known and x is not None]
+        # (a factor that states the whole attention scale makes the two that it is made of superfluous)
+        if kind == "yarn" and scaling.get("attention_factor") is not None:
+            other = [n for n in other if n not in ("mscale", "mscale_all_dim")]
+        if other:
+            raise _lib.TwilightError(f"scaling of rope_type {kind!r} has entries that are not supported: {', '.join(other)}")
+        if scaling.get("rope_theta") is not None and float(scaling["rope_theta"]) != float(base):
+            raise _lib.TwilightError(f"scaling states rope_theta {scaling['rope_theta']}, base is {base}")
+        part = scaling.get("partial_rotary_factor")
+        if part is not None and int(HEAD_DIM * part) != rotary_dim:
+            raise _lib.TwilightError(f"scaling states partial_rotary_factor {part}, rotary_dim is {rotary_dim}")
     pair = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
-    factor = 1.0 if scaling is None else float(scaling.get("factor", 1.0))
+    factor = 1.0 if scaling is None or kind == "default" else float(scaling["factor"])
     attention_scale = 1.0
     if kind == "dynamic":
-        limit = scaling["original_max_position_embeddings"]
+        limit = scaling[_LIMIT]
         n = max(limit, seq_len or limit)
         base = base * (factor * n / limit - (factor - 1)) ** (rotary_dim / (rotary_dim - 2))
     freqs = base ** (-pair / rotary_dim)
@@ -539,23 +570,23 @@ def rope_frequencies(rotary_dim: int = HEAD_DIM, base: float = 10000.0, *, scali
         freqs = freqs / factor
     elif kind == "llama3":
         low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
-        turns = scaling["original_max_position_embeddings"] * freqs / (2 * math.pi)  # within the original context
+        turns = scaling[_LIMIT] * freqs / (2 * math.pi)  # within the original context
         keep = ((turns - low) / (high - low)).clamp(0, 1)
         freqs = freqs * (keep + (1 - keep) / factor)
     elif kind == "yarn":
-        limit = scaling["original_max_position_embeddings"]
+        limit = scaling[_LIMIT]
 
         def index_of(turns):  # of the pair that makes this many turns within the original context
             return rotary_dim * math.log(limit / (turns * 2 * math.pi)) / (2 * math.log(base))
-        first = max(math.floor(index_of(float(scaling.get("beta_fast", 32)))), 0)
-        last = min(math.ceil(index_of(float(scaling.get("beta_slow", 1)))), rotary_dim - 1)
+        first, last = index_of(float(scaling.get("beta_fast") or 32)), index_of(float(scaling.get("beta_slow") or 1))
+        if scaling.get("truncate", True):
+            first, last = math.floor(first), math.ceil(last)
+        first, last = max(first, 0), min(last, rotary_dim - 1)
         ramp = ((pair / 2 - first) / max(last - first, 0.001)).clamp(0, 1)
         freqs = freqs * (1 - ramp + ramp / factor)
         attention_scale = scaling.get("attention_factor")
         if attention_scale is None:
             attention_scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
-    elif kind not in ("default", "dynamic"):
-        raise _lib.TwilightError(f"unknown rope_type {kind!r}")
     return freqs.to(device), float(attention_scale)
 
 

@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(kPlanThreads) prompt_plan_kernel(const AttnPar
 //   S[row][token] = Q K^T   m16n8k16, rows the M side (rows 8-15 are zero for NT = 1), K rows the B operand
 //   O^T[channel][row] += V^T P^T: P as the B operand has the layout of the S accumulators.
 // Each piece leaves a partial result per row; a KV head that several warps share has one from each.
-// Bound by reading K and V: 5.2 to 5.4 TB/s over 340 to 370 MB (0.8 of the measured copy), most of the rest its start.
+// Bound by reading K and V: 5.4 TB/s over 342 MB of 32 KV heads in a profile, 5.1 over 375 MB of 8 (0.82 and 0.77 of
+// the measured copy).
 constexpr int kRowStages = 3;
 constexpr int kPageKV = 2 * kPage * kD * 2;  // K page, V page: 8 KiB
 template <int NT>
@@ -560,7 +561,8 @@ __global__ void __launch_bounds__(256, 3) prompt_merge_kernel(const AttnParams p
   const int lane = threadIdx.x & 31, sub = lane & (L - 1);
   const int64_t rows = (int64_t)p.num_tokens * p.Hq;
   // (all of a warp makes the same number of rounds)
-  for (int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (32 / L); row0 < rows; row0 += (int64_t)gridDim.x * (256 / L)) {
+  for (int64_t row0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (32 / L); row0 < rows;
+       row0 += (int64_t)gridDim.x * (256 / L)) {
     const int64_t row = row0 + lane / L;
     const int tok = row < rows ? (int)(row / p.Hq) : -1, head = (int)(row - (int64_t)tok * p.Hq);
     // the row's partial results: n[0] of its sequence's segment, n[1] of its group's, `step` slots apart
@@ -688,9 +690,8 @@ static WorkspaceLayout workspace_layout(int64_t tokens, int64_t n_seg, int64_t H
   const int64_t row_parts = least(few * ((max_pages + kRowRunMin - 1) / kRowRunMin + 1), few * 2 + warps * kFewRows);
   // and of the tile kernel
   const int64_t whole = tokens * Hq * ((max_pages + kTileChunkMin - 1) / kTileChunkMin);
-  const int64_t tile_parts = tokens * G <= 8 ? 0
-                             : !prefix && max_pages <= kTileChunkMin ? 0
-                                                                     : least(whole, 6 * blocks * 2 * tt * G + (prefix ? tokens * Hq : 0));
+  const bool no_parts = tokens * G <= 8 || (!prefix && max_pages <= kTileChunkMin);
+  const int64_t tile_parts = no_parts ? 0 : least(whole, 6 * blocks * 2 * tt * G + (prefix ? tokens * Hq : 0));
   w.rows = row_parts + tile_parts;
   size_t at = 0;
   w.hdr = at;
@@ -843,7 +844,8 @@ extern "C" int twl_shared_prefix_attn(const void* q, int dtype, int64_t q_token_
   p.qo2 = group_indptr; p.indptr2 = prefix_indptr; p.indices2 = prefix_indices; p.last2 = prefix_last_page_len;
   p.n_second = num_groups; p.always_partial = 1; p.query_block = 1;
   p.num_tokens = batch; p.Hq = num_q_heads; p.Hkv = num_kv_heads; p.G = num_q_heads / num_kv_heads;
-  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G; // (a batch of up to sixteen rows per KV head is one row tile, its prefixes' too)
+  p.num_pages_total = num_pages_total; p.tok_tile = 128 / p.G;
+  // (a batch of up to sixteen rows per KV head is one row tile, its prefixes' too)
   p.row_tile = p.G <= 8 && batch * p.G > kFewRows ? 8 : 16;
   p.scale_log2 = sm_scale * 1.44269504088896341f;
   p.status = status;

@@ -19,7 +19,7 @@
 //
 // Bound: two products of 128 x 128 x 128 (512 clocks each at the tensor peak) and 128 x 128 exponentials (1024 clocks of the
 // special-function units) per subtile and step; with few rows per KV head, reading K and V.  8192 queries x 8192 keys, 32/8
-// heads: 823 us, 1335 TFLOP/s (0.81 of the measured bf16 peak; causal 1220), a step of both subtiles in 3400 clocks.
+// heads: 820 us, 1340 TFLOP/s (0.82 of the measured bf16 peak; causal 1230), a step of both subtiles in 3340 clocks.
 #include <cuda.h>
 
 #include <type_traits>
@@ -29,7 +29,7 @@
 namespace twl {
 
 constexpr int kTileThreads = 384;  // three warpgroups, the unit of the register split
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // (200: 4 % slower, 192: spills, 40 % slower)
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // (200: the same, 216: 1 % slower, 224: 5 %)
 static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * 168, "registers of the launch: 168 a thread at 384 threads");
 constexpr int kKStages = 3, kVStages = 2, kStages = kKStages + kVStages;
 constexpr int kStageBytes = 128 * kD * 2;      // 128 keys (or 128 query rows)
@@ -61,7 +61,8 @@ struct Item {
 
 struct TileShared {
   uint64_t item_full[2], item_empty[2];
-  uint64_t q_full, q_free, k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages], s_full[2], p_half[2], p_full[2], o_full[2], pair[2], drain;
+  uint64_t q_full, q_free, k_full[kKStages], k_empty[kKStages], v_full[kVStages], v_empty[kVStages];
+  uint64_t s_full[2], p_half[2], p_full[2], o_full[2], pair[2], drain;
   Item items[2];
   uint32_t tmem;
   int32_t hi[kInfoSlots];      // largest position of the tile's keys, INT_MAX when a page is missing

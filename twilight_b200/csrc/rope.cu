@@ -8,8 +8,8 @@
 // its sine and cosine, once per page and pair; the rotation is 32-bit and rounded once to the model type.
 //
 // Bound: HBM.  Every row is read once and written once; the INT4 slab and the metadata of a page are made from
-// the rows while they are in registers: 21K ragged tokens of 32/8 heads in 109 us, 4.9 TB/s.  The decode form (one token per
-// sequence) is bound by the latency of a launch and of three dependent loads (the sequence's entries, its page, the rows): 6 us.
+// the rows while they are in registers: 20K ragged tokens of 32/8 heads in 109 us, 4.7 TB/s.  The decode form (one token per
+// sequence) is bound by the latency of a launch and of three dependent loads (the sequence's entries, its page, the rows): 5 us.
 #include "common.cuh"
 
 namespace twl {
@@ -187,7 +187,7 @@ __device__ __forceinline__ uint4 rotate8(const uint4& u, const Angles<INTER>& g,
 // registers), V (copied) and q (half a warp takes a token and walks the heads with its sines in registers; where the
 // page has fewer new tokens, several half-warps share a token).  Rows move in 16-byte pieces, two (K, V) or four (q) of
 // them in flight per lane and 32 warps on an SM: with twice as many in flight and three quarters of the warps one token
-// for each of 256 sequences (32 KV heads) took 16.3 instead of 14.4 us, 21K tokens of prompts the same 108.
+// for each of 256 sequences (32 KV heads) took 16.3 instead of 14.4 us, 20K tokens of prompts the same 108.
 // Pages are found without a scan: sequence b owns the block slots from qo_indptr[b]/16 + 2b on, always as many as
 // the pages its new tokens can touch; a slot beyond them has nothing to do.
 template <typename T, bool INTER>
@@ -454,7 +454,7 @@ extern "C" int twl_rope_append_kv(const void* q, const void* k, const void* v, i
   p.wide = wide(q, q_token_stride, q_head_stride) && wide(k, k_token_stride, k_head_stride) &&
            wide(v, v_token_stride, v_head_stride) && wide(q_out, out_token_stride, out_head_stride);
   // One KV head (with its query heads) a block while there are fewer blocks than four per SM (decode: latency), then more,
-  // up to eight: a block's look-up of its page and the sines are worth more rows (prompts of 21K tokens, 32/8 heads: 108 us,
+  // up to eight: a block's look-up of its page and the sines are worth more rows (prompts of 20K tokens, 32/8 heads: 108 us,
   // with three times the blocks 160 us).
   const int64_t room = (int64_t)num_sms() * 4;
   int64_t heads = (slots * num_kv_heads + room - 1) / room;

@@ -1,5 +1,7 @@
 """Host side of the prompt operators: frequencies, argument checks and status codes (no kernel is launched)."""
 import math
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -223,3 +225,18 @@ def test_attention_status_codes():
         mp=2, pooled=256, scores=256, bp=256, bn=256, mk=2), **kw}.values(), None, None)
     assert select(budget=0) == select(pooled=None) == select(hq=5) == -1
     assert select(qb=24) == select(dtype=9) == -3 and select(ts=510) == -2 and select(mp=60000) == -5
+
+
+def test_kernels_wait_before_they_read():
+    """What an earlier kernel of the stream wrote is visible after griddepcontrol.wait only: in every kernel of the prompt
+    operators that wait comes before the first read of memory."""
+    csrc = Path(_lib.__file__).resolve().parent / "csrc"
+    found = []
+    for name in ("rope.cu", "prompt.cu", "prompt_tile.cu", "select.cu"):
+        for kernel in re.finditer(r"__global__ void .*?\b(\w+_kernel)\(.*?\n}\n", (csrc / name).read_text(), re.S):
+            if name == "select.cu" and "query_blocks" not in kernel.group(1):
+                continue
+            found.append(kernel.group(1))
+            before = kernel.group(0)[: kernel.group(0).index("pdl_wait();")]
+            assert not re.search(r"\bp\.\w+(\[|->)|__ld|ldg|load_|look_up|tma_|query_block", before.split("{", 1)[1]), found[-1]
+    assert len(found) == 9, found

@@ -621,3 +621,39 @@ def test_a_part_of_a_larger_batch(lead):
         ops.prompt_attn(wide, k, v, qo + lead, *tab, max_pages=most, out=out, status=status, **wargs)
         assert int(status) == 0 and torch.equal(out[lead: lead + t], want)
         assert (out[:lead] == 5).all() and (out[lead + t:] == 5).all()
+
+
+def test_calls_one_after_another_see_what_was_written_before_each():
+    """A long chunk, a few tokens and many single ones in one call (both attention kernels have work), over and over, with
+    queries, pages, page table and lengths rewritten by kernels right before each call: the same as with the GPU waited for."""
+    new = [300, 5] + [1] * 60
+    old = [900, 40] + [37 * i % 700 for i in range(60)]
+    rounds = []
+    for i in range(6):
+        shift = [max(0, x - 16 * i) for x in old]
+        rounds.append(make_prompt(new, shift, 8, 2, torch.bfloat16, seed=30 + i))
+    pages = max(r[1].shape[0] for r in rounds)
+    entries = max(r[4][1].numel() for r in rounds)
+    q, qo = torch.empty_like(rounds[0][0]), rounds[0][3]
+    k, v = (torch.empty(pages, 2, PAGE, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    ptr, idx, last = torch.empty(63, **I32), torch.empty(entries, **I32), torch.empty(62, **I32)
+    ws = torch.empty(ops.prompt_attn_workspace_bytes(q.shape[0], 62, 8, 2, 80), dtype=torch.uint8, device=DEV)
+
+    def one(r, wait):
+        x, kk, vv, _, tab, _ = r
+        for to, of in ((q, x), (k[: kk.shape[0]], kk), (v[: vv.shape[0]], vv), (ptr, tab[0]), (idx[: tab[1].numel()], tab[1]),
+                       (last, tab[2])):
+            to.copy_(of)
+        if wait:
+            torch.cuda.synchronize()
+        out = ops.prompt_attn(q, k, v, qo, ptr, idx, last, max_pages=80, workspace=ws)
+        if wait:
+            torch.cuda.synchronize()
+        return out
+
+    want = [one(r, True) for r in rounds]
+    got = [one(r, False) for r in rounds * 4]
+    assert all(torch.equal(x, want[i % 6]) for i, x in enumerate(got))
+    x, kk, vv, qo, tab, lens = rounds[-1]
+    out, lse = ops.prompt_attn(x, kk, vv, qo, *tab, max_pages=80, lse=True)
+    check_prompt(x, kk, vv, qo, tab, lens, out, lse)

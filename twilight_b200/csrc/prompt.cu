@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
   using Shape = RowShape<NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_wait();
-  pdl_release();  // the plan is complete: the tile kernel, which needs no more than that, may move in where a block ends
+  pdl_release();  // the tile kernel sets itself up where a block ends, and waits for the others
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int per = p.hdr->per_warp;

@@ -224,23 +224,11 @@ __device__ __forceinline__ void weights(const float* x, uint64_t scale, uint64_t
   }
 }
 
-// The kernels before this one are complete when it starts, but only their results in L2 are sure to be seen without the wait
-// that comes at the end: what they wrote is read there, past this SM's first-level cache.
-__device__ __forceinline__ Segment load_l2(const Segment* from) {
-  static_assert(sizeof(Segment) % 8 == 0, "in pieces of eight bytes");
-  union {
-    Segment s;
-    long long w[sizeof(Segment) / 8];
-  } u;
-#pragma unroll
-  for (int i = 0; i < (int)(sizeof(Segment) / 8); ++i) u.w[i] = __ldcg(reinterpret_cast<const long long*>(from) + i);
-  return u.s;
-}
 __device__ __forceinline__ Item load_item(const AttnParams& p, int i) {
   Item it;
-  const int4 w = __ldcg(p.tile_list + i / p.Hkv);
+  const int4 w = p.tile_list[i / p.Hkv];
   it.kvh = i % p.Hkv;
-  const Segment s = load_l2(p.segs + w.x);
+  const Segment s = p.segs[w.x];
   it.indices = (s.second ? p.indices2 : p.indices1) + s.kvbase;
   it.tok0 = s.tok0 + w.y;
   it.ntok = w.z;
@@ -254,7 +242,7 @@ __device__ __forceinline__ Item load_item(const AttnParams& p, int i) {
   if (p.block_pages) {
     const int64_t slot = (int64_t)(s.tok0 / p.query_block + w.x + w.y / p.query_block) * p.Hkv + it.kvh;
     it.list = p.block_pages + slot * p.max_k + it.page0;
-    avail = min(max(__ldcg(p.block_npages + slot), 0), p.max_k);
+    avail = min(max(p.block_npages[slot], 0), p.max_k);
   }
   it.n_pages = 0;
 #pragma unroll
@@ -271,7 +259,7 @@ __device__ __forceinline__ Item load_item(const AttnParams& p, int i) {
   it.n_tiles = max(it.steps[0], it.steps[1]);
   it.tail_page = -1;
   if (it.n_pages > 0 && (s.len & (kPage - 1)) != 0 &&
-      (it.list ? __ldcg(it.list + it.n_pages - 1) : it.page0 + it.n_pages - 1) == s.npages - 1)
+      (it.list ? it.list[it.n_pages - 1] : it.page0 + it.n_pages - 1) == s.npages - 1)
     it.tail_page = (it.n_pages - 1) & 7;
   it.pair = it.ntok <= p.tok_tile && it.n_tiles > 1;
   if (it.pair) {
@@ -321,9 +309,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  // No wait for the kernel before: that is the row kernel, which lets this one start once the plan is complete.  The two
-  // overlap; this one waits at its end, so that what follows it follows both.  (Reads past the first-level cache instead:
-  // see load_l2; 8K x 8K takes the same 820 us, causal 446 instead of 444.)
+  // Everything from here on reads what earlier kernels wrote (the plan, page tables, lists; Q, K and V by TMA), and only this wait
+  // makes that visible.  The kernel before is the row kernel, whose release lets the lines above run beside its last blocks.
+  pdl_wait();
   bool ok = true;
   uint32_t n_item = 0;  // items so far: slot n_item & 1 of the two
   // The next item, copied out of its slot; false at the end (or when a wait ran out: ok is false then).
@@ -341,7 +329,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
 
   if (warp == 10) {
     // ---- work items ----
-    const int n_items = __ldcg(&p.hdr->tile_items) * p.Hkv;
+    const int n_items = p.hdr->tile_items * p.Hkv;
     for (int i = blockIdx.x;; ++n_item) {
       Item it;
       if (i < n_items)
@@ -393,8 +381,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
         lp = -1;
         phys = -1;
         if (lane < 8 && at < it.n_pages) {
-          lp = it.list ? __ldcg(it.list + at) : it.page0 + at;
-          if (lp >= 0 && lp < it.npages) phys = __ldcg(it.indices + lp);
+          lp = it.list ? it.list[at] : it.page0 + at;
+          if (lp >= 0 && lp < it.npages) phys = it.indices[lp];
           if (phys < 0 || phys >= p.num_pages_total) {
             phys = -1;
             if (is_k) raise_flag(p.status, TWL_FLAG_BAD_INDEX);
@@ -746,7 +734,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
     }
   }
   if (!ok && lane == 0) raise_flag(p.status, TWL_FLAG_WAIT_LIMIT);
-  pdl_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == 9) {

@@ -657,3 +657,35 @@ def test_calls_one_after_another_see_what_was_written_before_each():
     x, kk, vv, qo, tab, lens = rounds[-1]
     out, lse = ops.prompt_attn(x, kk, vv, qo, *tab, max_pages=80, lse=True)
     check_prompt(x, kk, vv, qo, tab, lens, out, lse)
+
+
+def block_sums64(q, meta, qo, tab, lens, block, b, j, hkv):
+    """Scores of the pages before block j of sequence b in 64 bits, [pages, hkv], and the sums of their parts' sizes."""
+    a, e = int(qo[b]), int(qo[b + 1])
+    rows = q[a + j * block: min(e, a + (j + 1) * block)].double().unflatten(1, (hkv, -1))
+    n = (lens[b] - (e - a) + j * block) // PAGE
+    ids = tab[1][int(tab[0][b]): int(tab[0][b + 1])].long()[:n]
+    low, high = rows.clamp(max=0).sum((0, 2)), rows.clamp(min=0).sum((0, 2))
+    lo, hi = low * meta[ids, :, 0].double(), high * meta[ids, :, 1].double()
+    return (lo + hi).sum(-1), (lo.abs() + hi.abs()).sum(-1), rows.shape[0] * rows.shape[2]
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e-2, 1e-4, 1e-5])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_block_scores_are_32_bit_sums_whatever_the_queries_size(dtype, scale):
+    new, old, hq, hkv, block = [128, 90], [1000, 2500], 8, 2, 32
+    q, k, v, qo, tab, lens = make_prompt(new, old, hq, hkv, dtype, seed=40)
+    q = (q.float() * scale).to(dtype)
+    most = max((n + 15) // 16 for n in lens)
+    meta = ops.build_page_meta(k, *tab, max_pages=most)
+    slots = sum(new) // block + len(new)
+    scores = torch.zeros(slots, hkv, most, device=DEV)
+    ops.quest_select_blocks(q, meta, qo, *tab, 256, max_pages=most, query_block=block, page_scores=scores)
+    for b in range(len(new)):
+        for j in range((new[b] + block - 1) // block):
+            want, size, rows = block_sums64(q, meta, qo, tab, lens, block, b, j, hkv)
+            got = scores[int(qo[b]) // block + b + j, :, : want.shape[0]].T.double()
+            # In steps of 2^-24 of the sum of the parts' sizes: the pooled sums in 16 runs (rows/16 + 15 roundings, of numbers of
+            # one sign), their parts (4: 22 bits), tensor-core sums of 16 products and what they are added to (17 numbers cut off
+            # below 2 steps each, twice for every 32 numbers), sums of those (8)
+            assert ((got - want).abs() <= (rows / 16 + 15 + 4 + 68 + 8) * 2.0 ** -24 * size).all()

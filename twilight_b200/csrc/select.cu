@@ -772,54 +772,59 @@ __global__ void __launch_bounds__(256) pool_query_blocks_kernel(const BlockSelPa
 
 // block = 256 pages x 16 slots of one KV head on tensor cores: 16 pages at a time are a warp's A rows, taken from memory in
 // 16-byte pieces straight into the fragments as in quest_page_scores_mma_kernel, eight slots the columns.  The pooled
-// vectors are split into three bf16 (two fp16) numbers, each the rounded rest of the one before: 24 (22) bits, so the
-// products and their fp32 sums are as good as 32-bit ones.  They are scaled by a power of two near 1 / rows first,
-// which keeps fp16 in range.
+// vectors are split into three bf16 (two fp16) numbers, each the rounded rest of the one before: 24 (22) bits.  A vector is first
+// scaled by the power of two that takes its largest number to kTop: in fp16 the rests then stay normal numbers, whatever the size of
+// the queries.  The tensor cores cut off the bits of a sum that its largest number has no room for: in one run over
+// all 256 numbers that came to 2^-19.2 of the sum of the parts' sizes in fp16 (2^-21.2 in bf16); with the products of every 32 numbers
+// summed from zero, and those eight sums added in 32 bits, it is 2^-21.8 in both, in the same time.
 constexpr int kBlkPages = 256, kBlkSlots = 16, kBlkPitch = 288;  // elements of a row of pooled numbers: 32 more than it holds, for the banks
 template <typename T>
 struct BlkTerms {
-  static constexpr int kN = 2;
+  static constexpr int kN = 2, kTop = 14;  // largest number: 2^14 .. 2^15
 };
 template <>
 struct BlkTerms<__nv_bfloat16> {
-  static constexpr int kN = 3;
+  static constexpr int kN = 3, kTop = 0;
 };
 template <typename T>
 __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelParams p) {
-  constexpr int N = BlkTerms<T>::kN;
+  constexpr int N = BlkTerms<T>::kN, kTop = BlkTerms<T>::kTop;
   __shared__ alignas(16) T pooled[N][kBlkSlots][kBlkPitch];
   __shared__ int hist_s[kBlkSlots], seq_s[kBlkSlots];
   __shared__ float unscale_s[kBlkSlots];
   pdl_wait();
   const int slot0 = blockIdx.z * kBlkSlots, kvh = blockIdx.y, block_page = blockIdx.x * kBlkPages;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  __shared__ int rows_s[kBlkSlots];
   if (warp == 0) {
     const QueryBlock qb = query_blocks_from(p, slot0);
     if (lane < kBlkSlots) {
       const bool there = slot0 + lane < p.slots;
       hist_s[lane] = there ? history_pages(qb) : 0;
       seq_s[lane] = there ? qb.b : -1;
-      rows_s[lane] = qb.rows;
     }
   }
   __syncthreads();
   for (int i = warp; i < kBlkSlots; i += 8) {
-    const int hist = hist_s[i];
-    const int rows = max(1, rows_s[i] * (p.Hq / p.Hkv)), shift = 32 - __clz(rows);
-    if (lane == 0) unscale_s[i] = (float)(1u << shift);
-    if (hist > block_page) {
-      const float scale = 1.f / (float)(1u << shift);
-      const float* src = p.pooled + ((size_t)(slot0 + i) * p.Hkv + kvh) * 256;
+    if (hist_s[i] <= block_page) continue;
+    const float* src = p.pooled + ((size_t)(slot0 + i) * p.Hkv + kvh) * 256;
+    float x[8], top = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        float x = src[32 * k + lane] * scale;
+    for (int k = 0; k < 8; ++k) {
+      x[k] = src[32 * k + lane];
+      top = fmaxf(top, fabsf(x[k]));
+    }
+    // (both powers of two are normal numbers)
+    const uint32_t e = min(max(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23, (uint32_t)kTop + 1), 253u);
+    const float scale = __uint_as_float((254 + kTop - e) << 23);
+    if (lane == 0) unscale_s[i] = __uint_as_float((e - kTop) << 23);
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          const T y = Elem<T>::from_f(x);
-          pooled[n][i][32 * k + lane] = y;
-          x -= Elem<T>::to_f(y);
-        }
+    for (int k = 0; k < 8; ++k) {
+      x[k] *= scale;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const T y = Elem<T>::from_f(x[k]);
+        pooled[n][i][32 * k + lane] = y;
+        x[k] -= Elem<T>::to_f(y);
       }
     }
   }
@@ -850,13 +855,17 @@ __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelP
           if (n8 + 8 <= i0 || n8 >= i1) continue;
           float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int n = N - 1; n >= 0; --n)  // the small terms first
+          for (int c = 0; c < 8; ++c) {  // a piece's products from zero, its sum to the others' as a rounded 32-bit sum
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
+            for (int n = N - 1; n >= 0; --n) {  // the small terms first
               const uint4 w = *reinterpret_cast<const uint4*>(&pooled[n][n8 + g][32 * c + 8 * t]);
-              MmaTile<T>::run(acc, v[0][c].x, v[1][c].x, v[0][c].y, v[1][c].y, w.x, w.y);
-              MmaTile<T>::run(acc, v[0][c].z, v[1][c].z, v[0][c].w, v[1][c].w, w.z, w.w);
+              MmaTile<T>::run(part, v[0][c].x, v[1][c].x, v[0][c].y, v[1][c].y, w.x, w.y);
+              MmaTile<T>::run(part, v[0][c].z, v[1][c].z, v[0][c].w, v[1][c].w, w.z, w.w);
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += part[e];
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int s = n8 + 2 * t + (e & 1), page = page0 + g + 8 * (e >> 1);

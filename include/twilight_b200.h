@@ -393,9 +393,9 @@ TWL_API int twl_dequantize_k_pages(const uint8_t* k4_pages, const int32_t* page_
  * holds its first position on, and of the pages before that the max(1,budget/16)+(budget%16!=0) with the
  * largest sums over the block's rows (tokens x query heads of the KV head) of Quest's bound
  * sum_d max(q_d*kmax_d, q_d*kmin_d) (twilight/pyimpl/quest.py:37-99 applied to a block), ties to the
- * lower page, in fp32.  pooled: fp32 [slots][H_kv][256] and page_scores: fp32
- * [slots][H_kv][max_pages], caller scratch (kept as outputs for inspection: sums of min(q,0) and
- * max(q,0); scores of the pages before the block).
+ * lower page.  The choice is that of 64-bit sums (of finite q and kmeta).  pooled: fp32
+ * [slots][H_kv][256] and page_scores: fp32 [slots][H_kv][max_pages], caller scratch (kept as outputs for
+ * inspection: sums of min(q,0) and max(q,0); scores of the pages before the block, in 32 bits).
  *
  * twl_shared_prefix_attn: decode attention (one token per sequence) of groups of sequences that share a
  * prefix.  Group i is the sequences group_indptr[i]..group_indptr[i+1] of the batch; its prefix is a page

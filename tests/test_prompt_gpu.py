@@ -689,3 +689,87 @@ def test_block_scores_are_32_bit_sums_whatever_the_queries_size(dtype, scale):
             # one sign), their parts (4: 22 bits), tensor-core sums of 16 products and what they are added to (17 numbers cut off
             # below 2 steps each, twice for every 32 numbers), sums of those (8)
             assert ((got - want).abs() <= (rows / 16 + 15 + 4 + 68 + 8) * 2.0 ** -24 * size).all()
+
+
+def exact_lists(q, meta, qo, tab, lens, budget, block, hkv, got, count):
+    """Compares block lists with the 64-bit choice, ties to the lower page; the number of lists that had a choice."""
+    k = max(1, budget // PAGE) + (budget % PAGE != 0)
+    lists = 0
+    for b, total in enumerate(lens):
+        m = int(qo[b + 1]) - int(qo[b])
+        for j in range((m + block - 1) // block):
+            want = block_sums64(q, meta, qo, tab, lens, block, b, j, hkv)[0]
+            n, slot = want.shape[0], int(qo[b]) // block + b + j
+            best = want.sort(dim=0, stable=True, descending=True).indices[:k].sort(dim=0).values
+            assert torch.equal(got[slot, :, : min(k, n)].long().T, best), (b, j)
+            own = torch.arange(n, (total - m + min(m, (j + 1) * block) - 1) // PAGE + 1, device=DEV)
+            assert (count[slot] == best.shape[0] + own.shape[0]).all()
+            assert (got[slot, :, best.shape[0]: best.shape[0] + own.shape[0]] == own).all()
+            lists += hkv * (n > k)
+    return lists
+
+
+@pytest.mark.parametrize("case", [
+    # new, old, hq, hkv, budget, block, scale
+    ([1500, 700], [4000, 9000], 8, 8, 1024, 128, 1.0),
+    ([1500, 700], [4000, 9000], 16, 4, 4096, 64, 1.0),
+    ([700, 300], [4000, 2000], 8, 8, 1024, 64, 1e-3),
+    ([700, 300], [4000, 2000], 8, 8, 1024, 64, 1e-4),
+    ([40], [20000], 48, 1, 100, 16, 1e-2),
+], ids=[str(i) for i in range(5)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_chosen_pages_are_those_of_the_64_bit_sums(dtype, case):
+    new, old, hq, hkv, budget, block, scale = case
+    for seed in range(3):
+        q, k, v, qo, tab, lens = make_prompt(new, old, hq, hkv, dtype, seed=50 + seed)
+        q = (q.float() * scale).to(dtype)
+        most = max((n + 15) // 16 for n in lens)
+        meta = ops.build_page_meta(k, *tab, max_pages=most)
+        status = torch.zeros(1, **I32)
+        pages, count = ops.quest_select_blocks(q, meta, qo, *tab, budget, max_pages=most, query_block=block, status=status)
+        assert int(status) == 0
+        assert exact_lists(q, meta, qo, tab, lens, budget, block, hkv, pages, count) > 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("spread", ["one step in a few channels", "none", "no queries", "one page apart"])
+def test_chosen_pages_among_near_and_equal_scores(dtype, spread):
+    """Every page has (nearly) the same metadata: the cut lies among scores that 32 bits do not tell apart, or among equal ones,
+    where the lower page goes first."""
+    new, old, hq, hkv, budget, block = [70, 33], [3000, 5000], 4, 2, 700, 32
+    q, k, v, qo, tab, lens = make_prompt(new, old, hq, hkv, dtype, seed=60)
+    g = torch.Generator(device=DEV).manual_seed(61)
+    most = max((n + 15) // 16 for n in lens)
+    pages = k.shape[0]
+    base = torch.randn(1, hkv, 2, D, generator=g, device=DEV).abs()
+    base[:, :, 0] *= -1
+    meta = base.to(dtype).repeat(pages, 1, 1, 1).contiguous()
+    if spread == "one step in a few channels":
+        bits = meta.view(torch.int16)
+        some = torch.rand(meta.shape, generator=g, device=DEV) < 0.05
+        bits += some * torch.randint(-1, 2, meta.shape, generator=g, device=DEV, dtype=torch.int16)
+    if spread == "one page apart":
+        meta[int(tab[1][77])] *= 2.0
+    if spread == "no queries":
+        q = torch.zeros_like(q)
+    got = ops.quest_select_blocks(q, meta, qo, *tab, budget, max_pages=most, query_block=block)
+    assert exact_lists(q, meta, qo, tab, lens, budget, block, hkv, *got) > 0
+
+
+def test_sparse_prompts_against_the_definition():
+    """Selection and attention together, by the definition's own choice of pages."""
+    for new, old, hq, hkv, dtype, budget, block in (([500, 300], [2000, 100], 4, 4, torch.float16, 512, 128),
+                                                    ([260], [4000], 8, 2, torch.bfloat16, 1024, 64)):
+        q, k, v, qo, tab, lens = make_prompt(new, old, hq, hkv, dtype, seed=70)
+        most = max((n + 15) // 16 for n in lens)
+        meta = ops.build_page_meta(k, *tab, max_pages=most)
+        sel = ops.quest_select_blocks(q, meta, qo, *tab, budget, max_pages=most, query_block=block)
+        out, lse = ops.prompt_attn(q, k, v, qo, *tab, max_pages=most, block_pages=sel[0], block_npages=sel[1],
+                                   query_block=block, lse=True)
+
+        def pages_of(b, j, h):
+            want = block_sums64(q, meta, qo, tab, lens, block, b, j, hkv)[0][:, h]
+            best = want.sort(stable=True, descending=True).indices[: max(1, budget // PAGE) + (budget % PAGE != 0)]
+            return torch.cat([best, torch.arange(want.shape[0], most, device=DEV)])
+
+        check_prompt(q, k, v, qo, tab, lens, out, lse, True, pages_of, block)

@@ -426,22 +426,16 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 constexpr int kTopkThreads = 256;
 static_assert(kTopkThreads == kSelThreads, "the fused tail runs the selection with the scoring block");
 
-// Keeps the k best of src[0..n) (k < n) and writes their positions, ascending, to out[0..k).
-// Called by a whole block of kTopkThreads threads; keys: n words of shared memory.  Scores are
-// read through L2 because other blocks may have written them.
-__device__ void topk_row(const float* src, int n, int k, int32_t* out, uint32_t* keys, TopkScratch& sc) {
+// The k-th largest of keys[0..n) (k < n) and how many keys equal to it are among the k largest.  Called by a whole block of
+// kTopkThreads threads; kmin, kmax: the smallest and the largest of the keys that this thread has seen (or written: the keys
+// are read after a barrier), all of them between the threads.
+__device__ __forceinline__ void topk_threshold(const uint32_t* keys, int n, int k, uint32_t kmin, uint32_t kmax, TopkScratch& sc,
+                                               uint32_t& thr, int& take_eq) {
   int (&hist)[256] = sc.hist;
   int (&wsum)[33] = sc.wsum;
   uint32_t& sh_prefix = sc.prefix;
   int& sh_krem = sc.krem;
-  // keys, and the smallest and the largest of them: the leading bits they share need no pass
-  uint32_t kmin = 0xFFFFFFFFu, kmax = 0u;
-  for (int i = threadIdx.x; i < n; i += kTopkThreads) {
-    const uint32_t key = order_key(__ldcg(src + i));
-    keys[i] = key;
-    kmin = min(kmin, key);
-    kmax = max(kmax, key);
-  }
+  // the leading bits that the smallest and the largest key share need no pass
   kmin = __reduce_min_sync(0xffffffffu, kmin);
   kmax = __reduce_max_sync(0xffffffffu, kmax);
   if ((threadIdx.x & 31) == 0) {
@@ -508,8 +502,13 @@ __device__ void topk_row(const float* src, int n, int k, int32_t* out, uint32_t*
     top = shift;
     __syncthreads();
   }
-  const uint32_t thr = sh_prefix;  // k-th largest key
-  const int take_eq = sh_krem;     // how many keys equal to it are kept (lowest pages first)
+  thr = sh_prefix;
+  take_eq = sh_krem;
+}
+
+// Positions of the keys above thr and of the first take_eq equal to it, ascending, to out.
+__device__ __forceinline__ void topk_compact(const uint32_t* keys, int n, uint32_t thr, int take_eq, int32_t* out, TopkScratch& sc) {
+  int (&wsum)[33] = sc.wsum;
   // ordered compaction, 4 consecutive pages per thread per tile
   int base_gt = 0, base_eq = 0;
   for (int t0 = 0; t0 < n; t0 += kTopkThreads * 4) {
@@ -540,6 +539,22 @@ __device__ void topk_row(const float* src, int n, int k, int32_t* out, uint32_t*
     base_gt += total & 0xFFFF;
     base_eq += total >> 16;
   }
+}
+
+// Keeps the k best of src[0..n) (k < n) and writes their positions, ascending, to out[0..k), the lowest of equal ones first.
+// Called by a whole block of kTopkThreads threads; keys: n words of shared memory.  Scores are
+// read through L2 because other blocks may have written them.
+__device__ void topk_row(const float* src, int n, int k, int32_t* out, uint32_t* keys, TopkScratch& sc) {
+  uint32_t kmin = 0xFFFFFFFFu, kmax = 0u, thr;
+  int take_eq;
+  for (int i = threadIdx.x; i < n; i += kTopkThreads) {
+    const uint32_t key = order_key(__ldcg(src + i));
+    keys[i] = key;
+    kmin = min(kmin, key);
+    kmax = max(kmax, key);
+  }
+  topk_threshold(keys, n, k, kmin, kmax, sc, thr, take_eq);
+  topk_compact(keys, n, thr, take_eq, out, sc);
 }
 
 struct TopkParams {
@@ -656,8 +671,8 @@ static int launch_scores_g(const ScoreParams& p, cudaStream_t st) {
 // A block of query tokens (all their G heads of a KV head: rows r) picks its pages by the sum of Quest's bounds over
 // its rows, which is linear in the metadata,
 //   sum_r sum_d max(q_rd kmax_d, q_rd kmin_d) = sum_d (sum_r min(q_rd, 0)) kmin_d + (sum_r max(q_rd, 0)) kmax_d,
-// so a block is pooled once into 256 numbers and a page costs it 256 multiply-adds whatever its rows.  All of it
-// in 32 bits (or as good).  Three launches: pool, scores, selection.
+// so a block is pooled once into 256 numbers and a page costs it 256 multiply-adds whatever its rows.  Sums and scores
+// in 32 bits (or as good); scores too near the cut for that are decided in 64.  Three launches: pool, scores, selection.
 // Slots: query block j of sequence b is slot qo_indptr[b]/query_block + b + j.
 struct BlockSelParams {
   const void *q, *kmeta;
@@ -726,7 +741,7 @@ __device__ __forceinline__ int history_pages(const QueryBlock& r) {
 
 // block = (slot, KV head): 16 lanes of 8 channels x 16 rows at a time
 template <typename T>
-__global__ void __launch_bounds__(256) pool_query_blocks_kernel(const BlockSelParams p) {
+__global__ void __launch_bounds__(256, 4) pool_query_blocks_kernel(const BlockSelParams p) {
   __shared__ float part[16][2][kD];
   pdl_wait();
   const int slot = blockIdx.x, kvh = blockIdx.y, G = p.Hq / p.Hkv;
@@ -746,15 +761,18 @@ __global__ void __launch_bounds__(256) pool_query_blocks_kernel(const BlockSelPa
                                                     (kvh * G + r - tok * G) * kD) + c);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    for (int k = 0; k < 4; ++k) {  // the eight as a tree: three roundings instead of eight
+      float l[8][2], h[8][2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = Elem<T>::to_f2(u[k]);
-        lo[2 * k] += fminf(f.x, 0.f);
-        hi[2 * k] += fmaxf(f.x, 0.f);
-        lo[2 * k + 1] += fminf(f.y, 0.f);
-        hi[2 * k + 1] += fmaxf(f.y, 0.f);
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = Elem<T>::to_f2(k == 0 ? v[i].x : k == 1 ? v[i].y : k == 2 ? v[i].z : v[i].w);
+        l[i][0] = fminf(f.x, 0.f); l[i][1] = fminf(f.y, 0.f);
+        h[i][0] = fmaxf(f.x, 0.f); h[i][1] = fmaxf(f.y, 0.f);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        lo[2 * k + e] += ((l[0][e] + l[1][e]) + (l[2][e] + l[3][e])) + ((l[4][e] + l[5][e]) + (l[6][e] + l[7][e]));
+        hi[2 * k + e] += ((h[0][e] + h[1][e]) + (h[2][e] + h[3][e])) + ((h[4][e] + h[5][e]) + (h[6][e] + h[7][e]));
       }
     }
   }
@@ -764,10 +782,16 @@ __global__ void __launch_bounds__(256) pool_query_blocks_kernel(const BlockSelPa
     part[r0][1][8 * c + k] = hi[k];
   }
   __syncthreads();
-  float s = 0.f;
+  float s[16];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) s += (&part[r][0][0])[threadIdx.x];
-  p.pooled[((size_t)slot * p.Hkv + kvh) * 256 + threadIdx.x] = s;
+  for (int r = 0; r < 16; ++r) s[r] = (&part[r][0][0])[threadIdx.x];
+#pragma unroll
+  for (int w = 8; w > 0; w >>= 1)
+#pragma unroll
+    for (int r = 0; r < w; ++r) s[r] += s[r + w];
+  const size_t row = (size_t)slot * p.Hkv + kvh;
+  p.pooled[row * 256 + threadIdx.x] = s[0];
+  if (threadIdx.x == 0) p.block_pages[row * p.max_k] = 0;  // (see score_query_blocks_kernel)
 }
 
 // block = 256 pages x 16 slots of one KV head on tensor cores: 16 pages at a time are a warp's A rows, taken from memory in
@@ -777,6 +801,8 @@ __global__ void __launch_bounds__(256) pool_query_blocks_kernel(const BlockSelPa
 // the queries.  The tensor cores cut off the bits of a sum that its largest number has no room for: in one run over
 // all 256 numbers that came to 2^-19.2 of the sum of the parts' sizes in fp16 (2^-21.2 in bf16); with the products of every 32 numbers
 // summed from zero, and those eight sums added in 32 bits, it is 2^-21.8 in both, in the same time.
+// The bits of the largest |metadata| of the pages (of a 16-bit type: ordered as integers) go to the first entry of a row's list,
+// which is free until the selection writes it: the selection bounds the scores' errors by it.
 constexpr int kBlkPages = 256, kBlkSlots = 16, kBlkPitch = 288;  // elements of a row of pooled numbers: 32 more than it holds, for the banks
 template <typename T>
 struct BlkTerms {
@@ -829,6 +855,7 @@ __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelP
     }
   }
   __syncthreads();
+  uint32_t largest = 0;  // of lane's slot
   for (int page0 = block_page + warp * 16; page0 < block_page + kBlkPages; page0 += 128) {
     for (int i0 = 0; i0 < kBlkSlots;) {  // the slots of one sequence at a time
       const int b = seq_s[i0];
@@ -839,6 +866,7 @@ __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelP
         const int here = min(16, n_pages - page0);
         int phys[2];
         uint4 v[2][8];
+        uint32_t top = 0;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           phys[h] = g + 8 * h < here ? idx[g + 8 * h] : 0;
@@ -850,6 +878,16 @@ __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelP
 #pragma unroll
           for (int c = 0; c < 8; ++c) v[h][c] = ldg_stream_u4(src + 32 * c);
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (g + 8 * h >= here || phys[h] < 0) continue;
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[h][c].x & 0x7fff7fffu, v[h][c].y & 0x7fff7fffu),
+                                         __vmaxu2(v[h][c].z & 0x7fff7fffu, v[h][c].w & 0x7fff7fffu)));
+        }
+        top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
+        if (lane >= i0 && lane < i1) largest = max(largest, top);
 #pragma unroll
         for (int n8 = 0; n8 < kBlkSlots; n8 += 8) {
           if (n8 + 8 <= i0 || n8 >= i1) continue;
@@ -878,15 +916,101 @@ __global__ void __launch_bounds__(256) score_query_blocks_kernel(const BlockSelP
       i0 = i1;
     }
   }
+  if (lane < kBlkSlots && hist_s[lane] > block_page && largest > 0)
+    atomicMax(p.block_pages + ((size_t)(slot0 + lane) * p.Hkv + kvh) * p.max_k, (int)largest);
 }
 
 constexpr int kBlkKeys = 200 * 1024;  // shared memory for the keys of a row: 51200 pages
-// block = (slot, KV head): the budget's best of the pages before the block, then the pages it lies in
-__global__ void __launch_bounds__(kTopkThreads) select_query_blocks_kernel(const BlockSelParams p) {
+constexpr int kBlkPools = 8 * 2 * kD * (int)sizeof(double);
+constexpr int kBlkOpen = 128;  // open pages that are ranked one against the other
+
+// The block's pooled queries in 64 bits: part[0..256) (part: 8 x 256, one run of the rows a warp).
+template <typename T>
+__device__ __forceinline__ void pool_query_block64(const BlockSelParams& p, const QueryBlock& qb, int kvh, double* part) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.Hq / p.Hkv, rows = qb.rows * G;
+  double lo[4] = {}, hi[4] = {};
+  int tok = warp / G, g = warp - tok * G;
+  const int d_tok = 8 / G, d_g = 8 - d_tok * G;
+  const T* const q0 = static_cast<const T*>(p.q) + (int64_t)qb.row0 * p.q_ts + kvh * G * kD + 4 * lane;
+  for (int r0 = warp; r0 < rows; r0 += 64) {
+    uint2 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = make_uint2(0, 0);
+      if (r0 + 8 * i < rows) v[i] = __ldg(reinterpret_cast<const uint2*>(q0 + (int64_t)tok * p.q_ts + g * kD));
+      tok += d_tok;
+      g += d_g;
+      if (g >= G) {
+        g -= G;
+        ++tok;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 a = Elem<T>::to_f2(v[i].x), b = Elem<T>::to_f2(v[i].y);
+      const float f[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const double d = f[k];
+        if (f[k] < 0.f) lo[k] += d;
+        if (f[k] > 0.f) hi[k] += d;
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    part[warp * 256 + 4 * lane + k] = lo[k];
+    part[warp * 256 + kD + 4 * lane + k] = hi[k];
+  }
+  __syncthreads();
+  double s = 0.;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) s += part[w * 256 + threadIdx.x];
+  part[threadIdx.x] = s;  // (its own column: nobody else reads it before the barrier)
+  __syncthreads();
+}
+
+// sum_d of a page's metadata times w[0..256), in 64 bits, by a warp (every lane gets it).
+template <typename T>
+__device__ __forceinline__ double score_page64(const BlockSelParams& p, int phys, int kvh, const double* w) {
+  const int lane = threadIdx.x & 31;
+  const uint2* meta = reinterpret_cast<const uint2*>(static_cast<const T*>(p.kmeta) + ((size_t)phys * p.Hkv + kvh) * 2 * kD) + lane;
+  double s = 0.;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint2 v = __ldg(meta + h * 32);
+    const float2 a = Elem<T>::to_f2(v.x), b = Elem<T>::to_f2(v.y);
+    const double* x = w + h * kD + 4 * lane;
+    s += (double)a.x * x[0] + (double)a.y * x[1] + (double)b.x * x[2] + (double)b.y * x[3];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+
+// block = (slot, KV head): the budget's best of the pages before the block, then the pages it lies in.
+// Best by 64-bit sums.  The 32-bit scores are off by at most e, so with c the k-th best of them a page above c + 2e is kept, and one
+// below c - 2e is not.  What is between is open; where that is more than the places left, those pages are scored anew:
+//   up to kBlkOpen of them (most often two or three) with 64-bit products of the 32-bit pooled queries, and where two of these still are
+//   too near one another at the cut, of the queries pooled in 64 bits; ranked by comparing each with each;
+//   more of them (many nearly or wholly equal pages) with those, selected as the 32-bit scores are, by s - c rounded to 32 bits and
+//   then, where that ties at the cut, by what the rounding took.
+// Pages whose 64-bit sums are equal: the lower first.
+// Errors in steps of 2^-24 of |pooled|_1 max|metadata|, each counted at its worst: pooled queries (rows/128 + 7 roundings of
+// numbers of one sign), their split (4), tensor-core sums (17 numbers cut off below two steps each, twice for every 32 products: 68)
+// and the sum of those (8).  Measured, the scores are off by two steps at most.
+// 21 us for 512 rows of 1.9K pages and 256 query rows each (without the open pages 12, without those pooled again 13), 14 us for 752
+// rows of up to 500 pages and 128 query rows.
+template <typename T>
+__global__ void __launch_bounds__(kTopkThreads, 5) select_query_blocks_kernel(const BlockSelParams p) {
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ TopkScratch sc;
+  __shared__ double open_score[kBlkOpen], edge[2];
+  __shared__ int open_page[kBlkOpen];
+  __shared__ float sizes[kTopkThreads / 32];
+  __shared__ int n_sure, n_open;
   pdl_wait();
-  const int slot = blockIdx.x, kvh = blockIdx.y;
+  const int slot = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const QueryBlock qb = query_block_of(p, slot);
   if (qb.rows == 0) return;
   const size_t row = (size_t)slot * p.Hkv + kvh;
@@ -895,7 +1019,100 @@ __global__ void __launch_bounds__(kTopkThreads) select_query_blocks_kernel(const
   if (k == n) {
     for (int i = threadIdx.x; i < n; i += kTopkThreads) out[i] = i;
   } else if (k > 0) {
-    topk_row(p.scores + row * p.max_pages, n, k, out, keys, sc);
+    const float* src = p.scores + row * p.max_pages;
+    const uint16_t largest = (uint16_t)__ldcg(out);
+    const float pooled = p.pooled[row * 256 + threadIdx.x], size = warp_sum(fabsf(pooled));
+    uint32_t kmin = 0xFFFFFFFFu, kmax = 0u, thr;
+    int take_eq;
+    for (int i = threadIdx.x; i < n; i += kTopkThreads) {
+      const uint32_t key = order_key(__ldcg(src + i));
+      keys[i] = key;
+      kmin = min(kmin, key);
+      kmax = max(kmax, key);
+    }
+    if (lane == 0) sizes[warp] = size;
+    if (threadIdx.x == 0) n_sure = n_open = 0;
+    topk_threshold(keys, n, k, kmin, kmax, sc, thr, take_eq);
+    float step = 0.f;
+#pragma unroll
+    for (int w = 0; w < kTopkThreads / 32; ++w) step += sizes[w];
+    step *= Elem<T>::to_f(*reinterpret_cast<const T*>(&largest)) * 0x1p-24f;
+    // (one more for the roundings of this product)
+    const float pool_err = step * (float)((qb.rows * (p.Hq / p.Hkv) + 127) / 128 + 7 + 1), err = pool_err + step * (4 + 68 + 8);
+    const float cut = __uint_as_float(thr & 0x80000000u ? thr ^ 0x80000000u : ~thr);
+    // (an infinity or NaN among them, or nearly: the 32-bit scores decide, and no page that is not there is open)
+    if (fabsf(cut) + 2.f * err < 1e38f) {
+      const uint32_t k_lo = order_key(__fadd_rd(cut, -2.f * err)), k_hi = order_key(__fadd_ru(cut, 2.f * err));
+      int sure = 0;
+      for (int i = threadIdx.x; i < n; i += kTopkThreads) {
+        const uint32_t key = keys[i];
+        sure += key > k_hi;
+        if (key >= k_lo && key <= k_hi) {
+          const int at = atomicAdd(&n_open, 1);
+          if (at < kBlkOpen) open_page[at] = i;
+        }
+      }
+      sure = __reduce_add_sync(0xffffffffu, sure);
+      if (lane == 0 && sure > 0) atomicAdd(&n_sure, sure);
+      double* const part = reinterpret_cast<double*>(reinterpret_cast<uint8_t*>(keys) + ((size_t)p.max_pages * 4 + 15) / 16 * 16);
+      part[threadIdx.x] = pooled;
+      __syncthreads();
+      const int open = n_open, need = k - n_sure;
+      const int32_t* idx = p.indices + p.indptr[qb.b];
+      if (open == need) {
+        thr = k_lo - 1;  // all from k_lo on (a finite number's key is not the smallest)
+        take_eq = 0;
+      } else if (open <= kBlkOpen) {
+        for (int exact = 0;; ++exact) {
+          for (int j = warp; j < open; j += kTopkThreads / 32) {
+            const double s = score_page64<T>(p, idx[open_page[j]], kvh, part);
+            if (lane == 0) open_score[j] = s;
+          }
+          __syncthreads();
+          if (threadIdx.x < open) {
+            const double s = open_score[threadIdx.x];
+            const int page = open_page[threadIdx.x];
+            int rank = 0;
+            for (int j = 0; j < open; ++j) rank += open_score[j] > s || (open_score[j] == s && open_page[j] < page);
+            keys[page] = rank < need ? 0xFFFFFFFFu : 0u;
+            if (rank == need - 1) edge[0] = s;  // the last that is kept, the first that is not
+            if (rank == need) edge[1] = s;
+          }
+          __syncthreads();
+          if (exact || edge[0] - edge[1] > 2. * pool_err) break;
+          pool_query_block64<T>(p, qb, kvh, part);
+        }
+        thr = k_hi;  // those kept are above it now
+        take_eq = 0;
+      } else {
+        pool_query_block64<T>(p, qb, kvh, part);
+        uint32_t lo = k_lo, hi = k_hi;
+        for (int level = 0; level < 2; ++level) {
+          kmin = 0xFFFFFFFFu;
+          kmax = 0u;
+          for (int i0 = warp * 32; i0 < n; i0 += kTopkThreads) {  // a warp's own 32 keys
+            const int i = i0 + lane;
+            uint32_t key = i < n ? keys[i] : 0u;
+            const bool mine = i < n && key >= lo && key <= hi;
+            key = mine ? key : key > hi ? 0xFFFFFFFFu : 0u;
+            for (uint32_t left = __ballot_sync(0xffffffffu, mine); left; left &= left - 1) {
+              const int at = __ffs(left) - 1;
+              const double d = score_page64<T>(p, idx[i0 + at], kvh, part) - (double)cut;
+              const float f = level == 0 ? (float)d : (float)(d - (double)(float)d);
+              if (lane == at) key = order_key(f);  // (finite: between the keys of the others)
+            }
+            if (i < n) {
+              keys[i] = key;
+              kmin = min(kmin, key);
+              kmax = max(kmax, key);
+            }
+          }
+          topk_threshold(keys, n, k, kmin, kmax, sc, thr, take_eq);
+          lo = hi = thr;
+        }
+      }
+    }
+    topk_compact(keys, n, thr, take_eq, out, sc);
   }
   // its own pages, up to the one of its last position
   const int own = qb.last < 0 ? 0 : max(0, min(min(qb.last / kPage + 1, qb.pages) - n, p.max_k - k));
@@ -1017,8 +1234,9 @@ extern "C" int twl_quest_select_blocks(const void* q, int dtype, int64_t q_token
     TWL_CUDA_TRY(launch_chain(pool_query_blocks_kernel<__nv_bfloat16>, per_slot, dim3(256), 0, st, p));
     TWL_CUDA_TRY(launch_chain(score_query_blocks_kernel<__nv_bfloat16>, tiles, dim3(256), 0, st, p));
   }
-  static int8_t done[kSmemDevices];
-  TWL_CUDA_TRY(allow_smem(select_query_blocks_kernel, kBlkKeys, done));
-  TWL_CUDA_TRY(launch_chain(select_query_blocks_kernel, per_slot, dim3(kTopkThreads), smem, st, p));
+  static int8_t done[2][kSmemDevices];
+  auto* select = dtype == TWL_F16 ? select_query_blocks_kernel<__half> : select_query_blocks_kernel<__nv_bfloat16>;
+  TWL_CUDA_TRY(allow_smem(select, kBlkKeys + kBlkPools, done[dtype == TWL_F16]));
+  TWL_CUDA_TRY(launch_chain(select, per_slot, dim3(kTopkThreads), (smem + 15) / 16 * 16 + kBlkPools, st, p));
   return TWL_OK;
 }

@@ -796,7 +796,8 @@ def quest_select_blocks(q, kmeta, qo_indptr, kv_indptr, kv_indices, kv_last_page
                         page_scores=None, status=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Pages that every block of ``query_block`` queries (a multiple of 16) of a prompt attends to, for
     :func:`prompt_attn`: all from the page of its first position on, and of those before it the token budget's best
-    by the sum of Quest's bounds over the block's rows (twilight/pyimpl/quest.py:37-99 applied to a block).
+    by the sum of Quest's bounds over the block's rows (twilight/pyimpl/quest.py:37-99 applied to a block), as 64-bit
+    sums would choose them, ties to the lower page.
 
     Returns ``(block_pages [slots,Hkv,max_k] int32 ascending, block_npages [slots,Hkv] int32)`` with
     ``slots = T//query_block + batch``; block j of sequence b is row ``qo_indptr[b]//query_block + b + j``."""

@@ -240,3 +240,49 @@ def test_kernels_wait_before_they_read():
             before = kernel.group(0)[: kernel.group(0).index("pdl_wait();")]
             assert not re.search(r"\bp\.\w+(\[|->)|__ld|ldg|load_|look_up|tma_|query_block", before.split("{", 1)[1]), found[-1]
     assert len(found) == 9, found
+
+
+def planned_partials(own, sizes, prefix, hq, hkv):
+    """Partial rows that the plan kernel hands out for shared_prefix_attn (csrc/prompt.cu) on a GPU of 148 SMs: lengths in pages."""
+    g, sms, n = hq // hkv, 148, len(own)
+    row_tile = 8 if g <= 8 and n * g > 16 else 16
+    segs = [(1, x) for x in own] + list(zip(sizes, prefix))
+    few = [s for s in segs if s[0] * g <= row_tile]
+    tile = [(-(-t // (2 * (128 // g))) * hkv, t, pages) for t, pages in segs if t * g > row_tile]
+    per = max(4, -(-sum(hkv * p for t, p in few if t) // (sms * (8 if row_tile == 8 else 7))))
+    rows = sum(t * hq * (-(-p // per) + 1) for t, p in few)
+    tiles, work = sum(x[0] for x in tile), sum(x[0] * x[2] for x in tile)
+    share, tc = -(-work // sms), 0
+    if tiles < sms:
+        tc = (max(-(-work // (sms - tiles // 2)), 32) + 7) & ~7
+        for _ in range(3):
+            cut = [max(1, -(-p // tc)) for _, _, p in tile]
+            items = sum(x[0] * c for x, c in zip(tile, cut))
+            longest = max([0] + [-(-x[2] // c) for x, c in zip(tile, cut)])
+            if items <= sms:
+                break
+            tc = (tc * items // sms + 8) & ~7
+        if share * 5 < longest * 4 and share > 24 * 8:
+            tc = 0
+    if tc == 0:
+        tc = (max((share + 2) // 3, 128) + 7) & ~7
+    return rows + sum(max(1, -(-p // tc)) * t * hq for _, t, p in tile)
+
+
+@pytest.mark.parametrize("heads", [(1, 1), (8, 1), (32, 8), (9, 1), (16, 1), (17, 1), (32, 1), (33, 1), (48, 1), (96, 2), (64, 1), (128, 1)])
+def test_workspace_of_a_shared_prefix_holds_its_partial_results(heads):
+    lib, (hq, hkv) = _lib.load(), heads
+    shapes = [([4] * n, [n], [4]) for n in (1, 2, 3, 20, 64)] + [([32] * 1000, [1000], [32]), ([1] * 2000, [700, 1300], [32, 1])]
+    r = torch.Generator().manual_seed(hq)
+    for _ in range(60):
+        sizes = [int(torch.randint(0, 70, (1,), generator=r)) for _ in range(int(torch.randint(1, 5, (1,), generator=r)))]
+        top = (1, 4, 32, 40, 300, 3000)[int(torch.randint(6, (1,), generator=r))]
+        if sum(sizes):
+            shapes.append((torch.randint(0, top + 1, (sum(sizes),), generator=r).tolist(), sizes,
+                           torch.randint(0, top + 1, (len(sizes),), generator=r).tolist()))
+    for own, sizes, prefix in shapes:
+        most = max(1, max(own + prefix))
+        size = lib.twl_shared_prefix_workspace_bytes(len(own), len(sizes), hq, hkv, most)
+        # a partial row is 520 bytes; a segment 56, an item of the tile list (888 and more of them) 16, the header 256
+        room = (size - 256 - 56 * (len(own) + len(sizes)) - 16 * 888) // 520
+        assert planned_partials(own, sizes, prefix, hq, hkv) <= room, (len(own), sizes, most)

@@ -773,3 +773,25 @@ def test_sparse_prompts_against_the_definition():
             return torch.cat([best, torch.arange(want.shape[0], most, device=DEV)])
 
         check_prompt(q, k, v, qo, tab, lens, out, lse, True, pages_of, block)
+
+
+@pytest.mark.parametrize("heads", [(33, 1), (48, 1), (128, 2), (128, 1)])
+@pytest.mark.parametrize("batch", [1, 2, 3, 260])
+def test_shared_prefix_of_many_query_heads(heads, batch):
+    """A sequence's own part alone is more rows than the row kernel takes: both parts leave partial results of the tile kernel."""
+    hq, hkv = heads
+    own, prefix = [(1 + 13 * i) % 64 for i in range(batch)], [60]
+    total = sum((x + 15) // 16 for x in own + prefix)
+    ptr, idx, last = table(own, 4, 0, total)
+    pptr, pidx, plast = table(prefix, 4, idx.numel(), total)
+    k, v, lean, g = pool(total, hkv, torch.bfloat16, 80)
+    q = (torch.randn(batch, hkv, hq // hkv, D, generator=g, device=DEV) + 0.3 * lean).reshape(batch, hq, D).to(torch.bfloat16)
+    status = torch.zeros(1, **I32)
+    out = ops.shared_prefix_attn(q, k, v, torch.tensor([0, batch], **I32), pptr, pidx, plast, ptr, idx, last, max_pages=4, status=status)
+    assert int(status) == 0
+    gq = hq // hkv
+    for b in list(range(batch))[:: max(1, batch // 20)]:
+        for h in range(hkv):
+            kk, vv = (torch.cat([dense(x, pptr, pidx, 0, 60, h), dense(x, ptr, idx, b, own[b], h)]) for x in (k, v))
+            ref, _, p = attend64(q[b, h * gq: (h + 1) * gq].double(), kk, vv, torch.ones(gq, kk.shape[0], dtype=torch.bool, device=DEV))
+            assert ((out[b, h * gq: (h + 1) * gq].double() - ref).abs() <= tol_of(torch.bfloat16, p, vv, ref)).all(), (b, h)

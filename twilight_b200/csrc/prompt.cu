@@ -688,10 +688,11 @@ static WorkspaceLayout workspace_layout(int64_t tokens, int64_t n_seg, int64_t H
   // which are the warps and one or two more for each
   const int64_t few = least(tokens * Hq * (prefix ? 2 : 1), n_seg * kFewRows * Hkv);
   const int64_t row_parts = least(few * ((max_pages + kRowRunMin - 1) / kRowRunMin + 1), few * 2 + warps * kFewRows);
-  // and of the tile kernel
-  const int64_t whole = tokens * Hq * ((max_pages + kTileChunkMin - 1) / kTileChunkMin);
+  // and of the tile kernel: a row has those of one segment, or of two where a sequence's own token is more than few rows too
+  const int64_t once = tokens * Hq * (prefix && G > kFewRows ? 2 : 1);
+  const int64_t whole = once * ((max_pages + kTileChunkMin - 1) / kTileChunkMin);
   const bool no_parts = tokens * G <= 8 || (!prefix && max_pages <= kTileChunkMin);
-  const int64_t tile_parts = no_parts ? 0 : least(whole, 6 * blocks * 2 * tt * G + (prefix ? tokens * Hq : 0));
+  const int64_t tile_parts = no_parts ? 0 : least(whole, 6 * blocks * 2 * tt * G + (prefix ? once : 0));
   w.rows = row_parts + tile_parts;
   size_t at = 0;
   w.hdr = at;

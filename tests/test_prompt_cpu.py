@@ -286,3 +286,13 @@ def test_workspace_of_a_shared_prefix_holds_its_partial_results(heads):
         # a partial row is 520 bytes; a segment 56, an item of the tile list (888 and more of them) 16, the header 256
         room = (size - 256 - 56 * (len(own) + len(sizes)) - 16 * 888) // 520
         assert planned_partials(own, sizes, prefix, hq, hkv) <= room, (len(own), sizes, most)
+
+
+def test_rows_that_may_be_rotated_in_place_are_not_read_as_read_only():
+    """rope_append_kv's out may be q itself; ld.global.nc is undefined for memory that the kernel writes."""
+    text = (Path(_lib.__file__).resolve().parent / "csrc" / "rope.cu").read_text()
+    kernel = text[text.index("rope_append_kernel("): text.index("struct DequantParams")]
+    queries = kernel[kernel.index("static_cast<const T*>(p.q)"):]
+    assert "p.q)" not in kernel[: -len(queries)] and not re.search(r"load_row16|ldg", queries)
+    load_q = text[text.index("load_q16("): text.index("store_row16(")]
+    assert "ld.global" in load_q and ".nc" not in load_q and "ldg" not in load_q

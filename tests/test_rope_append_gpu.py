@@ -208,3 +208,20 @@ def test_rows_before_the_first_sequence_and_behind_the_last_are_left(lead):
     assert int(status) == 0 and torch.equal(out[lead: lead + t], want)
     assert torch.equal(kp, k_want) and torch.equal(vp, v_want)
     assert (out[:lead] == 5).all() and (out[lead + t:] == 5).all()
+
+
+@pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
+@pytest.mark.parametrize("pad", [0, 4])
+def test_in_place(case, pad):
+    """out as q itself: rows of a fused projection; with `pad` more elements a head they start anywhere in a 32-byte sector."""
+    new, old, hq, hkv, rotary, inter, dtype = case
+    (q, k, v), kp, vp, table, lens = make(new, old, hq, hkv, dtype)
+    freqs, scale = ops.rope_frequencies(rotary, device=DEV) if rotary else (None, 1.0)
+    kw = dict(interleaved=inter, attention_scale=scale)
+    want = ops.rope_append_kv(q, k, v, freqs, kp.clone(), vp.clone(), None, None, *table, **kw)
+    wide = torch.zeros(q.shape[0], hq + 1, D + pad, dtype=dtype, device=DEV)
+    mine = wide[:, :hq, :D]
+    mine.copy_(q)
+    got = ops.rope_append_kv(mine, k, v, freqs, kp, vp, None, None, *table, out=mine, **kw)
+    assert got.data_ptr() == mine.data_ptr() and torch.equal(got, want)
+    assert not wide[:, hq].any() and not wide[..., D:].any()

@@ -37,6 +37,18 @@ __device__ __forceinline__ uint4 load_row16(const T* p, int wide) {
   const uint2 a = ldg_stream_u2(p), b = ldg_stream_u2(p + 4);
   return make_uint4(a.x, a.y, b.x, b.y);
 }
+// The same of q, which may be written in place: the read-only loads above are undefined for memory that the kernel writes.
+template <typename T>
+__device__ __forceinline__ uint4 load_q16(const T* p, int wide) {
+  uint4 r;
+  if (wide)
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p) : "memory");
+  else
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%4];\n\tld.global.L1::no_allocate.v2.u32 {%2,%3}, [%4+8];"
+                 : "=&r"(r.x), "=&r"(r.y), "=&r"(r.z), "=&r"(r.w) : "l"(p) : "memory");
+  return r;
+}
 template <typename T>
 __device__ __forceinline__ void store_row16(T* p, const uint4& v, int wide) {
   if (wide) {
@@ -351,7 +363,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 4) rope_append_kernel(const R
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int h = kv0 * G + h_off + (i0 + i) * h_step;
-      if (mine && h < h_end) u[i] = load_row16(src + h * p.q_hs, p.wide);
+      if (mine && h < h_end) u[i] = load_q16(src + h * p.q_hs, p.wide);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -396,6 +396,9 @@ TWL_API int twl_dequantize_k_pages(const uint8_t* k4_pages, const int32_t* page_
  * lower page.  The choice is that of 64-bit sums (of finite q and kmeta).  pooled: fp32
  * [slots][H_kv][256] and page_scores: fp32 [slots][H_kv][max_pages], caller scratch (kept as outputs for
  * inspection: sums of min(q,0) and max(q,0); scores of the pages before the block, in 32 bits).
+ * block_npages of a slot that no block has is 0, as are those of a sequence whose offsets or last page
+ * length make no sense (flagged, TWL_FLAG_BAD_INDEX).  max_pages: the largest page count of a sequence;
+ * pages behind it are left out and flagged.
  *
  * twl_shared_prefix_attn: decode attention (one token per sequence) of groups of sequences that share a
  * prefix.  Group i is the sequences group_indptr[i]..group_indptr[i+1] of the batch; its prefix is a page

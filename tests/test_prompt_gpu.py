@@ -795,3 +795,50 @@ def test_shared_prefix_of_many_query_heads(heads, batch):
             kk, vv = (torch.cat([dense(x, pptr, pidx, 0, 60, h), dense(x, ptr, idx, b, own[b], h)]) for x in (k, v))
             ref, _, p = attend64(q[b, h * gq: (h + 1) * gq].double(), kk, vv, torch.ones(gq, kk.shape[0], dtype=torch.bool, device=DEV))
             assert ((out[b, h * gq: (h + 1) * gq].double() - ref).abs() <= tol_of(torch.bfloat16, p, vv, ref)).all(), (b, h)
+
+
+def test_selection_flags_what_it_leaves_out_and_counts_every_slot():
+    new, old, hq, hkv, block = [70, 0, 5, 130], [300, 900, 40, 1000], 8, 2, 32
+    q, k, v, qo, tab, lens = make_prompt(new, old, hq, hkv, torch.bfloat16, seed=90)
+    most = max((n + 15) // 16 for n in lens)
+    meta = torch.stack([k.amin(2), k.amax(2)], 2).contiguous()
+    slots = sum(new) // block + len(new)
+
+    def call(qo=qo, tab=tab, max_pages=most, rows=None):
+        status, count = torch.zeros(1, **I32), torch.full((slots, hkv), 99, **I32)
+        pages = ops.quest_select_blocks(q, meta, qo, *tab, 128, max_pages=max_pages, query_block=block, block_npages=count,
+                                        status=status)[0]
+        return pages, count, int(status)
+
+    def slots_of(b):
+        first = int(qo[b]) // block + b
+        return range(first, first + (new[b] + block - 1) // block)
+
+    used = sorted(s for b in range(4) for s in slots_of(b))
+    none = [s for s in range(slots) if s not in used]
+    pages, count, status = call()
+    assert status == 0 and none and (count[none] == 0).all() and (count[used] > 0).all() and (count <= pages.shape[2]).all()
+    # a sequence that makes no sense: flagged, without lists; the others as before
+    for b, last in ((0, 0), (3, 17)):
+        wrong = tab[2].clone()
+        wrong[b] = last
+        got_pages, got, status = call(tab=(tab[0], tab[1], wrong))
+        assert status == ops.FLAG_BAD_INDEX and (got[list(slots_of(b))] == 0).all()
+        for s in used:
+            if s not in slots_of(b):
+                assert torch.equal(got[s], count[s])
+                for h in range(hkv):
+                    assert torch.equal(got_pages[s, h, : count[s, h]], pages[s, h, : count[s, h]])
+    far = qo.clone()
+    far[4] += 1                                                 # more rows than q has
+    _, got, status = call(qo=far)
+    assert status == ops.FLAG_BAD_INDEX and (got[list(slots_of(3))] == 0).all()
+    # fewer pages than a sequence has: what is left out is flagged, and the lists stay in range
+    got_pages, got, status = call(max_pages=most - 1)
+    assert status == ops.FLAG_BAD_INDEX and (got <= got_pages.shape[2]).all()
+    for s in used:
+        for h in range(hkv):
+            x = got_pages[s, h, : got[s, h]]
+            assert (x[1:] > x[:-1]).all() and ((x >= 0) & (x < most - 1)).all()
+    # a sequence without new tokens has no lists to leave anything out of
+    assert call(max_pages=most)[2] == 0 and (lens[1] + 15) // 16 < most

@@ -684,6 +684,7 @@ struct BlockSelParams {
 };
 struct QueryBlock {
   int b, row0, rows, first, last, pages;  // sequence, first query row, tokens, positions of the first and last, its pages
+  int bad;  // the sequence's entries make no sense, or it has new tokens and more pages than max_pages
 };
 
 // The query blocks of consecutive slots, found by the warp together: lane i gets that of slot + i (i < 16; more than
@@ -701,7 +702,7 @@ __device__ __forceinline__ QueryBlock query_blocks_from(const BlockSelParams& p,
   const int b = min(lo + lane, p.batch - 1);
   const int t0 = p.qo_indptr[b], n_new = p.qo_indptr[b + 1] - t0;
   const int n_pages = p.indptr[b + 1] - p.indptr[b], ll = p.last_len[b];
-  const bool bad = t0 < 0 || t0 + n_new > p.num_tokens || (n_pages > 0 && (ll < 1 || ll > kPage));
+  const bool bad = t0 < 0 || n_new < 0 || t0 + n_new > p.num_tokens || n_pages < 0 || (n_pages > 0 && (ll < 1 || ll > kPage));
   const int len = n_pages > 0 && !bad ? (n_pages - 1) * kPage + ll : 0;
   const int first_slot = lo + lane < p.batch ? t0 / p.query_block + b : 0x7fffffff;
   int mine = 0;  // of the sequences looked at, which has this lane's slot
@@ -721,6 +722,7 @@ __device__ __forceinline__ QueryBlock query_blocks_from(const BlockSelParams& p,
   r.first = s_len - s_new + at;
   r.last = r.first + r.rows - 1;
   r.pages = min(max(s_pages, 0), p.max_pages);
+  r.bad = s_bad || (s_new > 0 && s_pages > p.max_pages);
   return r;
 }
 // The query block of one slot, for every lane of the warp.
@@ -732,6 +734,7 @@ __device__ __forceinline__ QueryBlock query_block_of(const BlockSelParams& p, in
   r.first = __shfl_sync(0xffffffffu, r.first, 0);
   r.last = __shfl_sync(0xffffffffu, r.last, 0);
   r.pages = __shfl_sync(0xffffffffu, r.pages, 0);
+  r.bad = __shfl_sync(0xffffffffu, r.bad, 0);
   return r;
 }
 // pages wholly before the block's first position: the ones it chooses from
@@ -1012,8 +1015,12 @@ __global__ void __launch_bounds__(kTopkThreads, 5) select_query_blocks_kernel(co
   pdl_wait();
   const int slot = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const QueryBlock qb = query_block_of(p, slot);
-  if (qb.rows == 0) return;
   const size_t row = (size_t)slot * p.Hkv + kvh;
+  if (qb.bad && threadIdx.x == 0) raise_flag(p.status, TWL_FLAG_BAD_INDEX);
+  if (qb.rows == 0) {  // no block has this slot
+    if (threadIdx.x == 0) p.block_npages[row] = 0;
+    return;
+  }
   int32_t* out = p.block_pages + row * p.max_k;
   const int n = history_pages(qb), k = min(min(n, p.budget_k), p.max_k);
   if (k == n) {

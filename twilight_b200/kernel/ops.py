@@ -800,7 +800,9 @@ def quest_select_blocks(q, kmeta, qo_indptr, kv_indptr, kv_indices, kv_last_page
     sums would choose them, ties to the lower page.
 
     Returns ``(block_pages [slots,Hkv,max_k] int32 ascending, block_npages [slots,Hkv] int32)`` with
-    ``slots = T//query_block + batch``; block j of sequence b is row ``qo_indptr[b]//query_block + b + j``."""
+    ``slots = T//query_block + batch``; block j of sequence b is row ``qo_indptr[b]//query_block + b + j``, rows without a
+    block have a count of 0.  ``max_pages``: the largest page count of a sequence (pages behind it are left out, and
+    flagged in ``status``, as sequences are whose entries make no sense)."""
     _queries(q)
     t, hq = q.shape[0], q.shape[1]
     batch = qo_indptr.numel() - 1

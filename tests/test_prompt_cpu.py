@@ -296,3 +296,36 @@ def test_rows_that_may_be_rotated_in_place_are_not_read_as_read_only():
     assert "p.q)" not in kernel[: -len(queries)] and not re.search(r"load_row16|ldg", queries)
     load_q = text[text.index("load_q16("): text.index("store_row16(")]
     assert "ld.global" in load_q and ".nc" not in load_q and "ldg" not in load_q
+
+
+def test_workspace_sizes_are_those_of_the_device_of_the_call(monkeypatch):
+    """A process with GPUs of different SM counts: a size asked for one is not given for the other."""
+    sms, current = {0: 100, 1: 148}, [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index, self.before = index, current[0]
+
+        def __enter__(self):
+            current[0] = self.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Library:
+        twl_prompt_attn_workspace_bytes = staticmethod(lambda *a: sms[current[0]] * a[0])
+        twl_shared_prefix_workspace_bytes = staticmethod(lambda *a: sms[current[0]] * a[0])
+
+    monkeypatch.setattr(_lib, "load", lambda: Library)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    for size, args in ((ops.prompt_attn_workspace_bytes, (999983, 1, 8, 2, 4)),
+                       (ops.shared_prefix_workspace_bytes, (999983, 1, 8, 2, 4))):
+        for _ in range(2):
+            for current[0] in (0, 1):
+                assert size(*args) == sms[current[0]] * 999983
+        current[0] = 0
+        assert size(*args, device="cuda:1") == 148 * 999983 and size(*args, device="cuda:0") == 100 * 999983
+        assert size(*args, device="cuda") == 100 * 999983 and current[0] == 0
+    ops._workspace_bytes.cache_clear()

@@ -739,11 +739,29 @@ def _workspace(t: Optional[torch.Tensor], nbytes: int, device) -> torch.Tensor:
 
 
 @functools.lru_cache(maxsize=1024)
+def _workspace_bytes(name: str, index: int, *sizes: int) -> int:
+    """(The sizes follow the GPU's SM count: asked with the device current that the call runs on.)"""
+    fn = getattr(_lib.load(), f"twl_{name}_workspace_bytes")
+    if index < 0:
+        return int(fn(*sizes))
+    with torch.cuda.device(index):
+        return int(fn(*sizes))
+
+
+def _device_index(device) -> int:
+    """The device's index, the current one's for None; -1 where there is none."""
+    index = None if device is None else torch.device(device).index
+    if index is None:
+        index = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    return index
+
+
 def prompt_attn_workspace_bytes(num_tokens: int, batch: int, num_q_heads: int, num_kv_heads: int, max_pages: int,
-                                query_block: int = 0) -> int:
-    """Bytes of :func:`prompt_attn`'s workspace; ``query_block`` is 0 without block lists."""
-    return int(_lib.load().twl_prompt_attn_workspace_bytes(num_tokens, batch, num_q_heads, num_kv_heads, max_pages,
-                                                           query_block))
+                                query_block: int = 0, *, device=None) -> int:
+    """Bytes of :func:`prompt_attn`'s workspace on ``device`` (None: the current one); ``query_block`` is 0 without block
+    lists."""
+    return _workspace_bytes("prompt_attn", _device_index(device), num_tokens, batch, num_q_heads, num_kv_heads, max_pages,
+                            query_block)
 
 
 def prompt_attn(q, k_pages, v_pages, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, *, max_pages: int,
@@ -778,8 +796,9 @@ def prompt_attn(q, k_pages, v_pages, qo_indptr, kv_indptr, kv_indices, kv_last_p
         query_block = 0
     _cuda(q)
     if t > 0:
-        workspace = _workspace(workspace, prompt_attn_workspace_bytes(t, batch, hq, hkv, max_pages, query_block), q.device)
         index = q.get_device()
+        workspace = _workspace(workspace, _workspace_bytes("prompt_attn", index, t, batch, hq, hkv, max_pages, query_block),
+                               q.device)
         _launch_small("prompt_attn", index,
                       ("k_pages", k_pages, "v_pages", v_pages, "qo_indptr", qo_indptr, "kv_indptr", kv_indptr,
                        "kv_indices", kv_indices, "kv_last_page_len", kv_last_page_len, "block_pages", block_pages,
@@ -852,9 +871,10 @@ def quest_select_blocks(q, kmeta, qo_indptr, kv_indptr, kv_indices, kv_last_page
     return block_pages, block_npages
 
 
-@functools.lru_cache(maxsize=1024)
-def shared_prefix_workspace_bytes(batch: int, num_groups: int, num_q_heads: int, num_kv_heads: int, max_pages: int) -> int:
-    return int(_lib.load().twl_shared_prefix_workspace_bytes(batch, num_groups, num_q_heads, num_kv_heads, max_pages))
+def shared_prefix_workspace_bytes(batch: int, num_groups: int, num_q_heads: int, num_kv_heads: int, max_pages: int, *,
+                                  device=None) -> int:
+    """Bytes of :func:`shared_prefix_attn`'s workspace on ``device`` (None: the current one)."""
+    return _workspace_bytes("shared_prefix", _device_index(device), batch, num_groups, num_q_heads, num_kv_heads, max_pages)
 
 
 def shared_prefix_attn(q, k_pages, v_pages, group_indptr, prefix_indptr, prefix_indices, prefix_last_page_len, kv_indptr,
@@ -888,8 +908,8 @@ def shared_prefix_attn(q, k_pages, v_pages, group_indptr, prefix_indptr, prefix_
     if b > 0:
         if max_pages is None:
             max_pages = max(prefix_indices.numel(), kv_indices.numel(), 1)
-        workspace = _workspace(workspace, shared_prefix_workspace_bytes(b, groups, hq, hkv, max_pages), q.device)
         index = q.get_device()
+        workspace = _workspace(workspace, _workspace_bytes("shared_prefix", index, b, groups, hq, hkv, max_pages), q.device)
         _launch_small("shared_prefix_attn", index,
                       ("k_pages", k_pages, "v_pages", v_pages, "group_indptr", group_indptr, "prefix_indptr", prefix_indptr,
                        "prefix_indices", prefix_indices, "prefix_last_page_len", prefix_last_page_len, "kv_indptr", kv_indptr,

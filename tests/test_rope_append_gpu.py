@@ -225,3 +225,20 @@ def test_in_place(case, pad):
     got = ops.rope_append_kv(mine, k, v, freqs, kp, vp, None, None, *table, out=mine, **kw)
     assert got.data_ptr() == mine.data_ptr() and torch.equal(got, want)
     assert not wide[:, hq].any() and not wide[..., D:].any()
+
+
+def test_strides_of_one_token_and_of_one_head_are_not_read():
+    for new, hq, hkv in (([1], 4, 2), ([9, 3], 1, 1), ([1], 1, 1)):
+        (q, k, v), kp, vp, table, lens = make(new, [20] * len(new), hq, hkv, torch.bfloat16)
+        freqs, _ = ops.rope_frequencies(device=DEV)
+        t = sum(new)
+
+        def odd(x):
+            x = x.contiguous()
+            return torch.as_strided(x, x.shape, (13 if t == 1 else x.stride(0), 7 if x.shape[1] == 1 else D, 1))
+
+        pools = [x.clone() for x in (kp, vp)]
+        want = ops.rope_append_kv(q, k, v, freqs, *pools, None, None, *table)
+        out = odd(torch.zeros(t, hq, D, dtype=q.dtype, device=DEV))
+        got = ops.rope_append_kv(odd(q), odd(k), odd(v), freqs, kp, vp, None, None, *table, out=out)
+        assert torch.equal(got, want) and torch.equal(kp, pools[0]) and torch.equal(vp, pools[1])

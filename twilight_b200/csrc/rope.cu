@@ -444,6 +444,10 @@ extern "C" int twl_rope_append_kv(const void* q, const void* k, const void* v, i
     return TWL_ERR_BAD_ARG;
   if (rotary_dim < 0 || (rotary_dim > 0 && !freqs)) return TWL_ERR_BAD_ARG;
   if (rotary_dim > kD || rotary_dim % (interleaved ? 8 : 16) != 0) return TWL_ERR_UNSUPPORTED;
+  // the strides of one token, and of one head, say nothing
+  if (num_tokens == 1) q_token_stride = k_token_stride = v_token_stride = out_token_stride = 0;
+  if (num_q_heads == 1) q_head_stride = out_head_stride = 0;
+  if (num_kv_heads == 1) k_head_stride = v_head_stride = 0;
   if (!strides_ok(q, q_token_stride, q_head_stride) || !strides_ok(k, k_token_stride, k_head_stride) ||
       !strides_ok(v, v_token_stride, v_head_stride) || !strides_ok(q_out, out_token_stride, out_head_stride) ||
       !aligned(k_pages, 16) || !aligned(v_pages, 16) || (k4_pages && !aligned(k4_pages, 16)) ||

@@ -842,3 +842,35 @@ def test_selection_flags_what_it_leaves_out_and_counts_every_slot():
             assert (x[1:] > x[:-1]).all() and ((x >= 0) & (x < most - 1)).all()
     # a sequence without new tokens has no lists to leave anything out of
     assert call(max_pages=most)[2] == 0 and (lens[1] + 15) // 16 < most
+
+
+@pytest.mark.parametrize("tokens, pages", [(3, (1 << 22) + 9), (40, (1 << 26) + 9)])
+def test_a_list_shorter_than_its_place_at_far_positions(tokens, pages):
+    """Positions beyond 2^26 and 2^30 (every page of the table is the same one): the places that a list leaves empty are no keys."""
+    k, v, lean, g = pool(1, 1, torch.bfloat16, 95)
+    q = torch.randn(tokens, 1, D, generator=g, device=DEV).to(torch.bfloat16)
+    ptr, last = torch.tensor([0, pages], **I32), torch.tensor([16], **I32)
+    idx = torch.zeros(pages, **I32)
+    slots = tokens // 64 + 1
+    lists, count = torch.zeros(slots, 1, 12, **I32), torch.ones(slots, 1, **I32)
+    status = torch.zeros(1, **I32)
+    out, lse = ops.prompt_attn(q, k, v, torch.tensor([0, tokens], **I32), ptr, idx, last, max_pages=pages, block_pages=lists,
+                               block_npages=count, query_block=64, lse=True, status=status)
+    assert int(status) == 0
+    ref, ref_lse, p = attend64(q[:, 0].double(), k[0, 0].double(), v[0, 0].double(),
+                               torch.ones(tokens, PAGE, dtype=torch.bool, device=DEV))
+    assert ((out[:, 0].double() - ref).abs() <= tol_of(torch.bfloat16, p, v[0, 0].double(), ref)).all()
+    assert ((lse[:, 0].double() - ref_lse).abs() <= 2.0 ** -18 + 2.0 ** -22 * ref_lse.abs()).all()
+
+
+def test_more_new_tokens_than_the_sequence_has():
+    """Queries before position 0 see nothing: zeros, whichever kernel takes them."""
+    for new, old in (([5], [-3]), ([300], [-100])):
+        lens = [new[0] + old[0]]
+        ptr, idx, last = table(lens, 3)
+        k, v, lean, g = pool(idx.numel(), 2, torch.float16, 96)
+        q = torch.randn(new[0], 4, D, generator=g, device=DEV).half()
+        qo = torch.tensor([0, new[0]], **I32)
+        out, lse = ops.prompt_attn(q, k, v, qo, ptr, idx, last, max_pages=20, lse=True)
+        check_prompt(q, k, v, qo, (ptr, idx, last), lens, out, lse)
+        assert not out[: -old[0]].any()

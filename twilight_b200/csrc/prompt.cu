@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
 #pragma unroll
   for (int j = 0; j < 4; ++j) to_off[j] = (2 * j + (lane >> 4)) * 256 + (((lane & 15) ^ (2 * j + (lane >> 4))) << 4);
   // lane j holds number 32*(page/32) + j of the piece's pages: logical page and physical id (or "none")
-  constexpr int kNone = 0x3fffff;  // a logical page behind every limit
+  constexpr int kNone = 0x7ffffff;  // a logical page behind every limit: its last position is 2^31 - 1
   int my_lp = kNone, my_phys = -1, window = -1, window_seg = -1;
   const auto look_up = [&]() {
     const int w = f.page >> 5;

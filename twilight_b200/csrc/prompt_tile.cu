@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       look_up(0, lp, phys);
       for (int t = 0; t < it.n_tiles; ++t) {
         const int group = phys < 0 ? gone : (phys * p.Hkv + it.kvh) * 2;
-        const int pos = phys < 0 ? 0x3fffffff : lp * kPage;
+        const int pos = phys < 0 ? 0x7fffffff : lp * kPage;
         const int hi = __reduce_max_sync(0xffffffffu, lane >= 8 ? -1 : phys < 0 ? 0x7fffffff : pos + kPage - 1);
         look_up(t + 1, lp, phys);
         ok = all_ok(mbar_wait(&empty[stage], (round & 1) ^ 1));
@@ -576,7 +576,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
       const int pair = it.pair;
       const int tok = (pair ? 0 : a * p.tok_tile) + tok_r;  // of the item
       const bool real = tok_r < p.tok_tile && tok < it.ntok;
-      const int limit = !real ? -1 : p.causal ? it.limit0 + tok : it.limit0;
+      const int limit = !real ? -1 : max(-1, p.causal ? it.limit0 + tok : it.limit0);
       float m = -INFINITY, l = 0.f;
       const int steps = a ? it.steps[1] : it.steps[0], steps_other = a ? it.steps[0] : it.steps[1];
       for (int j = 0; j < steps; ++j) {
@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
         if (masked) {
 #pragma unroll
           for (int pg = 0; pg < 8; ++pg) {
-            const int n = limit - sh.pos[slot][pg];  // keys 0..n of the page are seen
+            const int n = limit - sh.pos[slot][pg];  // keys 0..n of the page are seen (at least -2^31: limit is -1 or more)
 #pragma unroll
             for (int c = 0; c < kPage; ++c)
               if (c > n) x[16 * pg + c] = -INFINITY;

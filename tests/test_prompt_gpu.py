@@ -874,3 +874,28 @@ def test_more_new_tokens_than_the_sequence_has():
         out, lse = ops.prompt_attn(q, k, v, qo, ptr, idx, last, max_pages=20, lse=True)
         check_prompt(q, k, v, qo, (ptr, idx, last), lens, out, lse)
         assert not out[: -old[0]].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tokens", [2, 40])
+def test_many_small_weights_add_up(dtype, tokens):
+    """One key of weight 1 and 2^18 of 2^-26.5 each, 2^-8.5 together: rounded to fp16 as they are they would all be zero."""
+    n = 1 << 18
+    k, v = (torch.zeros(2, 1, PAGE, D, dtype=dtype, device=DEV) for _ in range(2))
+    k[0, 0, 0, 0] = 13.0
+    v[:] = torch.randn(2, 1, 1, D, generator=torch.Generator(device=DEV).manual_seed(97), device=DEV).to(dtype)
+    q = torch.zeros(tokens, 1, D, dtype=dtype, device=DEV)
+    q[:, 0, 0] = 16.0
+    idx = torch.ones(n // PAGE, **I32)
+    idx[0] = 0
+    tab = torch.tensor([0, n // PAGE], **I32), idx, torch.tensor([16], **I32)
+    kk, vv = (x[idx.long(), 0].reshape(-1, D).double() for x in (k, v))
+    keep = torch.ones(1, n, dtype=torch.bool, device=DEV)
+    ref, _, p = attend64(q[:1, 0].double(), kk, vv, keep)
+    tol = tol_of(dtype, p, vv, ref)
+    assert ((ref - vv[:1]).abs() > 2 * tol).any()               # the small ones count
+    out = ops.prompt_attn(q, k, v, torch.tensor([0, tokens], **I32), *tab, max_pages=n // PAGE, causal=False)
+    assert ((out[:, 0].double() - ref).abs() <= tol).all()
+    none = torch.zeros(tokens + 1, **I32), torch.zeros(0, **I32), torch.zeros(tokens, **I32)
+    out = ops.shared_prefix_attn(q, k, v, torch.tensor([0, tokens], **I32), *tab, *none)
+    assert ((out[:, 0].double() - ref).abs() <= tol).all()

@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
       float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[h], mx);
+      const float mn = fmaxf(m[h], mx - kTopWeight<T>);
       const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen so far: every weight is 2^-inf = 0
       fac[h] = ex2(m[h] - ref);
       moved |= mn != m[h];
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(RowShape<NT>::kWarps * 32) prompt_rows_kernel(
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = ex2(x[e] - ref);
       l[h] = l[h] * fac[h] + (x[0] + x[1]) + (x[2] + x[3]);
-      // weights go to the tensor cores in the model type (half a step of it each); their sum stays unrounded
+      // weights go to the tensor cores in the model type (half a step of it each, see kTopWeight); their sum stays unrounded
       pb[h][0] = pack2<T>(x[0], x[1]);
       pb[h][1] = pack2<T>(x[2], x[3]);
     }

@@ -16,6 +16,14 @@ namespace twl {
 
 constexpr int kFewRows = 16;  // most rows of a segment of the row kernel
 
+// The largest weight of a row, as a power of two: weights 2^(x - reference) go to the tensor cores in the model type, and fp16 rounds
+// those below 2^-14 in steps of 2^-24 and drops those below 2^-25.  Up here n weights are off by at most n 2^-40 of the largest one
+// altogether (n 2^-25 with the largest at 1: a step of fp16 from 32K keys on).  bf16 has the exponents of fp32.
+template <typename T>
+constexpr float kTopWeight = 15.f;
+template <>
+inline constexpr float kTopWeight<__nv_bfloat16> = 0.f;
+
 struct Segment {
   int32_t tok0, ntok;     // query tokens
   int32_t kvbase, npages; // its part of kv_indices (or of the prefix's)

@@ -9,8 +9,9 @@
 // The two subtiles share K and V and alternate on the tensor cores: while one subtile's weights are computed, the
 // other's products run.  An item of one subtile takes both places: they take its key tiles in turn, and their results
 // are joined at the end.  TMEM (512 columns): S of both (P takes the place of S once it is read), O of both.
-// The reference maximum m of a row is only moved when the true one has grown by more than 2^8, so O is rescaled a
-// few times per row; weights then stay below 2^8, which fp16 and the fp32 sums hold without loss.
+// The reference m of a row is only moved when its maximum has grown by more than 2^8, so O is rescaled a few times per row.  The
+// largest weight is between 1 and 2^8 in bf16, between 2^7 and 2^15 in fp16 (see kTopWeight): n weights are off by at most n 2^-32 of
+// the largest one altogether there.
 //
 // Warps: 0-3 and 4-7 softmax, 8 K pages, 11 V pages, 9 tensor-core issue, 10 work items (taken from a counter, two ahead).
 // K has three 32 KiB stages, V two.  A page is ONE copy: seen as [groups of 8 rows][halves of 64 channels][8 rows][64] it
@@ -208,7 +209,7 @@ __device__ __forceinline__ float max64(const float* x) {
   m[1] = max3(m[1], x[62], x[63]);
   return max3(max3(m[0], m[1], m[2]), m[3], m[3]);
 }
-// 64 weights 2^(x scale - ref) of a row: their sum in 32 bits, and themselves rounded to the model type (half a step each),
+// 64 weights 2^(x scale - ref) of a row: their sum in 32 bits, and themselves rounded to the model type (half a step each, see above),
 // in which they go to the tensor cores.  All on the special-function unit: with an eighth or a quarter of them by a polynomial
 // on the multiply-add pipes, 8K x 8K with 32/8 heads took 848 instead of 823 us.
 template <typename T>
@@ -606,13 +607,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) prompt_tile_kernel(const __gr
           __syncwarp();
         }
         const float top = max3(max64(x), max64(x + 64), -INFINITY) * scale;
-        // Move the reference only when it is 2^8 behind (or nothing was seen so far).  (Computing the first weights with the
-        // standing reference while the maximum is found was 2 % slower.)
+        // Move the reference, kTop below the maximum, only when that has grown by more than 2^8 (or nothing was seen so far).  (Computing
+        // the first weights with the standing reference while the maximum is found was 2 % slower.)
+        constexpr float kTop = kTopWeight<T> == 0.f ? 0.f : kTopWeight<T> - 8.f;
         float f = 1.f;
-        const bool move = !(top <= m + 8.f);  // from -inf: any finite maximum; a NaN moves it too
+        const bool move = !(top <= m + (kTop + 8.f));  // from -inf: any finite maximum; a NaN moves it too
         if (move) {
-          f = tile_ex2(m - top);
-          m = top;
+          f = tile_ex2(m - (top - kTop));
+          m = top - kTop;
           l *= f;
         }
         if (__any_sync(0xffffffffu, move) && j > 0) {

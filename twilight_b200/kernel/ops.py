@@ -775,7 +775,8 @@ def prompt_attn(q, k_pages, v_pages, qo_indptr, kv_indptr, kv_indices, kv_last_p
     :func:`quest_select_blocks` restrict every block of ``query_block`` queries to its pages.  ``max_pages``: the
     largest page count of a sequence.  Returns ``out [T,Hq,128]``, and with ``lse`` (True or a tensor) also the fp32
     ``[T,Hq]`` logarithms of the sums of exponentials.  ``workspace``: ``prompt_attn_workspace_bytes`` bytes, one for
-    each call that may overlap with another."""
+    each call that may overlap with another.  V must be finite also where a query does not see its token (its weight is
+    zero there); rows behind a sequence's end may hold anything."""
     _queries(q)
     t, hq = q.shape[0], q.shape[1]
     pages, hkv = _kv_pools(q, k_pages, v_pages)

@@ -899,3 +899,19 @@ def test_many_small_weights_add_up(dtype, tokens):
     none = torch.zeros(tokens + 1, **I32), torch.zeros(0, **I32), torch.zeros(tokens, **I32)
     out = ops.shared_prefix_attn(q, k, v, torch.tensor([0, tokens], **I32), *tab, *none)
     assert ((out[:, 0].double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_chosen_pages_of_the_longest_history(dtype):
+    """As many pages as the selection takes, a few hundred different ones: equal scores everywhere."""
+    pages, new, hkv, block = 51200, 40, 2, 32
+    k, v, lean, g = pool(300, hkv, dtype, 98)
+    meta = torch.stack([k.amin(2), k.amax(2)], 2).contiguous()
+    q = torch.randn(new, 4, D, generator=g, device=DEV).to(dtype)
+    idx = torch.randint(0, 300, (pages,), generator=g, device=DEV, dtype=torch.int32)
+    tab, qo = (torch.tensor([0, pages], **I32), idx, torch.tensor([16], **I32)), torch.tensor([0, new], **I32)
+    for budget in (16, 5000, 700000):
+        status = torch.zeros(1, **I32)
+        got = ops.quest_select_blocks(q, meta, qo, *tab, budget, max_pages=pages, query_block=block, status=status)
+        assert int(status) == 0
+        assert exact_lists(q, meta, qo, tab, [pages * PAGE], budget, block, hkv, *got) == 2 * hkv

@@ -393,7 +393,7 @@ TWL_API int twl_dequantize_k_pages(const uint8_t* k4_pages, const int32_t* page_
  * holds its first position on, and of the pages before that the max(1,budget/16)+(budget%16!=0) with the
  * largest sums over the block's rows (tokens x query heads of the KV head) of Quest's bound
  * sum_d max(q_d*kmax_d, q_d*kmin_d) (twilight/pyimpl/quest.py:37-99 applied to a block), ties to the
- * lower page.  The choice is that of 64-bit sums (of finite q and kmeta).  pooled: fp32
+ * lower page.  The choice is that of 64-bit sums (of scores up to 1e38).  pooled: fp32
  * [slots][H_kv][256] and page_scores: fp32 [slots][H_kv][max_pages], caller scratch (kept as outputs for
  * inspection: sums of min(q,0) and max(q,0); scores of the pages before the block, in 32 bits).
  * block_npages of a slot that no block has is 0, as are those of a sequence whose offsets or last page

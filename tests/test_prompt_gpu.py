@@ -915,3 +915,12 @@ def test_chosen_pages_of_the_longest_history(dtype):
         got = ops.quest_select_blocks(q, meta, qo, *tab, budget, max_pages=pages, query_block=block, status=status)
         assert int(status) == 0
         assert exact_lists(q, meta, qo, tab, [pages * PAGE], budget, block, hkv, *got) == 2 * hkv
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-36, 1e-38])
+def test_chosen_pages_of_queries_near_the_smallest_numbers(scale):
+    q, k, v, qo, tab, lens = make_prompt([100], [3000], 4, 2, torch.bfloat16, seed=99)
+    q = (q.double() * scale).to(torch.bfloat16)
+    meta = ops.build_page_meta(k, *tab, max_pages=200)
+    got = ops.quest_select_blocks(q, meta, qo, *tab, 500, max_pages=200, query_block=32)
+    assert exact_lists(q, meta, qo, tab, lens, 500, 32, 2, *got) > 0

@@ -8,7 +8,7 @@
 // Segments of at most 8 (or 16) rows go to the row kernel (a warp-level tensor-core tile of as many rows; bound by reading
 // K and V): all their (KV head, page) units in one line, cut into equal runs, one per warp of the GPU.  Longer
 // segments go to the tile kernel in tiles of up to 256 rows; where there are fewer of those than the GPU runs at once,
-// the keys are cut into chunks too.  Partial (maximum, sum, accumulator) triples are joined by the merge kernel.
+// the keys are cut into chunks too.  Partial (reference, sum, accumulator) triples are joined by the merge kernel.
 #pragma once
 #include "common.cuh"
 
@@ -66,7 +66,7 @@ struct AttnParams {
   int4* tile_list;  // {segment, first token, tokens, chunk}
   int32_t tile_cap;
   float* part_acc;  // [rows][128]
-  float2* part_ml;  // [rows] {maximum in log2 units, sum}
+  float2* part_ml;  // [rows] {reference in log2 units, sum of the weights}
   int64_t part_cap;
   int32_t* status;
 };

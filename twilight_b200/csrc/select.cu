@@ -1045,7 +1045,8 @@ __global__ void __launch_bounds__(kTopkThreads, 5) select_query_blocks_kernel(co
     for (int w = 0; w < kTopkThreads / 32; ++w) step += sizes[w];
     step *= Elem<T>::to_f(*reinterpret_cast<const T*>(&largest)) * 0x1p-24f;
     // (one more for the roundings of this product)
-    const float pool_err = step * (float)((qb.rows * (p.Hq / p.Hkv) + 127) / 128 + 7 + 1), err = pool_err + step * (4 + 68 + 8);
+    const float pool_err = step * (float)((qb.rows * (p.Hq / p.Hkv) + 127) / 128 + 7 + 1) + 0x1p-120f;  // (numbers below the normal ones)
+    const float err = pool_err + step * (4 + 68 + 8);
     const float cut = __uint_as_float(thr & 0x80000000u ? thr ^ 0x80000000u : ~thr);
     // (an infinity or NaN among them, or nearly: the 32-bit scores decide, and no page that is not there is open)
     if (fabsf(cut) + 2.f * err < 1e38f) {
